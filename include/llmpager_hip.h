@@ -219,6 +219,93 @@ int lp_mla_attn_decode_batch(lp_ctx* ctx, uint64_t q, uint64_t cache, uint64_t c
                              uint64_t ctx_out, uint64_t workspace, int batch, int heads, int qk_dim, int c_dim,
                              int max_seq, float scale, lp_stream s);
 
+/* ---- a batch's KV cache in pages -------------------------------------------
+ * No reference counterparts: the reference keeps one contiguous cache per
+ * sequence and steps through a batch or a prompt token by token
+ * (decode.rs:368-569).  Here the sequences of a batch, each with one new token
+ * or many, append and attend in one call. */
+
+enum { LP_KV_F16 = 0, LP_KV_Q4 = 1 };
+
+/* One layer's cache.  Its pools hold `pages` pages of page_rows rows for every
+ * KV head: page p of KV head g at pool + (p * kv_heads + g) * lp_kv_page_bytes,
+ * as fp16 [page_rows, head_dim] or as a q4 region [page_rows, head_dim] of
+ * group 32 (quant.rs:1-22: f16 scales, then nibbles holding q + 8).  Row r of
+ * sequence b is row r % page_rows of page table[b][r / page_rows].  An entry
+ * outside 0 .. pages - 1 holds no rows: nothing is appended to it and
+ * attention leaves its rows out.  Sequences may share pages that are only
+ * read. */
+typedef struct lp_kv_cache {
+    uint64_t k_pages, v_pages; /* device pools, 16-byte aligned */
+    uint64_t table;            /* device i32 [batch, max_pages] */
+    int32_t pages;
+    int32_t page_rows;         /* a power of two, 16 to 256 */
+    int32_t max_pages;         /* page_rows * max_pages at most 2^30 */
+    int32_t kv_heads;
+    int32_t head_dim;          /* 64 or 128 */
+    int32_t format;            /* LP_KV_F16 or LP_KV_Q4 */
+} lp_kv_cache;
+
+/* Bytes of one KV head's page (0 for a shape that lp_kv_cache does not take). */
+uint64_t lp_kv_page_bytes(int page_rows, int head_dim, int format);
+
+/* The new tokens of a batch: token t of sequence b, q_starts[b] <= t <
+ * q_starts[b + 1] (device i32 [batch + 1], rising), has position seq_lens[b] -
+ * (q_starts[b + 1] - t): seq_lens (device i32 [batch]) count the new tokens.
+ * Tokens behind the last sequence (q_starts[batch] .. tokens - 1) are padding
+ * and everything of theirs is left as it was.  At most 4096 sequences.
+ *
+ * Per token, rmsnorm of each query head with q_norm and each key head with
+ * k_norm (f32 [head_dim]; 0: none), NeoX rotate-half rope of both, pair
+ * (i, i + head_dim / 2) by position * inv_freq[i] (device f32 [head_dim / 2]),
+ * both factors times mscale; queries to q_out, keys and values into their
+ * pages.  q, k, v and q_out are f32 rows, tokens *_stride floats apart (a
+ * multiple of 4; 16-byte aligned), so they may be parts of one projection's
+ * output; q_out may be q.  An fp16 page rounds to nearest even.  A q4 page
+ * takes scale = max|x| / 7 of each group, rounded to 7 significant bits and kept
+ * within 2^-17 .. 896, and round(x / scale) within -7 .. 7 (NaN as 0), of
+ * values computed in 64 bits.  k_out, v_out (f32 [tokens, kv_heads, head_dim],
+ * or 0): also the rows as the pages hold them.  A position outside the table's
+ * width is not appended.  Two tokens with one place leave one of the two there. */
+int lp_kv_append_paged(lp_ctx* ctx, const lp_kv_cache* cache, uint64_t q, int q_stride, uint64_t k, int k_stride,
+                       uint64_t v, int v_stride, uint64_t q_norm, uint64_t k_norm, float eps, uint64_t inv_freq,
+                       float mscale, uint64_t q_out, int q_out_stride, uint64_t k_out, uint64_t v_out, int heads,
+                       uint64_t q_starts, uint64_t seq_lens, int batch, int tokens, lp_stream s);
+
+/* Causal attention of the batch's new tokens over their sequences' pages (their
+ * own rows among them: append first): out[t, h] = sum_r p_r v_r / sum_r p_r,
+ * p_r = e^(scale q[t, h] . k_r - max), over the rows r up to the token's
+ * position of KV head h / (heads / kv_heads).  A token without a row gets
+ * zeros.  max_q and max_seq bound the new tokens and the lengths of a
+ * sequence: a sequence's tokens past its first max_q are left as they were, a
+ * larger length is taken as max_seq (or as what the table's width holds).  The
+ * bounds decide how the work is split, so a capture may be replayed with other
+ * q_starts, seq_lens and tables within them.  q and out: f32 rows as above,
+ * which must not overlap.  workspace: lp_attn_paged_ws_bytes bytes, 256-byte
+ * aligned (0 bytes: may be 0); two calls that overlap need one each. */
+uint64_t lp_attn_paged_ws_bytes(const lp_kv_cache* cache, int heads, int batch, int tokens, int max_q, int max_seq);
+int lp_attn_paged(lp_ctx* ctx, const lp_kv_cache* cache, uint64_t q, int q_stride, uint64_t out, int out_stride,
+                  int heads, uint64_t q_starts, uint64_t seq_lens, int batch, int tokens, int max_q, int max_seq,
+                  float scale, uint64_t workspace, uint64_t ws_bytes, lp_stream s);
+
+/* ---- logits ---------------------------------------------------------------- */
+
+/* Log probabilities from rows of logits (f32 [vocab], `stride` floats apart;
+ * the reference computes them on the host, main.rs:339-371): logp[r] of the
+ * token targets[r] (i32 [rows]; a token outside the vocabulary gets 0; both 0:
+ * not wanted), entropy[r] in nats (0: not wanted), and the `top` (at most 64)
+ * tokens of the largest logits, largest first, the lowest id first of equal
+ * ones, with their log probabilities (ids i32, top_logp f32 [rows, top]).
+ * Logits of -inf are tokens that cannot be drawn.  A row with a NaN, with +inf
+ * or with nothing but -inf has NaN for its log probabilities and entropy; its
+ * ids are those of its numbers, and -1 where they end.  workspace:
+ * lp_logprobs_ws_bytes bytes, 256-byte aligned (0 bytes: may be 0); two calls
+ * that overlap need one each. */
+uint64_t lp_logprobs_ws_bytes(int rows, int vocab, int top);
+int lp_logprobs(lp_ctx* ctx, uint64_t logits, int stride, int rows, int vocab, uint64_t targets, uint64_t logp,
+                uint64_t entropy, int top, uint64_t ids, uint64_t top_logp, uint64_t workspace, uint64_t ws_bytes,
+                lp_stream s);
+
 /* ---- fused MoE layer ------------------------------------------------------ */
 
 enum { LP_GATING_SOFTMAX = 0, LP_GATING_SIGMOID = 1 };

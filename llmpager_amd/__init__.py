@@ -25,6 +25,9 @@ LIBPATH = os.path.join(LIBDIR, "libllmpager_hip.so")
 GATING_SOFTMAX = 0
 GATING_SIGMOID = 1
 
+KV_F16 = 0
+KV_Q4 = 1
+
 _lib = None
 
 
@@ -69,6 +72,13 @@ class WsLayout(C.Structure):
     _fields_ = [(n, C.c_uint64) for n in (
         "logits", "ids", "wts", "cnt", "gs", "perm", "inv", "uniq", "meta", "et", "act", "y", "xf", "xd",
         "sh_et", "sh_perm", "sh_act", "sh_y", "tiles", "actimg", "xexp", "disp", "total")]
+
+
+class KvCache(C.Structure):
+    """lp_kv_cache (include/llmpager_hip.h): one layer's KV cache in pages."""
+
+    _fields_ = [(n, C.c_uint64) for n in ("k_pages", "v_pages", "table")] + [
+        (n, C.c_int32) for n in ("pages", "page_rows", "max_pages", "kv_heads", "head_dim", "format")]
 
 
 def _sig(lib):
@@ -125,6 +135,14 @@ def _sig(lib):
         "lp_strided_copy": (i32, [vp, u64, i32, i32, u64, i32, i32, i32, i32, vp]),
         "lp_mla_batch_ws_bytes": (u64, [vp, i32, i32, i32]),
         "lp_mla_attn_decode_batch": (i32, [vp, u64, u64, u64, u64, u64, u64, i32, i32, i32, i32, i32, f32, vp]),
+        "lp_kv_page_bytes": (u64, [i32, i32, i32]),
+        "lp_kv_append_paged": (i32, [vp, P(KvCache), u64, i32, u64, i32, u64, i32, u64, u64, f32, u64, f32, u64, i32, u64,
+                                     u64, i32, u64, u64, i32, i32, vp]),
+        "lp_attn_paged_ws_bytes": (u64, [P(KvCache), i32, i32, i32, i32, i32]),
+        "lp_attn_paged": (i32, [vp, P(KvCache), u64, i32, u64, i32, i32, u64, u64, i32, i32, i32, i32, f32, u64, u64,
+                                vp]),
+        "lp_logprobs_ws_bytes": (u64, [i32, i32, i32]),
+        "lp_logprobs": (i32, [vp, u64, i32, i32, i32, u64, u64, u64, i32, u64, u64, u64, u64, vp]),
         "lp_moe_ws_layout_get": (i32, [P(LayerDesc), i32, P(WsLayout)]),
         "lp_moe_workspace_check": (i32, [P(LayerDesc), i32, i32, u64, u64]),
         "lp_moe_route": (i32, [vp, P(LayerDesc), u64, i32, u64, u64, vp]),
@@ -263,6 +281,11 @@ def route_expf_sweep(first: int, stride: int, n: int) -> np.ndarray:
     out = np.zeros(n, np.float32)
     lib().lp_route_expf_sweep(first, stride, n, _ptr(out))
     return out
+
+
+def kv_page_bytes(page_rows: int, head_dim: int, format: int) -> int:
+    """Bytes of one KV head's page (0 for a shape that KvCache does not take)."""
+    return int(lib().lp_kv_page_bytes(page_rows, head_dim, format))
 
 
 def dimage_bytes(cols: int) -> int:
@@ -541,6 +564,39 @@ class Kernels:
                               stream=None) -> None:
         _check(lib().lp_mla_attn_decode_batch(self.cuda.ctx, q, cache, cache_stride, seq_lens, ctx, ws, batch,
                                               heads, qk_dim, c_dim, max_seq, scale, stream))
+
+
+    # a batch's KV cache in pages, and logits (no kernels.rs counterparts)
+    def kv_append_paged(self, cache: KvCache, q: int, q_stride: int, k: int, k_stride: int, v: int, v_stride: int,
+                        q_norm: int, k_norm: int, eps: float, inv_freq: int, mscale: float, q_out: int,
+                        q_out_stride: int, k_out: int, v_out: int, heads: int, q_starts: int, seq_lens: int, batch: int,
+                        tokens: int, stream=None) -> None:
+        """Per-head norms and rope of a batch's new queries and keys, keys and
+        values into their pages (k_out, v_out: 0, or the rows as held)."""
+        _check(lib().lp_kv_append_paged(self.cuda.ctx, cache, q, q_stride, k, k_stride, v, v_stride, q_norm, k_norm,
+                                        eps, inv_freq, mscale, q_out, q_out_stride, k_out, v_out, heads, q_starts,
+                                        seq_lens, batch, tokens, stream))
+
+    def attn_paged_ws_bytes(self, cache: KvCache, heads: int, batch: int, tokens: int, max_q: int, max_seq: int) -> int:
+        return int(lib().lp_attn_paged_ws_bytes(cache, heads, batch, tokens, max_q, max_seq))
+
+    def attn_paged(self, cache: KvCache, q: int, q_stride: int, out: int, out_stride: int, heads: int, q_starts: int,
+                   seq_lens: int, batch: int, tokens: int, max_q: int, max_seq: int, scale: float, ws: int,
+                   stream=None, ws_bytes: int | None = None) -> None:
+        """Causal attention of a batch's new tokens over its pages.  `ws` is a
+        DevPtr or an address with `ws_bytes` given."""
+        _check(lib().lp_attn_paged(self.cuda.ctx, cache, q, q_stride, out, out_stride, heads, q_starts, seq_lens,
+                                   batch, tokens, max_q, max_seq, scale, ws, _ws_bytes(ws, ws_bytes), stream))
+
+    def logprobs_ws_bytes(self, rows: int, vocab: int, top: int) -> int:
+        return int(lib().lp_logprobs_ws_bytes(rows, vocab, top))
+
+    def logprobs(self, logits: int, stride: int, rows: int, vocab: int, targets: int, logp: int, entropy: int, top: int,
+                 ids: int, top_logp: int, ws: int, stream=None, ws_bytes: int | None = None) -> None:
+        """Log probabilities of given tokens, entropies and the `top`
+        alternatives of rows of logits."""
+        _check(lib().lp_logprobs(self.cuda.ctx, logits, stride, rows, vocab, targets, logp, entropy, top, ids, top_logp,
+                                 ws, _ws_bytes(ws, ws_bytes), stream))
 
 
 # ---- fused MoE layer ----------------------------------------------------------------

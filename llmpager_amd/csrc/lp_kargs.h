@@ -302,6 +302,59 @@ struct MlaBatchArgs {
     int32_t max_seq;                // rows per cache: seq_lens[b] is clamped to it on the device
 };
 
+// ---- a batch's KV cache in pages, and logits ---------------------------------
+
+constexpr int kQ4Group = 32;           // columns of a q4 page's scale
+// What an appended row's scales may be: 7 significant bits, so that a nibble
+// times its scale, and 72 scales, are exact in fp16.
+constexpr double kQ4MinScale = 1.0 / (1 << 17);
+constexpr double kQ4MaxScale = 896.0;
+constexpr int kPageRowsMin = 16, kPageRowsMax = 256;
+constexpr int kPagedMaxBatch = 4096;
+constexpr int kLogprobMaxTop = 64;
+
+// Bytes of one KV head's page.
+LPK_HD constexpr int page_bytes(int head_dim, int page_rows, bool q4) {
+    return page_rows * (q4 ? head_dim / kQ4Group * 2 + head_dim / 2 : head_dim * 2);
+}
+
+struct PagedCache {
+    uint64_t k_pages, v_pages;      // page p of KV head g at base + (p kv_heads + g) page_bytes
+    uint64_t table;                 // i32 [batch, max_pages]
+    int32_t pages, page_log2, max_pages, kv_heads;
+};
+
+struct KvAppendPagedArgs {
+    PagedCache c;
+    uint64_t q, k, v;               // f32, tokens *_stride floats apart
+    uint64_t q_norm, k_norm;        // f32 [head_dim] or 0
+    uint64_t inv_freq;              // f32 [head_dim / 2]
+    uint64_t q_out, k_out, v_out;   // k_out, v_out: f32 [tokens, kv_heads, head_dim] or 0
+    uint64_t q_starts, seq_lens;    // i32 [batch + 1], [batch]
+    int32_t q_stride, k_stride, v_stride, q_out_stride;
+    int32_t heads, batch, tokens;
+    int32_t parts, rows_per_part;   // waves per token, and the rows (q, k and v heads) of each
+    float eps, mscale;
+    int32_t pad0;
+};
+
+struct AttnPagedArgs {
+    PagedCache c;
+    uint64_t q, out;                // f32, tokens *_stride floats apart
+    uint64_t q_starts, seq_lens;
+    int32_t q_stride, out_stride;
+    int32_t heads, group, batch, tokens, max_q, max_seq;
+    float scale;
+    int32_t pad0;
+};
+
+struct LogprobArgs {
+    uint64_t logits, targets;       // f32 rows `stride` floats apart; i32 [rows] or 0
+    uint64_t logp, entropy;         // f32 [rows] (entropy may be 0)
+    uint64_t ids, top_logp;         // i32, f32 [rows, top]
+    int32_t stride, rows, vocab, top;
+};
+
 // ---- fused MoE layer ---------------------------------------------------------
 
 // Device-side view of one MoE layer's routing and expert tables.

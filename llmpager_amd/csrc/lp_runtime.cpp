@@ -128,6 +128,15 @@ enum Fn {
     kMidGateupRs,
     kMidDown,
     kMidDownRs,
+    kAppendF16D64,
+    kAppendF16D128,
+    kAppendQ4D64,
+    kAppendQ4D128,
+    kAttnPagedF16D64,
+    kAttnPagedF16D128,
+    kAttnPagedQ4D64,
+    kAttnPagedQ4D128,
+    kLogprobs,
     kNumFns
 };
 
@@ -180,11 +189,16 @@ const FnSpec kSpecs[kNumFns] = {
     {"lp_step.hsaco", "lp_attn_block_g16"},
     {"lp_mid.hsaco", "lp_mid_gateup"},       {"lp_mid.hsaco", "lp_mid_gateup_rs"},
     {"lp_mid.hsaco", "lp_mid_down"},         {"lp_mid.hsaco", "lp_mid_down_rs"},
+    {"lp_paged.hsaco", "lp_kv_append_f16_d64"}, {"lp_paged.hsaco", "lp_kv_append_f16_d128"},
+    {"lp_paged.hsaco", "lp_kv_append_q4_d64"}, {"lp_paged.hsaco", "lp_kv_append_q4_d128"},
+    {"lp_paged.hsaco", "lp_attn_paged_f16_d64"}, {"lp_paged.hsaco", "lp_attn_paged_f16_d128"},
+    {"lp_paged.hsaco", "lp_attn_paged_q4_d64"}, {"lp_paged.hsaco", "lp_attn_paged_q4_d128"},
+    {"lp_logits.hsaco", "lp_logprobs"},
 };
 
 const char* const kModules[] = {"lp_basic.hsaco", "lp_moe.hsaco", "lp_gemm.hsaco", "lp_attn.hsaco",
-                                "lp_step.hsaco", "lp_mid.hsaco"};
-constexpr int kNumModules = 6;
+                                "lp_step.hsaco", "lp_mid.hsaco", "lp_paged.hsaco", "lp_logits.hsaco"};
+constexpr int kNumModules = 8;
 
 std::string library_dir() {
     Dl_info info;
@@ -1028,6 +1042,137 @@ int lp_attn_block(lp_ctx* c, uint64_t q, uint64_t k, uint64_t v, uint64_t q_norm
     b.n_attn = attn_wgs(b.at, heads);
     const unsigned n_o = (unsigned)((hidden + 4 * kBlockRowsPerWave - 1) / (4 * kBlockRowsPerWave));
     return launch(c, (Fn)(kAttnBlockG1 + gi), dim3((unsigned)b.n_attn + n_o), dim3(256), 0, s, b);
+}
+
+// ---- a batch's KV cache in pages (lp_paged.hip) -------------------------------------
+
+uint64_t lp_kv_page_bytes(int page_rows, int head_dim, int format) {
+    if (page_rows < kPageRowsMin || page_rows > kPageRowsMax || (page_rows & (page_rows - 1)) ||
+        (head_dim != 64 && head_dim != 128) || (format != LP_KV_F16 && format != LP_KV_Q4))
+        return 0;
+    return (uint64_t)page_bytes(head_dim, page_rows, format == LP_KV_Q4);
+}
+
+// The cache as the kernels take it.  The rows that a table's width holds stay
+// below 2^30: positions are 32-bit, and a chunk past the last row of one still is.
+static int check_paged(const char* who, const lp_kv_cache* c, PagedCache* out) {
+    const std::string w(who);
+    if (!c) return fail(LP_E_INVALID, w + ": null cache");
+    if (c->format != LP_KV_F16 && c->format != LP_KV_Q4) return fail(LP_E_INVALID, w + ": unknown cache format");
+    if (c->head_dim != 64 && c->head_dim != 128) return fail(LP_E_UNSUPPORTED, w + ": head_dim must be 64 or 128");
+    if (c->page_rows < kPageRowsMin || c->page_rows > kPageRowsMax || (c->page_rows & (c->page_rows - 1)))
+        return fail(LP_E_UNSUPPORTED, w + ": page_rows must be a power of two, 16 to 256");
+    if (c->pages <= 0 || c->max_pages <= 0 || c->kv_heads <= 0)
+        return fail(LP_E_INVALID, w + ": pages, max_pages and kv_heads must be positive");
+    if ((int64_t)c->max_pages * c->page_rows > (1 << 30))
+        return fail(LP_E_UNSUPPORTED, w + ": max_pages x page_rows must be at most 2^30");
+    if (!c->k_pages || !c->v_pages || !c->table || c->k_pages % 16 || c->v_pages % 16 || c->table % 4)
+        return fail(LP_E_INVALID, w + ": null page pool or table, pools not 16-byte aligned, or table not 4-byte aligned");
+    int log2 = 4;
+    while ((1 << log2) < c->page_rows) ++log2;
+    *out = PagedCache{c->k_pages, c->v_pages, c->table, c->pages, log2, c->max_pages, c->kv_heads};
+    return LP_OK;
+}
+
+// f32 rows of `cols` floats, `stride` apart: 16-byte aligned, the rows apart
+// from one another.
+static int check_rows(const std::string& what, uint64_t p, int stride, int64_t cols) {
+    if (!p) return fail(LP_E_INVALID, what + " is null");
+    if (p % 16 || stride % 4) return fail(LP_E_UNSUPPORTED, what + " must be 16-byte aligned, its stride a multiple of 4");
+    if (stride < cols) return fail(LP_E_INVALID, what + ": the stride is smaller than a row");
+    return LP_OK;
+}
+
+static int check_batch(const char* who, int heads, int kv_heads, int batch, int tokens, uint64_t q_starts, uint64_t seq_lens) {
+    const std::string w(who);
+    if (heads <= 0 || heads % kv_heads) return fail(LP_E_INVALID, w + ": heads must be a multiple of kv_heads");
+    if (batch < 0 || tokens < 0) return fail(LP_E_INVALID, w + ": negative batch or tokens");
+    if (batch > kPagedMaxBatch) return fail(LP_E_UNSUPPORTED, w + ": at most " + std::to_string(kPagedMaxBatch) + " sequences");
+    if (batch && (!q_starts || !seq_lens || q_starts % 4 || seq_lens % 4))
+        return fail(LP_E_INVALID, w + ": q_starts or seq_lens null or not 4-byte aligned");
+    return LP_OK;
+}
+
+int lp_kv_append_paged(lp_ctx* c, const lp_kv_cache* cache, uint64_t q, int q_stride, uint64_t k, int k_stride,
+                       uint64_t v, int v_stride, uint64_t q_norm, uint64_t k_norm, float eps, uint64_t inv_freq,
+                       float mscale, uint64_t q_out, int q_out_stride, uint64_t k_out, uint64_t v_out, int heads,
+                       uint64_t q_starts, uint64_t seq_lens, int batch, int tokens, lp_stream s) {
+    KvAppendPagedArgs a{};
+    if (int r = check_paged("kv_append_paged", cache, &a.c)) return r;
+    if (int r = check_batch("kv_append_paged", heads, cache->kv_heads, batch, tokens, q_starts, seq_lens)) return r;
+    const int D = cache->head_dim;
+    if ((int64_t)heads + 2 * (int64_t)cache->kv_heads > INT32_MAX / 256)
+        return fail(LP_E_UNSUPPORTED, "kv_append_paged: too many heads");
+    if (int r = check_rows("kv_append_paged: q", q, q_stride, (int64_t)heads * D)) return r;
+    if (int r = check_rows("kv_append_paged: k", k, k_stride, (int64_t)cache->kv_heads * D)) return r;
+    if (int r = check_rows("kv_append_paged: v", v, v_stride, (int64_t)cache->kv_heads * D)) return r;
+    if (int r = check_rows("kv_append_paged: q_out", q_out, q_out_stride, (int64_t)heads * D)) return r;
+    if (!inv_freq || inv_freq % 8 || q_norm % 8 || k_norm % 8 || k_out % 16 || v_out % 16)
+        return fail(LP_E_INVALID, "kv_append_paged: null inv_freq, or a misaligned pointer");
+    if (int r = check_ctx(c)) return r;
+    if (!batch || !tokens) return LP_OK;
+    a.q = q, a.k = k, a.v = v, a.q_norm = q_norm, a.k_norm = k_norm, a.inv_freq = inv_freq;
+    a.q_out = q_out, a.k_out = k_out, a.v_out = v_out, a.q_starts = q_starts, a.seq_lens = seq_lens;
+    a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride, a.q_out_stride = q_out_stride;
+    a.heads = heads, a.batch = batch, a.tokens = tokens;
+    a.eps = eps, a.mscale = mscale;
+    const int rows = heads + 2 * cache->kv_heads, per = 256 / D;  // rows a wave takes at a time
+    a.rows_per_part = per;
+    a.parts = (rows + a.rows_per_part - 1) / a.rows_per_part;
+    const int64_t waves = (int64_t)tokens * a.parts;
+    if (waves > INT32_MAX / 256) return fail(LP_E_UNSUPPORTED, "kv_append_paged: too many tokens");
+    const Fn f = cache->format == LP_KV_Q4 ? (D == 64 ? kAppendQ4D64 : kAppendQ4D128)
+                                           : (D == 64 ? kAppendF16D64 : kAppendF16D128);
+    return launch(c, f, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, s, a);
+}
+
+uint64_t lp_attn_paged_ws_bytes(const lp_kv_cache*, int, int, int, int, int) { return 0; }
+
+int lp_attn_paged(lp_ctx* c, const lp_kv_cache* cache, uint64_t q, int q_stride, uint64_t out, int out_stride, int heads,
+                  uint64_t q_starts, uint64_t seq_lens, int batch, int tokens, int max_q, int max_seq, float scale,
+                  uint64_t workspace, uint64_t ws_bytes, lp_stream s) {
+    AttnPagedArgs a{};
+    if (int r = check_paged("attn_paged", cache, &a.c)) return r;
+    if (int r = check_batch("attn_paged", heads, cache->kv_heads, batch, tokens, q_starts, seq_lens)) return r;
+    const int D = cache->head_dim;
+    if (int r = check_rows("attn_paged: q", q, q_stride, (int64_t)heads * D)) return r;
+    if (int r = check_rows("attn_paged: out", out, out_stride, (int64_t)heads * D)) return r;
+    if (q == out) return fail(LP_E_INVALID, "attn_paged: out must not be q");
+    if (max_q < 0 || max_seq < 0) return fail(LP_E_INVALID, "attn_paged: negative max_q or max_seq");
+    if (int r = check_ctx(c)) return r;
+    if (!batch || !tokens || !max_q) return LP_OK;
+    (void)workspace, (void)ws_bytes;
+    a.q = q, a.out = out, a.q_starts = q_starts, a.seq_lens = seq_lens;
+    a.q_stride = q_stride, a.out_stride = out_stride;
+    a.heads = heads, a.group = heads / cache->kv_heads, a.batch = batch, a.tokens = tokens;
+    a.max_q = std::min(max_q, tokens);
+    a.max_seq = (int)std::min<int64_t>(max_seq, (int64_t)cache->max_pages * cache->page_rows);
+    a.scale = scale;
+    const int64_t waves = (int64_t)batch * a.max_q * heads;
+    if (waves > INT32_MAX / 256) return fail(LP_E_UNSUPPORTED, "attn_paged: too many queries");
+    const Fn f = cache->format == LP_KV_Q4 ? (D == 64 ? kAttnPagedQ4D64 : kAttnPagedQ4D128)
+                                           : (D == 64 ? kAttnPagedF16D64 : kAttnPagedF16D128);
+    return launch(c, f, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, s, a);
+}
+
+// ---- logits (lp_logits.hip) ---------------------------------------------------------
+
+uint64_t lp_logprobs_ws_bytes(int, int, int) { return 0; }
+
+int lp_logprobs(lp_ctx* c, uint64_t logits, int stride, int rows, int vocab, uint64_t targets, uint64_t logp,
+                uint64_t entropy, int top, uint64_t ids, uint64_t top_logp, uint64_t workspace, uint64_t ws_bytes,
+                lp_stream s) {
+    if (rows < 0 || vocab <= 0 || stride < vocab) return fail(LP_E_INVALID, "logprobs: need rows >= 0 and 1 <= vocab <= stride");
+    if (top < 0 || top > vocab) return fail(LP_E_INVALID, "logprobs: top must be 0 to vocab");
+    if (top > kLogprobMaxTop) return fail(LP_E_UNSUPPORTED, "logprobs: at most " + std::to_string(kLogprobMaxTop) + " alternatives");
+    if (!logits || logits % 4 || targets % 4 || logp % 4 || entropy % 4 || ids % 4 || top_logp % 4 ||
+        (targets != 0) != (logp != 0) || (top && (!ids || !top_logp)))
+        return fail(LP_E_INVALID, "logprobs: null or misaligned pointer (targets and logp go together)");
+    if (int r = check_ctx(c)) return r;
+    if (!rows) return LP_OK;
+    (void)workspace, (void)ws_bytes;
+    LogprobArgs a{logits, targets, logp, entropy, ids, top_logp, stride, rows, vocab, top};
+    return launch(c, kLogprobs, dim3((unsigned)rows), dim3(256), 0, s, a);
 }
 
 // ---- fused MoE layer --------------------------------------------------------------

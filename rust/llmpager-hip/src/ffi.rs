@@ -43,6 +43,9 @@ pub const LP_E_DEVICE: c_int = -5;
 pub const LP_GATING_SOFTMAX: i32 = 0;
 pub const LP_GATING_SIGMOID: i32 = 1;
 
+pub const LP_KV_F16: i32 = 0;
+pub const LP_KV_Q4: i32 = 1;
+
 pub const LP_LOOKUP_HIT: c_int = 0;
 pub const LP_LOOKUP_MISS: c_int = 1;
 pub const LP_LOOKUP_STALLED: c_int = 2;
@@ -52,6 +55,20 @@ pub const LP_PAGER_SRC_HOST: i32 = 1;
 pub const LP_PAGER_SRC_PACK: i32 = 2;
 
 pub const LP_NOALLOC_SCRATCH_BYTES: u64 = 16 << 20;
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug, Default)]
+pub struct lp_kv_cache {
+    pub k_pages: u64,
+    pub v_pages: u64,
+    pub table: u64,
+    pub pages: i32,
+    pub page_rows: i32,
+    pub max_pages: i32,
+    pub kv_heads: i32,
+    pub head_dim: i32,
+    pub format: i32,
+}
 
 #[repr(C)]
 #[derive(Clone, Copy, Debug, Default)]
@@ -254,6 +271,28 @@ extern "C" {
     pub fn lp_mla_attn_decode_batch(
         ctx: *mut lp_ctx, q: u64, cache: u64, cache_stride: u64, seq_lens: u64, ctx_out: u64, workspace: u64,
         batch: c_int, heads: c_int, qk_dim: c_int, c_dim: c_int, max_seq: c_int, scale: f32, s: lp_stream,
+    ) -> c_int;
+
+    // ---- a batch's KV cache in pages, and logits ----
+    pub fn lp_kv_page_bytes(page_rows: c_int, head_dim: c_int, format: c_int) -> u64;
+    pub fn lp_kv_append_paged(
+        ctx: *mut lp_ctx, cache: *const lp_kv_cache, q: u64, q_stride: c_int, k: u64, k_stride: c_int, v: u64,
+        v_stride: c_int, q_norm: u64, k_norm: u64, eps: f32, inv_freq: u64, mscale: f32, q_out: u64,
+        q_out_stride: c_int, k_out: u64, v_out: u64, heads: c_int, q_starts: u64, seq_lens: u64, batch: c_int,
+        tokens: c_int, s: lp_stream,
+    ) -> c_int;
+    pub fn lp_attn_paged_ws_bytes(
+        cache: *const lp_kv_cache, heads: c_int, batch: c_int, tokens: c_int, max_q: c_int, max_seq: c_int,
+    ) -> u64;
+    pub fn lp_attn_paged(
+        ctx: *mut lp_ctx, cache: *const lp_kv_cache, q: u64, q_stride: c_int, out: u64, out_stride: c_int,
+        heads: c_int, q_starts: u64, seq_lens: u64, batch: c_int, tokens: c_int, max_q: c_int, max_seq: c_int,
+        scale: f32, workspace: u64, ws_bytes: u64, s: lp_stream,
+    ) -> c_int;
+    pub fn lp_logprobs_ws_bytes(rows: c_int, vocab: c_int, top: c_int) -> u64;
+    pub fn lp_logprobs(
+        ctx: *mut lp_ctx, logits: u64, stride: c_int, rows: c_int, vocab: c_int, targets: u64, logp: u64,
+        entropy: u64, top: c_int, ids: u64, top_logp: u64, workspace: u64, ws_bytes: u64, s: lp_stream,
     ) -> c_int;
 
     // ---- the fused MoE layer ----

@@ -8,7 +8,7 @@
 use anyhow::{bail, Result};
 
 use crate::driver::{CUdeviceptr, CUstream, Cuda};
-use crate::ffi::{self, check, lp_moe_layer_desc, lp_moe_ws_layout};
+use crate::ffi::{self, check, lp_kv_cache, lp_moe_layer_desc, lp_moe_ws_layout};
 
 /// The code objects are loaded by [`Cuda::init`]; `Kernels` keeps the
 /// reference's shape (`load`, then `&self` methods taking `&Cuda`).
@@ -262,6 +262,72 @@ impl Kernels {
             )
         };
         check(rc, "mla_attn_decode_batch")
+    }
+
+    /// Bytes of one KV head's page of a paged cache (0 for a shape it does not take).
+    pub fn kv_page_bytes(&self, page_rows: i32, head_dim: i32, format: i32) -> u64 {
+        unsafe { ffi::lp_kv_page_bytes(page_rows, head_dim, format) }
+    }
+
+    /// A batch's new tokens: per-head norms and rope of the queries (to
+    /// `q_out`) and keys, keys and values into the cache's pages; `k_out` and
+    /// `v_out` (or 0) take the rows as the pages hold them.
+    #[allow(clippy::too_many_arguments)]
+    pub fn kv_append_paged(
+        &self, cuda: &Cuda, cache: &lp_kv_cache, q: CUdeviceptr, q_stride: i32, k: CUdeviceptr, k_stride: i32,
+        v: CUdeviceptr, v_stride: i32, q_norm: CUdeviceptr, k_norm: CUdeviceptr, eps: f32, inv_freq: CUdeviceptr,
+        mscale: f32, q_out: CUdeviceptr, q_out_stride: i32, k_out: CUdeviceptr, v_out: CUdeviceptr, heads: i32,
+        q_starts: CUdeviceptr, seq_lens: CUdeviceptr, batch: i32, tokens: i32, stream: CUstream,
+    ) -> Result<()> {
+        let rc = unsafe {
+            ffi::lp_kv_append_paged(
+                cuda.ctx, cache, q, q_stride, k, k_stride, v, v_stride, q_norm, k_norm, eps, inv_freq, mscale, q_out,
+                q_out_stride, k_out, v_out, heads, q_starts, seq_lens, batch, tokens, stream,
+            )
+        };
+        check(rc, "kv_append_paged")
+    }
+
+    /// Workspace bytes for [`Self::attn_paged`].
+    pub fn attn_paged_ws_bytes(&self, cache: &lp_kv_cache, heads: i32, batch: i32, tokens: i32, max_q: i32, max_seq: i32) -> u64 {
+        unsafe { ffi::lp_attn_paged_ws_bytes(cache, heads, batch, tokens, max_q, max_seq) }
+    }
+
+    /// Causal attention of a batch's new tokens over the cache's pages.
+    #[allow(clippy::too_many_arguments)]
+    pub fn attn_paged(
+        &self, cuda: &Cuda, cache: &lp_kv_cache, q: CUdeviceptr, q_stride: i32, out: CUdeviceptr, out_stride: i32,
+        heads: i32, q_starts: CUdeviceptr, seq_lens: CUdeviceptr, batch: i32, tokens: i32, max_q: i32, max_seq: i32,
+        scale: f32, ws: CUdeviceptr, ws_bytes: u64, stream: CUstream,
+    ) -> Result<()> {
+        let rc = unsafe {
+            ffi::lp_attn_paged(
+                cuda.ctx, cache, q, q_stride, out, out_stride, heads, q_starts, seq_lens, batch, tokens, max_q,
+                max_seq, scale, ws, ws_bytes, stream,
+            )
+        };
+        check(rc, "attn_paged")
+    }
+
+    /// Workspace bytes for [`Self::logprobs`].
+    pub fn logprobs_ws_bytes(&self, rows: i32, vocab: i32, top: i32) -> u64 {
+        unsafe { ffi::lp_logprobs_ws_bytes(rows, vocab, top) }
+    }
+
+    /// Log probabilities of given tokens, entropies and the `top` alternatives
+    /// of rows of logits.
+    #[allow(clippy::too_many_arguments)]
+    pub fn logprobs(
+        &self, cuda: &Cuda, logits: CUdeviceptr, stride: i32, rows: i32, vocab: i32, targets: CUdeviceptr,
+        logp: CUdeviceptr, entropy: CUdeviceptr, top: i32, ids: CUdeviceptr, top_logp: CUdeviceptr, ws: CUdeviceptr,
+        ws_bytes: u64, stream: CUstream,
+    ) -> Result<()> {
+        let rc = unsafe {
+            ffi::lp_logprobs(
+                cuda.ctx, logits, stride, rows, vocab, targets, logp, entropy, top, ids, top_logp, ws, ws_bytes, stream,
+            )
+        };
+        check(rc, "logprobs")
     }
 
     /// Workspace layout (and `total` bytes) of one MoE layer over `t` tokens.
