@@ -271,3 +271,533 @@ extern "C" __global__ void __launch_bounds__(256) lp_attn_paged_f16_d64(const At
 extern "C" __global__ void __launch_bounds__(256) lp_attn_paged_f16_d128(const AttnPagedArgs a) { attn_body<128, false>(a); }
 extern "C" __global__ void __launch_bounds__(256) lp_attn_paged_q4_d64(const AttnPagedArgs a) { attn_body<64, true>(a); }
 extern "C" __global__ void __launch_bounds__(256) lp_attn_paged_q4_d128(const AttnPagedArgs a) { attn_body<128, true>(a); }
+
+// ---------------------------------------------------------------------------
+// Attention of few query rows: up to 16 NT rows (new tokens x query heads of a
+// KV head) against a sequence's pages.  Bytes bound it, so it is laid out for
+// loads: a workgroup takes `span` rows of one (sequence, KV head) and each of
+// its waves walks chunks of CR rows of its own, without a barrier.
+//
+//   scores   S^T = K Q^T on v_mfma_f32_16x16x32_f16: cache rows as M, straight
+//            from global memory into registers, the query rows as N.  The
+//            queries are fp16 hi + lo images of q scale log2 e (2^-22 of it is
+//            left out), two MFMAs a step; a 4-bit key is its nibble placed in
+//            the mantissa of 64 + n, then one packed fma, n s - 72 s, exact as
+//            scales have 7 significant bits;
+//   softmax  lane (query n, kb) holds rows RB kb .. RB kb + RB - 1 of the chunk
+//            (M index m of tile t is row RB (m / 4) + 4 t + m % 4), so maximum,
+//            e^ and sum stay in the lane; the running maximum is raised only
+//            when a score passes it by 2^8, which spares the rescaling and the
+//            exchange between lanes;
+//   context  O^T = V^T P^T: the probabilities (hi + lo) are the B operand as
+//            they lie in the registers, and V^T comes from the chunk's value
+//            rows in LDS through the transposing reads, 4 x 16 fp16 or 16 x 16
+//            nibbles to a 16-lane group.
+//
+// Rows past the sequence, or of absent pages, are masked and their values
+// zeroed.  Rows that only some of the queries see (several new tokens) may hold
+// NaN or infinity, which zero probabilities would not keep out: where one does,
+// attn_rows_apart adds the chunk row by row.
+// ---------------------------------------------------------------------------
+namespace {
+
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef short v4i16_t __attribute__((ext_vector_type(4)));
+typedef int v2i32_t __attribute__((ext_vector_type(2)));
+
+#define LP_LDS __attribute__((address_space(3)))
+// LDS bytes are written as one type and read as another
+typedef uint16_t u16_any __attribute__((may_alias));
+typedef uint32_t u32_any __attribute__((may_alias));
+typedef uint64_t u64_any __attribute__((may_alias));
+typedef u32x4_t u32x4_any __attribute__((may_alias));
+typedef f32x4_t f32x4_any __attribute__((may_alias));
+typedef float2 float2_any __attribute__((may_alias));
+
+__device__ __forceinline__ f32x4_t mfma16(const u32x4_t& a, const u32x4_t& b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Two values as fp16, cut towards zero: with the next 11 bits of each in `lo`,
+// 2^-21 of a value is left out.
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+    hi = __builtin_bit_cast(uint32_t, h);
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a - (float)h[0], b - (float)h[1]));
+}
+
+// Eight nibbles times their scales: pairs (n0, n4), (n1, n5), (n2, n6), (n3, n7)
+// of q + 8, each pair by s (scales of its two) with c = -72 s.
+__device__ __forceinline__ uint32_t nibble_pair(uint32_t w, half2_t s, half2_t c) {
+    const half2_t v = __builtin_bit_cast(half2_t, and_or(w, 0x00f000f0u, 0x54005400u));
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(v, s, c));
+}
+__device__ __forceinline__ u32x4_t nibbles8(uint32_t w, const half2_t (&s)[4], const half2_t (&c)[4]) {
+    u32x4_t r;
+    r[0] = nibble_pair(w << 4, s[0], c[0]);
+    r[1] = nibble_pair(w, s[1], c[1]);
+    r[2] = nibble_pair(w >> 4, s[2], c[2]);
+    r[3] = nibble_pair(w >> 8, s[3], c[3]);
+    return r;
+}
+
+__device__ __forceinline__ bool odd_halves(uint32_t w) {  // a NaN or infinity among the two
+    return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u;
+}
+
+// The new tokens of sequence b and its rows, as the kernels take them.
+struct SeqView {
+    int t0, n, len;  // first token, tokens (at most max_q), rows
+    int p0;          // the first token's position
+};
+__device__ __forceinline__ SeqView seq_view(const AttnPagedArgs& a, int b) {
+    SeqView s;
+    s.t0 = gptr<int>(a.q_starts)[b];
+    const int n = gptr<int>(a.q_starts)[b + 1] - s.t0;
+    s.len = min(gptr<int>(a.seq_lens)[b], a.max_seq);
+    s.p0 = s.len - n;
+    s.n = min(n, a.max_q);
+    if (s.t0 < 0 || s.t0 > a.tokens - s.n) s.n = 0;  // starts that name no tokens
+    return s;
+}
+
+// A sequence's rows of one KV head per split, and the record of (sequence and
+// KV head bg, split, query row): D sums, then {maximum, sum} behind all of them.
+__device__ __forceinline__ uint64_t rec_index(const AttnPagedArgs& a, int bg, int split, int row) {
+    return ((uint64_t)(uint32_t)bg * (uint32_t)a.splits + (uint32_t)split) * (uint32_t)a.rows + (uint32_t)row;
+}
+template <int D>
+__device__ __forceinline__ uint64_t rec_sums(const AttnPagedArgs& a) {
+    return a.part + (uint64_t)(uint32_t)(a.batch * a.c.kv_heads) * (uint32_t)a.splits * (uint32_t)a.rows * (D * 4);
+}
+
+template <int D, bool Q4>
+struct FewRows {
+    static constexpr int CR = Q4 ? 64 : 32;            // rows per chunk
+    static constexpr int RB = CR / 4, MT = CR / 16;    // rows of a lane, 16-row tiles
+    static constexpr int G = D / 32, DT = D / 16;
+    static constexpr int RS = Q4 ? D / 2 + (D == 128 ? 16 : 8) : D * 2 + 32;  // LDS bytes of a value row
+    static constexpr int kScales = Q4 ? CR * G * 2 : 0;
+    static constexpr int kWave = CR * RS + 2 * kScales;                        // value rows, key scales, value scales
+    static constexpr int kMerge = 4 * 16 * (D + 4) * 4 + 4 * 16 * 8;           // the waves' sums of one query tile
+    static constexpr int kLds = 4 * kWave > kMerge ? 4 * kWave : kMerge;
+};
+
+template <int D, bool Q4, int NT>
+__device__ __forceinline__ void few_body(const AttnPagedArgs& a) {
+    using F = FewRows<D, Q4>;
+    constexpr int CR = F::CR, RB = F::RB, MT = F::MT, G = F::G, DT = F::DT, RS = F::RS;
+    constexpr int KS = D / 32;                       // MFMA steps of a score
+    constexpr int KW = Q4 ? D / 32 : D / 8;          // 32-bit words of a key row in a lane, and of a value row
+    __shared__ __align__(16) uint8_t lds[F::kLds];
+    const int wave = (int)(threadIdx.x >> 6), lane = lane_id(), n = lane & 15, kb = lane >> 4;
+    const int split = blockIdx.y, bg = blockIdx.x, b = bg / a.c.kv_heads, g = bg - b * a.c.kv_heads;
+    const SeqView sv = seq_view(a, b);
+    const int r0 = split * a.span, r1 = min(sv.len, r0 + a.span);
+    const int nrows = sv.n * a.group;
+    if (nrows <= 0 || (r0 >= r1 && split > 0)) return;  // whole workgroups
+    uint8_t* const mine = lds + wave * F::kWave;
+    const uint32_t vt = (uint32_t)(uintptr_t)(LP_LDS uint8_t*)mine;
+    LP_LDS uint8_t* const vl = (LP_LDS uint8_t*)mine;
+    LP_LDS u16_any* const ksl = (LP_LDS u16_any*)(mine + CR * RS);
+    LP_LDS u16_any* const vsl = (LP_LDS u16_any*)(mine + CR * RS + F::kScales);
+
+    // ---- chunks: page, keys, values
+    const int blk = (n >> 2) * RB;  // the lane's rows of a tile, within the chunk: blk + 4 t + n % 4
+    const int pmask = (1 << a.c.page_log2) - 1;
+    uint32_t kreg[MT][KW], vreg[MT][KW];
+    uint64_t ksr = 0, vsr = 0;
+    auto page_for = [&](int c) { return c < r1 ? page_of(a.c, b, c + blk) : -1; };
+    auto row_at = [&](int c, int pg) {  // byte offset in a pool of the page's first byte
+        return ((uint64_t)(uint32_t)max(pg, 0) * (uint32_t)a.c.kv_heads + (uint32_t)g) *
+               (uint32_t)(Q4 ? (G * 2 + D / 2) << a.c.page_log2 : (D * 2) << a.c.page_log2);
+    };
+    auto load_rows = [&](uint32_t (&r)[MT][KW], uint64_t& sr, uint64_t pool, int c, int pg) {
+        const uint32_t pr = (uint32_t)((c + blk) & pmask);
+        const uint64_t at = pool + row_at(c, pg);
+        if constexpr (Q4) {
+            // the scales of row blk + 4 kb + n % 4, all groups
+            const uint64_t sa = at + (pr + 4 * kb + (n & 3)) * (G * 2);
+            sr = G == 4 ? *gptr<uint64_t>(sa) : (uint64_t)*gptr<uint32_t>(sa);
+        }
+        const uint64_t ra = at + (Q4 ? (uint32_t)(G * 2) << a.c.page_log2 : 0u) + (pr + (n & 3)) * (uint32_t)(Q4 ? D / 2 : D * 2) +
+                            (Q4 ? kb * (D / 8) : kb * 16);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            if constexpr (Q4 && D == 64) {
+                const auto v = *gptr<uint64_t>(ra + t * 4 * (D / 2));
+                r[t][0] = (uint32_t)v, r[t][1] = (uint32_t)(v >> 32);
+            } else {
+#pragma unroll
+                for (int j = 0; j < KW / 4; ++j) {
+                    const u32x4_t v = *gptr<u32x4_t>(ra + t * 4 * (Q4 ? D / 2 : D * 2) + 64 * j);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) r[t][4 * j + i] = v[i];
+                }
+            }
+        }
+    };
+    int c = r0 + wave * CR, pg = -1, pg1 = -1;
+    if (c < r1) {
+        pg = page_for(c);
+        load_rows(kreg, ksr, a.c.k_pages, c, pg);
+        load_rows(vreg, vsr, a.c.v_pages, c, pg);
+        pg1 = page_for(c + 4 * CR);
+    }
+
+    // ---- the query rows' images: lane (n, kb), step j
+    u32x4_t qh[NT][KS], ql[NT][KS];
+    int last[NT];  // the last row that query n of a tile sees
+    const float qs = a.scale * 1.44269504088896341f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int row = nt * 16 + n, i = row / a.group, h = g * a.group + (row - i * a.group);
+        const bool on = row < nrows;
+        last[nt] = on ? sv.p0 + i : -1;
+        const uint64_t q = a.q + ((uint64_t)(uint32_t)(sv.t0 + (on ? i : 0)) * (uint32_t)a.q_stride + (uint32_t)((on ? h : 0) * D)) * 4;
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+            const int d = Q4 ? (D / 4) * kb + 8 * j : 32 * j + 8 * kb;
+            f32x4_t x0 = gptr<f32x4_t>(q + 4 * d)[0], x1 = gptr<f32x4_t>(q + 4 * d)[1];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) x0[u] = on ? x0[u] * qs : 0.0f, x1[u] = on ? x1[u] * qs : 0.0f;
+            uint32_t h4[4], l4[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if constexpr (Q4)
+                    split2(x0[u], x1[u], h4[u], l4[u]);
+                else
+                    split2(u < 2 ? x0[2 * u] : x1[2 * u - 4], u < 2 ? x0[2 * u + 1] : x1[2 * u - 3], h4[u], l4[u]);
+            }
+            qh[nt][j] = u32x4_t{h4[0], h4[1], h4[2], h4[3]};
+            ql[nt][j] = u32x4_t{l4[0], l4[1], l4[2], l4[3]};
+        }
+    }
+    // rows below `all` are seen by every query row there is
+    const int all = min(sv.p0 + 1, sv.len);
+
+    float m[NT], l[NT];
+    f32x4_t acc[NT][DT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        m[nt] = -INFINITY, l[nt] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[nt][d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    for (; c < r1; c += 4 * CR) {
+        const bool there = pg >= 0;
+        const bool whole = c + CR <= all && __ballot(!there) == 0;  // every row there and seen by all
+        // ---- scores
+        f32x4_t s[NT][MT];
+        if constexpr (Q4) {
+            if (G == 4)
+                *(LP_LDS u64_any*)(ksl + lane * G) = ksr;
+            else
+                *(LP_LDS u32_any*)(ksl + lane * G) = (uint32_t)ksr;
+            __builtin_amdgcn_wave_barrier();
+        }
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            half2_t sc[4], cc[4];
+            if constexpr (Q4) {
+                const _Float16 x = __builtin_bit_cast(_Float16, ksl[(16 * t + n) * G + (kb * G >> 2)]);
+                const half2_t x2 = {x, x}, y2 = x2 * (_Float16)-72.0f;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) sc[u] = x2, cc[u] = y2;
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) s[nt][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < KS; ++j) {
+                u32x4_t k;
+                if constexpr (Q4)
+                    k = nibbles8(kreg[t][j], sc, cc);
+                else
+                    k = u32x4_t{kreg[t][4 * j], kreg[t][4 * j + 1], kreg[t][4 * j + 2], kreg[t][4 * j + 3]};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    s[nt][t] = mfma16(k, qh[nt][j], s[nt][t]);
+                    s[nt][t] = mfma16(k, ql[nt][j], s[nt][t]);
+                }
+            }
+        }
+        const int cn = c + 4 * CR;
+        if (cn < r1) load_rows(kreg, ksr, a.c.k_pages, cn, pg1);
+        // ---- values to LDS, as they are; those of rows that are not there as zeros
+        bool odd = false;
+        {
+            if constexpr (Q4) {
+                const int r = blk + 4 * kb + (n & 3);
+                if (!(there && c + r < sv.len)) vsr = 0;
+                if (!whole) odd = odd_halves((uint32_t)vsr) || odd_halves((uint32_t)(vsr >> 32));
+                // the scale of row r in the order of the pairs: 0, 4, 1, 5, ... of eight
+                const int at = (r & ~7) + 2 * (r & 3) + (r >> 2 & 1);
+#pragma unroll
+                for (int u = 0; u < G; ++u) vsl[u * CR + at] = (uint16_t)(vsr >> (16 * u));
+            }
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const int r = blk + 4 * t + (n & 3);
+                if constexpr (!Q4) {
+                    if (!whole) {
+                        const bool in = there && c + r < sv.len;
+#pragma unroll
+                        for (int i = 0; i < KW; ++i) {
+                            vreg[t][i] = in ? vreg[t][i] : 0u;
+                            odd |= odd_halves(vreg[t][i]);
+                        }
+                    }
+                }
+                if constexpr (Q4 && D == 64) {
+                    *(LP_LDS u64_any*)(vl + r * RS + kb * 8) = (uint64_t)vreg[t][1] << 32 | vreg[t][0];
+                } else {
+#pragma unroll
+                    for (int j = 0; j < KW / 4; ++j)
+                        *(LP_LDS u32x4_any*)(vl + r * RS + kb * 16 + 64 * j) =
+                            u32x4_t{vreg[t][4 * j], vreg[t][4 * j + 1], vreg[t][4 * j + 2], vreg[t][4 * j + 3]};
+                }
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+        if (cn < r1) load_rows(vreg, vsr, a.c.v_pages, cn, pg1);
+        const int there_n = whole ? 1 : __shfl((int)there, 4 * kb, 64);  // the page of the lane's rows as a query
+        pg = pg1;
+        pg1 = page_for(cn + 4 * CR);
+        // ---- softmax: lane (n, kb), row RB kb + 4 t + v
+        u32x4_t ph[NT][CR / 32], pl[NT][CR / 32];
+        float p[NT][MT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            if (!whole) {
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int v = 0; v < 4; ++v)
+                        if (!there_n || c + RB * kb + 4 * t + v > last[nt]) s[nt][t][v] = -INFINITY;
+            }
+            float mx = s[nt][0][0];
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) mx = fmaxf(mx, s[nt][t][v]);
+            if (__ballot(mx > m[nt] + 8.0f)) {
+                mx = fmaxf(mx, shfl_xor(mx, 16));
+                mx = fmaxf(mx, shfl_xor(mx, 32));
+                const float mn = fmaxf(m[nt], mx);
+                // nothing seen so far: nothing to rescale
+                const float f = m[nt] == -INFINITY ? 0.0f : exp2_hw(m[nt] - mn);
+                l[nt] *= f;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) acc[nt][d] *= f;
+                m[nt] = mn;
+            }
+            const float base = m[nt] == -INFINITY ? 0.0f : m[nt];
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    p[nt][t][v] = exp2_hw(s[nt][t][v] - base);
+                    l[nt] += p[nt][t][v];
+                }
+#pragma unroll
+            for (int w = 0; w < CR / 32; ++w)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    uint32_t h, lo;
+                    if constexpr (Q4)
+                        split2(p[nt][2 * w][v], p[nt][2 * w + 1][v], h, lo);
+                    else
+                        split2(p[nt][v >> 1][2 * (v & 1)], p[nt][v >> 1][2 * (v & 1) + 1], h, lo);
+                    ph[nt][w][v] = h, pl[nt][w][v] = lo;
+                }
+        }
+        // ---- context
+        if (!whole && __ballot(odd)) {
+            // row by row, each for the queries that see it
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int v = 0; v < 4; ++v)
+                        for (int k = 0; k < 4; ++k) {
+                            const int r = RB * k + 4 * t + v;
+                            const float pk = __shfl(p[nt][t][v], n + 16 * k, 64);
+                            const int in = __shfl(there_n, 16 * k, 64);
+                            if (c + r > last[nt] || !in) continue;
+#pragma unroll
+                            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                                for (int u = 0; u < 4; ++u) {
+                                    const int dim = 16 * d + 4 * kb + u;
+                                    float x;
+                                    if constexpr (Q4) {
+                                        const int at = (r & ~7) + 2 * (r & 3) + (r >> 2 & 1);
+                                        x = f16_bits_to_f32(vsl[dim / 32 * CR + at]) *
+                                            (float)((int)(vl[r * RS + dim / 2] >> (4 * (dim & 1)) & 15) - 8);
+                                    } else {
+                                        x = f16_bits_to_f32(*(LP_LDS u16_any*)(vl + r * RS + 2 * dim));
+                                    }
+                                    acc[nt][d][u] = __builtin_fmaf(pk, x, acc[nt][d][u]);
+                                }
+                        }
+            __builtin_amdgcn_wave_barrier();
+            continue;
+        }
+        if constexpr (Q4) {
+#pragma unroll
+            for (int u = 0; u < G; ++u) {
+                half2_t sc[2][4], cc[2][4];
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const u32x4_t x = *(LP_LDS u32x4_any*)(vsl + u * CR + 16 * kb + 8 * w);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t y = x[i];  // (a bit cast of the element itself reads element 0)
+                        sc[w][i] = __builtin_bit_cast(half2_t, y);
+                        cc[w][i] = sc[w][i] * (_Float16)-72.0f;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int d = 2 * u + e;
+                    const v2i32_t x = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+                        (LP_LDS v2i32_t*)(uintptr_t)(vt + (uint32_t)((16 * kb + n) * RS + 8 * d)));
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) {
+                        const u32x4_t v = nibbles8((uint32_t)x[w], sc[w], cc[w]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            acc[nt][d] = mfma16(v, ph[nt][w], acc[nt][d]);
+                            acc[nt][d] = mfma16(v, pl[nt][w], acc[nt][d]);
+                        }
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const uint32_t at = vt + (uint32_t)((8 * kb + (n >> 2)) * RS + 32 * d + 8 * (n & 3));
+                const v4i16_t x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP_LDS v4i16_t*)(uintptr_t)at);
+                const v4i16_t x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP_LDS v4i16_t*)(uintptr_t)(at + 4 * RS));
+                const v2i32_t y0 = __builtin_bit_cast(v2i32_t, x0), y1 = __builtin_bit_cast(v2i32_t, x1);
+                const u32x4_t v = {(uint32_t)y0[0], (uint32_t)y0[1], (uint32_t)y1[0], (uint32_t)y1[1]};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    acc[nt][d] = mfma16(v, ph[nt][0], acc[nt][d]);
+                    acc[nt][d] = mfma16(v, pl[nt][0], acc[nt][d]);
+                }
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+
+    // ---- the waves' sums meet, a query tile at a time
+    constexpr int MS = D + 4;  // floats of a row there
+    float* const sum = reinterpret_cast<float*>(lds);  // [wave][n][MS]
+    float2_any* const ml = reinterpret_cast<float2_any*>(lds + 4 * 16 * MS * 4);
+    const bool direct = sv.len <= a.span;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        float lt = l[nt];
+        lt += shfl_xor(lt, 16);
+        lt += shfl_xor(lt, 32);
+        __syncthreads();
+#pragma unroll
+        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4_any*>(sum + (wave * 16 + n) * MS + 16 * d + 4 * kb) = acc[nt][d];
+        if (kb == 0) ml[wave * 16 + n] = make_float2(m[nt], lt);
+        __syncthreads();
+        constexpr int TR = D / 4;  // threads of a row
+#pragma unroll
+        for (int k = 0; k < 16 * TR; k += 256) {
+            const int q = (k + (int)threadIdx.x) / TR, d4 = (k + (int)threadIdx.x) % TR, row = nt * 16 + q;
+            if (row >= nrows) continue;
+            float M = -INFINITY, L = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) M = fmaxf(M, ml[w * 16 + q].x);
+            f32x4_t A = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float2 x = ml[w * 16 + q];
+                // a wave that saw numbers has a maximum; one that saw nothing, or NaN only, has none
+                const float f = x.x == -INFINITY ? 1.0f : exp2_hw(x.x - M);
+                L = __builtin_fmaf(f, x.y, L);
+                A += *reinterpret_cast<const f32x4_any*>(sum + (w * 16 + q) * MS + 4 * d4) * f;
+            }
+            if (direct) {
+                const int i = row / a.group, h = g * a.group + (row - i * a.group);
+                const uint64_t o = a.out + ((uint64_t)(uint32_t)(sv.t0 + i) * (uint32_t)a.out_stride + (uint32_t)(h * D)) * 4;
+                const float f = L == 0.0f ? 0.0f : 1.0f / L;
+                gptr_w<f32x4_t>(o)[d4] = A * f;
+            } else {
+                const uint64_t at = rec_index(a, bg, split, row);
+                gptr_w<f32x4_t>(a.part + at * (D * 4))[d4] = A;
+                if (d4 == 0) gptr_w<float2>(rec_sums<D>(a))[at] = make_float2(M, L);
+            }
+        }
+    }
+}
+
+}  // namespace
+
+#define LP_ATTN_FEW(NAME, D, Q4, NT) \
+    extern "C" __global__ void __launch_bounds__(256) lp_attn_few_##NAME(const AttnPagedArgs a) { few_body<D, Q4, NT>(a); }
+LP_ATTN_FEW(f16_d64, 64, false, 1)
+LP_ATTN_FEW(f16_d128, 128, false, 1)
+LP_ATTN_FEW(q4_d64, 64, true, 1)
+LP_ATTN_FEW(q4_d128, 128, true, 1)
+LP_ATTN_FEW(f16_d64_n2, 64, false, 2)
+LP_ATTN_FEW(f16_d128_n2, 128, false, 2)
+LP_ATTN_FEW(q4_d64_n2, 64, true, 2)
+LP_ATTN_FEW(q4_d128_n2, 128, true, 2)
+#undef LP_ATTN_FEW
+
+// The records of a query row of a sequence with several splits, joined: a wave
+// per row, its lanes the weights 2^(m_s - M), then D / 64 columns each.
+namespace {
+
+template <int D>
+__device__ __forceinline__ void join_body(const AttnPagedArgs& a) {
+    const int w = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6), lane = lane_id();
+    const int bg = w / a.rows, row = w - bg * a.rows, b = bg / a.c.kv_heads, g = bg - b * a.c.kv_heads;
+    if (b >= a.batch) return;
+    const SeqView sv = seq_view(a, b);
+    if (row >= sv.n * a.group || sv.len <= a.span) return;
+    const int S = (sv.len + a.span - 1) / a.span;
+    const uint64_t r0 = rec_index(a, bg, 0, row);
+    float2 x = make_float2(-INFINITY, 0.0f);
+    if (lane < S) x = gptr<float2>(rec_sums<D>(a))[r0 + (uint64_t)(uint32_t)lane * (uint32_t)a.rows];
+    const float M = wave_max(x.x);
+    const float f = x.x == -INFINITY ? 1.0f : exp2_hw(x.x - M);
+    float L = f * x.y;
+    for (int o = 32; o >= 1; o >>= 1) L += shfl_xor(L, o);
+    constexpr int C = D / 64;
+    float A[C] = {};
+#pragma unroll 8
+    for (int s = 0; s < S; ++s) {
+        const float fs = __shfl(f, s, 64);
+        const uint64_t at = a.part + (r0 + (uint64_t)(uint32_t)s * (uint32_t)a.rows) * (D * 4);
+        if constexpr (C == 2) {
+            const float2 v = gptr<float2>(at)[lane];
+            A[0] = __builtin_fmaf(fs, v.x, A[0]);
+            A[1] = __builtin_fmaf(fs, v.y, A[1]);
+        } else {
+            A[0] = __builtin_fmaf(fs, gptr<float>(at)[lane], A[0]);
+        }
+    }
+    const int i = row / a.group, h = g * a.group + (row - i * a.group);
+    const uint64_t o = a.out + ((uint64_t)(uint32_t)(sv.t0 + i) * (uint32_t)a.out_stride + (uint32_t)(h * D)) * 4;
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    if constexpr (C == 2)
+        gptr_w<float2>(o)[lane] = make_float2(A[0] * inv, A[1] * inv);
+    else
+        gptr_w<float>(o)[lane] = A[0] * inv;
+}
+
+}  // namespace
+
+extern "C" __global__ void __launch_bounds__(256) lp_attn_join_d64(const AttnPagedArgs a) { join_body<64>(a); }
+extern "C" __global__ void __launch_bounds__(256) lp_attn_join_d128(const AttnPagedArgs a) { join_body<128>(a); }

@@ -311,6 +311,8 @@ constexpr double kQ4MinScale = 1.0 / (1 << 17);
 constexpr double kQ4MaxScale = 896.0;
 constexpr int kPageRowsMin = 16, kPageRowsMax = 256;
 constexpr int kPagedMaxBatch = 4096;
+constexpr int kFewRows = 32;           // query rows of a (sequence, KV head) that lp_attn_few_* take
+constexpr int kPagedMaxSplits = 64;    // lp_attn_join_*: one split per lane
 constexpr int kLogprobMaxTop = 64;
 
 // Bytes of one KV head's page.
@@ -344,8 +346,10 @@ struct AttnPagedArgs {
     uint64_t q_starts, seq_lens;
     int32_t q_stride, out_stride;
     int32_t heads, group, batch, tokens, max_q, max_seq;
+    int32_t rows;                   // query rows of a (sequence, KV head): max_q group
+    int32_t splits, span;           // rows of the context per workgroup; records per query row
     float scale;
-    int32_t pad0;
+    uint64_t part;                  // the splits' records
 };
 
 struct LogprobArgs {

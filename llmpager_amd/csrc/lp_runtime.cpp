@@ -136,6 +136,16 @@ enum Fn {
     kAttnPagedF16D128,
     kAttnPagedQ4D64,
     kAttnPagedQ4D128,
+    kAttnFewF16D64,
+    kAttnFewF16D128,
+    kAttnFewQ4D64,
+    kAttnFewQ4D128,
+    kAttnFewF16D64N2,
+    kAttnFewF16D128N2,
+    kAttnFewQ4D64N2,
+    kAttnFewQ4D128N2,
+    kAttnJoinD64,
+    kAttnJoinD128,
     kLogprobs,
     kNumFns
 };
@@ -193,6 +203,11 @@ const FnSpec kSpecs[kNumFns] = {
     {"lp_paged.hsaco", "lp_kv_append_q4_d64"}, {"lp_paged.hsaco", "lp_kv_append_q4_d128"},
     {"lp_paged.hsaco", "lp_attn_paged_f16_d64"}, {"lp_paged.hsaco", "lp_attn_paged_f16_d128"},
     {"lp_paged.hsaco", "lp_attn_paged_q4_d64"}, {"lp_paged.hsaco", "lp_attn_paged_q4_d128"},
+    {"lp_paged.hsaco", "lp_attn_few_f16_d64"}, {"lp_paged.hsaco", "lp_attn_few_f16_d128"},
+    {"lp_paged.hsaco", "lp_attn_few_q4_d64"}, {"lp_paged.hsaco", "lp_attn_few_q4_d128"},
+    {"lp_paged.hsaco", "lp_attn_few_f16_d64_n2"}, {"lp_paged.hsaco", "lp_attn_few_f16_d128_n2"},
+    {"lp_paged.hsaco", "lp_attn_few_q4_d64_n2"}, {"lp_paged.hsaco", "lp_attn_few_q4_d128_n2"},
+    {"lp_paged.hsaco", "lp_attn_join_d64"}, {"lp_paged.hsaco", "lp_attn_join_d128"},
     {"lp_logits.hsaco", "lp_logprobs"},
 };
 
@@ -1126,7 +1141,62 @@ int lp_kv_append_paged(lp_ctx* c, const lp_kv_cache* cache, uint64_t q, int q_st
     return launch(c, f, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, s, a);
 }
 
-uint64_t lp_attn_paged_ws_bytes(const lp_kv_cache*, int, int, int, int, int) { return 0; }
+// How attention is split over the rows of a context: spans of whole chunks for
+// each wave of a workgroup, as long as the (sequence, KV head) pairs times the
+// spans of max_seq rows are about `wgs` workgroups, and at most
+// kPagedMaxSplits spans.
+static void paged_spans(int pairs, int max_seq, int step, int wgs, int* span, int* splits) {
+    const int64_t per = ((int64_t)pairs * max_seq + wgs - 1) / wgs;
+    const int64_t least = (max_seq + kPagedMaxSplits - 1) / kPagedMaxSplits;
+    *span = (int)((std::max<int64_t>({per, least, 1}) + step - 1) / step * step);
+    *splits = std::max(1, (int)(((int64_t)max_seq + *span - 1) / *span));
+}
+
+struct PagedPlan {
+    int max_q, max_seq, rows, span, splits;
+    uint64_t bytes;  // of the records
+};
+
+static PagedPlan paged_plan(const lp_kv_cache* c, int heads, int batch, int tokens, int max_q, int max_seq) {
+    PagedPlan p{};
+    p.max_q = std::min(max_q, tokens);
+    p.max_seq = (int)std::min<int64_t>(max_seq, (int64_t)c->max_pages * c->page_rows);
+    p.rows = p.max_q * (heads / c->kv_heads);
+    p.splits = 1, p.span = INT32_MAX;
+    const int pairs = batch * c->kv_heads;
+    if (p.rows <= kFewRows) paged_spans(pairs, p.max_seq, c->format == LP_KV_Q4 ? 256 : 128, 2048, &p.span, &p.splits);
+    if (p.splits > 1) p.bytes = (uint64_t)pairs * p.splits * p.rows * (c->head_dim + 2) * 4;
+    return p;
+}
+
+// One query row per (token, query head): their number per KV head and its
+// products with the sequences stay within 32 bits.
+static int check_queries(const lp_kv_cache* c, int heads, int batch, int tokens, int max_q, int max_seq) {
+    if (max_q < 0 || max_seq < 0) return fail(LP_E_INVALID, "attn_paged: negative max_q or max_seq");
+    if ((int64_t)batch * std::min(max_q, tokens) * heads > INT32_MAX / 256)
+        return fail(LP_E_UNSUPPORTED, "attn_paged: batch x max_q x heads must be below 2^23");
+    return LP_OK;
+}
+
+uint64_t lp_attn_paged_ws_bytes(const lp_kv_cache* cache, int heads, int batch, int tokens, int max_q, int max_seq) {
+    PagedCache pc;
+    if (check_paged("attn_paged", cache, &pc) || check_batch("attn_paged", heads, cache->kv_heads, batch, tokens, 4, 4) ||
+        check_queries(cache, heads, batch, tokens, max_q, max_seq))
+        return 0;
+    return paged_plan(cache, heads, batch, tokens, max_q, max_seq).bytes;
+}
+
+// A workspace of at least `need` bytes (none of 0).
+static int check_workspace(const char* who, uint64_t need, uint64_t ws, uint64_t ws_bytes) {
+    const std::string w(who);
+    if (!need) return LP_OK;
+    if (!ws) return fail(LP_E_INVALID, w + ": null workspace");
+    if (ws % 256) return fail(LP_E_UNSUPPORTED, w + ": the workspace must be 256-byte aligned");
+    if (ws_bytes < need)
+        return fail(LP_E_INVALID, w + ": the workspace has " + std::to_string(ws_bytes) + " bytes, the call needs " +
+                                      std::to_string(need));
+    return LP_OK;
+}
 
 int lp_attn_paged(lp_ctx* c, const lp_kv_cache* cache, uint64_t q, int q_stride, uint64_t out, int out_stride, int heads,
                   uint64_t q_starts, uint64_t seq_lens, int batch, int tokens, int max_q, int max_seq, float scale,
@@ -1138,18 +1208,25 @@ int lp_attn_paged(lp_ctx* c, const lp_kv_cache* cache, uint64_t q, int q_stride,
     if (int r = check_rows("attn_paged: q", q, q_stride, (int64_t)heads * D)) return r;
     if (int r = check_rows("attn_paged: out", out, out_stride, (int64_t)heads * D)) return r;
     if (q == out) return fail(LP_E_INVALID, "attn_paged: out must not be q");
-    if (max_q < 0 || max_seq < 0) return fail(LP_E_INVALID, "attn_paged: negative max_q or max_seq");
+    if (int r = check_queries(cache, heads, batch, tokens, max_q, max_seq)) return r;
+    const PagedPlan plan = paged_plan(cache, heads, batch, tokens, max_q, max_seq);
+    if (int r = check_workspace("attn_paged", plan.bytes, workspace, ws_bytes)) return r;
     if (int r = check_ctx(c)) return r;
     if (!batch || !tokens || !max_q) return LP_OK;
-    (void)workspace, (void)ws_bytes;
     a.q = q, a.out = out, a.q_starts = q_starts, a.seq_lens = seq_lens;
     a.q_stride = q_stride, a.out_stride = out_stride;
     a.heads = heads, a.group = heads / cache->kv_heads, a.batch = batch, a.tokens = tokens;
-    a.max_q = std::min(max_q, tokens);
-    a.max_seq = (int)std::min<int64_t>(max_seq, (int64_t)cache->max_pages * cache->page_rows);
+    a.max_q = plan.max_q, a.max_seq = plan.max_seq, a.rows = plan.rows;
+    a.splits = plan.splits, a.span = plan.span, a.part = workspace;
     a.scale = scale;
+    if (plan.rows <= kFewRows) {
+        const Fn f = (Fn)(kAttnFewF16D64 + (plan.rows > 16 ? 4 : 0) + (cache->format == LP_KV_Q4 ? 2 : 0) + (D == 128 ? 1 : 0));
+        if (int r = launch(c, f, dim3((unsigned)(batch * cache->kv_heads), (unsigned)plan.splits), dim3(256), 0, s, a)) return r;
+        if (plan.splits == 1) return LP_OK;
+        const int64_t rows = (int64_t)batch * cache->kv_heads * plan.rows;
+        return launch(c, D == 64 ? kAttnJoinD64 : kAttnJoinD128, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+    }
     const int64_t waves = (int64_t)batch * a.max_q * heads;
-    if (waves > INT32_MAX / 256) return fail(LP_E_UNSUPPORTED, "attn_paged: too many queries");
     const Fn f = cache->format == LP_KV_Q4 ? (D == 64 ? kAttnPagedQ4D64 : kAttnPagedQ4D128)
                                            : (D == 64 ? kAttnPagedF16D64 : kAttnPagedF16D128);
     return launch(c, f, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, s, a);
