@@ -195,84 +195,6 @@ extern "C" __global__ void __launch_bounds__(256) lp_kv_append_q4_d64(const KvAp
 extern "C" __global__ void __launch_bounds__(256) lp_kv_append_q4_d128(const KvAppendPagedArgs a) { append_body<128, true>(a); }
 
 // ---------------------------------------------------------------------------
-// Attention, a wave per (query token, head): 64 rows at a time, a row's score
-// per lane, an online softmax over the rows, then the context with the
-// dimensions across the lanes.
-// ---------------------------------------------------------------------------
-namespace {
-
-template <int D, bool Q4>
-__device__ __forceinline__ float row_value(uint64_t page, int log2, int row, int d) {
-    if constexpr (Q4) {
-        const float s = f16_bits_to_f32(gptr<uint16_t>(page)[row * (D / 32) + d / 32]);
-        const uint32_t n = gptr<uint8_t>(page + (uint32_t)(D / 16 << log2))[row * (D / 2) + d / 2];
-        return s * (float)((int)(n >> (4 * (d & 1)) & 15) - 8);
-    } else {
-        return f16_bits_to_f32(gptr<uint16_t>(page)[row * D + d]);
-    }
-}
-
-template <int D, bool Q4>
-__device__ __forceinline__ void attn_body(const AttnPagedArgs& a) {
-    __shared__ float qs[4][D];
-    const int wave = (int)(threadIdx.x >> 6), lane = lane_id();
-    const int w = (int)blockIdx.x * 4 + wave;
-    const int h = w % a.heads, i = w / a.heads % a.max_q, b = w / a.heads / a.max_q;
-    if (b >= a.batch) return;
-    const int t0 = gptr<int>(a.q_starts)[b], n = gptr<int>(a.q_starts)[b + 1] - t0, t = t0 + i;
-    if (i >= n || t < 0 || t >= a.tokens) return;
-    const int len = min(gptr<int>(a.seq_lens)[b], a.max_seq);
-    const int pos = len - n + i, g = h / a.group;
-    const uint64_t q = a.q + ((uint64_t)t * (uint32_t)a.q_stride + (uint32_t)(h * D)) * 4;
-    for (int d = lane; d < D; d += 64) qs[wave][d] = gptr<float>(q)[d];
-    __builtin_amdgcn_wave_barrier();
-    constexpr int DL = D / 64;
-    float m = -INFINITY, l = 0.0f, acc[DL] = {};
-    for (int r0 = 0; r0 <= pos; r0 += 64) {
-        const int row = r0 + lane;
-        const int pg = row <= pos ? page_of(a.c, b, row) : -1;
-        const int pr = row & ((1 << a.c.page_log2) - 1);
-        float s = -INFINITY;
-        if (pg >= 0) {
-            const uint64_t at = page_at<D, Q4>(a.c, a.c.k_pages, pg, g);
-            s = 0.0f;
-            for (int d = 0; d < D; ++d) s = __builtin_fmaf(qs[wave][d], row_value<D, Q4>(at, a.c.page_log2, pr, d), s);
-            s *= a.scale;
-        }
-        const float mn = fmaxf(m, wave_max(s));
-        const float alpha = mn == -INFINITY ? 1.0f : expf(m - mn);
-        const float p = pg < 0 || mn == -INFINITY ? 0.0f : expf(s - mn);
-        float sum = p;
-        for (int o = 32; o >= 1; o >>= 1) sum += shfl_xor(sum, o);
-        l = __builtin_fmaf(l, alpha, sum);
-        m = mn;
-#pragma unroll
-        for (int u = 0; u < DL; ++u) acc[u] *= alpha;
-        uint64_t seen = __ballot(pg >= 0);
-        while (seen) {
-            const int k = __builtin_ctzll(seen);
-            seen &= seen - 1;
-            const float pk = __shfl(p, k, 64);
-            const uint64_t at = page_at<D, Q4>(a.c, a.c.v_pages, __shfl(pg, k, 64), g);
-            const int kr = (r0 + k) & ((1 << a.c.page_log2) - 1);
-#pragma unroll
-            for (int u = 0; u < DL; ++u)
-                acc[u] = __builtin_fmaf(pk, row_value<D, Q4>(at, a.c.page_log2, kr, lane + 64 * u), acc[u]);
-        }
-    }
-    const uint64_t o = a.out + ((uint64_t)t * (uint32_t)a.out_stride + (uint32_t)(h * D)) * 4;
-#pragma unroll
-    for (int u = 0; u < DL; ++u) gptr_w<float>(o)[lane + 64 * u] = l == 0.0f ? 0.0f : acc[u] / l;
-}
-
-}  // namespace
-
-extern "C" __global__ void __launch_bounds__(256) lp_attn_paged_f16_d64(const AttnPagedArgs a) { attn_body<64, false>(a); }
-extern "C" __global__ void __launch_bounds__(256) lp_attn_paged_f16_d128(const AttnPagedArgs a) { attn_body<128, false>(a); }
-extern "C" __global__ void __launch_bounds__(256) lp_attn_paged_q4_d64(const AttnPagedArgs a) { attn_body<64, true>(a); }
-extern "C" __global__ void __launch_bounds__(256) lp_attn_paged_q4_d128(const AttnPagedArgs a) { attn_body<128, true>(a); }
-
-// ---------------------------------------------------------------------------
 // Attention of few query rows: up to 16 NT rows (new tokens x query heads of a
 // KV head) against a sequence's pages.  Bytes bound it, so it is laid out for
 // loads: a workgroup takes `span` rows of one (sequence, KV head) and each of
@@ -364,6 +286,11 @@ __device__ __forceinline__ SeqView seq_view(const AttnPagedArgs& a, int b) {
     return s;
 }
 
+// The rows that a query row of the sequence sees.
+__device__ __forceinline__ int seen_rows(const AttnPagedArgs& a, const SeqView& s, int row) {
+    return max(0, min(s.p0 + row / a.group + 1, s.len));
+}
+
 // A sequence's rows of one KV head per split, and the record of (sequence and
 // KV head bg, split, query row): D sums, then {maximum, sum} behind all of them.
 __device__ __forceinline__ uint64_t rec_index(const AttnPagedArgs& a, int bg, int split, int row) {
@@ -396,9 +323,10 @@ __device__ __forceinline__ void few_body(const AttnPagedArgs& a) {
     const int wave = (int)(threadIdx.x >> 6), lane = lane_id(), n = lane & 15, kb = lane >> 4;
     const int split = blockIdx.y, bg = blockIdx.x, b = bg / a.c.kv_heads, g = bg - b * a.c.kv_heads;
     const SeqView sv = seq_view(a, b);
-    const int r0 = split * a.span, r1 = min(sv.len, r0 + a.span);
     const int nrows = sv.n * a.group;
-    if (nrows <= 0 || (r0 >= r1 && split > 0)) return;  // whole workgroups
+    if (nrows <= 0) return;  // whole workgroups, here and below
+    const int vis = seen_rows(a, sv, nrows - 1), r0 = split * a.span, r1 = min(vis, r0 + a.span);
+    if (r0 >= r1 && split > 0) return;
     uint8_t* const mine = lds + wave * F::kWave;
     const uint32_t vt = (uint32_t)(uintptr_t)(LP_LDS uint8_t*)mine;
     LP_LDS uint8_t* const vl = (LP_LDS uint8_t*)mine;
@@ -477,7 +405,7 @@ __device__ __forceinline__ void few_body(const AttnPagedArgs& a) {
         }
     }
     // rows below `all` are seen by every query row there is
-    const int all = min(sv.p0 + 1, sv.len);
+    const int all = seen_rows(a, sv, 0);
 
     float m[NT], l[NT];
     f32x4_t acc[NT][DT];
@@ -531,7 +459,7 @@ __device__ __forceinline__ void few_body(const AttnPagedArgs& a) {
         {
             if constexpr (Q4) {
                 const int r = blk + 4 * kb + (n & 3);
-                if (!(there && c + r < sv.len)) vsr = 0;
+                if (!(there && c + r < r1)) vsr = 0;
                 if (!whole) odd = odd_halves((uint32_t)vsr) || odd_halves((uint32_t)(vsr >> 32));
                 // the scale of row r in the order of the pairs: 0, 4, 1, 5, ... of eight
                 const int at = (r & ~7) + 2 * (r & 3) + (r >> 2 & 1);
@@ -543,7 +471,7 @@ __device__ __forceinline__ void few_body(const AttnPagedArgs& a) {
                 const int r = blk + 4 * t + (n & 3);
                 if constexpr (!Q4) {
                     if (!whole) {
-                        const bool in = there && c + r < sv.len;
+                        const bool in = there && c + r < r1;
 #pragma unroll
                         for (int i = 0; i < KW; ++i) {
                             vreg[t][i] = in ? vreg[t][i] : 0u;
@@ -699,7 +627,7 @@ __device__ __forceinline__ void few_body(const AttnPagedArgs& a) {
     constexpr int MS = D + 4;  // floats of a row there
     float* const sum = reinterpret_cast<float*>(lds);  // [wave][n][MS]
     float2_any* const ml = reinterpret_cast<float2_any*>(lds + 4 * 16 * MS * 4);
-    const bool direct = sv.len <= a.span;
+    const bool direct = vis <= a.span;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         float lt = l[nt];
@@ -755,6 +683,315 @@ LP_ATTN_FEW(q4_d64_n2, 64, true, 2)
 LP_ATTN_FEW(q4_d128_n2, 128, true, 2)
 #undef LP_ATTN_FEW
 
+// ---------------------------------------------------------------------------
+// Attention of many query rows: a workgroup takes 128 of a (sequence, KV head)'s
+// query rows, 32 a wave, and walks the rows of the context that they see in
+// chunks of 64, as fp16 in LDS for its four waves: the next chunk's rows are
+// written there (4-bit ones multiplied out on the way, columns of eight in the
+// order of nibbles8) and the one's after it are on their way to registers while
+// this chunk is worked on, one barrier a chunk.
+//
+// Matrix work bounds it: fp32 queries and probabilities cost two fp16 MFMAs a
+// product.  As above S^T = K Q^T and O^T = V^T P^T, on v_mfma_f32_32x32x16_f16: the
+// queries' images stay in registers, the probabilities are the B operand where
+// they lie (lane (query n, h), value r: row 8 (r / 4) + 4 h + r % 4 of 32), V^T
+// comes through transposing reads of 4 x 16 blocks, and a row read from LDS
+// serves the hi and the lo product.  Key rows are padded by 16 bytes (16 rows'
+// 16-byte pieces then cover the banks), value rows by 64 (four rows' 32 bytes and
+// their neighbours' do).
+// ---------------------------------------------------------------------------
+namespace {
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ f32x16_t mfma32(const u32x4_t& a, const u32x4_t& b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+}
+
+template <int D>
+struct ManyRows {
+    static constexpr int CR = 64;
+    static constexpr int RSK = D * 2 + 16, RSV = D * 2 + 64;
+    static constexpr int kBuf = CR * (RSK + RSV);
+    static constexpr int kFlags = 2 * kBuf;          // per buffer: 4 waves' ballots of rows there, 4 words of odd values
+    static constexpr int kLds = kFlags + 2 * (4 * 8 + 4 * 4);
+};
+
+template <int D, bool Q4>
+__device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
+    using M = ManyRows<D>;
+    constexpr int CR = M::CR, RSK = M::RSK, RSV = M::RSV, G = D / 32;
+    constexpr int KS = D / 16, DT = D / 32;
+    constexpr int W = Q4 ? D / 32 : D / 8;  // 32-bit words of a row's quarter
+    __shared__ __align__(16) uint8_t lds[M::kLds];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = lane_id(), n = lane & 31, h = lane >> 5;
+    // consecutive ids go round the XCDs: each takes one run of (sequence, KV
+    // head)s, whose rows its L2 then serves to their query tiles
+    const int total = (int)gridDim.x, xcd = (int)blockIdx.x % kXcds, idx = (int)blockIdx.x / kXcds;
+    const int id = idx + xcd * (total / kXcds) + min(xcd, total % kXcds);
+    const int split = id % a.splits, tile = a.tiles - 1 - id / a.splits % a.tiles, bg = id / a.splits / a.tiles;
+    const int b = bg / a.c.kv_heads, g = bg - b * a.c.kv_heads;
+    const SeqView sv = seq_view(a, b);
+    const int nrows = sv.n * a.group, row0 = tile * kManyRows;
+    if (row0 >= nrows) return;  // whole workgroups, here and below
+    const int vis = seen_rows(a, sv, min(row0 + kManyRows, nrows) - 1);
+    const int r0 = split * a.span, r1 = min(vis, r0 + a.span);
+    if (r0 >= r1 && split > 0) return;
+    const uint32_t lbase = (uint32_t)(uintptr_t)(LP_LDS uint8_t*)lds;
+    LP_LDS uint8_t* const ll = (LP_LDS uint8_t*)lds;
+
+    // ---- staging: thread (row tid / 4, quarter tid % 4) of a chunk
+    const int srow = tid >> 2, quarter = tid & 3;
+    const int pmask = (1 << a.c.page_log2) - 1;
+
+    uint32_t kreg[W], vreg[W];
+    uint32_t ks = 0, vs = 0;
+    auto page_for = [&](int c) { return c + srow < r1 ? page_of(a.c, b, c + srow) : -1; };
+    auto load_rows = [&](uint32_t (&r)[W], uint32_t& s, uint64_t pool, int c, int pg) {
+        const uint32_t pr = (uint32_t)((c + srow) & pmask);
+        const uint64_t at = page_at<D, Q4>(a.c, pool, max(pg, 0), g);
+        if constexpr (Q4) {
+            s = gptr<uint16_t>(at)[pr * G + (quarter * G >> 2)];
+            const uint64_t ra = at + ((uint32_t)(G * 2) << a.c.page_log2) + pr * (D / 2) + quarter * (D / 8);
+            if constexpr (D == 64) {
+                const uint64_t v = *gptr<uint64_t>(ra);
+                r[0] = (uint32_t)v, r[1] = (uint32_t)(v >> 32);
+            } else {
+                const u32x4_t v = *gptr<u32x4_t>(ra);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) r[i] = v[i];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < W / 4; ++j) {
+                const u32x4_t v = *gptr<u32x4_t>(at + pr * (D * 2) + 16 * quarter + 64 * j);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) r[4 * j + i] = v[i];
+            }
+        }
+    };
+    auto store_rows = [&](int buf, int c, int pg) {
+        const bool in = c + srow < r1 && pg >= 0;
+        bool odd = false;
+        const uint32_t kd = (uint32_t)(buf * M::kBuf + srow * RSK), vd = (uint32_t)(buf * M::kBuf + CR * RSK + srow * RSV);
+        if constexpr (Q4) {
+            const uint32_t ke = in ? ks | ks << 16 : 0u, ve = in ? vs | vs << 16 : 0u;
+            odd = odd_halves(ve);
+            half2_t sk[4], ck[4], sw[4], cw[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                sk[i] = __builtin_bit_cast(half2_t, ke), ck[i] = sk[i] * (_Float16)-72.0f;
+                sw[i] = __builtin_bit_cast(half2_t, ve), cw[i] = sw[i] * (_Float16)-72.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                *(LP_LDS u32x4_any*)(ll + kd + quarter * (16 * W) + 16 * i) = nibbles8(kreg[i], sk, ck);
+                *(LP_LDS u32x4_any*)(ll + vd + quarter * (16 * W) + 16 * i) = nibbles8(vreg[i], sw, cw);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                vreg[i] = in ? vreg[i] : 0u;
+                odd |= odd_halves(vreg[i]);
+            }
+#pragma unroll
+            for (int j = 0; j < W / 4; ++j) {
+                *(LP_LDS u32x4_any*)(ll + kd + 16 * quarter + 64 * j) = u32x4_t{kreg[4 * j], kreg[4 * j + 1], kreg[4 * j + 2], kreg[4 * j + 3]};
+                *(LP_LDS u32x4_any*)(ll + vd + 16 * quarter + 64 * j) = u32x4_t{vreg[4 * j], vreg[4 * j + 1], vreg[4 * j + 2], vreg[4 * j + 3]};
+            }
+        }
+        const uint64_t there = __ballot(in);
+        const int any = __ballot(odd) != 0;
+        if (lane == 0) {
+            *(LP_LDS u64_any*)(ll + M::kFlags + buf * 48 + wave * 8) = there;
+            *(LP_LDS u32_any*)(ll + M::kFlags + buf * 48 + 32 + wave * 4) = any;
+        }
+    };
+    int pg = -1, pg1 = -1;  // of the chunk in the registers, and of the one after it
+    if (r0 < r1) {
+        pg = page_for(r0);
+        load_rows(kreg, ks, a.c.k_pages, r0, pg);
+        load_rows(vreg, vs, a.c.v_pages, r0, pg);
+        pg1 = page_for(r0 + CR);
+    }
+
+    // ---- the wave's query rows
+    const int row = row0 + 32 * wave + n, qi = row / a.group, qh_ = g * a.group + (row - qi * a.group);
+    const bool on = row < nrows;
+    const int last = on ? sv.p0 + qi : -1;
+    const int wrow = min(row0 + 32 * wave + 31, nrows - 1);
+    const int wvis = row0 + 32 * wave < nrows ? seen_rows(a, sv, wrow) : 0;        // rows that one of the wave's sees
+    const int wall = row0 + 32 * wave < nrows ? seen_rows(a, sv, row0 + 32 * wave) : 0;  // rows that all of them see
+    u32x4_t qh[KS], ql[KS];
+    {
+        const float qs = a.scale * 1.44269504088896341f;
+        const uint64_t q = a.q + ((uint64_t)(uint32_t)(sv.t0 + (on ? qi : 0)) * (uint32_t)a.q_stride + (uint32_t)((on ? qh_ : 0) * D)) * 4;
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+            f32x4_t x0 = gptr<f32x4_t>(q + 64 * j + 32 * h)[0], x1 = gptr<f32x4_t>(q + 64 * j + 32 * h)[1];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) x0[u] = on ? x0[u] * qs : 0.0f, x1[u] = on ? x1[u] * qs : 0.0f;
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if constexpr (Q4)
+                    split2(x0[u], x1[u], hi[u], lo[u]);
+                else
+                    split2(u < 2 ? x0[2 * u] : x1[2 * u - 4], u < 2 ? x0[2 * u + 1] : x1[2 * u - 3], hi[u], lo[u]);
+            }
+            qh[j] = u32x4_t{hi[0], hi[1], hi[2], hi[3]};
+            ql[j] = u32x4_t{lo[0], lo[1], lo[2], lo[3]};
+        }
+    }
+    float m = -INFINITY, l = 0.0f;
+    f32x16_t acc[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[d][r] = 0.0f;
+
+    if (r0 < r1) {
+        store_rows(0, r0, pg);
+        pg = pg1;
+        if (r0 + CR < r1) {
+            load_rows(kreg, ks, a.c.k_pages, r0 + CR, pg);
+            load_rows(vreg, vs, a.c.v_pages, r0 + CR, pg);
+        }
+        pg1 = page_for(r0 + 2 * CR);
+        __syncthreads();
+    }
+    int buf = 0;
+    for (int c = r0; c < r1; c += CR, buf ^= 1) {
+        if (c + CR < r1) {
+            store_rows(buf ^ 1, c + CR, pg);
+            pg = pg1;
+            if (c + 2 * CR < r1) {
+                load_rows(kreg, ks, a.c.k_pages, c + 2 * CR, pg);
+                load_rows(vreg, vs, a.c.v_pages, c + 2 * CR, pg);
+            }
+            pg1 = page_for(c + 3 * CR);
+        }
+        const uint32_t kt = (uint32_t)(buf * M::kBuf), vt = kt + CR * RSK;
+        for (int t = 0; t < CR / 32; ++t) {
+            const int ct = c + 32 * t;
+            if (ct >= wvis) break;
+            uint64_t there[2];  // four bits a row
+#pragma unroll
+            for (int i = 0; i < 2; ++i) there[i] = *(LP_LDS u64_any*)(ll + M::kFlags + buf * 48 + (2 * t + i) * 8);
+            const bool whole = ct + 32 <= wall && __builtin_amdgcn_readfirstlane((int)((there[0] & there[1]) == ~0ull));
+            // ---- scores
+            f32x16_t s;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < KS; ++j) {
+                const u32x4_t k = *(LP_LDS u32x4_any*)(ll + kt + (uint32_t)((32 * t + n) * RSK + 32 * j + 16 * h));
+                s = mfma32(k, qh[j], s);
+                s = mfma32(k, ql[j], s);
+            }
+            if (!whole) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int rr = 8 * (r / 4) + 4 * h + r % 4;
+                    const bool in = there[r / 8] >> (4 * (rr & 15)) & 1;
+                    if (!in || ct + rr > last) s[r] = -INFINITY;
+                }
+            }
+            // ---- softmax
+            float mx = s[0];
+#pragma unroll
+            for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+            if (__ballot(mx > m + 8.0f)) {
+                mx = fmaxf(mx, shfl_xor(mx, 32));
+                const float mn = fmaxf(m, mx);
+                const float f = m == -INFINITY ? 0.0f : exp2_hw(m - mn);
+                l *= f;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) acc[d] *= f;
+                m = mn;
+            }
+            const float base = m == -INFINITY ? 0.0f : m;
+            float p[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                p[r] = exp2_hw(s[r] - base);
+                l += p[r];
+            }
+            // ---- context
+            if (!whole) {
+                int odd = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) odd |= *(LP_LDS u32_any*)(ll + M::kFlags + buf * 48 + 32 + i * 4);
+                if (__builtin_amdgcn_readfirstlane(odd)) {
+                    // row by row, each for the queries that see it
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        for (int k = 0; k < 2; ++k) {
+                            const int rr = 8 * (r / 4) + 4 * k + r % 4;
+                            const float pk = __shfl(p[r], n + 32 * k, 64);
+                            if (ct + rr > last || !(there[r / 8] >> (4 * (rr & 15)) & 1)) continue;
+#pragma unroll
+                            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) {
+                                    const int at = 32 * d + 8 * (e / 4) + 4 * h + e % 4;
+                                    const uint32_t x = *(LP_LDS u16_any*)(ll + vt + (uint32_t)((32 * t + rr) * RSV + 2 * at));
+                                    acc[d][e] = __builtin_fmaf(pk, f16_bits_to_f32(x), acc[d][e]);
+                                }
+                        }
+                    continue;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) split2(p[8 * j + 2 * u], p[8 * j + 2 * u + 1], hi[u], lo[u]);
+                const u32x4_t ph = {hi[0], hi[1], hi[2], hi[3]}, pl = {lo[0], lo[1], lo[2], lo[3]};
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    const uint32_t at = lbase + vt + (uint32_t)((32 * t + 16 * j + 4 * h + (lane >> 2 & 3)) * RSV + 64 * d +
+                                                                32 * (lane >> 4 & 1) + 8 * (lane & 3));
+                    const v4i16_t x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP_LDS v4i16_t*)(uintptr_t)at);
+                    const v4i16_t x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP_LDS v4i16_t*)(uintptr_t)(at + 8 * RSV));
+                    const v2i32_t y0 = __builtin_bit_cast(v2i32_t, x0), y1 = __builtin_bit_cast(v2i32_t, x1);
+                    const u32x4_t v = {(uint32_t)y0[0], (uint32_t)y0[1], (uint32_t)y1[0], (uint32_t)y1[1]};
+                    acc[d] = mfma32(v, ph, acc[d]);
+                    acc[d] = mfma32(v, pl, acc[d]);
+                }
+            }
+        }
+        __syncthreads();
+    }
+    if (!on) return;  // the halves of a query row are on or off together
+    l += shfl_xor(l, 32);
+    const bool direct = vis <= a.span;
+    const uint64_t rec = rec_index(a, bg, split, row);
+    const float f = !direct ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+    const uint64_t o = direct ? a.out + ((uint64_t)(uint32_t)(sv.t0 + qi) * (uint32_t)a.out_stride + (uint32_t)(qh_ * D)) * 4
+                              : a.part + rec * (D * 4);
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float x0 = acc[d][4 * e] * f, x1 = acc[d][4 * e + 1] * f, x2 = acc[d][4 * e + 2] * f, x3 = acc[d][4 * e + 3] * f;
+            if constexpr (Q4) {  // place 4 h + r of eight holds column (4 h + r) / 2 + 4 (r % 2)
+                gptr_w<float2>(o + (32 * d + 8 * e + 2 * h) * 4)[0] = make_float2(x0, x2);
+                gptr_w<float2>(o + (32 * d + 8 * e + 2 * h + 4) * 4)[0] = make_float2(x1, x3);
+            } else {
+                gptr_w<f32x4_t>(o + (32 * d + 8 * e + 4 * h) * 4)[0] = f32x4_t{x0, x1, x2, x3};
+            }
+        }
+    if (!direct && h == 0) gptr_w<float2>(rec_sums<D>(a))[rec] = make_float2(m, l);
+}
+
+}  // namespace
+
+extern "C" __global__ void __launch_bounds__(256, 2) lp_attn_many_f16_d64(const AttnPagedArgs a) { many_body<64, false>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) lp_attn_many_f16_d128(const AttnPagedArgs a) { many_body<128, false>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) lp_attn_many_q4_d64(const AttnPagedArgs a) { many_body<64, true>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) lp_attn_many_q4_d128(const AttnPagedArgs a) { many_body<128, true>(a); }
+
 // The records of a query row of a sequence with several splits, joined: a wave
 // per row, its lanes the weights 2^(m_s - M), then D / 64 columns each.
 namespace {
@@ -765,8 +1002,12 @@ __device__ __forceinline__ void join_body(const AttnPagedArgs& a) {
     const int bg = w / a.rows, row = w - bg * a.rows, b = bg / a.c.kv_heads, g = bg - b * a.c.kv_heads;
     if (b >= a.batch) return;
     const SeqView sv = seq_view(a, b);
-    if (row >= sv.n * a.group || sv.len <= a.span) return;
-    const int S = (sv.len + a.span - 1) / a.span;
+    const int nrows = sv.n * a.group;
+    if (row >= nrows) return;
+    // the rows that its workgroup walked
+    const int vis = seen_rows(a, sv, a.rows <= kFewRows ? nrows - 1 : min(row / kManyRows * kManyRows + kManyRows, nrows) - 1);
+    if (vis <= a.span) return;  // written directly
+    const int S = (vis + a.span - 1) / a.span;
     const uint64_t r0 = rec_index(a, bg, 0, row);
     float2 x = make_float2(-INFINITY, 0.0f);
     if (lane < S) x = gptr<float2>(rec_sums<D>(a))[r0 + (uint64_t)(uint32_t)lane * (uint32_t)a.rows];

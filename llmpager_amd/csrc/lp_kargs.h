@@ -312,6 +312,7 @@ constexpr double kQ4MaxScale = 896.0;
 constexpr int kPageRowsMin = 16, kPageRowsMax = 256;
 constexpr int kPagedMaxBatch = 4096;
 constexpr int kFewRows = 32;           // query rows of a (sequence, KV head) that lp_attn_few_* take
+constexpr int kManyRows = 128;         // query rows of a workgroup of lp_attn_many_*
 constexpr int kPagedMaxSplits = 64;    // lp_attn_join_*: one split per lane
 constexpr int kLogprobMaxTop = 64;
 
@@ -348,6 +349,8 @@ struct AttnPagedArgs {
     int32_t heads, group, batch, tokens, max_q, max_seq;
     int32_t rows;                   // query rows of a (sequence, KV head): max_q group
     int32_t splits, span;           // rows of the context per workgroup; records per query row
+    int32_t tiles;                  // lp_attn_many_*: workgroups of kManyRows query rows
+    int32_t pad0;
     float scale;
     uint64_t part;                  // the splits' records
 };

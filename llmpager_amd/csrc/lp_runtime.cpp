@@ -132,10 +132,10 @@ enum Fn {
     kAppendF16D128,
     kAppendQ4D64,
     kAppendQ4D128,
-    kAttnPagedF16D64,
-    kAttnPagedF16D128,
-    kAttnPagedQ4D64,
-    kAttnPagedQ4D128,
+    kAttnManyF16D64,
+    kAttnManyF16D128,
+    kAttnManyQ4D64,
+    kAttnManyQ4D128,
     kAttnFewF16D64,
     kAttnFewF16D128,
     kAttnFewQ4D64,
@@ -201,8 +201,8 @@ const FnSpec kSpecs[kNumFns] = {
     {"lp_mid.hsaco", "lp_mid_down"},         {"lp_mid.hsaco", "lp_mid_down_rs"},
     {"lp_paged.hsaco", "lp_kv_append_f16_d64"}, {"lp_paged.hsaco", "lp_kv_append_f16_d128"},
     {"lp_paged.hsaco", "lp_kv_append_q4_d64"}, {"lp_paged.hsaco", "lp_kv_append_q4_d128"},
-    {"lp_paged.hsaco", "lp_attn_paged_f16_d64"}, {"lp_paged.hsaco", "lp_attn_paged_f16_d128"},
-    {"lp_paged.hsaco", "lp_attn_paged_q4_d64"}, {"lp_paged.hsaco", "lp_attn_paged_q4_d128"},
+    {"lp_paged.hsaco", "lp_attn_many_f16_d64"}, {"lp_paged.hsaco", "lp_attn_many_f16_d128"},
+    {"lp_paged.hsaco", "lp_attn_many_q4_d64"}, {"lp_paged.hsaco", "lp_attn_many_q4_d128"},
     {"lp_paged.hsaco", "lp_attn_few_f16_d64"}, {"lp_paged.hsaco", "lp_attn_few_f16_d128"},
     {"lp_paged.hsaco", "lp_attn_few_q4_d64"}, {"lp_paged.hsaco", "lp_attn_few_q4_d128"},
     {"lp_paged.hsaco", "lp_attn_few_f16_d64_n2"}, {"lp_paged.hsaco", "lp_attn_few_f16_d128_n2"},
@@ -1153,7 +1153,7 @@ static void paged_spans(int pairs, int max_seq, int step, int wgs, int* span, in
 }
 
 struct PagedPlan {
-    int max_q, max_seq, rows, span, splits;
+    int max_q, max_seq, rows, tiles, span, splits;
     uint64_t bytes;  // of the records
 };
 
@@ -1164,7 +1164,11 @@ static PagedPlan paged_plan(const lp_kv_cache* c, int heads, int batch, int toke
     p.rows = p.max_q * (heads / c->kv_heads);
     p.splits = 1, p.span = INT32_MAX;
     const int pairs = batch * c->kv_heads;
-    if (p.rows <= kFewRows) paged_spans(pairs, p.max_seq, c->format == LP_KV_Q4 ? 256 : 128, 2048, &p.span, &p.splits);
+    p.tiles = (p.rows + kManyRows - 1) / kManyRows;
+    if (p.rows > kFewRows)
+        paged_spans(pairs * p.tiles, p.max_seq, 64, 512, &p.span, &p.splits);
+    else
+        paged_spans(pairs, p.max_seq, c->format == LP_KV_Q4 ? 256 : 128, 2048, &p.span, &p.splits);
     if (p.splits > 1) p.bytes = (uint64_t)pairs * p.splits * p.rows * (c->head_dim + 2) * 4;
     return p;
 }
@@ -1219,17 +1223,18 @@ int lp_attn_paged(lp_ctx* c, const lp_kv_cache* cache, uint64_t q, int q_stride,
     a.max_q = plan.max_q, a.max_seq = plan.max_seq, a.rows = plan.rows;
     a.splits = plan.splits, a.span = plan.span, a.part = workspace;
     a.scale = scale;
+    const int pairs = batch * cache->kv_heads, which = (cache->format == LP_KV_Q4 ? 2 : 0) + (D == 128 ? 1 : 0);
     if (plan.rows <= kFewRows) {
-        const Fn f = (Fn)(kAttnFewF16D64 + (plan.rows > 16 ? 4 : 0) + (cache->format == LP_KV_Q4 ? 2 : 0) + (D == 128 ? 1 : 0));
-        if (int r = launch(c, f, dim3((unsigned)(batch * cache->kv_heads), (unsigned)plan.splits), dim3(256), 0, s, a)) return r;
-        if (plan.splits == 1) return LP_OK;
-        const int64_t rows = (int64_t)batch * cache->kv_heads * plan.rows;
-        return launch(c, D == 64 ? kAttnJoinD64 : kAttnJoinD128, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+        const Fn f = (Fn)(kAttnFewF16D64 + (plan.rows > 16 ? 4 : 0) + which);
+        if (int r = launch(c, f, dim3((unsigned)pairs, (unsigned)plan.splits), dim3(256), 0, s, a)) return r;
+    } else {
+        a.tiles = plan.tiles;
+        const unsigned wgs = (unsigned)((int64_t)pairs * plan.tiles * plan.splits);
+        if (int r = launch(c, (Fn)(kAttnManyF16D64 + which), dim3(wgs), dim3(256), 0, s, a)) return r;
     }
-    const int64_t waves = (int64_t)batch * a.max_q * heads;
-    const Fn f = cache->format == LP_KV_Q4 ? (D == 64 ? kAttnPagedQ4D64 : kAttnPagedQ4D128)
-                                           : (D == 64 ? kAttnPagedF16D64 : kAttnPagedF16D128);
-    return launch(c, f, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, s, a);
+    if (plan.splits == 1) return LP_OK;
+    const int64_t rows = (int64_t)pairs * plan.rows;
+    return launch(c, D == 64 ? kAttnJoinD64 : kAttnJoinD128, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
 }
 
 // ---- logits (lp_logits.hip) ---------------------------------------------------------
