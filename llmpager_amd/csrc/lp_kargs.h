@@ -314,6 +314,9 @@ constexpr int kPagedMaxBatch = 4096;
 constexpr int kFewRows = 32;           // query rows of a (sequence, KV head) that lp_attn_few_* take
 constexpr int kManyRows = 128;         // query rows of a workgroup of lp_attn_many_*
 constexpr int kPagedMaxSplits = 64;    // lp_attn_join_*: one split per lane
+constexpr int kLogprobStep = 4096;     // logits of a workgroup's step
+constexpr int kLogprobMaxParts = 64;   // lp_logprobs_join: one part per lane
+constexpr int kLogprobMaxVocab = 1 << 30;
 constexpr int kLogprobMaxTop = 64;
 
 // Bytes of one KV head's page.
@@ -359,8 +362,11 @@ struct LogprobArgs {
     uint64_t logits, targets;       // f32 rows `stride` floats apart; i32 [rows] or 0
     uint64_t logp, entropy;         // f32 [rows] (entropy may be 0)
     uint64_t ids, top_logp;         // i32, f32 [rows, top]
+    uint64_t part;                  // records [rows, parts] of logprob_rec(top) bytes
     int32_t stride, rows, vocab, top;
+    int32_t parts, per_part;        // workgroups of a row, and the logits of each (a multiple of kLogprobStep)
 };
+LPK_HD constexpr int logprob_rec(int top) { return 32 + (8 * top + 31) / 32 * 32; }
 
 // ---- fused MoE layer ---------------------------------------------------------
 

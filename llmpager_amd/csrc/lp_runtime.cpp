@@ -147,6 +147,8 @@ enum Fn {
     kAttnJoinD64,
     kAttnJoinD128,
     kLogprobs,
+    kLogprobsTop,
+    kLogprobsJoin,
     kNumFns
 };
 
@@ -208,7 +210,8 @@ const FnSpec kSpecs[kNumFns] = {
     {"lp_paged.hsaco", "lp_attn_few_f16_d64_n2"}, {"lp_paged.hsaco", "lp_attn_few_f16_d128_n2"},
     {"lp_paged.hsaco", "lp_attn_few_q4_d64_n2"}, {"lp_paged.hsaco", "lp_attn_few_q4_d128_n2"},
     {"lp_paged.hsaco", "lp_attn_join_d64"}, {"lp_paged.hsaco", "lp_attn_join_d128"},
-    {"lp_logits.hsaco", "lp_logprobs"},
+    {"lp_logits.hsaco", "lp_logprobs"},      {"lp_logits.hsaco", "lp_logprobs_top"},
+    {"lp_logits.hsaco", "lp_logprobs_join"},
 };
 
 const char* const kModules[] = {"lp_basic.hsaco", "lp_moe.hsaco", "lp_gemm.hsaco", "lp_attn.hsaco",
@@ -1239,7 +1242,23 @@ int lp_attn_paged(lp_ctx* c, const lp_kv_cache* cache, uint64_t q, int q_stride,
 
 // ---- logits (lp_logits.hip) ---------------------------------------------------------
 
-uint64_t lp_logprobs_ws_bytes(int, int, int) { return 0; }
+// A row's parts: about 2048 workgroups in all, each of whole steps (a part's
+// first 16-byte piece may begin before the row does, so up to 3 logits more
+// than the row has are shared out).
+static void logprob_parts(int rows, int vocab, int* parts, int* per) {
+    const int steps = (int)(((int64_t)vocab + 3 + kLogprobStep - 1) / kLogprobStep);
+    const int want = std::max(1, std::min({2048 / std::max(rows, 1), steps, kLogprobMaxParts}));
+    const int each = (steps + want - 1) / want;
+    *per = each * kLogprobStep;
+    *parts = (steps + each - 1) / each;
+}
+
+uint64_t lp_logprobs_ws_bytes(int rows, int vocab, int top) {
+    if (rows <= 0 || vocab <= 0 || vocab > kLogprobMaxVocab || top < 0 || top > kLogprobMaxTop) return 0;
+    int parts, per;
+    logprob_parts(rows, vocab, &parts, &per);
+    return parts > 1 ? (uint64_t)rows * parts * logprob_rec(top) : 0;
+}
 
 int lp_logprobs(lp_ctx* c, uint64_t logits, int stride, int rows, int vocab, uint64_t targets, uint64_t logp,
                 uint64_t entropy, int top, uint64_t ids, uint64_t top_logp, uint64_t workspace, uint64_t ws_bytes,
@@ -1250,11 +1269,17 @@ int lp_logprobs(lp_ctx* c, uint64_t logits, int stride, int rows, int vocab, uin
     if (!logits || logits % 4 || targets % 4 || logp % 4 || entropy % 4 || ids % 4 || top_logp % 4 ||
         (targets != 0) != (logp != 0) || (top && (!ids || !top_logp)))
         return fail(LP_E_INVALID, "logprobs: null or misaligned pointer (targets and logp go together)");
+    if (vocab > kLogprobMaxVocab) return fail(LP_E_UNSUPPORTED, "logprobs: at most 2^30 logits a row");
+    if (int r = check_workspace("logprobs", lp_logprobs_ws_bytes(rows, vocab, top), workspace, ws_bytes)) return r;
     if (int r = check_ctx(c)) return r;
     if (!rows) return LP_OK;
-    (void)workspace, (void)ws_bytes;
-    LogprobArgs a{logits, targets, logp, entropy, ids, top_logp, stride, rows, vocab, top};
-    return launch(c, kLogprobs, dim3((unsigned)rows), dim3(256), 0, s, a);
+    LogprobArgs a{logits, targets, logp, entropy, ids, top_logp, workspace, stride, rows, vocab, top, 1, 0};
+    logprob_parts(rows, vocab, &a.parts, &a.per_part);
+    const int64_t wgs = (int64_t)rows * a.parts;
+    if (wgs > INT32_MAX / 256) return fail(LP_E_UNSUPPORTED, "logprobs: too many rows");
+    if (int r = launch(c, top ? kLogprobsTop : kLogprobs, dim3((unsigned)wgs), dim3(256), 0, s, a)) return r;
+    if (a.parts == 1) return LP_OK;
+    return launch(c, kLogprobsJoin, dim3((unsigned)rows), dim3(256), 0, s, a);
 }
 
 // ---- fused MoE layer --------------------------------------------------------------
