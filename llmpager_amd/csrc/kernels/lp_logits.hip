@@ -106,6 +106,20 @@ struct Best {
         tv = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), top - 1));
         tid = __builtin_amdgcn_readlane(id, top - 1);
     }
+    // A value that at least `top` lanes' mx reach: the largest whose 12 last
+    // bits, in the order of their bit patterns, are zero.  What is below it is
+    // not among the best of anything that holds those mx.
+    static __device__ __forceinline__ float reached(float mx, int top) {
+        const uint32_t b = __float_as_uint(mx), key = b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
+        uint32_t at = 0;
+#pragma unroll
+        for (int bit = 31; bit >= 12; --bit) {
+            const uint32_t t = at | 1u << bit;
+            at = __popcll(__ballot(key >= t)) >= top ? t : at;
+        }
+        // (the patterns below -inf's are NaNs)
+        return fmaxf(at & 0x80000000u ? __uint_as_float(at ^ 0x80000000u) : __uint_as_float(~at), -INFINITY);
+    }
     // each lane's (x, i) where `on`
     __device__ __forceinline__ void take(float x, int i, bool on, int top) {
         uint64_t left = ~0ull;
@@ -201,13 +215,16 @@ __device__ __forceinline__ void scan(const LogprobArgs& a, int row, int part, Su
         for (int i = 1; i < kPer; ++i) mx = fmaxf(mx, xs[i]);
         t.add(xs, mx);
         if constexpr (TOP) {
-            if (__ballot(mx >= best.tv)) {
+            const uint64_t b = __ballot(mx >= best.tv);
+            if (b) {
+                // many: first what the block's own best are not below
+                const float least = __popcll(b) > 8 ? Best::reached(mx, a.top) : -INFINITY;
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
                         const int id = e + 4 * (lane + 64 * j) - skew + u;
-                        best.take(xs[4 * j + u], id, id >= 0 && id < n, a.top);
+                        best.take(xs[4 * j + u], id, xs[4 * j + u] >= least && id >= 0 && id < n, a.top);
                     }
             }
         }

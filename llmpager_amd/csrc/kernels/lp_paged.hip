@@ -57,6 +57,60 @@ __device__ __forceinline__ double round7(double d) {
     return __builtin_bit_cast(double, b >> 46 << 46);
 }
 
+// 1 / sqrt(a), a > 0: the fp32 one and two Newton steps, 2^-24 -> 2^-47 -> 64 bits.
+// (a far from 1 is brought into fp32's range by the powers of two of its exponent.)
+__device__ __forceinline__ double rsqrt_f64(double a) {
+    const int e = __builtin_amdgcn_frexp_exp(a) & ~1;
+    const double m = __builtin_amdgcn_ldexp(a, -e);  // 0.5 .. 2
+    double y = (double)__builtin_amdgcn_rsqf((float)m);
+    y = __builtin_fma(0.5 * y, __builtin_fma(-m * y, y, 1.0), y);
+    y = __builtin_fma(0.5 * y, __builtin_fma(-m * y, y, 1.0), y);
+    return __builtin_amdgcn_ldexp(y, -e / 2);
+}
+
+// x / d with inv = 1 / d to a unit or so: the quotient corrected by its
+// remainder, so that one that is a number of 53 bits comes out as it.
+__device__ __forceinline__ double div_by(double x, double d, double inv) {
+    const double q = x * inv;
+    return __builtin_fma(__builtin_fma(-q, d, x), inv, q);
+}
+
+// 1 / s, s of 7 significant bits within the normal fp32 numbers.
+__device__ __forceinline__ double rcp_f64(double s) {
+    double y = (double)__builtin_amdgcn_rcpf((float)s);
+    y = __builtin_fma(__builtin_fma(-s, y, 1.0), y, y);
+    return __builtin_fma(__builtin_fma(-s, y, 1.0), y, y);
+}
+
+// sin and cos of r, |r| <= pi: Taylor's series about the nearest multiple of
+// pi / 2, whose first term left out is below 2^-53 there.
+__device__ __forceinline__ void sincos_f64(double r, double& sn, double& cs) {
+    const double k = rint(r * 0.63661977236758138);
+    const double x = __builtin_fma(-k, 6.1232339957367660e-17, __builtin_fma(-k, 1.5707963267948966, r));
+    const double z = x * x;
+    auto by_z = [&](double y, double c0) { return __builtin_fma(y, z, c0); };
+    double s = by_z(-7.6471637318198164e-13, 1.6059043836821613e-10);  // 1 / 15!, 1 / 13!, ...
+    s = by_z(s, -2.5052108385441720e-8);
+    s = by_z(s, 2.7557319223985893e-6);
+    s = by_z(s, -1.9841269841269841e-4);
+    s = by_z(s, 8.3333333333333333e-3);
+    s = by_z(s, -0.16666666666666667);
+    s = by_z(s, 1.0);
+    double c = by_z(4.7794773323873853e-14, -1.1470745597729725e-11);  // 1 / 16!, 1 / 14!, ...
+    c = by_z(c, 2.0876756987868099e-9);
+    c = by_z(c, -2.7557319223985888e-7);
+    c = by_z(c, 2.4801587301587302e-5);
+    c = by_z(c, -1.3888888888888889e-3);
+    c = by_z(c, 4.1666666666666667e-2);
+    c = by_z(c, -0.5);
+    c = by_z(c, 1.0);
+    s *= x;
+    const int q = (int)k & 3;
+    const double a = q & 1 ? c : s, b = q & 1 ? s : c;
+    sn = q & 2 ? -a : a;
+    cs = (q + 1) & 2 ? -b : b;
+}
+
 // The token's sequence (batch for a token behind the last one): the sequences
 // that end at or before it.
 __device__ __forceinline__ int sequence_of(uint64_t q_starts, int batch, int token) {
@@ -78,8 +132,14 @@ __device__ __forceinline__ int sequence_of(uint64_t q_starts, int batch, int tok
 //
 // Everything up to the last rounding is in 64 bits: the angle pos inv_freq of a
 // far position needs it, and a 4-bit code then is that of the exact value
-// whatever the order of the sums.
+// whatever the order of the sums.  Vector fp64 runs at fp32's rate here, but
+// its divisions, square roots and sines are long: they are short series and
+// Newton steps from fp32 (2,115 tokens of 32 + 2 x 4 heads into 4-bit pages, 100
+// MB in all: 41 us with the library's, 27.4 with these, 3.6 TB/s).
 // ---------------------------------------------------------------------------
+// (by value: a choice between members of a block makes the compiler keep it in memory)
+__device__ __forceinline__ uint64_t pick(bool c, uint64_t a, uint64_t b) { return c ? a : b; }
+
 template <int D, bool Q4>
 __device__ __forceinline__ void append_body(const KvAppendPagedArgs& a) {
     constexpr int LPR = D / 4, RPW = 64 / LPR, G = D / 32;
@@ -99,40 +159,50 @@ __device__ __forceinline__ void append_body(const KvAppendPagedArgs& a) {
         const double ang = (double)pos * (double)(u ? fr.y : fr.x);
         const double k = rint(ang * 0.15915494309189535);
         const double r = __builtin_fma(-k, 2.4492935982947064e-16, __builtin_fma(-k, 6.283185307179586, ang));
-        sincos(r, &sn[u], &cs[u]);
+        sincos_f64(r, sn[u], cs[u]);
         cs[u] *= (double)a.mscale;
         sn[u] *= (double)a.mscale;
     }
     const int H = a.heads, KV = a.c.kv_heads, rows = H + 2 * KV;
     const int r1 = min(rows, (w % a.parts + 1) * a.rows_per_part);
-    for (int r = w % a.parts * a.rows_per_part; r < r1; r += RPW) {
+    const uint64_t qt = a.q + (uint64_t)token * (uint32_t)a.q_stride * 4, kt = a.k + (uint64_t)token * (uint32_t)a.k_stride * 4;
+    const uint64_t vt = a.v + (uint64_t)token * (uint32_t)a.v_stride * 4;
+    const uint64_t qw = a.q_norm, kw = a.k_norm, kout = a.k_out, vout = a.v_out;
+    const uint64_t kpage = page_at<D, Q4>(a.c, a.c.k_pages, max(page, 0), 0), vpage = page_at<D, Q4>(a.c, a.c.v_pages, max(page, 0), 0);
+    // a row's floats and its norm's weights; the next rows' are on their way
+    // while these are worked on
+    float2 f0, f1, w0, w1;
+    auto load = [&](int row) {
+        f0 = f1 = make_float2(0.0f, 0.0f), w0 = w1 = make_float2(1.0f, 1.0f);
+        if (row >= r1) return;
+        const bool isq = row < H, isk = !isq && row < H + KV;
+        const int head = isq ? row : isk ? row - H : row - H - KV;
+        const uint64_t src = pick(isq, qt, pick(isk, kt, vt)) + (uint32_t)(head * D * 4);
+        f0 = gptr<float2>(src)[j];
+        f1 = gptr<float2>(src)[LPR + j];
+        const uint64_t nw = pick(isq, qw, pick(isk, kw, 0));
+        if (nw) {
+            w0 = gptr<float2>(nw)[j];
+            w1 = gptr<float2>(nw)[LPR + j];
+        }
+    };
+    const int rfirst = w % a.parts * a.rows_per_part;
+    load(rfirst + sub);
+    for (int r = rfirst; r < r1; r += RPW) {
         const int row = r + sub;
         const bool on = row < r1, isq = row < H, isk = !isq && row < H + KV;
         const int head = isq ? row : isk ? row - H : row - H - KV;
-        const uint64_t src = (isq ? a.q : isk ? a.k : a.v) +
-                             ((uint64_t)token * (uint32_t)(isq ? a.q_stride : isk ? a.k_stride : a.v_stride) +
-                              (uint32_t)(head * D)) * 4;
-        float2 f0 = make_float2(0.0f, 0.0f), f1 = f0, w0 = make_float2(1.0f, 1.0f), w1 = w0;
-        if (on) {
-            f0 = gptr<float2>(src)[j];
-            f1 = gptr<float2>(src)[LPR + j];
-            const uint64_t nw = isq ? a.q_norm : isk ? a.k_norm : 0;
-            if (nw) {
-                w0 = gptr<float2>(nw)[j];
-                w1 = gptr<float2>(nw)[LPR + j];
-            }
-        }
         double x[4] = {f0.x, f0.y, f1.x, f1.y};
+        const double wt[4] = {w0.x, w0.y, w1.x, w1.y};
+        load(row + RPW);
         double ss = x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3];
         ss = row16_f64(ss, [](double p, double q) { return p + q; });
         if constexpr (LPR == 32) ss += __shfl_xor(ss, 16, 64);
         if (isq || isk) {
-            if (isq ? a.q_norm != 0 : a.k_norm != 0) {
-                const double inv = 1.0 / sqrt(ss / (double)D + (double)a.eps);
-                x[0] *= inv * (double)w0.x;
-                x[1] *= inv * (double)w0.y;
-                x[2] *= inv * (double)w1.x;
-                x[3] *= inv * (double)w1.y;
+            if (pick(isq, qw, kw)) {
+                const double inv = rsqrt_f64(ss / (double)D + (double)a.eps);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) x[u] *= inv * wt[u];
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -146,8 +216,9 @@ __device__ __forceinline__ void append_body(const KvAppendPagedArgs& a) {
             gptr_w<float2>(dst)[j] = make_float2((float)x[0], (float)x[1]);
             gptr_w<float2>(dst)[LPR + j] = make_float2((float)x[2], (float)x[3]);
         }
+        if (!__ballot(on && !isq)) continue;  // queries only
         float2 held[2];
-        const uint64_t pg = page_at<D, Q4>(a.c, isk ? a.c.k_pages : a.c.v_pages, max(page, 0), isq ? 0 : head);
+        const uint64_t pg = pick(isk, kpage, vpage) + (uint32_t)(isq ? 0 : head) * (uint32_t)page_bytes(D, 1 << a.c.page_log2, Q4);
         const bool store = on && !isq && page >= 0;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -155,9 +226,11 @@ __device__ __forceinline__ void append_body(const KvAppendPagedArgs& a) {
             if constexpr (Q4) {
                 // the group's scale; a NaN counts as zero, so that a 4-bit row holds numbers only
                 const double m = row16_f64(fmax(fmax(fabs(x0), fabs(x1)), 0.0), [](double p, double q) { return fmax(p, q); });
-                const double s = fmin(fmax(round7(m / 7.0), kQ4MinScale), kQ4MaxScale);
-                const int c0 = x0 == x0 ? (int)fmin(fmax(rint(x0 / s), -7.0), 7.0) : 0;
-                const int c1 = x1 == x1 ? (int)fmin(fmax(rint(x1 / s), -7.0), 7.0) : 0;
+                const double s = fmax(round7(div_by(fmin(m, 7.0 * kQ4MaxScale), 7.0, 1.0 / 7.0)), kQ4MinScale), is = rcp_f64(s);
+                auto code = [&](double y) {  // (8 scales are cut as 7 are: no infinities from here)
+                    return y == y ? (int)fmin(fmax(rint(div_by(fmin(fmax(y, -8.0 * s), 8.0 * s), s, is)), -7.0), 7.0) : 0;
+                };
+                const int c0 = code(x0), c1 = code(x1);
                 held[u] = make_float2((float)(c0 * s), (float)(c1 * s));
                 // eight columns' nibbles meet in a word
                 uint32_t n = (uint32_t)((c0 + 8) | (c1 + 8) << 4) << (8 * (lane & 3));
@@ -178,7 +251,7 @@ __device__ __forceinline__ void append_body(const KvAppendPagedArgs& a) {
                         (uint32_t)__builtin_bit_cast(uint16_t, h0) | (uint32_t)__builtin_bit_cast(uint16_t, h1) << 16;
             }
         }
-        const uint64_t ko = isk ? a.k_out : a.v_out;
+        const uint64_t ko = pick(isk, kout, vout);
         if (on && !isq && ko) {
             const uint64_t dst = ko + ((uint64_t)token * (uint32_t)KV + (uint32_t)head) * (D * 4);
             gptr_w<float2>(dst)[j] = held[0];

@@ -1135,7 +1135,12 @@ int lp_kv_append_paged(lp_ctx* c, const lp_kv_cache* cache, uint64_t q, int q_st
     a.heads = heads, a.batch = batch, a.tokens = tokens;
     a.eps = eps, a.mscale = mscale;
     const int rows = heads + 2 * cache->kv_heads, per = 256 / D;  // rows a wave takes at a time
-    a.rows_per_part = per;
+    // Waves that share a token's rows: one pass each while the tokens are few,
+    // else about 8192 in all, so that the angles are made less often and a
+    // wave's next rows load behind its present ones (2,115 tokens of 32 + 2 x 4
+    // heads: 8,192 waves 27.4 us, 24,576 32.6).
+    const int want = std::max(1, std::min(8192 / tokens, (rows + per - 1) / per));
+    a.rows_per_part = ((rows + want - 1) / want + per - 1) / per * per;
     a.parts = (rows + a.rows_per_part - 1) / a.rows_per_part;
     const int64_t waves = (int64_t)tokens * a.parts;
     if (waves > INT32_MAX / 256) return fail(LP_E_UNSUPPORTED, "kv_append_paged: too many tokens");
