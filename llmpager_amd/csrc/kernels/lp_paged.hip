@@ -267,33 +267,6 @@ extern "C" __global__ void __launch_bounds__(256) lp_kv_append_f16_d128(const Kv
 extern "C" __global__ void __launch_bounds__(256) lp_kv_append_q4_d64(const KvAppendPagedArgs a) { append_body<64, true>(a); }
 extern "C" __global__ void __launch_bounds__(256) lp_kv_append_q4_d128(const KvAppendPagedArgs a) { append_body<128, true>(a); }
 
-// ---------------------------------------------------------------------------
-// Attention of few query rows: up to 16 NT rows (new tokens x query heads of a
-// KV head) against a sequence's pages.  Bytes bound it, so it is laid out for
-// loads: a workgroup takes `span` rows of one (sequence, KV head) and each of
-// its waves walks chunks of CR rows of its own, without a barrier.
-//
-//   scores   S^T = K Q^T on v_mfma_f32_16x16x32_f16: cache rows as M, straight
-//            from global memory into registers, the query rows as N.  The
-//            queries are fp16 hi + lo images of q scale log2 e (2^-22 of it is
-//            left out), two MFMAs a step; a 4-bit key is its nibble placed in
-//            the mantissa of 64 + n, then one packed fma, n s - 72 s, exact as
-//            scales have 7 significant bits;
-//   softmax  lane (query n, kb) holds rows RB kb .. RB kb + RB - 1 of the chunk
-//            (M index m of tile t is row RB (m / 4) + 4 t + m % 4), so maximum,
-//            e^ and sum stay in the lane; the running maximum is raised only
-//            when a score passes it by 2^8, which spares the rescaling and the
-//            exchange between lanes;
-//   context  O^T = V^T P^T: the probabilities (hi + lo) are the B operand as
-//            they lie in the registers, and V^T comes from the chunk's value
-//            rows in LDS through the transposing reads, 4 x 16 fp16 or 16 x 16
-//            nibbles to a 16-lane group.
-//
-// Rows past the sequence, or of absent pages, are masked and their values
-// zeroed.  Rows that only some of the queries see (several new tokens) may hold
-// NaN or infinity, which zero probabilities would not keep out: where one does,
-// attn_rows_apart adds the chunk row by row.
-// ---------------------------------------------------------------------------
 namespace {
 
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
@@ -374,202 +347,316 @@ __device__ __forceinline__ uint64_t rec_sums(const AttnPagedArgs& a) {
     return a.part + (uint64_t)(uint32_t)(a.batch * a.c.kv_heads) * (uint32_t)a.splits * (uint32_t)a.rows * (D * 4);
 }
 
+// ---------------------------------------------------------------------------
+// Attention of few query rows: up to 16 NT rows (new tokens x query heads of a
+// KV head) against a sequence's pages.
+//
+//   work     a unit is one chunk of CR rows for each of a workgroup's four waves.
+//            A launch has about as many workgroups as fit the chip, and each
+//            takes one part of a (sequence, KV head) pair: `per` units, the
+//            fewest with which all parts find a workgroup, by the lengths that
+//            are in memory then.  The parts of a pair leave records {maximum,
+//            sum, sums} and count themselves; the last to do so joins them
+//            (few_join), and nothing waits.  (Equal shares that begin and end
+//            inside pairs would be more even, but a workgroup's second part
+//            costs its whole chain of round trips again: 32 sequences of up to
+//            8,192 4-bit rows 34.5 us.)
+//   loads    straight into LDS, no registers: the next chunk's keys are sent for
+//            once the scores have read this one's, its values once the context
+//            has; the waits count what was sent for since.  The pages of the
+//            next chunks are looked up together, 64 blocks of 16 rows at a time.
+//   scores   S^T = K Q^T on v_mfma_f32_16x16x32_f16: cache rows as M, the query
+//            rows as N, as fp16 hi + lo images of q scale log2 e (2^-21 of it is
+//            left out), two MFMAs a step, begun at minus the running maximum.
+//   softmax  lane (query n, kb) holds rows 16 t + 4 kb + v of the chunk, so e^ of
+//            them stays in the lane; the running maximum is raised only when a
+//            score passes it by 2^8, which spares the rescaling and the exchange
+//            between lanes.
+//   context  O^T = V^T P^T: the probabilities (hi + lo) are the B operand where
+//            they lie, V^T comes through the transposing LDS reads (4 x 16 fp16
+//            or 16 x 16 nibbles to a 16-lane group), a row of ones gives the sum.
+//
+// fp16 rows lie in LDS as they are, 16-byte pieces changed round within the row
+// (few_turn) so that 16 rows' same piece, and the four rows of a transposing
+// read, each cover the banks.  4-bit rows lie by pieces: piece p of row r in slot
+// r ^ 4 (r / 16) of 64, which does the same; a nibble becomes 64 + n in the
+// mantissa, then one packed fma, n s - 72 s, exact as scales have 7 significant
+// bits.  Their scales are turned into the order of the nibble pairs.
+//
+// Rows past the sequence, or of absent pages, are masked and their values
+// zeroed.  fp16 rows that only some of the queries see (several new tokens) may
+// hold NaN or infinity, which zero probabilities would not keep out: a chunk
+// with one is added row by row.
+// ---------------------------------------------------------------------------
 template <int D, bool Q4>
-struct FewRows {
-    static constexpr int CR = Q4 ? 64 : 32;            // rows per chunk
-    static constexpr int RB = CR / 4, MT = CR / 16;    // rows of a lane, 16-row tiles
-    static constexpr int G = D / 32, DT = D / 16;
-    static constexpr int RS = Q4 ? D / 2 + (D == 128 ? 16 : 8) : D * 2 + 32;  // LDS bytes of a value row
-    static constexpr int kScales = Q4 ? CR * G * 2 : 0;
-    static constexpr int kWave = CR * RS + 2 * kScales;                        // value rows, key scales, value scales
-    static constexpr int kMerge = 4 * 16 * (D + 4) * 4 + 4 * 16 * 8;           // the waves' sums of one query tile
+struct Few {
+    static constexpr int CR = Q4 ? 64 : 32, MT = CR / 16, G = D / 32, DT = D / 16, KS = D / 32;
+    static constexpr int kRow = Q4 ? D / 2 : D * 2;          // bytes
+    static constexpr int kRows = CR * kRow;                  // of a chunk's keys or values
+    static constexpr int PC = kRows / 1024;                  // loads of a wave for them
+    static constexpr int SP = Q4 ? G / 2 : 0;                // and 4-byte pieces of a row's scales
+    static constexpr int kVals = kRows, kKScale = 2 * kRows, kVScale = kKScale + SP * 256, kTurned = kVScale + SP * 256;
+    static constexpr int kWave = kTurned + (Q4 ? 2 * CR * G * 2 : 0);  // values' scales s and -72 s, turned
+    static constexpr int kKeyOps = PC + 2 * SP, kValOps = PC;
+    static constexpr int MS = D + 4;                         // floats of a row in the merge
+    static constexpr int kMerge = 4 * 16 * MS * 4 + 4 * 16 * 8;
     static constexpr int kLds = 4 * kWave > kMerge ? 4 * kWave : kMerge;
+    static_assert(kFewRows * kFewParts * 4 <= kMerge, "the parts' weights fit");
 };
 
-template <int D, bool Q4, int NT>
-__device__ __forceinline__ void few_body(const AttnPagedArgs& a) {
-    using F = FewRows<D, Q4>;
-    constexpr int CR = F::CR, RB = F::RB, MT = F::MT, G = F::G, DT = F::DT, RS = F::RS;
-    constexpr int KS = D / 32;                       // MFMA steps of a score
-    constexpr int KW = Q4 ? D / 32 : D / 8;          // 32-bit words of a key row in a lane, and of a value row
-    __shared__ __align__(16) uint8_t lds[F::kLds];
-    const int wave = (int)(threadIdx.x >> 6), lane = lane_id(), n = lane & 15, kb = lane >> 4;
-    const int split = blockIdx.y, bg = blockIdx.x, b = bg / a.c.kv_heads, g = bg - b * a.c.kv_heads;
-    const SeqView sv = seq_view(a, b);
-    const int nrows = sv.n * a.group;
-    if (nrows <= 0) return;  // whole workgroups, here and below
-    const int vis = seen_rows(a, sv, nrows - 1), r0 = split * a.span, r1 = min(vis, r0 + a.span);
-    if (r0 >= r1 && split > 0) return;
-    uint8_t* const mine = lds + wave * F::kWave;
-    const uint32_t vt = (uint32_t)(uintptr_t)(LP_LDS uint8_t*)mine;
-    LP_LDS uint8_t* const vl = (LP_LDS uint8_t*)mine;
-    LP_LDS u16_any* const ksl = (LP_LDS u16_any*)(mine + CR * RS);
-    LP_LDS u16_any* const vsl = (LP_LDS u16_any*)(mine + CR * RS + F::kScales);
+// Where an fp16 row keeps piece p (16 bytes).
+template <int D>
+__device__ __forceinline__ int few_turn(int row, int p) {
+    if constexpr (D == 128) return p ^ ((row & 7) << 1 | (row >> 3 & 1));
+    return p ^ ((row >> 1 & 3) << 1 | (row >> 3 & 1));
+}
 
-    // ---- chunks: page, keys, values
-    const int blk = (n >> 2) * RB;  // the lane's rows of a tile, within the chunk: blk + 4 t + n % 4
-    const int pmask = (1 << a.c.page_log2) - 1;
-    uint32_t kreg[MT][KW], vreg[MT][KW];
-    uint64_t ksr = 0, vsr = 0;
-    auto page_for = [&](int c) { return c < r1 ? page_of(a.c, b, c + blk) : -1; };
-    auto row_at = [&](int c, int pg) {  // byte offset in a pool of the page's first byte
-        return ((uint64_t)(uint32_t)max(pg, 0) * (uint32_t)a.c.kv_heads + (uint32_t)g) *
-               (uint32_t)(Q4 ? (G * 2 + D / 2) << a.c.page_log2 : (D * 2) << a.c.page_log2);
-    };
-    auto load_rows = [&](uint32_t (&r)[MT][KW], uint64_t& sr, uint64_t pool, int c, int pg) {
-        const uint32_t pr = (uint32_t)((c + blk) & pmask);
-        const uint64_t at = pool + row_at(c, pg);
-        if constexpr (Q4) {
-            // the scales of row blk + 4 kb + n % 4, all groups
-            const uint64_t sa = at + (pr + 4 * kb + (n & 3)) * (G * 2);
-            sr = G == 4 ? *gptr<uint64_t>(sa) : (uint64_t)*gptr<uint32_t>(sa);
+// Bytes a lane from its address to LDS address lds + 16 (4) lane, lds uniform:
+// in flight until the caller waits.
+__device__ __forceinline__ void to_lds16(uint64_t addr, uint32_t lds) {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(addr), "{m0}"(lds) : "memory");
+}
+__device__ __forceinline__ void to_lds4(uint64_t addr, uint32_t lds) {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(addr), "{m0}"(lds) : "memory");
+}
+
+// At most `n` of this wave's loads are outstanding and none of its LDS reads; no
+// access moves across.
+template <int n>
+__device__ __forceinline__ void wait_loads() {
+    __builtin_amdgcn_s_waitcnt((n & 15) | (n >> 4) << 14 | 7 << 4);
+    asm volatile("" ::: "memory");
+}
+
+// A sequence's units (none without new tokens).
+__device__ __forceinline__ int few_units(const AttnPagedArgs& a, int b, int unit) {
+    if (b >= a.batch) return 0;
+    const SeqView s = seq_view(a, b);
+    return s.n > 0 ? max(1, (max(0, min(s.p0 + s.n, s.len)) + unit - 1) / unit) : 0;
+}
+
+// The S parts' records from `first` on joined by the workgroup that counted
+// last.  They were written through to agent scope in this launch; the sums, whole
+// cache lines that nothing here has read before, are read as usual, maximum and
+// sum of a row, which share a line with other pairs', at agent scope.
+template <int D>
+__device__ __forceinline__ void few_join(const AttnPagedArgs& a, uint8_t* lds, const SeqView& sv, int g, int nrows, int first, int S) {
+    float* const wt = reinterpret_cast<float*>(lds);  // [row][kFewParts]
+    const int wave = (int)(threadIdx.x >> 6), lane = lane_id();
+    const uint64_t* const ml = reinterpret_cast<const uint64_t*>(a.part + (uint64_t)(uint32_t)(a.shares * a.rows) * (D * 4));
+    for (int row = wave; row < nrows; row += 4) {
+        float m = -INFINITY, l = 0.0f;
+        if (lane < S) {
+            const uint64_t u = agent_load(ml + ((first + lane) * a.rows + row));
+            m = __uint_as_float((uint32_t)u), l = __uint_as_float((uint32_t)(u >> 32));
         }
-        const uint64_t ra = at + (Q4 ? (uint32_t)(G * 2) << a.c.page_log2 : 0u) + (pr + (n & 3)) * (uint32_t)(Q4 ? D / 2 : D * 2) +
-                            (Q4 ? kb * (D / 8) : kb * 16);
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            if constexpr (Q4 && D == 64) {
-                const auto v = *gptr<uint64_t>(ra + t * 4 * (D / 2));
-                r[t][0] = (uint32_t)v, r[t][1] = (uint32_t)(v >> 32);
-            } else {
-#pragma unroll
-                for (int j = 0; j < KW / 4; ++j) {
-                    const u32x4_t v = *gptr<u32x4_t>(ra + t * 4 * (Q4 ? D / 2 : D * 2) + 64 * j);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) r[t][4 * j + i] = v[i];
-                }
-            }
-        }
-    };
-    int c = r0 + wave * CR, pg = -1, pg1 = -1;
-    if (c < r1) {
-        pg = page_for(c);
-        load_rows(kreg, ksr, a.c.k_pages, c, pg);
-        load_rows(vreg, vsr, a.c.v_pages, c, pg);
-        pg1 = page_for(c + 4 * CR);
+        const float M = wave_max(m);
+        const float f = m == -INFINITY ? 1.0f : exp2_hw(m - M);  // no maximum: nothing seen (sums 0), or NaN only
+        float L = f * l;
+        for (int o = 32; o >= 1; o >>= 1) L += shfl_xor(L, o);
+        if (lane < S) wt[row * kFewParts + lane] = L == 0.0f ? 0.0f : f / L;
     }
+    __syncthreads();
+    constexpr int TR = D / 4;
+    for (int k = (int)threadIdx.x; k < nrows * TR; k += 256) {
+        const int row = k / TR, d4 = k % TR, i = row / a.group, h = g * a.group + (row - i * a.group);
+        f32x4_t A = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+        for (int s = 0; s < S; ++s)
+            A += gptr<f32x4_t>(a.part + (uint64_t)(uint32_t)((first + s) * a.rows + row) * (D * 4))[d4] * wt[row * kFewParts + s];
+        const uint64_t o = a.out + ((uint64_t)(uint32_t)(sv.t0 + i) * (uint32_t)a.out_stride + (uint32_t)(h * D)) * 4;
+        gptr_w<f32x4_t>(o)[d4] = A;
+    }
+}
 
-    // ---- the query rows' images: lane (n, kb), step j
+// One part of a pair: units [u0, u1) of (sequence view sv, KV head g).
+template <int D, bool Q4, int NT>
+__device__ __forceinline__ void few_part(const AttnPagedArgs& a, uint8_t* lds, const SeqView& sv, int b, int g, int u0, int u1,
+                                         bool direct) {
+    using F = Few<D, Q4>;
+    constexpr int CR = F::CR, MT = F::MT, G = F::G, DT = F::DT, PC = F::PC, SP = F::SP, KS = F::KS;
+    const int wave = (int)(threadIdx.x >> 6), lane = lane_id(), n = lane & 15, kb = lane >> 4;
+    const int nrows = sv.n * a.group;
+    const int r1 = (int)min((int64_t)seen_rows(a, sv, nrows - 1), (int64_t)u1 * (4 * CR));
+    LP_LDS uint8_t* const mine = (LP_LDS uint8_t*)(lds + wave * F::kWave);
+    const uint32_t base = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)mine);
+
+    // ---- loads
+    const int pmask = (1 << a.c.page_log2) - 1;
+    const uint32_t pbytes = (uint32_t)page_bytes(D, 1 << a.c.page_log2, Q4);
+    // lane MT k + i: the page of rows 16 i .. of the wave's chunk k from c on
+    auto look_up = [&](int c) {
+        const int row = c + 4 * CR * (lane / MT) + 16 * (lane % MT);
+        return row < r1 ? page_of(a.c, b, row) : -1;
+    };
+    int pages = -1, taken = 0;  // looked up, and chunks of them whose keys were sent for
+    int pg = -1;                // of the last one's: 4-bit rows the lane's block's, fp16 the chunk's block's in lanes 0, 1
+    uint64_t rows_at = 0;       // 4-bit rows: the lane's, of the last one
+    const int myrow = lane ^ 4 * kb;  // 4-bit rows: the lane's
+    auto page_off = [&](int p) {
+        return ((uint64_t)(uint32_t)max(p, 0) * (uint32_t)a.c.kv_heads + (uint32_t)g) * pbytes;
+    };
+    // fp16: the wave's load p brings rows (1024 / kRow) p .. in
+    auto send_f16 = [&](uint64_t pool, int c, uint32_t at) {
+        constexpr int RL = 1024 / F::kRow, RP = F::kRow / 16;
+        const int row = lane / RP;
+#pragma unroll
+        for (int p = 0; p < PC; ++p) {
+            const int r = RL * p + row, blk = RL * p / 16;
+            const uint64_t page = pool + page_off(__builtin_amdgcn_readlane(pg, blk)) +
+                                  (uint32_t)((c + RL * p) & pmask) * (uint32_t)F::kRow;
+            to_lds16(page + (uint32_t)(row * F::kRow + 16 * few_turn<D>(r, lane % RP)), at + 1024 * p);
+        }
+    };
+    auto send_keys = [&](int c) {
+        if (taken == 64 / MT) pages = look_up(c), taken = 0;
+        pg = __shfl(pages, MT * taken + (Q4 ? kb : lane & 1), 64);
+        ++taken;
+        if constexpr (Q4) {
+            const uint64_t at = page_off(pg);
+            const uint32_t pr = (uint32_t)((c + myrow) & pmask);
+            rows_at = at + ((uint32_t)(G * 2) << a.c.page_log2) + pr * (D / 2);
+            const uint64_t sc = at + pr * (G * 2);
+#pragma unroll
+            for (int p = 0; p < SP; ++p) to_lds4(a.c.k_pages + sc + 4 * p, base + F::kKScale + 256 * p);
+#pragma unroll
+            for (int p = 0; p < SP; ++p) to_lds4(a.c.v_pages + sc + 4 * p, base + F::kVScale + 256 * p);
+#pragma unroll
+            for (int p = 0; p < PC; ++p) to_lds16(a.c.k_pages + rows_at + 16 * p, base + 1024 * p);
+        } else {
+            send_f16(a.c.k_pages, c, base);
+        }
+    };
+    auto send_values = [&](int c) {
+        if constexpr (Q4) {
+#pragma unroll
+            for (int p = 0; p < PC; ++p) to_lds16(a.c.v_pages + rows_at + 16 * p, base + F::kVals + 1024 * p);
+        } else {
+            send_f16(a.c.v_pages, c, base + F::kVals);
+        }
+    };
+    int c = (u0 * 4 + wave) * CR;
+    if (c < r1) pages = look_up(c);
+
+    // ---- the query rows' images: lane (n, kb), step j: 8 columns, 4-bit ones in the order of nibbles8
     u32x4_t qh[NT][KS], ql[NT][KS];
     int last[NT];  // the last row that query n of a tile sees
-    const float qs = a.scale * 1.44269504088896341f;
+    {
+        f32x4_t x[NT][KS][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const int row = nt * 16 + n, i = row / a.group, h = g * a.group + (row - i * a.group);
-        const bool on = row < nrows;
-        last[nt] = on ? sv.p0 + i : -1;
-        const uint64_t q = a.q + ((uint64_t)(uint32_t)(sv.t0 + (on ? i : 0)) * (uint32_t)a.q_stride + (uint32_t)((on ? h : 0) * D)) * 4;
+        for (int nt = 0; nt < NT; ++nt) {
+            const int row = min(nt * 16 + n, nrows - 1), i = row / a.group, h = g * a.group + (row - i * a.group);
+            last[nt] = nt * 16 + n < nrows ? sv.p0 + i : -1;
+            const uint64_t q = a.q + ((uint64_t)(uint32_t)(sv.t0 + i) * (uint32_t)a.q_stride + (uint32_t)(h * D)) * 4 +
+                               (Q4 ? D : 32) * kb;
 #pragma unroll
-        for (int j = 0; j < KS; ++j) {
-            const int d = Q4 ? (D / 4) * kb + 8 * j : 32 * j + 8 * kb;
-            f32x4_t x0 = gptr<f32x4_t>(q + 4 * d)[0], x1 = gptr<f32x4_t>(q + 4 * d)[1];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) x0[u] = on ? x0[u] * qs : 0.0f, x1[u] = on ? x1[u] * qs : 0.0f;
-            uint32_t h4[4], l4[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                if constexpr (Q4)
-                    split2(x0[u], x1[u], h4[u], l4[u]);
-                else
-                    split2(u < 2 ? x0[2 * u] : x1[2 * u - 4], u < 2 ? x0[2 * u + 1] : x1[2 * u - 3], h4[u], l4[u]);
+            for (int j = 0; j < KS; ++j) {
+                x[nt][j][0] = gptr<f32x4_t>(q)[Q4 ? 2 * j : 8 * j];
+                x[nt][j][1] = gptr<f32x4_t>(q)[Q4 ? 2 * j + 1 : 8 * j + 1];
             }
-            qh[nt][j] = u32x4_t{h4[0], h4[1], h4[2], h4[3]};
-            ql[nt][j] = u32x4_t{l4[0], l4[1], l4[2], l4[3]};
         }
+        if (c < r1) {
+            send_keys(c);
+            send_values(c);
+        }
+        const float qs = a.scale * 1.44269504088896341f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < KS; ++j) {
+                const f32x4_t y = x[nt][j][0] * qs, z = x[nt][j][1] * qs;
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    if constexpr (Q4)
+                        split2(y[u], z[u], hi[u], lo[u]);
+                    else
+                        split2(u < 2 ? y[2 * u] : z[2 * u - 4], u < 2 ? y[2 * u + 1] : z[2 * u - 3], hi[u], lo[u]);
+                }
+                qh[nt][j] = u32x4_t{hi[0], hi[1], hi[2], hi[3]};
+                ql[nt][j] = u32x4_t{lo[0], lo[1], lo[2], lo[3]};
+            }
     }
-    // rows below `all` are seen by every query row there is
-    const int all = seen_rows(a, sv, 0);
+    const int all = seen_rows(a, sv, 0);  // rows below it are seen by every query row
 
-    float m[NT], l[NT];
-    f32x4_t acc[NT][DT];
+    float m[NT];  // the running maximum, -inf before the first score
+    f32x4_t acc[NT][DT], sum[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        m[nt] = -INFINITY, l[nt] = 0.0f;
+        m[nt] = -INFINITY, sum[nt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int d = 0; d < DT; ++d) acc[nt][d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int d = 0; d < DT; ++d) acc[nt][d] = sum[nt];
     }
     for (; c < r1; c += 4 * CR) {
-        const bool there = pg >= 0;
-        const bool whole = c + CR <= all && __ballot(!there) == 0;  // every row there and seen by all
+        wait_loads<F::kValOps>();  // the keys (and scales) are here
+        // a bit per block of 16 rows: its page is there
+        const uint64_t pages_in = __ballot(pg >= 0);
+        uint32_t there = 0;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) there |= (uint32_t)(pages_in >> (Q4 ? 16 * t : t) & 1) << t;
+        const bool whole = c + CR <= all && there == (1u << MT) - 1;  // all there and seen by all
+        if constexpr (Q4) {
+            // the value scales by group, in the order of the pairs of rows (t even, t
+            // odd) that a lane group multiplies; of rows that are not there 0
+            const bool in = pg >= 0 && c + myrow < r1;
+            const int at = 16 * (myrow >> 2 & 3) + 8 * (kb >> 1) + 2 * (myrow & 3) + (kb & 1);
+#pragma unroll
+            for (int p = 0; p < SP; ++p) {
+                uint32_t v = *(LP_LDS u32_any*)(mine + F::kVScale + 256 * p + 4 * lane);
+                v = in ? v : 0u;
+                const half2_t y = __builtin_bit_cast(half2_t, v) * (_Float16)-72.0f;
+                const uint32_t w = __builtin_bit_cast(uint32_t, y);
+                LP_LDS u16_any* const t = (LP_LDS u16_any*)(mine + F::kTurned) + 4 * p * CR + at;
+                t[0] = (uint16_t)v, t[2 * CR] = (uint16_t)(v >> 16);
+                t[CR] = (uint16_t)w, t[3 * CR] = (uint16_t)(w >> 16);
+            }
+        }
         // ---- scores
         f32x4_t s[NT][MT];
-        if constexpr (Q4) {
-            if (G == 4)
-                *(LP_LDS u64_any*)(ksl + lane * G) = ksr;
-            else
-                *(LP_LDS u32_any*)(ksl + lane * G) = (uint32_t)ksr;
-            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const float from = m[nt] == -INFINITY ? 0.0f : -m[nt];
+#pragma unroll
+            for (int t = 0; t < MT; ++t) s[nt][t] = f32x4_t{from, from, from, from};
         }
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-            half2_t sc[4], cc[4];
+            u32x4_t k[KS];
             if constexpr (Q4) {
-                const _Float16 x = __builtin_bit_cast(_Float16, ksl[(16 * t + n) * G + (kb * G >> 2)]);
+                const int slot = 16 * t + (n ^ 4 * t), gr = kb * G >> 2;  // the lane's columns' group
+                const uint16_t sx = *(LP_LDS u16_any*)(mine + F::kKScale + 256 * (gr >> 1) + 4 * slot + 2 * (gr & 1));
+                const _Float16 x = __builtin_bit_cast(_Float16, sx);
                 const half2_t x2 = {x, x}, y2 = x2 * (_Float16)-72.0f;
+                const half2_t sc[4] = {x2, x2, x2, x2}, cc[4] = {y2, y2, y2, y2};
+                if constexpr (D == 128) {
+                    const u32x4_t w = *(LP_LDS u32x4_any*)(mine + kb * 1024 + slot * 16);
 #pragma unroll
-                for (int u = 0; u < 4; ++u) sc[u] = x2, cc[u] = y2;
+                    for (int j = 0; j < KS; ++j) k[j] = nibbles8(w[j], sc, cc);
+                } else {
+                    const uint64_t w = *(LP_LDS u64_any*)(mine + (kb >> 1) * 1024 + slot * 16 + 8 * (kb & 1));
+                    k[0] = nibbles8((uint32_t)w, sc, cc);
+                    k[1] = nibbles8((uint32_t)(w >> 32), sc, cc);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < KS; ++j)
+                    k[j] = *(LP_LDS u32x4_any*)(mine + (16 * t + n) * F::kRow + 16 * few_turn<D>(n, 4 * j + kb));
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) s[nt][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int j = 0; j < KS; ++j) {
-                u32x4_t k;
-                if constexpr (Q4)
-                    k = nibbles8(kreg[t][j], sc, cc);
-                else
-                    k = u32x4_t{kreg[t][4 * j], kreg[t][4 * j + 1], kreg[t][4 * j + 2], kreg[t][4 * j + 3]};
+            for (int j = 0; j < KS; ++j)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    s[nt][t] = mfma16(k, qh[nt][j], s[nt][t]);
-                    s[nt][t] = mfma16(k, ql[nt][j], s[nt][t]);
+                    s[nt][t] = mfma16(k[j], qh[nt][j], s[nt][t]);
+                    s[nt][t] = mfma16(k[j], ql[nt][j], s[nt][t]);
                 }
-            }
         }
-        const int cn = c + 4 * CR;
-        if (cn < r1) load_rows(kreg, ksr, a.c.k_pages, cn, pg1);
-        // ---- values to LDS, as they are; those of rows that are not there as zeros
-        bool odd = false;
-        {
-            if constexpr (Q4) {
-                const int r = blk + 4 * kb + (n & 3);
-                if (!(there && c + r < r1)) vsr = 0;
-                if (!whole) odd = odd_halves((uint32_t)vsr) || odd_halves((uint32_t)(vsr >> 32));
-                // the scale of row r in the order of the pairs: 0, 4, 1, 5, ... of eight
-                const int at = (r & ~7) + 2 * (r & 3) + (r >> 2 & 1);
-#pragma unroll
-                for (int u = 0; u < G; ++u) vsl[u * CR + at] = (uint16_t)(vsr >> (16 * u));
-            }
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                const int r = blk + 4 * t + (n & 3);
-                if constexpr (!Q4) {
-                    if (!whole) {
-                        const bool in = there && c + r < r1;
-#pragma unroll
-                        for (int i = 0; i < KW; ++i) {
-                            vreg[t][i] = in ? vreg[t][i] : 0u;
-                            odd |= odd_halves(vreg[t][i]);
-                        }
-                    }
-                }
-                if constexpr (Q4 && D == 64) {
-                    *(LP_LDS u64_any*)(vl + r * RS + kb * 8) = (uint64_t)vreg[t][1] << 32 | vreg[t][0];
-                } else {
-#pragma unroll
-                    for (int j = 0; j < KW / 4; ++j)
-                        *(LP_LDS u32x4_any*)(vl + r * RS + kb * 16 + 64 * j) =
-                            u32x4_t{vreg[t][4 * j], vreg[t][4 * j + 1], vreg[t][4 * j + 2], vreg[t][4 * j + 3]};
-                }
-            }
+        const bool more = c + 4 * CR < r1;
+        if (more) {
+            wait_loads<63>();  // the keys and scales are read
+            send_keys(c + 4 * CR);
         }
-        __builtin_amdgcn_wave_barrier();
-        if (cn < r1) load_rows(vreg, vsr, a.c.v_pages, cn, pg1);
-        const int there_n = whole ? 1 : __shfl((int)there, 4 * kb, 64);  // the page of the lane's rows as a query
-        pg = pg1;
-        pg1 = page_for(cn + 4 * CR);
-        // ---- softmax: lane (n, kb), row RB kb + 4 t + v
+        // ---- softmax: lane (n, kb), row 16 t + 4 kb + v
         u32x4_t ph[NT][CR / 32], pl[NT][CR / 32];
-        float p[NT][MT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             if (!whole) {
@@ -577,113 +664,136 @@ __device__ __forceinline__ void few_body(const AttnPagedArgs& a) {
                 for (int t = 0; t < MT; ++t)
 #pragma unroll
                     for (int v = 0; v < 4; ++v)
-                        if (!there_n || c + RB * kb + 4 * t + v > last[nt]) s[nt][t][v] = -INFINITY;
+                        if (!(there >> t & 1) || c + 16 * t + 4 * kb + v > last[nt]) s[nt][t][v] = -INFINITY;
             }
             float mx = s[nt][0][0];
 #pragma unroll
             for (int t = 0; t < MT; ++t)
 #pragma unroll
                 for (int v = 0; v < 4; ++v) mx = fmaxf(mx, s[nt][t][v]);
-            if (__ballot(mx > m[nt] + 8.0f)) {
+            if (__ballot(mx > (m[nt] == -INFINITY ? -INFINITY : 8.0f))) {
                 mx = fmaxf(mx, shfl_xor(mx, 16));
                 mx = fmaxf(mx, shfl_xor(mx, 32));
-                const float mn = fmaxf(m[nt], mx);
-                // nothing seen so far: nothing to rescale
-                const float f = m[nt] == -INFINITY ? 0.0f : exp2_hw(m[nt] - mn);
-                l[nt] *= f;
+                const bool first = m[nt] == -INFINITY;
+                const float by = first ? (mx == -INFINITY ? 0.0f : mx) : fmaxf(mx, 0.0f);
+                const float f = first ? 0.0f : exp2_hw(-by);
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) s[nt][t][v] -= by;
+                sum[nt] *= f;
 #pragma unroll
                 for (int d = 0; d < DT; ++d) acc[nt][d] *= f;
-                m[nt] = mn;
+                m[nt] = first ? mx : m[nt] + by;
             }
-            const float base = m[nt] == -INFINITY ? 0.0f : m[nt];
-#pragma unroll
-            for (int t = 0; t < MT; ++t)
-#pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                    p[nt][t][v] = exp2_hw(s[nt][t][v] - base);
-                    l[nt] += p[nt][t][v];
-                }
 #pragma unroll
             for (int w = 0; w < CR / 32; ++w)
 #pragma unroll
                 for (int v = 0; v < 4; ++v) {
-                    uint32_t h, lo;
+                    uint32_t hi, lo;
                     if constexpr (Q4)
-                        split2(p[nt][2 * w][v], p[nt][2 * w + 1][v], h, lo);
+                        split2(exp2_hw(s[nt][2 * w][v]), exp2_hw(s[nt][2 * w + 1][v]), hi, lo);
                     else
-                        split2(p[nt][v >> 1][2 * (v & 1)], p[nt][v >> 1][2 * (v & 1) + 1], h, lo);
-                    ph[nt][w][v] = h, pl[nt][w][v] = lo;
+                        split2(exp2_hw(s[nt][v >> 1][2 * (v & 1)]), exp2_hw(s[nt][v >> 1][2 * (v & 1) + 1]), hi, lo);
+                    ph[nt][w][v] = hi, pl[nt][w][v] = lo;
                 }
         }
         // ---- context
-        if (!whole && __ballot(odd)) {
+        if (more)
+            wait_loads<F::kKeyOps>();  // the values are here
+        else
+            wait_loads<0>();
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int w = 0; w < CR / 32; ++w) {
+                const u32x4_t one = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+                sum[nt] = mfma16(one, ph[nt][w], sum[nt]);
+                sum[nt] = mfma16(one, pl[nt][w], sum[nt]);
+            }
+        bool apart = false;
+        if constexpr (!Q4) {
+            if (!whole) {
+                // rows that are not there: zeros; an odd value among the others
+                bool odd = false;
+                for (int i = lane; i < F::kRows / 16; i += 64) {
+                    const int r = i / (F::kRow / 16);
+                    LP_LDS u32x4_any* const at = (LP_LDS u32x4_any*)(mine + F::kVals + 16 * i);
+                    u32x4_t x = *at;
+                    const bool in = (there >> (r >> 4) & 1) && c + r < r1;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        x[u] = in ? x[u] : 0u;
+                        odd |= odd_halves(x[u]);
+                    }
+                    *at = x;
+                }
+                apart = __ballot(odd) != 0;
+                __builtin_amdgcn_wave_barrier();
+            }
+        }
+        if (apart) {
             // row by row, each for the queries that see it
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int t = 0; t < MT; ++t)
+                for (int e = 0; e < 8; ++e) {
+                    const int t = e / 4, v = e % 4;  // its probability: half e % 2 of word e / 2
+                    const half2_t hi = __builtin_bit_cast(half2_t, (uint32_t)ph[nt][0][e / 2]), lo = __builtin_bit_cast(half2_t, (uint32_t)pl[nt][0][e / 2]);
+                    const float p = (float)hi[e % 2] + (float)lo[e % 2];
+#pragma unroll 1
+                    for (int k = 0; k < 4; ++k) {
+                        const int r = 16 * t + 4 * k + v;
+                        const float pk = __shfl(p, n + 16 * k, 64);
+                        if (c + r > last[nt] || !(there >> t & 1)) continue;
 #pragma unroll
-                    for (int v = 0; v < 4; ++v)
-                        for (int k = 0; k < 4; ++k) {
-                            const int r = RB * k + 4 * t + v;
-                            const float pk = __shfl(p[nt][t][v], n + 16 * k, 64);
-                            const int in = __shfl(there_n, 16 * k, 64);
-                            if (c + r > last[nt] || !in) continue;
+                        for (int d = 0; d < DT; ++d)
 #pragma unroll
-                            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                                for (int u = 0; u < 4; ++u) {
-                                    const int dim = 16 * d + 4 * kb + u;
-                                    float x;
-                                    if constexpr (Q4) {
-                                        const int at = (r & ~7) + 2 * (r & 3) + (r >> 2 & 1);
-                                        x = f16_bits_to_f32(vsl[dim / 32 * CR + at]) *
-                                            (float)((int)(vl[r * RS + dim / 2] >> (4 * (dim & 1)) & 15) - 8);
-                                    } else {
-                                        x = f16_bits_to_f32(*(LP_LDS u16_any*)(vl + r * RS + 2 * dim));
-                                    }
-                                    acc[nt][d][u] = __builtin_fmaf(pk, x, acc[nt][d][u]);
-                                }
-                        }
-            __builtin_amdgcn_wave_barrier();
-            continue;
-        }
-        if constexpr (Q4) {
+                            for (int u = 0; u < 4; ++u) {
+                                const int dim = 16 * d + 4 * kb + u;
+                                const uint32_t x = *(LP_LDS u16_any*)(mine + F::kVals + r * F::kRow + 16 * few_turn<D>(r, dim / 8) + 2 * (dim % 8));
+                                acc[nt][d][u] = __builtin_fmaf(pk, f16_bits_to_f32(x), acc[nt][d][u]);
+                            }
+                    }
+                }
+        } else if constexpr (Q4) {
+            const uint32_t va = base + F::kVals + (uint32_t)(((n >> 2) * 16 + ((4 * kb + (n & 3)) ^ 4 * (n >> 2))) * 16);
 #pragma unroll
             for (int u = 0; u < G; ++u) {
                 half2_t sc[2][4], cc[2][4];
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
-                    const u32x4_t x = *(LP_LDS u32x4_any*)(vsl + u * CR + 16 * kb + 8 * w);
+                    LP_LDS u16_any* const at = (LP_LDS u16_any*)(mine + F::kTurned) + 2 * u * CR + 16 * kb + 8 * w;
+                    const u32x4_t x = *(LP_LDS u32x4_any*)at, y = *(LP_LDS u32x4_any*)(at + CR);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const uint32_t y = x[i];  // (a bit cast of the element itself reads element 0)
-                        sc[w][i] = __builtin_bit_cast(half2_t, y);
-                        cc[w][i] = sc[w][i] * (_Float16)-72.0f;
+                        const uint32_t xi = x[i], yi = y[i];  // (a bit cast of the element itself reads element 0)
+                        sc[w][i] = __builtin_bit_cast(half2_t, xi), cc[w][i] = __builtin_bit_cast(half2_t, yi);
                     }
                 }
+                v2i32_t x[2];
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int d = 2 * u + e;
-                    const v2i32_t x = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
-                        (LP_LDS v2i32_t*)(uintptr_t)(vt + (uint32_t)((16 * kb + n) * RS + 8 * d)));
+                for (int e = 0; e < 2; ++e)
+                    x[e] = __builtin_amdgcn_ds_read_tr4_b64_v2i32((LP_LDS v2i32_t*)(uintptr_t)(va + u * 1024 + 8 * e));
 #pragma unroll
-                    for (int w = 0; w < 2; ++w) {
-                        const u32x4_t v = nibbles8((uint32_t)x[w], sc[w], cc[w]);
+                for (int w = 0; w < 2; ++w)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const u32x4_t v = nibbles8((uint32_t)x[e][w], sc[w], cc[w]);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            acc[nt][d] = mfma16(v, ph[nt][w], acc[nt][d]);
-                            acc[nt][d] = mfma16(v, pl[nt][w], acc[nt][d]);
+                            acc[nt][2 * u + e] = mfma16(v, ph[nt][w], acc[nt][2 * u + e]);
+                            acc[nt][2 * u + e] = mfma16(v, pl[nt][w], acc[nt][2 * u + e]);
                         }
                     }
-                }
             }
         } else {
+            const int vr = 4 * kb + (n >> 2);  // and 16 rows further
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                const uint32_t at = vt + (uint32_t)((8 * kb + (n >> 2)) * RS + 32 * d + 8 * (n & 3));
+                const uint32_t at = base + F::kVals + (uint32_t)(vr * F::kRow + 16 * few_turn<D>(vr, 2 * d + (n >> 1 & 1)) + 8 * (n & 1));
                 const v4i16_t x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP_LDS v4i16_t*)(uintptr_t)at);
-                const v4i16_t x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP_LDS v4i16_t*)(uintptr_t)(at + 4 * RS));
+                const v4i16_t x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP_LDS v4i16_t*)(uintptr_t)(at + 16 * F::kRow));
                 const v2i32_t y0 = __builtin_bit_cast(v2i32_t, x0), y1 = __builtin_bit_cast(v2i32_t, x1);
                 const u32x4_t v = {(uint32_t)y0[0], (uint32_t)y0[1], (uint32_t)y1[0], (uint32_t)y1[1]};
 #pragma unroll
@@ -693,23 +803,23 @@ __device__ __forceinline__ void few_body(const AttnPagedArgs& a) {
                 }
             }
         }
-        __builtin_amdgcn_wave_barrier();
+        if (more) {
+            wait_loads<63>();  // the values are read
+            send_values(c + 4 * CR);
+        }
     }
 
-    // ---- the waves' sums meet, a query tile at a time
-    constexpr int MS = D + 4;  // floats of a row there
-    float* const sum = reinterpret_cast<float*>(lds);  // [wave][n][MS]
+    // ---- the waves' sums meet, a query tile at a time: the output, or the part's record
+    constexpr int MS = F::MS;
+    float* const sums = reinterpret_cast<float*>(lds);  // [wave][n][MS]
     float2_any* const ml = reinterpret_cast<float2_any*>(lds + 4 * 16 * MS * 4);
-    const bool direct = vis <= a.span;
+    const uint64_t rml = a.part + (uint64_t)(uint32_t)(a.shares * a.rows) * (D * 4);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        float lt = l[nt];
-        lt += shfl_xor(lt, 16);
-        lt += shfl_xor(lt, 32);
         __syncthreads();
 #pragma unroll
-        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4_any*>(sum + (wave * 16 + n) * MS + 16 * d + 4 * kb) = acc[nt][d];
-        if (kb == 0) ml[wave * 16 + n] = make_float2(m[nt], lt);
+        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4_any*>(sums + (wave * 16 + n) * MS + 16 * d + 4 * kb) = acc[nt][d];
+        if (kb == 0) ml[wave * 16 + n] = make_float2(m[nt], sum[nt][0]);
         __syncthreads();
         constexpr int TR = D / 4;  // threads of a row
 #pragma unroll
@@ -723,10 +833,9 @@ __device__ __forceinline__ void few_body(const AttnPagedArgs& a) {
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
                 const float2 x = ml[w * 16 + q];
-                // a wave that saw numbers has a maximum; one that saw nothing, or NaN only, has none
-                const float f = x.x == -INFINITY ? 1.0f : exp2_hw(x.x - M);
+                const float f = x.x == -INFINITY ? 1.0f : exp2_hw(x.x - M);  // as in few_join
                 L = __builtin_fmaf(f, x.y, L);
-                A += *reinterpret_cast<const f32x4_any*>(sum + (w * 16 + q) * MS + 4 * d4) * f;
+                A += *reinterpret_cast<const f32x4_any*>(sums + (w * 16 + q) * MS + 4 * d4) * f;
             }
             if (direct) {
                 const int i = row / a.group, h = g * a.group + (row - i * a.group);
@@ -734,26 +843,94 @@ __device__ __forceinline__ void few_body(const AttnPagedArgs& a) {
                 const float f = L == 0.0f ? 0.0f : 1.0f / L;
                 gptr_w<f32x4_t>(o)[d4] = A * f;
             } else {
-                const uint64_t at = rec_index(a, bg, split, row);
-                gptr_w<f32x4_t>(a.part + at * (D * 4))[d4] = A;
-                if (d4 == 0) gptr_w<float2>(rec_sums<D>(a))[at] = make_float2(M, L);
+                const uint32_t at = blockIdx.x * (uint32_t)a.rows + (uint32_t)row;
+                uint64_t* const o = reinterpret_cast<uint64_t*>(a.part + (uint64_t)at * (D * 4) + 16 * d4);
+                const float a0 = A[0], a1 = A[1], a2 = A[2], a3 = A[3];
+                agent_store(o, (uint64_t)__float_as_uint(a1) << 32 | __float_as_uint(a0));
+                agent_store(o + 1, (uint64_t)__float_as_uint(a3) << 32 | __float_as_uint(a2));
+                if (d4 == 0)
+                    agent_store(reinterpret_cast<uint64_t*>(rml) + at, (uint64_t)__float_as_uint(L) << 32 | __float_as_uint(M));
             }
         }
     }
 }
 
+template <int D, bool Q4, int NT>
+__device__ __forceinline__ void few_body(const AttnPagedArgs& a) {
+    using F = Few<D, Q4>;
+    constexpr int kUnit = 4 * F::CR;
+    __shared__ __align__(1024) uint8_t lds[F::kLds];
+    __shared__ int flag;
+    const int lane = lane_id(), kv = a.c.kv_heads;
+    int b, g, part = 0, parts = 1, per = INT32_MAX / kUnit;
+    if (a.shares) {
+        // units in a lane each (64 sequences), or in LDS
+        int* const many = reinterpret_cast<int*>(lds);
+        const bool lanes = a.batch <= 64;
+        int mine = 0, total = 0;
+        if (lanes) {
+            mine = few_units(a, lane, kUnit);
+            total = wave_incl_scan(mine);
+            total = __builtin_amdgcn_readlane(total, 63);
+        } else {
+            for (int i = threadIdx.x; i < (a.batch + 63 & ~63); i += 256) many[i] = few_units(a, i, kUnit);
+            __syncthreads();
+            for (int i = 0; i < a.batch; i += 64) total += __builtin_amdgcn_readlane(wave_incl_scan(many[i + lane]), 63);
+        }
+        auto parts_of = [&](int u) { return (u + per - 1) / per; };
+        per = max((total * kv + a.shares - 1) / a.shares, a.min_units);
+        for (;; per += (per + 7) / 8) {
+            int n = 0;
+            for (int i = 0; i < a.batch; i += 64) n += __builtin_amdgcn_readlane(wave_incl_scan(parts_of(lanes ? mine : many[i + lane])), 63);
+            if (n * kv <= a.shares) break;  // one part a pair always fits
+        }
+        // the sequence whose parts hold the workgroup's number
+        int before = 0, at = (int)blockIdx.x;
+        for (b = 0;; b += 64) {
+            if (b >= a.batch) return;  // whole workgroups, here and below
+            const int n = parts_of(lanes ? mine : many[b + lane]), incl = before + kv * wave_incl_scan(n);
+            const int i = __popcll(__ballot(incl <= at));
+            if (i < 64) {
+                parts = __builtin_amdgcn_readlane(n, i);
+                at -= __builtin_amdgcn_readlane(incl, i) - kv * parts;
+                b += i;
+                break;
+            }
+            before = __builtin_amdgcn_readlane(incl, 63);
+        }
+        g = at / parts, part = at - g * parts;
+        if (!lanes) __syncthreads();  // the LDS is free
+    } else {  // a workgroup per pair
+        b = (int)blockIdx.x / kv, g = (int)blockIdx.x - b * kv;
+    }
+    const SeqView sv = seq_view(a, b);
+    if (sv.n <= 0) return;
+    few_part<D, Q4, NT>(a, lds, sv, b, g, part * per, part * per + per, parts == 1);
+    if (parts == 1) return;
+    int* const count = reinterpret_cast<int*>(a.sync) + b * kv + g;
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const int o = atomicAdd(count, 1);
+        if (o == parts - 1) agent_store(count, 0);  // the last: zero for the next launch
+        flag = o;
+    }
+    __syncthreads();
+    if (flag == parts - 1) few_join<D>(a, lds, sv, g, sv.n * a.group, (int)blockIdx.x - part, parts);
+}
+
 }  // namespace
 
-#define LP_ATTN_FEW(NAME, D, Q4, NT) \
-    extern "C" __global__ void __launch_bounds__(256) lp_attn_few_##NAME(const AttnPagedArgs a) { few_body<D, Q4, NT>(a); }
-LP_ATTN_FEW(f16_d64, 64, false, 1)
-LP_ATTN_FEW(f16_d128, 128, false, 1)
-LP_ATTN_FEW(q4_d64, 64, true, 1)
-LP_ATTN_FEW(q4_d128, 128, true, 1)
-LP_ATTN_FEW(f16_d64_n2, 64, false, 2)
-LP_ATTN_FEW(f16_d128_n2, 128, false, 2)
-LP_ATTN_FEW(q4_d64_n2, 64, true, 2)
-LP_ATTN_FEW(q4_d128_n2, 128, true, 2)
+#define LP_ATTN_FEW(NAME, WAVES, D, Q4, NT) \
+    extern "C" __global__ void __launch_bounds__(256, WAVES) lp_attn_few_##NAME(const AttnPagedArgs a) { few_body<D, Q4, NT>(a); }
+LP_ATTN_FEW(f16_d64, 2, 64, false, 1)
+LP_ATTN_FEW(f16_d128, 2, 128, false, 1)
+LP_ATTN_FEW(q4_d64, 3, 64, true, 1)
+LP_ATTN_FEW(q4_d128, 3, 128, true, 1)
+LP_ATTN_FEW(f16_d64_n2, 2, 64, false, 2)
+LP_ATTN_FEW(f16_d128_n2, 1, 128, false, 2)
+LP_ATTN_FEW(q4_d64_n2, 2, 64, true, 2)
+LP_ATTN_FEW(q4_d128_n2, 1, 128, true, 2)
 #undef LP_ATTN_FEW
 
 // ---------------------------------------------------------------------------
@@ -999,6 +1176,7 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
                     // row by row, each for the queries that see it
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
+#pragma unroll 1
                         for (int k = 0; k < 2; ++k) {
                             const int rr = 8 * (r / 4) + 4 * k + r % 4;
                             const float pk = __shfl(p[r], n + 32 * k, 64);
@@ -1078,7 +1256,7 @@ __device__ __forceinline__ void join_body(const AttnPagedArgs& a) {
     const int nrows = sv.n * a.group;
     if (row >= nrows) return;
     // the rows that its workgroup walked
-    const int vis = seen_rows(a, sv, a.rows <= kFewRows ? nrows - 1 : min(row / kManyRows * kManyRows + kManyRows, nrows) - 1);
+    const int vis = seen_rows(a, sv, min(row / kManyRows * kManyRows + kManyRows, nrows) - 1);
     if (vis <= a.span) return;  // written directly
     const int S = (vis + a.span - 1) / a.span;
     const uint64_t r0 = rec_index(a, bg, 0, row);

@@ -32,7 +32,9 @@ constexpr int kStepSyncAttn = 17 * kSyncStride;
 constexpr int kStepSyncGemv = kStepSyncAttn + kAttnFusedMaxKvHeads * kSyncStride;
 constexpr int kStepSyncDone = kStepSyncGemv + kSyncStride;  // KV (or query) heads complete
 constexpr int kStepSyncErr = kStepSyncDone + kSyncStride;   // waits that gave up (lp_step_errors_sync)
-constexpr int kSyncWords = kStepSyncErr + kSyncStride;
+constexpr int kPagedSync = kStepSyncErr + kSyncStride;      // paged attention: one per (sequence, KV head)
+constexpr int kPagedPairs = 2048;      // of those whose contexts may be taken in parts
+constexpr int kSyncWords = kPagedSync + kPagedPairs;
 constexpr int kMaxTopK = 16;           // largest top_k the device router accepts
 constexpr int kMaxExperts = 1024;      // largest expert count the device router accepts
 constexpr int kTopkFusedMaxT = 8;      // largest T routed by the one-workgroup top-k + dispatch kernel
@@ -313,6 +315,8 @@ constexpr int kPageRowsMin = 16, kPageRowsMax = 256;
 constexpr int kPagedMaxBatch = 4096;
 constexpr int kFewRows = 32;           // query rows of a (sequence, KV head) that lp_attn_few_* take
 constexpr int kManyRows = 128;         // query rows of a workgroup of lp_attn_many_*
+constexpr int kFewParts = 64;          // most parts of a pair's context there
+constexpr int kFewBatch = 1024;        // and sequences, for their units fit the LDS
 constexpr int kPagedMaxSplits = 64;    // lp_attn_join_*: one split per lane
 constexpr int kLogprobStep = 4096;     // logits of a workgroup's step
 constexpr int kLogprobMaxParts = 64;   // lp_logprobs_join: one part per lane
@@ -351,11 +355,15 @@ struct AttnPagedArgs {
     int32_t q_stride, out_stride;
     int32_t heads, group, batch, tokens, max_q, max_seq;
     int32_t rows;                   // query rows of a (sequence, KV head): max_q group
-    int32_t splits, span;           // rows of the context per workgroup; records per query row
-    int32_t tiles;                  // lp_attn_many_*: workgroups of kManyRows query rows
-    int32_t pad0;
     float scale;
-    uint64_t part;                  // the splits' records
+    uint64_t part;                  // records of the parts of a context
+    // lp_attn_few_*: workgroups for the pairs' parts (0: a workgroup per pair), the
+    // fewest units of a part, arrival counters of the pairs
+    int32_t shares, min_units;
+    uint64_t sync;
+    // lp_attn_many_*: workgroups of kManyRows query rows; rows of the context per
+    // workgroup, and records per query row
+    int32_t tiles, splits, span, pad0;
 };
 
 struct LogprobArgs {

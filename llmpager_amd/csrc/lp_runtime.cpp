@@ -1161,7 +1161,9 @@ static void paged_spans(int pairs, int max_seq, int step, int wgs, int* span, in
 }
 
 struct PagedPlan {
-    int max_q, max_seq, rows, tiles, span, splits;
+    int max_q, max_seq, rows;
+    int shares, min_units;    // few query rows
+    int tiles, span, splits;  // many
     uint64_t bytes;  // of the records
 };
 
@@ -1172,12 +1174,20 @@ static PagedPlan paged_plan(const lp_kv_cache* c, int heads, int batch, int toke
     p.rows = p.max_q * (heads / c->kv_heads);
     p.splits = 1, p.span = INT32_MAX;
     const int pairs = batch * c->kv_heads;
-    p.tiles = (p.rows + kManyRows - 1) / kManyRows;
-    if (p.rows > kFewRows)
+    if (p.rows <= kFewRows) {
+        // a workgroup's unit: a chunk for each of its four waves
+        const int unit = c->format == LP_KV_Q4 ? 256 : 128;
+        const int units = std::max(1, (p.max_seq + unit - 1) / unit);
+        p.min_units = (units + kFewParts - 1) / kFewParts;
+        const int cap = 512;  // two workgroups a CU
+        if (pairs <= kPagedPairs && batch <= kFewBatch && units > 1)
+            p.shares = (int)std::min<int64_t>(std::max(cap, pairs), (int64_t)pairs * units);
+        p.bytes = (uint64_t)p.shares * p.rows * (c->head_dim * 4 + 8);
+    } else {
+        p.tiles = (p.rows + kManyRows - 1) / kManyRows;
         paged_spans(pairs * p.tiles, p.max_seq, 64, 512, &p.span, &p.splits);
-    else
-        paged_spans(pairs, p.max_seq, c->format == LP_KV_Q4 ? 256 : 128, 2048, &p.span, &p.splits);
-    if (p.splits > 1) p.bytes = (uint64_t)pairs * p.splits * p.rows * (c->head_dim + 2) * 4;
+        if (p.splits > 1) p.bytes = (uint64_t)pairs * p.splits * p.rows * (c->head_dim + 2) * 4;
+    }
     return p;
 }
 
@@ -1233,13 +1243,17 @@ int lp_attn_paged(lp_ctx* c, const lp_kv_cache* cache, uint64_t q, int q_stride,
     a.scale = scale;
     const int pairs = batch * cache->kv_heads, which = (cache->format == LP_KV_Q4 ? 2 : 0) + (D == 128 ? 1 : 0);
     if (plan.rows <= kFewRows) {
+        // without counters of this stream, or with more pairs than there are: a
+        // workgroup per pair
+        const int slot = plan.shares ? sync_slot(c, s) : -1;
+        a.shares = slot >= 0 ? plan.shares : 0, a.min_units = plan.min_units;
+        a.sync = slot >= 0 ? sync_words(c, slot) + kPagedSync * 4 : 0;
         const Fn f = (Fn)(kAttnFewF16D64 + (plan.rows > 16 ? 4 : 0) + which);
-        if (int r = launch(c, f, dim3((unsigned)pairs, (unsigned)plan.splits), dim3(256), 0, s, a)) return r;
-    } else {
-        a.tiles = plan.tiles;
-        const unsigned wgs = (unsigned)((int64_t)pairs * plan.tiles * plan.splits);
-        if (int r = launch(c, (Fn)(kAttnManyF16D64 + which), dim3(wgs), dim3(256), 0, s, a)) return r;
+        return launch(c, f, dim3((unsigned)(a.shares ? a.shares : pairs)), dim3(256), 0, s, a);
     }
+    a.tiles = plan.tiles;
+    const unsigned wgs = (unsigned)((int64_t)pairs * plan.tiles * plan.splits);
+    if (int r = launch(c, (Fn)(kAttnManyF16D64 + which), dim3(wgs), dim3(256), 0, s, a)) return r;
     if (plan.splits == 1) return LP_OK;
     const int64_t rows = (int64_t)pairs * plan.rows;
     return launch(c, D == 64 ? kAttnJoinD64 : kAttnJoinD128, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
