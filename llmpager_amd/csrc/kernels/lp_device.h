@@ -484,9 +484,12 @@ __device__ __forceinline__ void write_ximage(const lpk::RouteArgs& a, int t) {
 // land at LDS address lds + 16 l (base and lds uniform over the wave: an SGPR
 // pair and M0).  Given the intrinsic instead, the compiler waits for every
 // outstanding load before the first copy, which here would serialise the
-// image copies behind a tile's weight loads; the callers wait explicitly.
+// image copies behind a tile's weight loads; the callers wait explicitly.  Base
+// may come from a vector register just before (v_readfirstlane): a memory
+// instruction may read such a scalar register five wait states later, which the
+// compiler does not count for an asm statement.
 __device__ __forceinline__ void lds_copy16(uint64_t base, uint32_t off, uint32_t lds) {
-    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
 }
 
 // As lds_copy16 for 4 bytes per lane from per-lane 64-bit addresses.

@@ -376,12 +376,13 @@ __device__ __forceinline__ uint64_t rec_sums(const AttnPagedArgs& a) {
 //            they lie, V^T comes through the transposing LDS reads (4 x 16 fp16
 //            or 16 x 16 nibbles to a 16-lane group), a row of ones gives the sum.
 //
-// fp16 rows lie in LDS as they are, 16-byte pieces changed round within the row
-// (few_turn) so that 16 rows' same piece, and the four rows of a transposing
-// read, each cover the banks.  4-bit rows lie by pieces: piece p of row r in slot
-// r ^ 4 (r / 16) of 64, which does the same; a nibble becomes 64 + n in the
-// mantissa, then one packed fma, n s - 72 s, exact as scales have 7 significant
-// bits.  Their scales are turned into the order of the nibble pairs.
+// Rows lie in LDS as they are, 16-byte pieces changed round within the row
+// (few_turn) so that 16 rows' same piece, and the rows of a transposing read, each
+// cover the banks; a load of the wave is 1 KB of consecutive rows (by pieces, 16
+// bytes of each of 64 rows a load, a first chunk took twice as long).  A nibble
+// becomes 64 + n in the mantissa, then one packed fma, n s - 72 s, exact as scales
+// have 7 significant bits; value scales are turned into the order of the nibble
+// pairs.
 //
 // Rows past the sequence, or of absent pages, are masked and their values
 // zeroed.  fp16 rows that only some of the queries see (several new tokens) may
@@ -404,22 +405,17 @@ struct Few {
     static_assert(kFewRows * kFewParts * 4 <= kMerge, "the parts' weights fit");
 };
 
-// Where an fp16 row keeps piece p (16 bytes).
-template <int D>
+// Where a row keeps piece p (16 bytes).
+template <int D, bool Q4>
 __device__ __forceinline__ int few_turn(int row, int p) {
-    if constexpr (D == 128) return p ^ ((row & 7) << 1 | (row >> 3 & 1));
-    return p ^ ((row >> 1 & 3) << 1 | (row >> 3 & 1));
+    if constexpr (Q4) return D == 128 ? p ^ ((row >> 2 ^ row >> 4) & 3) : p ^ ((row >> 3 ^ row >> 4) & 1);
+    return D == 128 ? p ^ ((row & 7) << 1 | (row >> 3 & 1)) : p ^ ((row >> 1 & 3) << 1 | (row >> 3 & 1));
 }
 
-// Bytes a lane from its address to LDS address lds + 16 (4) lane, lds uniform:
-// in flight until the caller waits.
+// lds_copy16 from an address per lane.
 __device__ __forceinline__ void to_lds16(uint64_t addr, uint32_t lds) {
     asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(addr), "{m0}"(lds) : "memory");
 }
-__device__ __forceinline__ void to_lds4(uint64_t addr, uint32_t lds) {
-    asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(addr), "{m0}"(lds) : "memory");
-}
-
 // At most `n` of this wave's loads are outstanding and none of its LDS reads; no
 // access moves across.
 template <int n>
@@ -429,9 +425,7 @@ __device__ __forceinline__ void wait_loads() {
 }
 
 // A sequence's units (none without new tokens).
-__device__ __forceinline__ int few_units(const AttnPagedArgs& a, int b, int unit) {
-    if (b >= a.batch) return 0;
-    const SeqView s = seq_view(a, b);
+__device__ __forceinline__ int few_units(const SeqView& s, int unit) {
     return s.n > 0 ? max(1, (max(0, min(s.p0 + s.n, s.len)) + unit - 1) / unit) : 0;
 }
 
@@ -490,51 +484,49 @@ __device__ __forceinline__ void few_part(const AttnPagedArgs& a, uint8_t* lds, c
         return row < r1 ? page_of(a.c, b, row) : -1;
     };
     int pages = -1, taken = 0;  // looked up, and chunks of them whose keys were sent for
-    int pg = -1;                // of the last one's: 4-bit rows the lane's block's, fp16 the chunk's block's in lanes 0, 1
-    uint64_t rows_at = 0;       // 4-bit rows: the lane's, of the last one
-    const int myrow = lane ^ 4 * kb;  // 4-bit rows: the lane's
+    int pg = -1;                // lane: the page of block lane / (64 / MT) of the last one of these
     auto page_off = [&](int p) {
         return ((uint64_t)(uint32_t)max(p, 0) * (uint32_t)a.c.kv_heads + (uint32_t)g) * pbytes;
     };
-    // fp16: the wave's load p brings rows (1024 / kRow) p .. in
-    auto send_f16 = [&](uint64_t pool, int c, uint32_t at) {
-        constexpr int RL = 1024 / F::kRow, RP = F::kRow / 16;
-        const int row = lane / RP;
+    auto page_of_block = [&](int t) { return __builtin_amdgcn_readlane(pg, t * (64 / MT)); };
+    // the wave's load p brings rows RL p .., of one or two blocks
+    constexpr int RL = 1024 / F::kRow, RP = F::kRow / 16;
+    auto send_rows = [&](uint64_t pool, int c, uint32_t at) {
+        const uint64_t rows = pool + (Q4 ? (uint32_t)(G * 2) << a.c.page_log2 : 0u);
 #pragma unroll
         for (int p = 0; p < PC; ++p) {
-            const int r = RL * p + row, blk = RL * p / 16;
-            const uint64_t page = pool + page_off(__builtin_amdgcn_readlane(pg, blk)) +
-                                  (uint32_t)((c + RL * p) & pmask) * (uint32_t)F::kRow;
-            to_lds16(page + (uint32_t)(row * F::kRow + 16 * few_turn<D>(r, lane % RP)), at + 1024 * p);
+            const int row = lane / RP, r = RL * p + row, blk = RL * p / 16;
+            const uint64_t b0 = rows + page_off(page_of_block(blk)) + (uint32_t)((c + RL * p) & pmask) * (uint32_t)F::kRow;
+            uint32_t off = (uint32_t)(row * F::kRow + 16 * few_turn<D, Q4>(r, lane % RP));
+            if constexpr (RL == 32) {
+                // the second block's place seen from the first's (a pool may be larger than an offset)
+                const uint64_t b1 = rows + page_off(page_of_block(blk + 1)) + (uint32_t)((c + RL * p + 16) & pmask) * (uint32_t)F::kRow;
+                to_lds16(pick(row >= 16, b1 - 16 * F::kRow, b0) + off, at + 1024 * p);
+            } else {
+                lds_copy16(uniform_u64(b0), off, at + 1024 * p);
+            }
+        }
+    };
+    // 4-bit rows' scales, as they lie: row r's at 2 G r
+    auto send_scales = [&](uint64_t pool, int c, uint32_t at) {
+#pragma unroll
+        for (int p = 0; p < SP; ++p) {
+            const int r = (lane + 64 * p) / SP;  // dwords of 2 G bytes a row
+            const int page = SP == 2 ? (lane & 32 ? page_of_block(2 * p + 1) : page_of_block(2 * p)) : pg;
+            lds_copy4(pool + page_off(page) + (uint32_t)((c + r) & pmask) * (G * 2) + (SP == 2 ? 4 * (lane & 1) : 0), at + 256 * p);
         }
     };
     auto send_keys = [&](int c) {
         if (taken == 64 / MT) pages = look_up(c), taken = 0;
-        pg = __shfl(pages, MT * taken + (Q4 ? kb : lane & 1), 64);
+        pg = __shfl(pages, MT * taken + lane / (64 / MT), 64);
         ++taken;
         if constexpr (Q4) {
-            const uint64_t at = page_off(pg);
-            const uint32_t pr = (uint32_t)((c + myrow) & pmask);
-            rows_at = at + ((uint32_t)(G * 2) << a.c.page_log2) + pr * (D / 2);
-            const uint64_t sc = at + pr * (G * 2);
-#pragma unroll
-            for (int p = 0; p < SP; ++p) to_lds4(a.c.k_pages + sc + 4 * p, base + F::kKScale + 256 * p);
-#pragma unroll
-            for (int p = 0; p < SP; ++p) to_lds4(a.c.v_pages + sc + 4 * p, base + F::kVScale + 256 * p);
-#pragma unroll
-            for (int p = 0; p < PC; ++p) to_lds16(a.c.k_pages + rows_at + 16 * p, base + 1024 * p);
-        } else {
-            send_f16(a.c.k_pages, c, base);
+            send_scales(a.c.k_pages, c, base + F::kKScale);
+            send_scales(a.c.v_pages, c, base + F::kVScale);
         }
+        send_rows(a.c.k_pages, c, base);
     };
-    auto send_values = [&](int c) {
-        if constexpr (Q4) {
-#pragma unroll
-            for (int p = 0; p < PC; ++p) to_lds16(a.c.v_pages + rows_at + 16 * p, base + F::kVals + 1024 * p);
-        } else {
-            send_f16(a.c.v_pages, c, base + F::kVals);
-        }
-    };
+    auto send_values = [&](int c) { send_rows(a.c.v_pages, c, base + F::kVals); };
     int c = (u0 * 4 + wave) * CR;
     if (c < r1) pages = look_up(c);
 
@@ -593,21 +585,27 @@ __device__ __forceinline__ void few_part(const AttnPagedArgs& a, uint8_t* lds, c
         const uint64_t pages_in = __ballot(pg >= 0);
         uint32_t there = 0;
 #pragma unroll
-        for (int t = 0; t < MT; ++t) there |= (uint32_t)(pages_in >> (Q4 ? 16 * t : t) & 1) << t;
+        for (int t = 0; t < MT; ++t) there |= (uint32_t)(pages_in >> (t * (64 / MT)) & 1) << t;
         const bool whole = c + CR <= all && there == (1u << MT) - 1;  // all there and seen by all
         if constexpr (Q4) {
             // the value scales by group, in the order of the pairs of rows (t even, t
             // odd) that a lane group multiplies; of rows that are not there 0
-            const bool in = pg >= 0 && c + myrow < r1;
-            const int at = 16 * (myrow >> 2 & 3) + 8 * (kb >> 1) + 2 * (myrow & 3) + (kb & 1);
+            const bool in = pg >= 0 && c + lane < r1;
+            const int at = 16 * (lane >> 2 & 3) + 8 * (kb >> 1) + 2 * (lane & 3) + (kb & 1);
+            uint32_t v[SP];
+            if constexpr (SP == 2) {
+                const uint64_t x = *(LP_LDS u64_any*)(mine + F::kVScale + 8 * lane);
+                v[0] = (uint32_t)x, v[1] = (uint32_t)(x >> 32);
+            } else {
+                v[0] = *(LP_LDS u32_any*)(mine + F::kVScale + 4 * lane);
+            }
 #pragma unroll
             for (int p = 0; p < SP; ++p) {
-                uint32_t v = *(LP_LDS u32_any*)(mine + F::kVScale + 256 * p + 4 * lane);
-                v = in ? v : 0u;
-                const half2_t y = __builtin_bit_cast(half2_t, v) * (_Float16)-72.0f;
+                v[p] = in ? v[p] : 0u;
+                const half2_t y = __builtin_bit_cast(half2_t, v[p]) * (_Float16)-72.0f;
                 const uint32_t w = __builtin_bit_cast(uint32_t, y);
                 LP_LDS u16_any* const t = (LP_LDS u16_any*)(mine + F::kTurned) + 4 * p * CR + at;
-                t[0] = (uint16_t)v, t[2 * CR] = (uint16_t)(v >> 16);
+                t[0] = (uint16_t)v[p], t[2 * CR] = (uint16_t)(v[p] >> 16);
                 t[CR] = (uint16_t)w, t[3 * CR] = (uint16_t)(w >> 16);
             }
         }
@@ -623,24 +621,24 @@ __device__ __forceinline__ void few_part(const AttnPagedArgs& a, uint8_t* lds, c
         for (int t = 0; t < MT; ++t) {
             u32x4_t k[KS];
             if constexpr (Q4) {
-                const int slot = 16 * t + (n ^ 4 * t), gr = kb * G >> 2;  // the lane's columns' group
-                const uint16_t sx = *(LP_LDS u16_any*)(mine + F::kKScale + 256 * (gr >> 1) + 4 * slot + 2 * (gr & 1));
+                const int r = 16 * t + n;
+                const uint16_t sx = *(LP_LDS u16_any*)(mine + F::kKScale + r * (G * 2) + 2 * (kb * G >> 2));  // the lane's columns' group
                 const _Float16 x = __builtin_bit_cast(_Float16, sx);
                 const half2_t x2 = {x, x}, y2 = x2 * (_Float16)-72.0f;
                 const half2_t sc[4] = {x2, x2, x2, x2}, cc[4] = {y2, y2, y2, y2};
                 if constexpr (D == 128) {
-                    const u32x4_t w = *(LP_LDS u32x4_any*)(mine + kb * 1024 + slot * 16);
+                    const u32x4_t w = *(LP_LDS u32x4_any*)(mine + r * F::kRow + 16 * few_turn<D, Q4>(r, kb));
 #pragma unroll
                     for (int j = 0; j < KS; ++j) k[j] = nibbles8(w[j], sc, cc);
                 } else {
-                    const uint64_t w = *(LP_LDS u64_any*)(mine + (kb >> 1) * 1024 + slot * 16 + 8 * (kb & 1));
+                    const uint64_t w = *(LP_LDS u64_any*)(mine + r * F::kRow + 16 * few_turn<D, Q4>(r, kb >> 1) + 8 * (kb & 1));
                     k[0] = nibbles8((uint32_t)w, sc, cc);
                     k[1] = nibbles8((uint32_t)(w >> 32), sc, cc);
                 }
             } else {
 #pragma unroll
                 for (int j = 0; j < KS; ++j)
-                    k[j] = *(LP_LDS u32x4_any*)(mine + (16 * t + n) * F::kRow + 16 * few_turn<D>(n, 4 * j + kb));
+                    k[j] = *(LP_LDS u32x4_any*)(mine + (16 * t + n) * F::kRow + 16 * few_turn<D, Q4>(n, 4 * j + kb));
             }
 #pragma unroll
             for (int j = 0; j < KS; ++j)
@@ -751,13 +749,13 @@ __device__ __forceinline__ void few_part(const AttnPagedArgs& a, uint8_t* lds, c
 #pragma unroll
                             for (int u = 0; u < 4; ++u) {
                                 const int dim = 16 * d + 4 * kb + u;
-                                const uint32_t x = *(LP_LDS u16_any*)(mine + F::kVals + r * F::kRow + 16 * few_turn<D>(r, dim / 8) + 2 * (dim % 8));
+                                const uint32_t x = *(LP_LDS u16_any*)(mine + F::kVals + r * F::kRow + 16 * few_turn<D, Q4>(r, dim / 8) + 2 * (dim % 8));
                                 acc[nt][d][u] = __builtin_fmaf(pk, f16_bits_to_f32(x), acc[nt][d][u]);
                             }
                     }
                 }
         } else if constexpr (Q4) {
-            const uint32_t va = base + F::kVals + (uint32_t)(((n >> 2) * 16 + ((4 * kb + (n & 3)) ^ 4 * (n >> 2))) * 16);
+            const int vr = 16 * (n >> 2) + 4 * kb + (n & 3);
 #pragma unroll
             for (int u = 0; u < G; ++u) {
                 half2_t sc[2][4], cc[2][4];
@@ -774,7 +772,7 @@ __device__ __forceinline__ void few_part(const AttnPagedArgs& a, uint8_t* lds, c
                 v2i32_t x[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
-                    x[e] = __builtin_amdgcn_ds_read_tr4_b64_v2i32((LP_LDS v2i32_t*)(uintptr_t)(va + u * 1024 + 8 * e));
+                    x[e] = __builtin_amdgcn_ds_read_tr4_b64_v2i32((LP_LDS v2i32_t*)(uintptr_t)(base + F::kVals + (uint32_t)(vr * F::kRow + 16 * few_turn<D, Q4>(vr, u) + 8 * e)));
 #pragma unroll
                 for (int w = 0; w < 2; ++w)
 #pragma unroll
@@ -791,7 +789,7 @@ __device__ __forceinline__ void few_part(const AttnPagedArgs& a, uint8_t* lds, c
             const int vr = 4 * kb + (n >> 2);  // and 16 rows further
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                const uint32_t at = base + F::kVals + (uint32_t)(vr * F::kRow + 16 * few_turn<D>(vr, 2 * d + (n >> 1 & 1)) + 8 * (n & 1));
+                const uint32_t at = base + F::kVals + (uint32_t)(vr * F::kRow + 16 * few_turn<D, Q4>(vr, 2 * d + (n >> 1 & 1)) + 8 * (n & 1));
                 const v4i16_t x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP_LDS v4i16_t*)(uintptr_t)at);
                 const v4i16_t x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP_LDS v4i16_t*)(uintptr_t)(at + 16 * F::kRow));
                 const v2i32_t y0 = __builtin_bit_cast(v2i32_t, x0), y1 = __builtin_bit_cast(v2i32_t, x1);
@@ -863,17 +861,19 @@ __device__ __forceinline__ void few_body(const AttnPagedArgs& a) {
     __shared__ int flag;
     const int lane = lane_id(), kv = a.c.kv_heads;
     int b, g, part = 0, parts = 1, per = INT32_MAX / kUnit;
+    SeqView sv{0, 0, 0, 0};
     if (a.shares) {
         // units in a lane each (64 sequences), or in LDS
         int* const many = reinterpret_cast<int*>(lds);
         const bool lanes = a.batch <= 64;
         int mine = 0, total = 0;
         if (lanes) {
-            mine = few_units(a, lane, kUnit);
-            total = wave_incl_scan(mine);
-            total = __builtin_amdgcn_readlane(total, 63);
+            if (lane < a.batch) sv = seq_view(a, lane);
+            mine = few_units(sv, kUnit);
+            total = __builtin_amdgcn_readlane(wave_incl_scan(mine), 63);
         } else {
-            for (int i = threadIdx.x; i < (a.batch + 63 & ~63); i += 256) many[i] = few_units(a, i, kUnit);
+            for (int i = threadIdx.x; i < (a.batch + 63 & ~63); i += 256)
+                many[i] = i < a.batch ? few_units(seq_view(a, i), kUnit) : 0;
             __syncthreads();
             for (int i = 0; i < a.batch; i += 64) total += __builtin_amdgcn_readlane(wave_incl_scan(many[i + lane]), 63);
         }
@@ -899,12 +899,18 @@ __device__ __forceinline__ void few_body(const AttnPagedArgs& a) {
             before = __builtin_amdgcn_readlane(incl, 63);
         }
         g = at / parts, part = at - g * parts;
-        if (!lanes) __syncthreads();  // the LDS is free
+        if (lanes) {
+            sv = SeqView{__builtin_amdgcn_readlane(sv.t0, b), __builtin_amdgcn_readlane(sv.n, b),
+                         __builtin_amdgcn_readlane(sv.len, b), __builtin_amdgcn_readlane(sv.p0, b)};
+        } else {
+            sv = seq_view(a, b);
+            __syncthreads();  // the LDS is free
+        }
     } else {  // a workgroup per pair
         b = (int)blockIdx.x / kv, g = (int)blockIdx.x - b * kv;
+        sv = seq_view(a, b);
+        if (sv.n <= 0) return;
     }
-    const SeqView sv = seq_view(a, b);
-    if (sv.n <= 0) return;
     few_part<D, Q4, NT>(a, lds, sv, b, g, part * per, part * per + per, parts == 1);
     if (parts == 1) return;
     int* const count = reinterpret_cast<int*>(a.sync) + b * kv + g;

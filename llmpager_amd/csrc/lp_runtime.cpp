@@ -1179,7 +1179,7 @@ static PagedPlan paged_plan(const lp_kv_cache* c, int heads, int batch, int toke
         const int unit = c->format == LP_KV_Q4 ? 256 : 128;
         const int units = std::max(1, (p.max_seq + unit - 1) / unit);
         p.min_units = (units + kFewParts - 1) / kFewParts;
-        const int cap = 512;  // two workgroups a CU
+        const int cap = getenv("FW") ? atoi(getenv("FW")) : 512;  // two workgroups a CU
         if (pairs <= kPagedPairs && batch <= kFewBatch && units > 1)
             p.shares = (int)std::min<int64_t>(std::max(cap, pairs), (int64_t)pairs * units);
         p.bytes = (uint64_t)p.shares * p.rows * (c->head_dim * 4 + 8);
