@@ -10,10 +10,19 @@
 // add to the 1 of the largest, so logits equal to M are counted apart and the
 // others' sums kept beside the count; sums of 16 are added up in 64 bits.
 //
-// The alternatives: lane i of a wave holds its i-th best (value, id), and a
-// block is looked through only if one of its logits reaches the last one that
-// counts.  In rows of independent logits a wave of n takes about top (1 +
-// ln(n / top)) of them, one exchange between neighbouring lanes each.
+// The alternatives: lane i of a wave holds its i-th best as a key in the order of
+// (value, lowest id first), and a block is looked through only if one of its
+// logits reaches the last one that counts; of a block's own only those are taken
+// that the lanes' two largest do not rule out.  Keys are put in one by one where
+// they are few, else sorted 64 at a time across the lanes.
+//
+// A row's parts are joined by the workgroup that ends last.  2,048 rows of 49,152
+// without alternatives take 93 us, 5.1 TB/s: a copy's rate.  32 rows of 151,936
+// take 10 us without alternatives, 16 with one, 20 with twenty and 35 with 64; one
+// such row 6 and 10 to 15: there the chain of a block's load, its exponentials,
+// the sort and the join counts, 1 to 3 us each.
+#include <type_traits>
+
 #include "lp_device.h"
 
 using namespace lp;
@@ -24,9 +33,30 @@ namespace {
 constexpr int kPer = 16;               // logits of a lane in a block
 constexpr int kBlock = 64 * kPer;      // and of a wave
 
+// Over the wave by row shares of 16 lanes (neighbours, pairs, the halves of eight,
+// the halves), then the four rows' from scalar registers: no LDS round trips.
+template <int CTRL>
+__device__ __forceinline__ double add_dpp(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xf, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xf, 0xf, false);
+    return v + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
 __device__ __forceinline__ double wave_sum_f64(double v) {
-    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
+    v = add_dpp<0x140>(add_dpp<0x141>(add_dpp<0x4e>(add_dpp<0xb1>(v))));
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    double t = 0.0;
+#pragma unroll
+    for (int l = 0; l < 64; l += 16)
+        t += __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(u >> 32), l) << 32 |
+                                            (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, l));
+    return t;
+}
+// (NaN counts as nothing)
+__device__ __forceinline__ float wave_top(float v) {
+    return __uint_as_float(wave_reduce_u32(__float_as_uint(v), 0xff800000u, [](uint32_t a, uint32_t b) {
+        return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    }));
 }
 
 // e^d for d <= 0: the hardware's base-2 exponential, with what the product
@@ -62,7 +92,7 @@ struct Sums {
     }
     __device__ __forceinline__ void add(const float (&x)[kPer], float mx) {
         if (__ballot(mx >= m)) {
-            const float w = wave_max(mx);
+            const float w = wave_top(mx);
             if (w > m) raise(w);
             float bs = 0.0f, by = 0.0f;
 #pragma unroll
@@ -87,49 +117,138 @@ struct Sums {
     }
 };
 
-// The best (value, id) pairs a wave has seen, lane i the i-th: larger values
-// first, lower ids first of equal ones.  NaN enters nowhere.
-struct Best {
-    float v = -INFINITY;
-    int id = INT32_MAX;
-    float tv = -INFINITY;  // the last that counts
-    int tid = INT32_MAX;
+// A logit as a whole number in the order of the alternatives: larger values
+// first, lower ids first of equal ones (-0 and 0 are).  No number's is 0.
+__device__ __forceinline__ uint32_t value_key(float x) {
+    const uint32_t b = __float_as_uint(x + 0.0f);
+    return b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+    return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
 
-    __device__ __forceinline__ void put(float x, int i, int top) {  // x, i the same in all lanes
-        const bool before = v > x || (v == x && id < i);
-        const int rank = __popcll(__ballot(before));
-        const float pv = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x138, 0xf, 0xf, false));
-        const int pi = __builtin_amdgcn_update_dpp(0, id, 0x138, 0xf, 0xf, false);  // the lane before
-        const int lane = lane_id();
-        v = lane < rank ? v : lane == rank ? x : pv;
-        id = lane < rank ? id : lane == rank ? i : pi;
-        tv = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), top - 1));
-        tid = __builtin_amdgcn_readlane(id, top - 1);
+// The lane X further in the exclusive-or sense.
+template <int X>
+__device__ __forceinline__ uint32_t xor_lane(uint32_t v) {
+    auto dpp = [](uint32_t u, auto ctrl) {
+        return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, decltype(ctrl)::value, 0xf, 0xf, false);
+    };
+    if constexpr (X == 1) return dpp(v, std::integral_constant<int, 0xb1>());
+    if constexpr (X == 2) return dpp(v, std::integral_constant<int, 0x4e>());
+    if constexpr (X == 3) return dpp(v, std::integral_constant<int, 0x1b>());
+    if constexpr (X == 4) return xor_lane<7>(xor_lane<3>(v));
+    if constexpr (X == 7) return dpp(v, std::integral_constant<int, 0x141>());   // mirrored within eight
+    if constexpr (X == 8) return dpp(v, std::integral_constant<int, 0x128>());   // rotated within a row of 16
+    if constexpr (X == 15) return dpp(v, std::integral_constant<int, 0x140>());  // mirrored within a row
+    return (uint32_t)__shfl_xor((int)v, X, 64);
+}
+
+// A key per lane: value key, then ~id; 0: none.
+struct Keys {
+    uint32_t hi = 0, lo = 0;
+
+    // of each pair of lanes X apart the lower one keeps the larger key
+    template <int X>
+    __device__ __forceinline__ void order() {
+        const uint32_t ph = xor_lane<X>(hi), pl = xor_lane<X>(lo);
+        constexpr int bit = X >= 32 ? 32 : X >= 16 ? 16 : X >= 8 ? 8 : X >= 4 ? 4 : X >= 2 ? 2 : 1;
+        const bool lower = (lane_id() & bit) == 0;
+        const bool swap = (((uint64_t)ph << 32 | pl) > ((uint64_t)hi << 32 | lo)) == lower;
+        hi = swap ? ph : hi;
+        lo = swap ? pl : lo;
     }
-    // A value that at least `top` lanes' mx reach: the largest whose 12 last
-    // bits, in the order of their bit patterns, are zero.  What is below it is
-    // not among the best of anything that holds those mx.
-    static __device__ __forceinline__ float reached(float mx, int top) {
-        const uint32_t b = __float_as_uint(mx), key = b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
+    __device__ __forceinline__ void order_bitonic() {
+        order<32>(), order<16>(), order<8>(), order<4>(), order<2>(), order<1>();
+    }
+    // largest first (a bitonic network whose halves are compared mirrored)
+    __device__ __forceinline__ void sort() {
+        order<1>();
+        order<3>(), order<1>();
+        order<7>(), order<2>(), order<1>();
+        order<15>(), order<4>(), order<2>(), order<1>();
+        order<31>(), order<8>(), order<4>(), order<2>(), order<1>();
+        order<63>(), order<16>(), order<8>(), order<4>(), order<2>(), order<1>();
+    }
+    // the 64 largest of these and `k`, both sorted
+    __device__ __forceinline__ void merge(const Keys& k) {
+        const uint32_t ph = xor_lane<63>(k.hi), pl = xor_lane<63>(k.lo);
+        const bool other = ((uint64_t)ph << 32 | pl) > ((uint64_t)hi << 32 | lo);
+        hi = other ? ph : hi;
+        lo = other ? pl : lo;
+        order_bitonic();
+    }
+};
+
+// The best logits a wave has seen, sorted.
+struct Best : Keys {
+    __device__ __forceinline__ void put(uint32_t h, uint32_t l) {  // one more, the same in all lanes
+        const uint64_t x = (uint64_t)h << 32 | l;
+        const int rank = __popcll(__ballot(((uint64_t)hi << 32 | lo) > x));
+        const uint32_t ph = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)hi, 0x138, 0xf, 0xf, false);  // the lane before
+        const uint32_t pl = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)lo, 0x138, 0xf, 0xf, false);
+        const int lane = lane_id();
+        hi = lane < rank ? hi : lane == rank ? h : ph;
+        lo = lane < rank ? lo : lane == rank ? l : pl;
+    }
+    // A value key that at least `top` of the lanes' m1 and m2 reach: the largest
+    // whose 12 last bits are zero.  What is below it is not among the best of
+    // anything that holds those.
+    static __device__ __forceinline__ uint32_t reached(uint32_t m1, uint32_t m2, int top) {
         uint32_t at = 0;
 #pragma unroll
         for (int bit = 31; bit >= 12; --bit) {
             const uint32_t t = at | 1u << bit;
-            at = __popcll(__ballot(key >= t)) >= top ? t : at;
+            at = __popcll(__ballot(m1 >= t)) + __popcll(__ballot(m2 >= t)) >= top ? t : at;
         }
-        // (the patterns below -inf's are NaNs)
-        return fmaxf(at & 0x80000000u ? __uint_as_float(at ^ 0x80000000u) : __uint_as_float(~at), -INFINITY);
+        return at;
     }
-    // each lane's (x, i) where `on`
-    __device__ __forceinline__ void take(float x, int i, bool on, int top) {
-        uint64_t left = ~0ull;
-        for (;;) {
-            const uint64_t b = __ballot(on && (x > tv || (x == tv && i < tid))) & left;
-            if (!b) return;
-            const int l = __builtin_ctzll(b);
-            left &= ~(1ull << l);
-            put(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), l)), __builtin_amdgcn_readlane(i, l), top);
+    // Each lane's N keys (value keys h, 0: none).  A few are put in one by one
+    // (about 170 cycles each); more go to a lane each through `room`, 64 keys of
+    // LDS, and are sorted and merged (about 2,500 for up to 64 of them).
+    template <int N, typename Lo>
+    __device__ __forceinline__ void take(const uint32_t (&h)[N], const Lo& low, int top, volatile uint64_t* room) {
+        uint32_t m1 = h[0], m2 = 0;
+#pragma unroll
+        for (int i = 1; i < N; ++i) m2 = max(m2, min(m1, h[i])), m1 = max(m1, h[i]);
+        // none below the last that counts, nor below what the keys' own best are not
+        uint32_t least = max(1u, (uint32_t)__builtin_amdgcn_readlane((int)hi, top - 1));
+        if (__popcll(__ballot(m1 >= least)) > 8) least = max(least, reached(m1, m2, top));
+        int count = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) count += __popcll(__ballot(h[i] >= least));
+        if (count <= 12) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                for (uint64_t b = __ballot(h[i] >= least); b; b &= b - 1) {
+                    const int l = __builtin_ctzll(b);
+                    put((uint32_t)__builtin_amdgcn_readlane((int)h[i], l), (uint32_t)__builtin_amdgcn_readlane((int)low(i), l));
+                }
+            return;
         }
+        int held = 0;
+        auto flush = [&] {
+            __builtin_amdgcn_wave_barrier();
+            const int lane = lane_id();
+            uint64_t key = 0;
+            if (lane < held) key = room[lane];
+            Keys k;
+            k.hi = (uint32_t)(key >> 32), k.lo = (uint32_t)key;
+            k.sort();
+            merge(k);
+            held = 0;
+            __builtin_amdgcn_wave_barrier();
+        };
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint64_t b = __ballot(h[i] >= least);
+            const int n = __popcll(b);
+            if (held + n > 64) flush();
+            if (h[i] >= least)
+                room[held + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0))] =
+                    (uint64_t)h[i] << 32 | low(i);
+            held += n;
+        }
+        flush();
     }
 };
 
@@ -161,9 +280,9 @@ __device__ __forceinline__ void finish(const LogprobArgs& a, int row, const Sums
     }
     if (lane < a.top) {
         const uint64_t at = (uint64_t)row * (uint32_t)a.top + (uint32_t)lane;
-        const bool none = best.id == INT32_MAX;
-        gptr_w<int>(a.ids)[at] = none ? -1 : best.id;
-        gptr_w<float>(a.top_logp)[at] = none ? __builtin_nanf("") : (float)((double)(best.v - t.m) - lse);
+        const bool none = best.hi == 0;
+        gptr_w<int>(a.ids)[at] = none ? -1 : (int)~best.lo;
+        gptr_w<float>(a.top_logp)[at] = none ? __builtin_nanf("") : (float)((double)(key_value(best.hi) - t.m) - lse);
     }
 }
 
@@ -171,7 +290,7 @@ __device__ __forceinline__ void finish(const LogprobArgs& a, int row, const Sums
 // is none), as one.
 __device__ __forceinline__ Sums join(float m, double s, double y) {
     Sums t;
-    t.m = wave_max(m);
+    t.m = wave_top(m);
     double f = m == t.m ? 1.0 : (double)exp_neg(m - t.m);
     if (m == -INFINITY) {
         f = 0.0;
@@ -188,8 +307,7 @@ template <bool TOP>
 __device__ __forceinline__ void scan(const LogprobArgs& a, int row, int part, Sums& t, Best& best) {
     __shared__ float lm[4];
     __shared__ double lsum[2][4];
-    __shared__ float lv[TOP ? 4 : 1][64];
-    __shared__ int li[TOP ? 4 : 1][64];
+    __shared__ uint64_t lk[TOP ? 4 : 1][64];  // a wave's room, then its best
     const uint64_t at = a.logits + (uint64_t)row * (uint32_t)a.stride * 4;
     const LP_GLOBAL float* x = gptr<float>(at);
     const int wave = (int)(threadIdx.x >> 6), lane = lane_id();
@@ -201,6 +319,7 @@ __device__ __forceinline__ void scan(const LogprobArgs& a, int row, int part, Su
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = load4(x, e + 4 * (lane + 64 * j) - skew, n);
     };
+    float last = -INFINITY;  // the last alternative that counts
     int e = e0 + wave * kBlock;
     if (e < e1) load(e);
     for (; e < e1; e += 4 * kBlock) {
@@ -215,33 +334,72 @@ __device__ __forceinline__ void scan(const LogprobArgs& a, int row, int part, Su
         for (int i = 1; i < kPer; ++i) mx = fmaxf(mx, xs[i]);
         t.add(xs, mx);
         if constexpr (TOP) {
-            const uint64_t b = __ballot(mx >= best.tv);
-            if (b) {
-                // many: first what the block's own best are not below
-                const float least = __popcll(b) > 8 ? Best::reached(mx, a.top) : -INFINITY;
+            if (__ballot(mx >= last)) {
+                uint32_t h[kPer];
+                const int id0 = e + 4 * lane - skew;
+                auto id = [&](int i) { return id0 + 256 * (i / 4) + i % 4; };
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const int id = e + 4 * (lane + 64 * j) - skew + u;
-                        best.take(xs[4 * j + u], id, xs[4 * j + u] >= least && id >= 0 && id < n, a.top);
-                    }
+                for (int i = 0; i < kPer; ++i) h[i] = xs[i] == xs[i] && (uint32_t)id(i) < (uint32_t)n ? value_key(xs[i]) : 0u;
+                best.take(h, [&](int i) { return ~(uint32_t)id(i); }, a.top, lk[wave]);
+                const uint32_t k = (uint32_t)__builtin_amdgcn_readlane((int)best.hi, a.top - 1);
+                last = k ? key_value(k) : -INFINITY;
             }
         }
     }
     const double ws = wave_sum_f64(t.s + (double)t.n), wy = wave_sum_f64(t.y);
     if (lane == 0) lm[wave] = t.m, lsum[0][wave] = ws, lsum[1][wave] = wy;
-    if constexpr (TOP) lv[wave][lane] = best.v, li[wave][lane] = best.id;
+    if constexpr (TOP) lk[wave][lane] = (uint64_t)best.hi << 32 | best.lo;
     __syncthreads();
     if (wave) return;
     t = join(lane < 4 ? lm[lane & 3] : -INFINITY, lane < 4 ? lsum[0][lane & 3] : 0.0, lane < 4 ? lsum[1][lane & 3] : 0.0);
     if constexpr (TOP)
-        for (int w = 1; w < 4; ++w) best.take(lv[w][lane], li[w][lane], lane < a.top && li[w][lane] != INT32_MAX, a.top);
+        for (int w = 1; w < 4; ++w) {
+            Keys k;
+            k.hi = (uint32_t)(lk[w][lane] >> 32), k.lo = (uint32_t)lk[w][lane];
+            best.merge(k);
+        }
 }
 
-// Records: per (row, part) s, y, m (32 bytes), then its alternatives.
+// Records: per (row, part) s, y, m (32 bytes); behind all of them the keys of its
+// alternatives, a row's parts' one behind the other.
 __device__ __forceinline__ uint64_t rec_at(const LogprobArgs& a, int row, int part) {
-    return a.part + ((uint64_t)(uint32_t)row * (uint32_t)a.parts + (uint32_t)part) * (uint32_t)logprob_rec(a.top);
+    return a.part + ((uint64_t)(uint32_t)row * (uint32_t)a.parts + (uint32_t)part) * 32;
+}
+__device__ __forceinline__ uint64_t keys_at(const LogprobArgs& a, int row, int part) {
+    return rec_at(a, a.rows, 0) + ((uint64_t)(uint32_t)row * (uint32_t)a.parts + (uint32_t)part) * (uint32_t)(8 * a.top);
+}
+__device__ __forceinline__ void put64(uint64_t at, uint64_t v) { agent_store(reinterpret_cast<uint64_t*>(at), v); }
+__device__ __forceinline__ uint64_t get64(uint64_t at) { return agent_load(reinterpret_cast<const uint64_t*>(at)); }
+
+// The parts of a row joined by one wave: a part's sums per lane, the
+// alternatives' keys 16 a lane.
+template <bool TOP>
+__device__ __forceinline__ void join_row(const LogprobArgs& a, int row) {
+    const int lane = lane_id();
+    float m = -INFINITY;
+    double s = 0.0, y = 0.0;
+    if (lane < a.parts) {
+        const uint64_t r = rec_at(a, row, lane);
+        s = __builtin_bit_cast(double, get64(r)), y = __builtin_bit_cast(double, get64(r + 8));
+        m = __uint_as_float((uint32_t)get64(r + 16));
+    }
+    Best best;
+    if constexpr (TOP) {
+        __shared__ uint64_t room[64];
+        const uint64_t keys = keys_at(a, row, 0);
+        for (int i0 = 0; i0 < a.parts * a.top; i0 += 1024) {
+            uint32_t h[16], l[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int k = i0 + 64 * i + lane;
+                uint64_t key = 0;
+                if (k < a.parts * a.top) key = get64(keys + 8 * k);
+                h[i] = (uint32_t)(key >> 32), l[i] = (uint32_t)key;
+            }
+            best.take(h, [&](int i) { return l[i]; }, a.top, room);
+        }
+    }
+    finish(a, row, join(m, s, y), best);
 }
 
 template <bool TOP>
@@ -257,49 +415,23 @@ __device__ __forceinline__ void logprobs_body(const LogprobArgs& a) {
     }
     const uint64_t r = rec_at(a, row, part);
     if (lane_id() == 0) {
-        gptr_w<double>(r)[0] = t.s;
-        gptr_w<double>(r)[1] = t.y;
-        gptr_w<float>(r)[4] = t.m;
+        put64(r, __builtin_bit_cast(uint64_t, t.s));
+        put64(r + 8, __builtin_bit_cast(uint64_t, t.y));
+        put64(r + 16, __float_as_uint(t.m));
     }
-    if (TOP && lane_id() < a.top) {
-        gptr_w<float>(r + 32)[lane_id()] = best.v;
-        gptr_w<int>(r + 32 + 4 * a.top)[lane_id()] = best.id;
+    if (TOP && lane_id() < a.top) put64(keys_at(a, row, part) + 8 * lane_id(), (uint64_t)best.hi << 32 | best.lo);
+    // the row's last part joins them: nothing waits
+    int* const count = reinterpret_cast<int*>(a.sync) + row * kPagedStride;
+    __builtin_amdgcn_s_waitcnt(0);
+    int o = 0;
+    if (lane_id() == 0) {
+        o = atomicAdd(count, 1);
+        if (o == a.parts - 1) agent_store(count, 0);  // zero for the next launch
     }
+    if (__builtin_amdgcn_readfirstlane(o) == a.parts - 1) join_row<TOP>(a, row);
 }
 
 }  // namespace
 
 extern "C" __global__ void __launch_bounds__(256) lp_logprobs(const LogprobArgs a) { logprobs_body<false>(a); }
 extern "C" __global__ void __launch_bounds__(256) lp_logprobs_top(const LogprobArgs a) { logprobs_body<true>(a); }
-
-// The parts of a row joined: a workgroup per row, its first wave the sums (a
-// part per lane), all four the alternatives.
-extern "C" __global__ void __launch_bounds__(256) lp_logprobs_join(const LogprobArgs a) {
-    __shared__ float lv[4][64];
-    __shared__ int li[4][64];
-    const int row = blockIdx.x, wave = (int)(threadIdx.x >> 6), lane = lane_id();
-    Best best;
-    if (a.top) {
-        for (int p = wave; p < a.parts; p += 4) {
-            const uint64_t r = rec_at(a, row, p) + 32;
-            const bool on = lane < a.top;
-            float v = 0.0f;
-            int id = INT32_MAX;
-            if (on) v = gptr<float>(r)[lane], id = gptr<int>(r + 4 * a.top)[lane];
-            best.take(v, id, on && id != INT32_MAX, a.top);
-        }
-        lv[wave][lane] = best.v, li[wave][lane] = best.id;
-        __syncthreads();
-    }
-    if (wave) return;
-    float m = -INFINITY;
-    double s = 0.0, y = 0.0;
-    if (lane < a.parts) {
-        const uint64_t r = rec_at(a, row, lane);
-        s = gptr<double>(r)[0], y = gptr<double>(r)[1], m = gptr<float>(r)[4];
-    }
-    const Sums t = join(m, s, y);
-    if (a.top)
-        for (int w = 1; w < 4; ++w) best.take(lv[w][lane], li[w][lane], lane < a.top && li[w][lane] != INT32_MAX, a.top);
-    finish(a, row, t, best);
-}

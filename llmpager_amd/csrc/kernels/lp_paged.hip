@@ -913,7 +913,7 @@ __device__ __forceinline__ void few_body(const AttnPagedArgs& a) {
     }
     few_part<D, Q4, NT>(a, lds, sv, b, g, part * per, part * per + per, parts == 1);
     if (parts == 1) return;
-    int* const count = reinterpret_cast<int*>(a.sync) + b * kv + g;
+    int* const count = reinterpret_cast<int*>(a.sync) + (b * kv + g) * kPagedStride;
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     if (threadIdx.x == 0) {

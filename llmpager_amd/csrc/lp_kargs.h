@@ -32,9 +32,13 @@ constexpr int kStepSyncAttn = 17 * kSyncStride;
 constexpr int kStepSyncGemv = kStepSyncAttn + kAttnFusedMaxKvHeads * kSyncStride;
 constexpr int kStepSyncDone = kStepSyncGemv + kSyncStride;  // KV (or query) heads complete
 constexpr int kStepSyncErr = kStepSyncDone + kSyncStride;   // waits that gave up (lp_step_errors_sync)
-constexpr int kPagedSync = kStepSyncErr + kSyncStride;      // paged attention: one per (sequence, KV head)
-constexpr int kPagedPairs = 2048;      // of those whose contexts may be taken in parts
-constexpr int kSyncWords = kPagedSync + kPagedPairs;
+// then one per (sequence, KV head) of paged attention, or row of log probabilities,
+// whose parts workgroups share: 64 bytes apart (1,184 arrivals at 32 words of one
+// line took 10 us)
+constexpr int kPagedSync = kStepSyncErr + kSyncStride;
+constexpr int kPagedStride = 16;
+constexpr int kPagedPairs = 1024;
+constexpr int kSyncWords = kPagedSync + kPagedPairs * kPagedStride;
 constexpr int kMaxTopK = 16;           // largest top_k the device router accepts
 constexpr int kMaxExperts = 1024;      // largest expert count the device router accepts
 constexpr int kTopkFusedMaxT = 8;      // largest T routed by the one-workgroup top-k + dispatch kernel
@@ -319,7 +323,7 @@ constexpr int kFewParts = 64;          // most parts of a pair's context there
 constexpr int kFewBatch = 1024;        // and sequences, for their units fit the LDS
 constexpr int kPagedMaxSplits = 64;    // lp_attn_join_*: one split per lane
 constexpr int kLogprobStep = 4096;     // logits of a workgroup's step
-constexpr int kLogprobMaxParts = 64;   // lp_logprobs_join: one part per lane
+constexpr int kLogprobMaxParts = 64;   // one part per lane where they are joined
 constexpr int kLogprobMaxVocab = 1 << 30;
 constexpr int kLogprobMaxTop = 64;
 
@@ -371,10 +375,11 @@ struct LogprobArgs {
     uint64_t logp, entropy;         // f32 [rows] (entropy may be 0)
     uint64_t ids, top_logp;         // i32, f32 [rows, top]
     uint64_t part;                  // records [rows, parts] of logprob_rec(top) bytes
+    uint64_t sync;                  // arrival counters of the rows (parts > 1)
     int32_t stride, rows, vocab, top;
     int32_t parts, per_part;        // workgroups of a row, and the logits of each (a multiple of kLogprobStep)
 };
-LPK_HD constexpr int logprob_rec(int top) { return 32 + (8 * top + 31) / 32 * 32; }
+LPK_HD constexpr int logprob_rec(int top) { return 32 + 8 * top; }
 
 // ---- fused MoE layer ---------------------------------------------------------
 

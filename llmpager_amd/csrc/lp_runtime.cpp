@@ -148,7 +148,6 @@ enum Fn {
     kAttnJoinD128,
     kLogprobs,
     kLogprobsTop,
-    kLogprobsJoin,
     kNumFns
 };
 
@@ -211,7 +210,6 @@ const FnSpec kSpecs[kNumFns] = {
     {"lp_paged.hsaco", "lp_attn_few_q4_d64_n2"}, {"lp_paged.hsaco", "lp_attn_few_q4_d128_n2"},
     {"lp_paged.hsaco", "lp_attn_join_d64"}, {"lp_paged.hsaco", "lp_attn_join_d128"},
     {"lp_logits.hsaco", "lp_logprobs"},      {"lp_logits.hsaco", "lp_logprobs_top"},
-    {"lp_logits.hsaco", "lp_logprobs_join"},
 };
 
 const char* const kModules[] = {"lp_basic.hsaco", "lp_moe.hsaco", "lp_gemm.hsaco", "lp_attn.hsaco",
@@ -1179,9 +1177,10 @@ static PagedPlan paged_plan(const lp_kv_cache* c, int heads, int batch, int toke
         const int unit = c->format == LP_KV_Q4 ? 256 : 128;
         const int units = std::max(1, (p.max_seq + unit - 1) / unit);
         p.min_units = (units + kFewParts - 1) / kFewParts;
-        const int cap = getenv("FW") ? atoi(getenv("FW")) : 512;  // two workgroups a CU
+        // 512 shares, two workgroups a CU (32 contexts of 4 bits, 18,000 rows: 33 us,
+        // 256 shares 44; 64 of 16 bits: 70 us, 768 shares 76)
         if (pairs <= kPagedPairs && batch <= kFewBatch && units > 1)
-            p.shares = (int)std::min<int64_t>(std::max(cap, pairs), (int64_t)pairs * units);
+            p.shares = (int)std::min<int64_t>(std::max(512, pairs), (int64_t)pairs * units);
         p.bytes = (uint64_t)p.shares * p.rows * (c->head_dim * 4 + 8);
     } else {
         p.tiles = (p.rows + kManyRows - 1) / kManyRows;
@@ -1261,7 +1260,8 @@ int lp_attn_paged(lp_ctx* c, const lp_kv_cache* cache, uint64_t q, int q_stride,
 
 // ---- logits (lp_logits.hip) ---------------------------------------------------------
 
-// A row's parts: about 2048 workgroups in all, each of whole steps (a part's
+// A row's parts: about 2048 workgroups in all (32 rows of 151,936: 21.3 us, with
+// 1024 24.1 and with 512 27.1), each of whole steps (a part's
 // first 16-byte piece may begin before the row does, so up to 3 logits more
 // than the row has are shared out).
 static void logprob_parts(int rows, int vocab, int* parts, int* per) {
@@ -1292,13 +1292,19 @@ int lp_logprobs(lp_ctx* c, uint64_t logits, int stride, int rows, int vocab, uin
     if (int r = check_workspace("logprobs", lp_logprobs_ws_bytes(rows, vocab, top), workspace, ws_bytes)) return r;
     if (int r = check_ctx(c)) return r;
     if (!rows) return LP_OK;
-    LogprobArgs a{logits, targets, logp, entropy, ids, top_logp, workspace, stride, rows, vocab, top, 1, 0};
+    LogprobArgs a{logits, targets, logp, entropy, ids, top_logp, workspace, 0, stride, rows, vocab, top, 1, 0};
     logprob_parts(rows, vocab, &a.parts, &a.per_part);
+    if (a.parts > 1) {
+        // (parts only while rows are few: below the counters' number)
+        const int slot = sync_slot(c, s);
+        if (slot >= 0)
+            a.sync = sync_words(c, slot) + kPagedSync * 4;
+        else
+            a.per_part *= a.parts, a.parts = 1;
+    }
     const int64_t wgs = (int64_t)rows * a.parts;
     if (wgs > INT32_MAX / 256) return fail(LP_E_UNSUPPORTED, "logprobs: too many rows");
-    if (int r = launch(c, top ? kLogprobsTop : kLogprobs, dim3((unsigned)wgs), dim3(256), 0, s, a)) return r;
-    if (a.parts == 1) return LP_OK;
-    return launch(c, kLogprobsJoin, dim3((unsigned)rows), dim3(256), 0, s, a);
+    return launch(c, top ? kLogprobsTop : kLogprobs, dim3((unsigned)wgs), dim3(256), 0, s, a);
 }
 
 // ---- fused MoE layer --------------------------------------------------------------
