@@ -289,12 +289,17 @@ __device__ __forceinline__ f32x4_t mfma16(const u32x4_t& a, const u32x4_t& b, f3
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Two values as fp16, cut towards zero: with the next 11 bits of each in `lo`,
-// 2^-21 of a value is left out.
+// Two values as fp16, cut towards zero, and what that leaves out of each, rounded
+// to fp16 (one mixed multiply-add each): 2^-22 of a value is left out.
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
     const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
     hi = __builtin_bit_cast(uint32_t, h);
-    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a - (float)h[0], b - (float)h[1]));
+    const half2_t x = __builtin_bit_cast(half2_t, h);
+    float minus;  // behind the asm lest -1 x + a become a subtraction of its own
+    asm("" : "=s"(minus) : "0"(-1.0f));
+    half2_t y;
+    y[0] = (_Float16)__builtin_fmaf((float)x[0], minus, a), y[1] = (_Float16)__builtin_fmaf((float)x[1], minus, b);
+    lo = __builtin_bit_cast(uint32_t, y);
 }
 
 // Eight nibbles times their scales: pairs (n0, n4), (n1, n5), (n2, n6), (n3, n7)
@@ -969,9 +974,25 @@ struct ManyRows {
     static constexpr int CR = 64;
     static constexpr int RSK = D * 2 + 16, RSV = D * 2 + 64;
     static constexpr int kBuf = CR * (RSK + RSV);
-    static constexpr int kFlags = 2 * kBuf;          // per buffer: 4 waves' ballots of rows there, 4 words of odd values
-    static constexpr int kLds = kFlags + 2 * (4 * 8 + 4 * 4);
+    static constexpr int kFlags = 2 * kBuf;  // 4 waves' ballots of rows there per buffer, 4 words of odd values
+    static constexpr int kLds = kFlags + 2 * 4 * 8 + 4 * 4;
 };
+
+// The order of what stands between two scheduling barriers: N pairs of matrix
+// instructions, the R reads of LDS of a pair two pairs before it, and V vector
+// instructions behind each.
+template <int N, int R, int V>
+__device__ __forceinline__ void mix() {
+    __builtin_amdgcn_sched_group_barrier(0x100, 2 * R, 0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x402, V, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (i + 2 < N) __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+        __builtin_amdgcn_sched_group_barrier(0x402, V, 0);
+    }
+}
 
 template <int D, bool Q4>
 __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
@@ -980,7 +1001,7 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
     constexpr int KS = D / 16, DT = D / 32;
     constexpr int W = Q4 ? D / 32 : D / 8;  // 32-bit words of a row's quarter
     __shared__ __align__(16) uint8_t lds[M::kLds];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = lane_id(), n = lane & 31, h = lane >> 5;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = lane_id(), n = lane & 31, h = lane >> 5;
     // the longest first: the last tiles of all pairs, then those before them (pair
     // by pair, each kept to an XCD: ragged prompts 75.6 us against 61.7)
     const int pairs = a.batch * a.c.kv_heads, id = (int)blockIdx.x;
@@ -1025,13 +1046,19 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
             }
         }
     };
-    auto store_rows = [&](int buf, int c, int pg) {
+    // ODD: only what is no finite number of the values; else that is left out, and
+    // `strange` says that there was some.
+    int strange = 0;
+    auto store_rows = [&](auto odd_pass, int buf, int c, int pg) {
+        constexpr bool ODD = decltype(odd_pass)::value;
         const bool in = c + srow < r1 && pg >= 0;
-        bool odd = false;
         const uint32_t kd = (uint32_t)(buf * M::kBuf + srow * RSK), vd = (uint32_t)(buf * M::kBuf + CR * RSK + srow * RSV);
         if constexpr (Q4) {
-            const uint32_t ke = in ? ks | ks << 16 : 0u, ve = in ? vs | vs << 16 : 0u;
-            odd = odd_halves(ve);
+            const uint32_t ke = in ? ks | ks << 16 : 0u;
+            uint32_t ve = in ? vs | vs << 16 : 0u;
+            const bool odd = odd_halves(ve);
+            strange |= odd;
+            ve = odd == ODD ? ve : 0u;
             half2_t sk[4], ck[4], sw[4], cw[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -1044,10 +1071,19 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
                 *(LP_LDS u32x4_any*)(ll + vd + quarter * (16 * W) + 16 * i) = nibbles8(vreg[i], sw, cw);
             }
         } else {
+            bool odd = false;
 #pragma unroll
             for (int i = 0; i < W; ++i) {
                 vreg[i] = in ? vreg[i] : 0u;
                 odd |= odd_halves(vreg[i]);
+            }
+            strange |= odd;
+            if (ODD || odd) {
+#pragma unroll
+                for (int i = 0; i < W; ++i) {
+                    const uint32_t lo = vreg[i] & 0xffffu, hi = vreg[i] & 0xffff0000u;
+                    vreg[i] = (odd_halves(lo) == ODD ? lo : 0u) | (odd_halves(hi) == ODD ? hi : 0u);
+                }
             }
 #pragma unroll
             for (int j = 0; j < W / 4; ++j) {
@@ -1055,13 +1091,10 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
                 *(LP_LDS u32x4_any*)(ll + vd + 16 * quarter + 64 * j) = u32x4_t{vreg[4 * j], vreg[4 * j + 1], vreg[4 * j + 2], vreg[4 * j + 3]};
             }
         }
-        const uint64_t there = __ballot(in);
-        const int any = __ballot(odd) != 0;
-        if (lane == 0) {
-            *(LP_LDS u64_any*)(ll + M::kFlags + buf * 48 + wave * 8) = there;
-            *(LP_LDS u32_any*)(ll + M::kFlags + buf * 48 + 32 + wave * 4) = any;
-        }
+        *(LP_LDS u64_any*)(ll + M::kFlags + buf * 32 + wave * 8) = __ballot(in);  // one word, from all lanes
     };
+    using Finite = std::false_type;
+    using Odd = std::true_type;
     int pg = -1, pg1 = -1;  // of the chunk in the registers, and of the one after it
     if (r0 < r1) {
         pg = page_for(r0);
@@ -1098,6 +1131,11 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
             ql[j] = u32x4_t{lo[0], lo[1], lo[2], lo[3]};
         }
     }
+    // the lane's places in a chunk: a key row's piece, and its share of 4 x 16 values
+    // (behind the asm so that what is added to them stays in the reads' offsets)
+    uint32_t klane = lbase + (uint32_t)(n * RSK + 16 * h);
+    uint32_t vlane = lbase + (uint32_t)(CR * RSK + (4 * h + (lane >> 2 & 3)) * RSV + 32 * (lane >> 4 & 1) + 8 * (lane & 3));
+    asm volatile("" : "+v"(klane), "+v"(vlane));
     float m = -INFINITY, l = 0.0f;
     f32x16_t acc[DT];
 #pragma unroll
@@ -1105,8 +1143,9 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[d][r] = 0.0f;
 
-    if (r0 < r1) {
-        store_rows(0, r0, pg);
+    const bool none = r0 >= r1;
+    if (!none) {
+        store_rows(Finite(), 0, r0, pg);
         pg = pg1;
         if (r0 + CR < r1) {
             load_rows(kreg, ks, a.c.k_pages, r0 + CR, pg);
@@ -1116,9 +1155,82 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
         __syncthreads();
     }
     int buf = 0;
-    for (int c = r0; c < r1; c += CR, buf ^= 1) {
+    auto scores = [&](int t) {
+        const uint32_t kt = klane + (uint32_t)(buf * M::kBuf);
+        f32x16_t s;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+            const u32x4_t k = *(LP_LDS u32x4_any*)(uintptr_t)(kt + (uint32_t)(32 * t * RSK + 32 * j));
+            s = mfma32(k, qh[j], s);
+            s = mfma32(k, ql[j], s);
+        }
+        return s;
+    };
+    // what rows c + 32 t.. hold no value for, and what the query does not see
+    auto mask = [&](int c, int t, f32x16_t& s) {
+        int h4 = 4 * h;  // behind the asm so that nothing of this is kept in registers meanwhile
+        asm volatile("" : "+v"(h4));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint64_t there = *(LP_LDS u64_any*)(ll + M::kFlags + buf * 32 + (2 * t + i) * 8);  // four bits a row
+#pragma unroll
+            for (int r = 8 * i; r < 8 * i + 8; ++r) {
+                const int rr = 8 * (r / 4) + h4 + r % 4;
+                if (!(there >> (4 * (rr & 15)) & 1) || c + 32 * t + rr > last) s[r] = -INFINITY;
+            }
+        }
+    };
+    auto top = [&](const f32x16_t& s) {
+        float mx = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+        return mx;
+    };
+    // to a larger maximum; what the sums so far are multiplied by
+    auto raise = [&](float mx) {
+        mx = fmaxf(mx, shfl_xor(mx, 32));
+        const float mn = fmaxf(m, mx);
+        const float f = m == -INFINITY ? 0.0f : exp2_hw(m - mn);
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[d] *= f;
+        m = mn;
+        return f;
+    };
+    auto exps = [&](f32x16_t& s) {
+        const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = exp2_hw(s[r] - base);
+    };
+    auto add = [&](const f32x16_t& s) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) l += s[r];
+    };
+    auto context = [&](int t, const f32x16_t& p) {
+        const uint32_t vt = vlane + (uint32_t)(buf * M::kBuf);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) split2(p[8 * j + 2 * u], p[8 * j + 2 * u + 1], hi[u], lo[u]);
+            const u32x4_t ph = {hi[0], hi[1], hi[2], hi[3]}, pl = {lo[0], lo[1], lo[2], lo[3]};
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const uint32_t at = vt + (uint32_t)((32 * t + 16 * j) * RSV + 64 * d);
+                const v4i16_t x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP_LDS v4i16_t*)(uintptr_t)at);
+                const v4i16_t x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP_LDS v4i16_t*)(uintptr_t)(at + 8 * RSV));
+                const v2i32_t y0 = __builtin_bit_cast(v2i32_t, x0), y1 = __builtin_bit_cast(v2i32_t, x1);
+                const u32x4_t v = {(uint32_t)y0[0], (uint32_t)y0[1], (uint32_t)y1[0], (uint32_t)y1[1]};
+                acc[d] = mfma32(v, ph, acc[d]);
+                acc[d] = mfma32(v, pl, acc[d]);
+            }
+        }
+    };
+    auto stage = [&](int c) {  // the next chunk to LDS, the one after it under way
         if (c + CR < r1) {
-            store_rows(buf ^ 1, c + CR, pg);
+            store_rows(Finite(), buf ^ 1, c + CR, pg);
             pg = pg1;
             if (c + 2 * CR < r1) {
                 load_rows(kreg, ks, a.c.k_pages, c + 2 * CR, pg);
@@ -1126,98 +1238,84 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
             }
             pg1 = page_for(c + 3 * CR);
         }
-        const uint32_t kt = (uint32_t)(buf * M::kBuf), vt = kt + CR * RSK;
-        for (int t = 0; t < CR / 32; ++t) {
-            const int ct = c + 32 * t;
-            if (ct >= wvis) break;
-            uint64_t there[2];  // four bits a row
+    };
+    for (int c = r0; c < r1; c += CR, buf ^= 1) {
+        stage(c);
+        if (c < wvis) {
+            uint64_t there = ~0ull;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) there[i] = *(LP_LDS u64_any*)(ll + M::kFlags + buf * 48 + (2 * t + i) * 8);
-            const bool whole = ct + 32 <= wall && __builtin_amdgcn_readfirstlane((int)((there[0] & there[1]) == ~0ull));
-            // ---- scores
-            f32x16_t s;
+            for (int i = 0; i < 4; ++i) there &= *(LP_LDS u64_any*)(ll + M::kFlags + buf * 32 + i * 8);
+            const bool whole = c + CR <= wall && __builtin_amdgcn_readfirstlane((int)(there == ~0ull));
+            // one half's exponentials behind the other half's products
+            f32x16_t s0 = scores(0);
+            if (!whole) mask(c, 0, s0);
+            float mx = top(s0);
+            if (__ballot(mx > m + 8.0f)) raise(mx);
+            __builtin_amdgcn_sched_barrier(0);
+            f32x16_t s1 = scores(1);
+            exps(s0);
+            add(s0);
+            asm volatile("" : "+v"(s0), "+v"(l));  // here, not where they are used
+            mix<KS, 1, 6>();
+            __builtin_amdgcn_sched_barrier(0);
+            if (!whole) mask(c, 1, s1);
+            mx = top(s1);
+            if (__ballot(mx > m + 8.0f)) s0 *= raise(mx);
+            __builtin_amdgcn_sched_barrier(0);
+            context(0, s0);
+            exps(s1);
+            add(s1);
+            mix<2 * DT, 2, 6>();
+            __builtin_amdgcn_sched_barrier(0);
+            context(1, s1);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __syncthreads();
+    }
+    // ---- values that are no finite numbers: again, these alone, row by row and each
+    // for the queries that see it (a product with 0 would make a NaN of those of others)
+    if (!none) {
+        if (lane == 0) *(LP_LDS u32_any*)(ll + M::kFlags + 64 + wave * 4) = 0;
+        if (__ballot(strange) && lane == 0) *(LP_LDS u32_any*)(ll + M::kFlags + 64 + wave * 4) = 1;
+        __syncthreads();
+        int any = 0;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = 0.0f;
-#pragma unroll
-            for (int j = 0; j < KS; ++j) {
-                const u32x4_t k = *(LP_LDS u32x4_any*)(ll + kt + (uint32_t)((32 * t + n) * RSK + 32 * j + 16 * h));
-                s = mfma32(k, qh[j], s);
-                s = mfma32(k, ql[j], s);
-            }
-            if (!whole) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int rr = 8 * (r / 4) + 4 * h + r % 4;
-                    const bool in = there[r / 8] >> (4 * (rr & 15)) & 1;
-                    if (!in || ct + rr > last) s[r] = -INFINITY;
-                }
-            }
-            // ---- softmax
-            float mx = s[0];
-#pragma unroll
-            for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-            if (__ballot(mx > m + 8.0f)) {
-                mx = fmaxf(mx, shfl_xor(mx, 32));
-                const float mn = fmaxf(m, mx);
-                const float f = m == -INFINITY ? 0.0f : exp2_hw(m - mn);
-                l *= f;
-#pragma unroll
-                for (int d = 0; d < DT; ++d) acc[d] *= f;
-                m = mn;
-            }
-            const float base = m == -INFINITY ? 0.0f : m;
-            float p[16];
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                p[r] = exp2_hw(s[r] - base);
-                l += p[r];
-            }
-            // ---- context
-            if (!whole) {
-                int odd = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) odd |= *(LP_LDS u32_any*)(ll + M::kFlags + buf * 48 + 32 + i * 4);
-                if (__builtin_amdgcn_readfirstlane(odd)) {
-                    // row by row, each for the queries that see it
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
+        for (int i = 0; i < 4; ++i) any |= *(LP_LDS u32_any*)(ll + M::kFlags + 64 + i * 4);
+        buf = 0;
+        if (__builtin_amdgcn_readfirstlane(any))
 #pragma unroll 1
-                        for (int k = 0; k < 2; ++k) {
-                            const int rr = 8 * (r / 4) + 4 * k + r % 4;
-                            const float pk = __shfl(p[r], n + 32 * k, 64);
-                            if (ct + rr > last || !(there[r / 8] >> (4 * (rr & 15)) & 1)) continue;
+            for (int c = r0; c < r1; c += CR) {
+                pg = page_for(c);
+                load_rows(kreg, ks, a.c.k_pages, c, pg);
+                load_rows(vreg, vs, a.c.v_pages, c, pg);
+                store_rows(Odd(), 0, c, pg);
+                __syncthreads();
+#pragma unroll 1
+                for (int t = 0; t < 2; ++t) {
+                    if (c + 32 * t >= wvis) break;
+                    f32x16_t s = scores(t);
+                    mask(c, t, s);
+                    exps(s);
+#pragma unroll 1
+                    for (int i = 0; i < 32; ++i) {
+                        const int r = i >> 1, rr = 32 * t + 8 * (r / 4) + 4 * (i & 1) + r % 4;
+                        const float pk = __shfl(s[0], n + 32 * (i & 1), 64);
+                        const uint32_t at = (uint32_t)(CR * RSK + rr * RSV + 8 * h);
+                        if (c + rr <= last)
 #pragma unroll
                             for (int d = 0; d < DT; ++d)
 #pragma unroll
                                 for (int e = 0; e < 16; ++e) {
-                                    const int at = 32 * d + 8 * (e / 4) + 4 * h + e % 4;
-                                    const uint32_t x = *(LP_LDS u16_any*)(ll + vt + (uint32_t)((32 * t + rr) * RSV + 2 * at));
-                                    acc[d][e] = __builtin_fmaf(pk, f16_bits_to_f32(x), acc[d][e]);
+                                    const uint32_t x = *(LP_LDS u16_any*)(ll + at + 2 * (32 * d + 8 * (e / 4) + e % 4));
+                                    if (x) acc[d][e] = __builtin_fmaf(pk, f16_bits_to_f32(x), acc[d][e]);
                                 }
-                        }
-                    continue;
+                        if (i & 1)  // the next two rows' probabilities
+#pragma unroll
+                            for (int e = 0; e < 15; ++e) s[e] = s[e + 1];
+                    }
                 }
+                __syncthreads();
             }
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                uint32_t hi[4], lo[4];
-#pragma unroll
-                for (int u = 0; u < 4; ++u) split2(p[8 * j + 2 * u], p[8 * j + 2 * u + 1], hi[u], lo[u]);
-                const u32x4_t ph = {hi[0], hi[1], hi[2], hi[3]}, pl = {lo[0], lo[1], lo[2], lo[3]};
-#pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    const uint32_t at = lbase + vt + (uint32_t)((32 * t + 16 * j + 4 * h + (lane >> 2 & 3)) * RSV + 64 * d +
-                                                                32 * (lane >> 4 & 1) + 8 * (lane & 3));
-                    const v4i16_t x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP_LDS v4i16_t*)(uintptr_t)at);
-                    const v4i16_t x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP_LDS v4i16_t*)(uintptr_t)(at + 8 * RSV));
-                    const v2i32_t y0 = __builtin_bit_cast(v2i32_t, x0), y1 = __builtin_bit_cast(v2i32_t, x1);
-                    const u32x4_t v = {(uint32_t)y0[0], (uint32_t)y0[1], (uint32_t)y1[0], (uint32_t)y1[1]};
-                    acc[d] = mfma32(v, ph, acc[d]);
-                    acc[d] = mfma32(v, pl, acc[d]);
-                }
-            }
-        }
-        __syncthreads();
     }
     if (!on) return;  // the halves of a query row are on or off together
     l += shfl_xor(l, 32);

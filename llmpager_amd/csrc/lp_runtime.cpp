@@ -1147,14 +1147,14 @@ int lp_kv_append_paged(lp_ctx* c, const lp_kv_cache* cache, uint64_t q, int q_st
     return launch(c, f, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, s, a);
 }
 
-// How attention is split over the rows of a context: spans of whole chunks for
-// each wave of a workgroup, as long as the (sequence, KV head) pairs times the
-// spans of max_seq rows are about `wgs` workgroups, and at most
-// kPagedMaxSplits spans.
-static void paged_spans(int pairs, int max_seq, int step, int wgs, int* span, int* splits) {
-    const int64_t per = ((int64_t)pairs * max_seq + wgs - 1) / wgs;
-    const int64_t least = (max_seq + kPagedMaxSplits - 1) / kPagedMaxSplits;
-    *span = (int)((std::max<int64_t>({per, least, 1}) + step - 1) / step * step);
+// How attention of many query rows is split over the rows of a context: into as
+// many spans of whole chunks of 64 (at most kPagedMaxSplits) as keep `wgs`
+// workgroups of them at once on the card, for the last of a few more would
+// run alone (48 tiles of 6,000 rows: 480 workgroups SPLIT_NEW us, 528 SPLIT_OLD).
+static void paged_spans(int64_t wgs, int max_seq, int* span, int* splits) {
+    const int most = (int)std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(wgs, 1), kPagedMaxSplits));
+    const int each = (int)(((int64_t)max_seq + most - 1) / most);
+    *span = std::max(64, (each + 63) / 64 * 64);
     *splits = std::max(1, (int)(((int64_t)max_seq + *span - 1) / *span));
 }
 
@@ -1184,7 +1184,7 @@ static PagedPlan paged_plan(const lp_kv_cache* c, int heads, int batch, int toke
         p.bytes = (uint64_t)p.shares * p.rows * (c->head_dim * 4 + 8);
     } else {
         p.tiles = (p.rows + kManyRows - 1) / kManyRows;
-        paged_spans(pairs * p.tiles, p.max_seq, 64, 512, &p.span, &p.splits);
+        paged_spans((int64_t)pairs * p.tiles, p.max_seq, &p.span, &p.splits);
         if (p.splits > 1) p.bytes = (uint64_t)pairs * p.splits * p.rows * (c->head_dim + 2) * 4;
     }
     return p;
