@@ -964,6 +964,7 @@ LP_ATTN_FEW(q4_d128_n2, 1, 128, true, 2)
 namespace {
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ f32x16_t mfma32(const u32x4_t& a, const u32x4_t& b, f32x16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
@@ -977,22 +978,6 @@ struct ManyRows {
     static constexpr int kFlags = 2 * kBuf;  // 4 waves' ballots of rows there per buffer, 4 words of odd values
     static constexpr int kLds = kFlags + 2 * 4 * 8 + 4 * 4;
 };
-
-// The order of what stands between two scheduling barriers: N pairs of matrix
-// instructions, the R reads of LDS of a pair two pairs before it, and V vector
-// instructions behind each.
-template <int N, int R, int V>
-__device__ __forceinline__ void mix() {
-    __builtin_amdgcn_sched_group_barrier(0x100, 2 * R, 0);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x402, V, 0);
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        if (i + 2 < N) __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
-        __builtin_amdgcn_sched_group_barrier(0x402, V, 0);
-    }
-}
 
 template <int D, bool Q4>
 __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
@@ -1022,7 +1007,10 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
 
     uint32_t kreg[W], vreg[W];
     uint32_t ks = 0, vs = 0;
-    auto page_for = [&](int c) { return c + srow < r1 ? page_of(a.c, b, c + srow) : -1; };
+    auto page_for = [&](int c) {
+        const int p = page_of(a.c, b, min(c + srow, r1 - 1));
+        return c + srow < r1 ? p : -1;
+    };
     auto load_rows = [&](uint32_t (&r)[W], uint32_t& s, uint64_t pool, int c, int pg) {
         const uint32_t pr = (uint32_t)((c + srow) & pmask);
         const uint64_t at = page_at<D, Q4>(a.c, pool, max(pg, 0), g);
@@ -1046,55 +1034,67 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
             }
         }
     };
+    using Finite = std::false_type;
+    using Odd = std::true_type;
     // ODD: only what is no finite number of the values; else that is left out, and
-    // `strange` says that there was some.
+    // `strange` says that there was some.  The values of rows that are not there are 0.
     int strange = 0;
-    auto store_rows = [&](auto odd_pass, int buf, int c, int pg) {
+    // (16-bit ones: whether a wave's rows under way need that, and it done)
+    auto special = [&](int c, int pg) {
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+            most = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, most),
+                                                                          __builtin_bit_cast(u16x2_t, vreg[i] & 0x7fff7fffu)));
+        return __ballot(odd_halves(most) || c + srow >= r1 || pg < 0) != 0;
+    };
+    auto mend = [&](auto odd_pass, int c, int pg) {
         constexpr bool ODD = decltype(odd_pass)::value;
         const bool in = c + srow < r1 && pg >= 0;
-        const uint32_t kd = (uint32_t)(buf * M::kBuf + srow * RSK), vd = (uint32_t)(buf * M::kBuf + CR * RSK + srow * RSV);
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const uint32_t lo = in ? vreg[i] & 0xffffu : 0u, hi = in ? vreg[i] & 0xffff0000u : 0u;
+            strange |= odd_halves(lo) || odd_halves(hi);
+            vreg[i] = (odd_halves(lo) == ODD ? lo : 0u) | (odd_halves(hi) == ODD ? hi : 0u);
+        }
+    };
+    // a chunk to LDS, in KS pieces
+    struct Scales {
+        half2_t s[4], c[4];
+    } ksc, vsc;
+    auto store_begin = [&](auto odd_pass, int buf, int c, int pg) {
+        constexpr bool ODD = decltype(odd_pass)::value;
+        const bool in = c + srow < r1 && pg >= 0;
         if constexpr (Q4) {
             const uint32_t ke = in ? ks | ks << 16 : 0u;
             uint32_t ve = in ? vs | vs << 16 : 0u;
             const bool odd = odd_halves(ve);
             strange |= odd;
             ve = odd == ODD ? ve : 0u;
-            half2_t sk[4], ck[4], sw[4], cw[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                sk[i] = __builtin_bit_cast(half2_t, ke), ck[i] = sk[i] * (_Float16)-72.0f;
-                sw[i] = __builtin_bit_cast(half2_t, ve), cw[i] = sw[i] * (_Float16)-72.0f;
-            }
-#pragma unroll
-            for (int i = 0; i < W; ++i) {
-                *(LP_LDS u32x4_any*)(ll + kd + quarter * (16 * W) + 16 * i) = nibbles8(kreg[i], sk, ck);
-                *(LP_LDS u32x4_any*)(ll + vd + quarter * (16 * W) + 16 * i) = nibbles8(vreg[i], sw, cw);
-            }
-        } else {
-            bool odd = false;
-#pragma unroll
-            for (int i = 0; i < W; ++i) {
-                vreg[i] = in ? vreg[i] : 0u;
-                odd |= odd_halves(vreg[i]);
-            }
-            strange |= odd;
-            if (ODD || odd) {
-#pragma unroll
-                for (int i = 0; i < W; ++i) {
-                    const uint32_t lo = vreg[i] & 0xffffu, hi = vreg[i] & 0xffff0000u;
-                    vreg[i] = (odd_halves(lo) == ODD ? lo : 0u) | (odd_halves(hi) == ODD ? hi : 0u);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < W / 4; ++j) {
-                *(LP_LDS u32x4_any*)(ll + kd + 16 * quarter + 64 * j) = u32x4_t{kreg[4 * j], kreg[4 * j + 1], kreg[4 * j + 2], kreg[4 * j + 3]};
-                *(LP_LDS u32x4_any*)(ll + vd + 16 * quarter + 64 * j) = u32x4_t{vreg[4 * j], vreg[4 * j + 1], vreg[4 * j + 2], vreg[4 * j + 3]};
+                ksc.s[i] = __builtin_bit_cast(half2_t, ke), ksc.c[i] = ksc.s[i] * (_Float16)-72.0f;
+                vsc.s[i] = __builtin_bit_cast(half2_t, ve), vsc.c[i] = vsc.s[i] * (_Float16)-72.0f;
             }
         }
         *(LP_LDS u64_any*)(ll + M::kFlags + buf * 32 + wave * 8) = __ballot(in);  // one word, from all lanes
     };
-    using Finite = std::false_type;
-    using Odd = std::true_type;
+    auto store_piece = [&](int buf, int j) {
+        const int i = j >> 1;
+        const uint32_t at = (uint32_t)(buf * M::kBuf + (j & 1 ? CR * RSK + srow * RSV : srow * RSK));
+        if constexpr (Q4)
+            *(LP_LDS u32x4_any*)(ll + at + quarter * (16 * W) + 16 * i) =
+                j & 1 ? nibbles8(vreg[i], vsc.s, vsc.c) : nibbles8(kreg[i], ksc.s, ksc.c);
+        else
+            *(LP_LDS u32x4_any*)(ll + at + 16 * quarter + 64 * i) =
+                j & 1 ? u32x4_t{vreg[4 * i], vreg[4 * i + 1], vreg[4 * i + 2], vreg[4 * i + 3]}
+                      : u32x4_t{kreg[4 * i], kreg[4 * i + 1], kreg[4 * i + 2], kreg[4 * i + 3]};
+    };
+    auto store_rows = [&](auto odd_pass, int buf, int c, int pg) {
+        store_begin(odd_pass, buf, c, pg);
+#pragma unroll
+        for (int j = 0; j < KS; ++j) store_piece(buf, j);
+    };
     int pg = -1, pg1 = -1;  // of the chunk in the registers, and of the one after it
     if (r0 < r1) {
         pg = page_for(r0);
@@ -1143,29 +1143,34 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[d][r] = 0.0f;
 
+    auto load_next = [&](int c) {  // (rows behind the last are some page's)
+        pg = pg1;
+        load_rows(kreg, ks, a.c.k_pages, c, pg);
+        load_rows(vreg, vs, a.c.v_pages, c, pg);
+        pg1 = page_for(c + CR);
+    };
     const bool none = r0 >= r1;
     if (!none) {
+        if (!Q4 && special(r0, pg)) mend(Finite(), r0, pg);
         store_rows(Finite(), 0, r0, pg);
-        pg = pg1;
-        if (r0 + CR < r1) {
-            load_rows(kreg, ks, a.c.k_pages, r0 + CR, pg);
-            load_rows(vreg, vs, a.c.v_pages, r0 + CR, pg);
-        }
-        pg1 = page_for(r0 + 2 * CR);
+        load_next(r0 + CR);
+        if (!Q4 && special(r0 + CR, pg)) mend(Finite(), r0 + CR, pg);
         __syncthreads();
     }
     int buf = 0;
-    auto scores = [&](int t) {
-        const uint32_t kt = klane + (uint32_t)(buf * M::kBuf);
+    auto keys = [&](int t, int j) {
+        return *(LP_LDS u32x4_any*)(uintptr_t)(klane + (uint32_t)(buf * M::kBuf + 32 * t * RSK + 32 * j));
+    };
+    auto values = [&](int i) {  // rows 16 (i / DT).., columns 32 (i % DT)..
+        const uint32_t at = vlane + (uint32_t)(buf * M::kBuf + 16 * (i / DT) * RSV + 64 * (i % DT));
+        const v2i32_t x = __builtin_bit_cast(v2i32_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP_LDS v4i16_t*)(uintptr_t)at));
+        const v2i32_t y = __builtin_bit_cast(v2i32_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP_LDS v4i16_t*)(uintptr_t)(at + 8 * RSV)));
+        return u32x4_t{(uint32_t)x[0], (uint32_t)x[1], (uint32_t)y[0], (uint32_t)y[1]};
+    };
+    auto zero = [] {
         f32x16_t s;
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = 0.0f;
-#pragma unroll
-        for (int j = 0; j < KS; ++j) {
-            const u32x4_t k = *(LP_LDS u32x4_any*)(uintptr_t)(kt + (uint32_t)(32 * t * RSK + 32 * j));
-            s = mfma32(k, qh[j], s);
-            s = mfma32(k, ql[j], s);
-        }
         return s;
     };
     // what rows c + 32 t.. hold no value for, and what the query does not see
@@ -1188,88 +1193,101 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
         for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
         return mx;
     };
-    // to a larger maximum; what the sums so far are multiplied by
+    // to a larger maximum; what the sums so far are to be multiplied by
     auto raise = [&](float mx) {
         mx = fmaxf(mx, shfl_xor(mx, 32));
         const float mn = fmaxf(m, mx);
         const float f = m == -INFINITY ? 0.0f : exp2_hw(m - mn);
         l *= f;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) acc[d] *= f;
         m = mn;
         return f;
     };
-    auto exps = [&](f32x16_t& s) {
-        const float base = m == -INFINITY ? 0.0f : m;
+    auto scale = [&](float f) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = exp2_hw(s[r] - base);
+        for (int d = 0; d < DT; ++d) acc[d] *= f;
     };
-    auto add = [&](const f32x16_t& s) {
+    // piece j of KS of a half's probabilities, and their images
+    auto probs = [&](const f32x16_t& s, float base, int j, uint32_t (&hi)[8], uint32_t (&lo)[8]) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) l += s[r];
-    };
-    auto context = [&](int t, const f32x16_t& p) {
-        const uint32_t vt = vlane + (uint32_t)(buf * M::kBuf);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) split2(p[8 * j + 2 * u], p[8 * j + 2 * u + 1], hi[u], lo[u]);
-            const u32x4_t ph = {hi[0], hi[1], hi[2], hi[3]}, pl = {lo[0], lo[1], lo[2], lo[3]};
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                const uint32_t at = vt + (uint32_t)((32 * t + 16 * j) * RSV + 64 * d);
-                const v4i16_t x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP_LDS v4i16_t*)(uintptr_t)at);
-                const v4i16_t x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP_LDS v4i16_t*)(uintptr_t)(at + 8 * RSV));
-                const v2i32_t y0 = __builtin_bit_cast(v2i32_t, x0), y1 = __builtin_bit_cast(v2i32_t, x1);
-                const u32x4_t v = {(uint32_t)y0[0], (uint32_t)y0[1], (uint32_t)y1[0], (uint32_t)y1[1]};
-                acc[d] = mfma32(v, ph, acc[d]);
-                acc[d] = mfma32(v, pl, acc[d]);
-            }
+        for (int u = 8 / KS * j; u < 8 / KS * (j + 1); ++u) {
+            const float x = exp2_hw(s[2 * u] - base), y = exp2_hw(s[2 * u + 1] - base);
+            l += x, l += y;
+            split2(x, y, hi[u], lo[u]);
+            asm volatile("" : "+v"(hi[u]), "+v"(lo[u]), "+v"(l));  // here, not where they are used
         }
     };
-    auto stage = [&](int c) {  // the next chunk to LDS, the one after it under way
-        if (c + CR < r1) {
-            store_rows(Finite(), buf ^ 1, c + CR, pg);
-            pg = pg1;
-            if (c + 2 * CR < r1) {
-                load_rows(kreg, ks, a.c.k_pages, c + 2 * CR, pg);
-                load_rows(vreg, vs, a.c.v_pages, c + 2 * CR, pg);
-            }
-            pg1 = page_for(c + 3 * CR);
-        }
-    };
+    auto part = [](const uint32_t (&x)[8], int j) { return u32x4_t{x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]}; };
+    // A chunk in four rows of KS steps (2 DT is as many), each of two matrix
+    // instructions, a read of LDS for those two steps on, and a share of the vector
+    // work: half 0's scores with the next chunk's rows to LDS; half 1's with half 0's
+    // probabilities; half 0's context with half 1's; half 1's.
+    static_assert(KS == 2 * DT && 8 % KS == 0);
+    auto step_end = [] { __builtin_amdgcn_sched_barrier(0); };
     for (int c = r0; c < r1; c += CR, buf ^= 1) {
-        stage(c);
-        if (c < wvis) {
-            uint64_t there = ~0ull;
+        u32x4_t x[3], y[3];
+        x[0] = keys(0, 0), x[1] = keys(0, 1);
+        uint64_t there = ~0ull;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) there &= *(LP_LDS u64_any*)(ll + M::kFlags + buf * 32 + i * 8);
+        for (int i = 0; i < 4; ++i) there &= *(LP_LDS u64_any*)(ll + M::kFlags + buf * 32 + i * 8);
+        f32x16_t s0 = zero();
+        store_begin(Finite(), buf ^ 1, c + CR, pg);
+        step_end();
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+            x[(j + 2) % 3] = keys((j + 2) / KS, (j + 2) % KS);
+            s0 = mfma32(x[j % 3], qh[j], s0);
+            s0 = mfma32(x[j % 3], ql[j], s0);
+            store_piece(buf ^ 1, j);
+            step_end();
+        }
+        load_next(c + 2 * CR);
+        if (c < wvis) {
             const bool whole = c + CR <= wall && __builtin_amdgcn_readfirstlane((int)(there == ~0ull));
-            // one half's exponentials behind the other half's products
-            f32x16_t s0 = scores(0);
             if (!whole) mask(c, 0, s0);
             float mx = top(s0);
-            if (__ballot(mx > m + 8.0f)) raise(mx);
-            __builtin_amdgcn_sched_barrier(0);
-            f32x16_t s1 = scores(1);
-            exps(s0);
-            add(s0);
-            asm volatile("" : "+v"(s0), "+v"(l));  // here, not where they are used
-            mix<KS, 1, 6>();
-            __builtin_amdgcn_sched_barrier(0);
+            if (__ballot(mx > m + 8.0f)) scale(raise(mx));
+            float base = m == -INFINITY ? 0.0f : m;
+            uint32_t hi[8], lo[8];
+            f32x16_t s1 = zero();
+            step_end();
+#pragma unroll
+            for (int j = 0; j < KS; ++j) {
+                if (j + 2 < KS)
+                    x[(KS + j + 2) % 3] = keys(1, j + 2);
+                else
+                    y[j + 2 - KS] = values(j + 2 - KS);
+                s1 = mfma32(x[(KS + j) % 3], qh[j], s1);
+                s1 = mfma32(x[(KS + j) % 3], ql[j], s1);
+                probs(s0, base, j, hi, lo);
+                step_end();
+            }
             if (!whole) mask(c, 1, s1);
             mx = top(s1);
-            if (__ballot(mx > m + 8.0f)) s0 *= raise(mx);
-            __builtin_amdgcn_sched_barrier(0);
-            context(0, s0);
-            exps(s1);
-            add(s1);
-            mix<2 * DT, 2, 6>();
-            __builtin_amdgcn_sched_barrier(0);
-            context(1, s1);
-            __builtin_amdgcn_sched_barrier(0);
+            const bool up = __ballot(mx > m + 8.0f);
+            float f = 1.0f;
+            if (up) f = raise(mx);
+            base = m == -INFINITY ? 0.0f : m;
+            uint32_t hi1[8], lo1[8];
+            step_end();
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                y[(i + 2) % 3] = values(i + 2);
+                acc[i % DT] = mfma32(y[i % 3], part(hi, i / DT), acc[i % DT]);
+                acc[i % DT] = mfma32(y[i % 3], part(lo, i / DT), acc[i % DT]);
+                probs(s1, base, i, hi1, lo1);
+                step_end();
+            }
+            if (up) scale(f);
+            step_end();
+#pragma unroll
+            for (int i = KS; i < 2 * KS; ++i) {
+                if (i + 2 < 2 * KS) y[(i + 2) % 3] = values(i + 2);
+                acc[i % DT] = mfma32(y[i % 3], part(hi1, i / DT - 2), acc[i % DT]);
+                acc[i % DT] = mfma32(y[i % 3], part(lo1, i / DT - 2), acc[i % DT]);
+                step_end();
+            }
         }
+        if (!Q4 && special(c + 2 * CR, pg)) mend(Finite(), c + 2 * CR, pg);
         __syncthreads();
     }
     // ---- values that are no finite numbers: again, these alone, row by row and each
@@ -1288,14 +1306,23 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
                 pg = page_for(c);
                 load_rows(kreg, ks, a.c.k_pages, c, pg);
                 load_rows(vreg, vs, a.c.v_pages, c, pg);
+                if (!Q4) mend(Odd(), c, pg);
                 store_rows(Odd(), 0, c, pg);
                 __syncthreads();
 #pragma unroll 1
                 for (int t = 0; t < 2; ++t) {
                     if (c + 32 * t >= wvis) break;
-                    f32x16_t s = scores(t);
+                    f32x16_t s = zero();
+#pragma unroll
+                    for (int j = 0; j < KS; ++j) {
+                        const u32x4_t k = keys(t, j);
+                        s = mfma32(k, qh[j], s);
+                        s = mfma32(k, ql[j], s);
+                    }
                     mask(c, t, s);
-                    exps(s);
+                    const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r] = exp2_hw(s[r] - base);
 #pragma unroll 1
                     for (int i = 0; i < 32; ++i) {
                         const int r = i >> 1, rr = 32 * t + 8 * (r / 4) + 4 * (i & 1) + r % 4;
