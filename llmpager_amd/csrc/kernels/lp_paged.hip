@@ -947,10 +947,10 @@ LP_ATTN_FEW(q4_d128_n2, 1, 128, true, 2)
 // ---------------------------------------------------------------------------
 // Attention of many query rows: a workgroup takes 128 of a (sequence, KV head)'s
 // query rows, 32 a wave, and walks the rows of the context that they see in
-// chunks of 64, as fp16 in LDS for its four waves: the next chunk's rows are
-// written there (4-bit ones multiplied out on the way, columns of eight in the
-// order of nibbles8) and the one's after it are on their way to registers while
-// this chunk is worked on, one barrier a chunk.
+// chunks of 64, as fp16 in LDS for its four waves, one barrier a chunk: the next
+// chunk's rows are written there (4-bit ones multiplied out on the way, columns of
+// eight in the order of nibbles8) and the one's after it sent for while this one is
+// worked on.
 //
 // Matrix work bounds it: fp32 queries and probabilities cost two fp16 MFMAs a
 // product.  As above S^T = K Q^T and O^T = V^T P^T, on v_mfma_f32_32x32x16_f16: the
@@ -959,7 +959,16 @@ LP_ATTN_FEW(q4_d128_n2, 1, 128, true, 2)
 // comes through transposing reads of 4 x 16 blocks, and a row read from LDS
 // serves the hi and the lo product.  Key rows are padded by 16 bytes (16 rows'
 // 16-byte pieces then cover the banks), value rows by 64 (four rows' 32 bytes and
-// their neighbours' do).
+// their neighbours' do).  The order of the instructions is given: every two MFMAs
+// have the reads for those two steps on and a share of the vector work beside them
+// (left to the compiler, each pair waited for its own reads: 526 us against 432).
+// What would hold the accumulators twice, a branch that computes them in another
+// way, stays out of the loop.
+//
+// 2,048 tokens of 32 heads behind 6,000 rows of 16 bits: 419 us, 563 TFLOP/s of the
+// formula's and twice that of MFMA work, what a large fp16 product reaches; 12 x 80
+// query rows of 4 heads behind 6,000 rows of 4 bits: 36 us, of which a chunk takes
+// about 3 us and the launch with what comes before the first one 10.
 // ---------------------------------------------------------------------------
 namespace {
 
@@ -987,10 +996,15 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
     constexpr int W = Q4 ? D / 32 : D / 8;  // 32-bit words of a row's quarter
     __shared__ __align__(16) uint8_t lds[M::kLds];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = lane_id(), n = lane & 31, h = lane >> 5;
-    // the longest first: the last tiles of all pairs, then those before them (pair
-    // by pair, each kept to an XCD: ragged prompts 75.6 us against 61.7)
-    const int pairs = a.batch * a.c.kv_heads, id = (int)blockIdx.x;
-    const int split = id % a.splits, bg = id / a.splits % pairs, tile = a.tiles - 1 - id / a.splits / pairs;
+    // The longest first: the last tiles of all pairs, then those before them (pair
+    // by pair, each kept to an XCD: ragged prompts 75.6 us against 61.7), and the
+    // last spans, which may be short, behind the others.  Where all are on the card
+    // at once, two a CU, the second ones from the shortest up (426 us against 419).
+    const int pairs = a.batch * a.c.kv_heads, total = pairs * a.tiles;
+    int id = (int)blockIdx.x % total;
+    const int split = (int)blockIdx.x / total;
+    if (id >= 256 && total <= 512) id = total - 1 - (id - 256);
+    const int bg = id % pairs, tile = a.tiles - 1 - id / pairs;
     const int b = bg / a.c.kv_heads, g = bg - b * a.c.kv_heads;
     const SeqView sv = seq_view(a, b);
     const int nrows = sv.n * a.group, row0 = tile * kManyRows;
