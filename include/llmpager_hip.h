@@ -281,8 +281,10 @@ int lp_kv_append_paged(lp_ctx* ctx, const lp_kv_cache* cache, uint64_t q, int q_
  * larger length is taken as max_seq (or as what the table's width holds).  The
  * bounds decide how the work is split, so a capture may be replayed with other
  * q_starts, seq_lens and tables within them.  q and out: f32 rows as above,
- * which must not overlap.  workspace: lp_attn_paged_ws_bytes bytes, 256-byte
- * aligned (0 bytes: may be 0); two calls that overlap need one each. */
+ * which must not overlap.  The products take q scale log2(e) as two fp16 images:
+ * below 2^16.  Scales in q4 pages are finite, as the append leaves them.
+ * workspace: lp_attn_paged_ws_bytes bytes, 256-byte aligned (0 bytes: may be 0);
+ * two calls that overlap, replays of graphs among them, need one each. */
 uint64_t lp_attn_paged_ws_bytes(const lp_kv_cache* cache, int heads, int batch, int tokens, int max_q, int max_seq);
 int lp_attn_paged(lp_ctx* ctx, const lp_kv_cache* cache, uint64_t q, int q_stride, uint64_t out, int out_stride,
                   int heads, uint64_t q_starts, uint64_t seq_lens, int batch, int tokens, int max_q, int max_seq,
@@ -300,7 +302,7 @@ int lp_attn_paged(lp_ctx* ctx, const lp_kv_cache* cache, uint64_t q, int q_strid
  * or with nothing but -inf has NaN for its log probabilities and entropy; its
  * ids are those of its numbers, and -1 where they end.  workspace:
  * lp_logprobs_ws_bytes bytes, 256-byte aligned (0 bytes: may be 0); two calls
- * that overlap need one each. */
+ * that overlap, replays of graphs among them, need one each. */
 uint64_t lp_logprobs_ws_bytes(int rows, int vocab, int top);
 int lp_logprobs(lp_ctx* ctx, uint64_t logits, int stride, int rows, int vocab, uint64_t targets, uint64_t logp,
                 uint64_t entropy, int top, uint64_t ids, uint64_t top_logp, uint64_t workspace, uint64_t ws_bytes,

@@ -198,7 +198,7 @@ struct Best : Keys {
 #pragma unroll
         for (int bit = 31; bit >= 12; --bit) {
             const uint32_t t = at | 1u << bit;
-            at = __popcll(__ballot(m1 >= t)) + __popcll(__ballot(m2 >= t)) >= top ? t : at;
+            at = (int)(__popcll(__ballot(m1 >= t)) + __popcll(__ballot(m2 >= t))) >= top ? t : at;
         }
         return at;
     }
@@ -435,3 +435,9 @@ __device__ __forceinline__ void logprobs_body(const LogprobArgs& a) {
 
 extern "C" __global__ void __launch_bounds__(256) lp_logprobs(const LogprobArgs a) { logprobs_body<false>(a); }
 extern "C" __global__ void __launch_bounds__(256) lp_logprobs_top(const LogprobArgs a) { logprobs_body<true>(a); }
+
+// Arrival counters that are not a stream's own, before the launch that counts.
+extern "C" __global__ void __launch_bounds__(256) lp_clear_words(const ClearArgs a) {
+    const int i = (int)(blockIdx.x * 256 + threadIdx.x);
+    if (i < a.n) agent_store(reinterpret_cast<int*>(a.at) + i, 0);
+}

@@ -516,7 +516,7 @@ __device__ __forceinline__ void few_part(const AttnPagedArgs& a, uint8_t* lds, c
     auto send_scales = [&](uint64_t pool, int c, uint32_t at) {
 #pragma unroll
         for (int p = 0; p < SP; ++p) {
-            const int r = (lane + 64 * p) / SP;  // dwords of 2 G bytes a row
+            const int r = (lane + 64 * p) / (SP ? SP : 1);  // dwords of 2 G bytes a row
             const int page = SP == 2 ? (lane & 32 ? page_of_block(2 * p + 1) : page_of_block(2 * p)) : pg;
             lds_copy4(pool + page_off(page) + (uint32_t)((c + r) & pmask) * (G * 2) + (SP == 2 ? 4 * (lane & 1) : 0), at + 256 * p);
         }

@@ -381,6 +381,11 @@ struct LogprobArgs {
 };
 LPK_HD constexpr int logprob_rec(int top) { return 32 + 8 * top; }
 
+struct ClearArgs {
+    uint64_t at;  // 32-bit words to be 0
+    int32_t n, pad0;
+};
+
 // ---- fused MoE layer ---------------------------------------------------------
 
 // Device-side view of one MoE layer's routing and expert tables.

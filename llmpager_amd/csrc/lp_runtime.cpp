@@ -148,6 +148,7 @@ enum Fn {
     kAttnJoinD128,
     kLogprobs,
     kLogprobsTop,
+    kClearWords,
     kNumFns
 };
 
@@ -210,6 +211,7 @@ const FnSpec kSpecs[kNumFns] = {
     {"lp_paged.hsaco", "lp_attn_few_q4_d64_n2"}, {"lp_paged.hsaco", "lp_attn_few_q4_d128_n2"},
     {"lp_paged.hsaco", "lp_attn_join_d64"}, {"lp_paged.hsaco", "lp_attn_join_d128"},
     {"lp_logits.hsaco", "lp_logprobs"},      {"lp_logits.hsaco", "lp_logprobs_top"},
+    {"lp_logits.hsaco", "lp_clear_words"},
 };
 
 const char* const kModules[] = {"lp_basic.hsaco", "lp_moe.hsaco", "lp_gemm.hsaco", "lp_attn.hsaco",
@@ -1161,8 +1163,35 @@ struct PagedPlan {
     int max_q, max_seq, rows;
     int shares, min_units;    // few query rows
     int tiles, span, splits;  // many
-    uint64_t bytes;  // of the records
+    uint64_t bytes;           // of the records and, with shares, the pairs' counters
 };
+
+// Records, and behind them `counters` arrival counters.
+static uint64_t counters_at(uint64_t records) { return (records + 63) / 64 * 64; }
+static uint64_t with_counters(uint64_t records, int counters) { return counters_at(records) + (uint64_t)counters * kPagedStride * 4; }
+
+// The arrival counters of a call whose last workgroups join the others' parts: its
+// stream's, zero between launches.  But what the caller captures into a graph may
+// be replayed beside other calls of that stream and other graphs captured from it,
+// and a stream may be one more than the context has counters for: there they are
+// the workspace's, cleared by a launch of its own.
+static int join_counters(lp_ctx* c, lp_stream s, uint64_t at, int n, uint64_t* sync) {
+    bool ours;
+    {
+        std::lock_guard<std::mutex> g(c->sync_mu);
+        ours = c->cap_slot >= 0 && c->cap_stream == (hipStream_t)s;
+    }
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    if (!ours && hipStreamIsCapturing((hipStream_t)s, &st) != hipSuccess) (void)hipGetLastError();
+    const int slot = ours || st == hipStreamCaptureStatusNone ? sync_slot(c, s) : -1;
+    if (slot >= 0) {
+        *sync = sync_words(c, slot) + kPagedSync * 4;
+        return LP_OK;
+    }
+    *sync = at;
+    ClearArgs a{at, n * kPagedStride, 0};
+    return launch(c, kClearWords, dim3((unsigned)((a.n + 255) / 256)), dim3(256), 0, s, a);
+}
 
 static PagedPlan paged_plan(const lp_kv_cache* c, int heads, int batch, int tokens, int max_q, int max_seq) {
     PagedPlan p{};
@@ -1180,7 +1209,7 @@ static PagedPlan paged_plan(const lp_kv_cache* c, int heads, int batch, int toke
         // 256 shares 44; 64 of 16 bits: 70 us, 768 shares 76)
         if (pairs <= kPagedPairs && batch <= kFewBatch && units > 1)
             p.shares = (int)std::min<int64_t>(std::max(512, pairs), (int64_t)pairs * units);
-        p.bytes = (uint64_t)p.shares * p.rows * (c->head_dim * 4 + 8);
+        if (p.shares) p.bytes = with_counters((uint64_t)p.shares * p.rows * (c->head_dim * 4 + 8), pairs);
     } else {
         p.tiles = (p.rows + kManyRows - 1) / kManyRows;
         paged_spans((int64_t)pairs * p.tiles, p.max_seq, &p.span, &p.splits);
@@ -1191,7 +1220,7 @@ static PagedPlan paged_plan(const lp_kv_cache* c, int heads, int batch, int toke
 
 // One query row per (token, query head): their number per KV head and its
 // products with the sequences stay within 32 bits.
-static int check_queries(const lp_kv_cache* c, int heads, int batch, int tokens, int max_q, int max_seq) {
+static int check_queries(int heads, int batch, int tokens, int max_q, int max_seq) {
     if (max_q < 0 || max_seq < 0) return fail(LP_E_INVALID, "attn_paged: negative max_q or max_seq");
     if ((int64_t)batch * std::min(max_q, tokens) * heads > INT32_MAX / 256)
         return fail(LP_E_UNSUPPORTED, "attn_paged: batch x max_q x heads must be below 2^23");
@@ -1201,7 +1230,7 @@ static int check_queries(const lp_kv_cache* c, int heads, int batch, int tokens,
 uint64_t lp_attn_paged_ws_bytes(const lp_kv_cache* cache, int heads, int batch, int tokens, int max_q, int max_seq) {
     PagedCache pc;
     if (check_paged("attn_paged", cache, &pc) || check_batch("attn_paged", heads, cache->kv_heads, batch, tokens, 4, 4) ||
-        check_queries(cache, heads, batch, tokens, max_q, max_seq))
+        check_queries(heads, batch, tokens, max_q, max_seq))
         return 0;
     return paged_plan(cache, heads, batch, tokens, max_q, max_seq).bytes;
 }
@@ -1228,7 +1257,7 @@ int lp_attn_paged(lp_ctx* c, const lp_kv_cache* cache, uint64_t q, int q_stride,
     if (int r = check_rows("attn_paged: q", q, q_stride, (int64_t)heads * D)) return r;
     if (int r = check_rows("attn_paged: out", out, out_stride, (int64_t)heads * D)) return r;
     if (q == out) return fail(LP_E_INVALID, "attn_paged: out must not be q");
-    if (int r = check_queries(cache, heads, batch, tokens, max_q, max_seq)) return r;
+    if (int r = check_queries(heads, batch, tokens, max_q, max_seq)) return r;
     const PagedPlan plan = paged_plan(cache, heads, batch, tokens, max_q, max_seq);
     if (int r = check_workspace("attn_paged", plan.bytes, workspace, ws_bytes)) return r;
     if (int r = check_ctx(c)) return r;
@@ -1241,11 +1270,10 @@ int lp_attn_paged(lp_ctx* c, const lp_kv_cache* cache, uint64_t q, int q_stride,
     a.scale = scale;
     const int pairs = batch * cache->kv_heads, which = (cache->format == LP_KV_Q4 ? 2 : 0) + (D == 128 ? 1 : 0);
     if (plan.rows <= kFewRows) {
-        // without counters of this stream, or with more pairs than there are: a
-        // workgroup per pair
-        const int slot = plan.shares ? sync_slot(c, s) : -1;
-        a.shares = slot >= 0 ? plan.shares : 0, a.min_units = plan.min_units;
-        a.sync = slot >= 0 ? sync_words(c, slot) + kPagedSync * 4 : 0;
+        // (no shares, with more pairs than there are counters: a workgroup per pair)
+        a.shares = plan.shares, a.min_units = plan.min_units;
+        if (a.shares)
+            if (int r = join_counters(c, s, workspace + plan.bytes - (uint64_t)pairs * kPagedStride * 4, pairs, &a.sync)) return r;
         const Fn f = (Fn)(kAttnFewF16D64 + (plan.rows > 16 ? 4 : 0) + which);
         return launch(c, f, dim3((unsigned)(a.shares ? a.shares : pairs)), dim3(256), 0, s, a);
     }
@@ -1275,7 +1303,7 @@ uint64_t lp_logprobs_ws_bytes(int rows, int vocab, int top) {
     if (rows <= 0 || vocab <= 0 || vocab > kLogprobMaxVocab || top < 0 || top > kLogprobMaxTop) return 0;
     int parts, per;
     logprob_parts(rows, vocab, &parts, &per);
-    return parts > 1 ? (uint64_t)rows * parts * logprob_rec(top) : 0;
+    return parts > 1 ? with_counters((uint64_t)rows * parts * logprob_rec(top), rows) : 0;
 }
 
 int lp_logprobs(lp_ctx* c, uint64_t logits, int stride, int rows, int vocab, uint64_t targets, uint64_t logp,
@@ -1293,16 +1321,10 @@ int lp_logprobs(lp_ctx* c, uint64_t logits, int stride, int rows, int vocab, uin
     if (!rows) return LP_OK;
     LogprobArgs a{logits, targets, logp, entropy, ids, top_logp, workspace, 0, stride, rows, vocab, top, 1, 0};
     logprob_parts(rows, vocab, &a.parts, &a.per_part);
-    if (a.parts > 1) {
-        // (parts only while rows are few: below the counters' number)
-        const int slot = sync_slot(c, s);
-        if (slot >= 0)
-            a.sync = sync_words(c, slot) + kPagedSync * 4;
-        else
-            a.per_part *= a.parts, a.parts = 1;
-    }
     const int64_t wgs = (int64_t)rows * a.parts;
     if (wgs > INT32_MAX / 256) return fail(LP_E_UNSUPPORTED, "logprobs: too many rows");
+    if (a.parts > 1)  // (only while rows are few: below the counters' number)
+        if (int r = join_counters(c, s, workspace + counters_at((uint64_t)wgs * logprob_rec(top)), rows, &a.sync)) return r;
     return launch(c, top ? kLogprobsTop : kLogprobs, dim3((unsigned)wgs), dim3(256), 0, s, a);
 }
 

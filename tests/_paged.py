@@ -2,6 +2,8 @@
 the paged append, attention and log probability tests check against."""
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 
 import llmpager_amd as lp
@@ -187,3 +189,32 @@ def logprobs(x, targets, top):
     tp = np.take_along_axis(p, ids, 1)
     gone = np.isnan(np.take_along_axis(x, ids, 1))
     return logp, ent, np.where(gone, -1, ids), np.where(gone, np.nan, tp)
+
+
+class HipGraph:
+    """What `launches(stream)` does, captured through the HIP runtime itself, as a
+    program with graphs of its own does (not lp_graph_capture_*)."""
+
+    _hip = None
+
+    def __init__(self, stream, launches):
+        if HipGraph._hip is None:  # the runtime that the library has loaded
+            with open("/proc/self/maps") as f:
+                HipGraph._hip = ctypes.CDLL(next(x.split()[-1] for x in f if "libamdhip64" in x))
+        self.graph, self.exec = ctypes.c_void_p(), ctypes.c_void_p()
+        self._call("hipStreamBeginCapture", ctypes.c_void_p(stream), 2)  # relaxed
+        try:
+            launches(stream)
+        finally:
+            self._call("hipStreamEndCapture", ctypes.c_void_p(stream), ctypes.byref(self.graph))
+        self._call("hipGraphInstantiate", ctypes.byref(self.exec), self.graph, None, None, ctypes.c_size_t(0))
+
+    def _call(self, name, *args):
+        assert getattr(self._hip, name)(*args) == 0, name
+
+    def launch(self, stream):
+        self._call("hipGraphLaunch", self.exec, ctypes.c_void_p(stream))
+
+    def close(self):
+        self._call("hipGraphExecDestroy", self.exec)
+        self._call("hipGraphDestroy", self.graph)

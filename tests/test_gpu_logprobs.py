@@ -9,7 +9,7 @@ import numpy as np
 import pytest
 
 import llmpager_amd as lp
-from _paged import logprobs
+from _paged import HipGraph, logprobs
 
 pytestmark = pytest.mark.gpu
 
@@ -182,3 +182,67 @@ def test_captured(cuda, K):
     cuda.destroy_stream(s)
     for p in (dx, dt, dl, de, di, dp, ws):
         cuda.free_device(p)
+
+
+@pytest.mark.parametrize("rows,vocab,top", [(2100, 4200, 2), (1024, 8300, 1), (1025, 9000, 64), (64, 33000, 64)])
+def test_many_rows(cuda, K, rows, vocab, top):
+    """Rows in parts and whole, around the number that have counters."""
+    rng = np.random.default_rng(rows)
+    x = rng.standard_normal((rows, vocab)).astype(np.float32)
+    _check(cuda, K, x, rng.integers(0, vocab, rows), top)
+
+
+@pytest.mark.parametrize("top", [1, 20, 64])
+def test_best_logits_in_one_place(cuda, K, top):
+    """The largest all in one lane's logits, in one block, and in a row's last part."""
+    rng = np.random.default_rng(top)
+    x = rng.standard_normal((4, 70001)).astype(np.float32)
+    x[0, 8192:8192 + 4 * 64 * 16:256] += 50   # one lane's, 16 blocks
+    x[1, 4096:4096 + 100] += np.arange(100, dtype=np.float32)
+    x[2, -80:] = 30
+    x[3, :] = np.float32(-2.5)                # all equal
+    _check(cuda, K, x, [8192, 4196, 70000, 0], top)
+
+
+def test_graphs_of_one_stream_replayed_at_once(cuda, K):
+    """Two graphs that the program captured itself from one stream, replayed on two
+    others beside eager calls on that stream."""
+    rng = np.random.default_rng(8)
+    R, V, top = 3, 90001, 12
+    xs = [rng.standard_normal((R, V)).astype(np.float32) for _ in range(3)]
+    mem = []
+    for x in xs:
+        mem.append([cuda.upload(x), cuda.upload(np.arange(R, dtype=np.int32))] +
+                   [cuda.alloc_device(n) for n in (R * 4, R * 4, R * top * 4, R * top * 4, K.logprobs_ws_bytes(R, V, top))])
+    cuda.sync()
+
+    def launch(i, stream):
+        dx, dt, dl, de, di, dp, ws = mem[i]
+        for _ in range(3):
+            K.logprobs(dx, V, R, V, dt, dl, de, top, di, dp, ws, stream, ws_bytes=ws.nbytes)
+
+    s, s0, s1 = (cuda.stream() for _ in range(3))
+    g0, g1 = (HipGraph(s, lambda st, i=i: launch(i, st)) for i in range(2))
+    for _ in range(4):
+        for m in mem:
+            cuda.htod_async(m[4], np.full((R, top), 7, np.int32), s)
+        cuda.sync()
+        for _ in range(5):
+            g0.launch(s0)
+            g1.launch(s1)
+            launch(2, s)
+        for st in (s, s0, s1):
+            cuda.sync_stream(st)
+        for x, m in zip(xs, mem):
+            wl, we, wi, wt = logprobs(x, np.arange(R), top)
+            _same(cuda.download(m[2], (R,), np.float32), wl)
+            _same(cuda.download(m[3], (R,), np.float32), we)
+            assert np.array_equal(cuda.download(m[4], (R, top), np.int32), wi)
+            _same(cuda.download(m[5], (R, top), np.float32), wt)
+    g0.close()
+    g1.close()
+    for st in (s, s0, s1):
+        cuda.destroy_stream(st)
+    for m in mem:
+        for p in m:
+            cuda.free_device(p)

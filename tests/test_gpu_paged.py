@@ -14,7 +14,7 @@ import numpy as np
 import pytest
 
 import llmpager_amd as lp
-from _paged import Batch, q4
+from _paged import Batch, HipGraph, q4
 
 pytestmark = pytest.mark.gpu
 
@@ -430,4 +430,100 @@ def test_captured_step_replayed_with_other_lengths(cuda, K, fmt):
         assert np.array_equal(cuda.download(do, (batch, heads, dim), np.float32, s), out)
     g.close()
     cuda.destroy_stream(s)
+    B.free()
+
+
+@FORMATS
+@pytest.mark.parametrize("new,past,heads,kv", [
+    ([1] * 70, [11 * b for b in range(70)], 4, 2),          # more sequences than lanes
+    ([1 + b % 3 for b in range(130)], [b for b in range(130)], 8, 1),
+    ([1] * 1030, [b % 90 for b in range(1030)], 2, 1),      # more than share their contexts out
+    ([1] * 600, [b % 50 for b in range(600)], 4, 4),        # more (sequence, KV head)s than have counters
+    ([20 + b % 7 for b in range(66)], [3 * b for b in range(66)], 8, 2),
+])
+def test_attention_many_sequences(cuda, K, fmt, new, past, heads, kv):
+    _check_attn(K, Batch(cuda, new, past, heads, kv, 64, 16, fmt, seed=len(new)))
+
+
+@FORMATS
+@pytest.mark.parametrize("new,past", [([9, 40], [3000, 1500]), ([70, 33], [4100, 64]), ([64], [6000]), ([128], [191])])
+def test_attention_many_rows_of_long_contexts(cuda, K, fmt, new, past):
+    """Contexts in spans that end inside a sequence and behind the shorter one."""
+    _check_attn(K, Batch(cuda, new, past, 8, 2, 128, 32, fmt, seed=40))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new,past", [([48], [2000]), ([130], [500])])
+def test_attention_seen_rows_that_are_no_numbers(cuda, K, dim, new, past):
+    """Infinities in a value row that the later tokens see and the earlier do not,
+    among them two of one column with opposite signs; a value row of NaN that all
+    see in some columns."""
+    B = Batch(cuda, new, past, 8, 2, dim, 16, lp.KV_F16, seed=41)
+    v = np.ones((2, dim), np.float16)
+    v[:, 3], v[:, 7] = np.inf, -np.inf
+    B.put(past[0] + 20, None, v)
+    w = np.zeros((2, dim), np.float16)
+    w[:, 7] = np.inf
+    B.put(past[0] + 30, None, w)
+    u = np.zeros((2, dim), np.float16)
+    u[0, 5] = np.nan
+    B.put(100, None, u)
+    _check_attn(K, B)
+
+
+@pytest.mark.parametrize("new,past", [([1, 1], [3000, 40]), ([3, 30], [900, 70])])
+def test_graphs_of_one_stream_replayed_at_once(cuda, K, new, past):
+    """Two graphs that the program captured itself from one stream, replayed on two
+    others beside eager calls on that stream: three workspaces, nothing else shared."""
+    Bs = [Batch(cuda, new, past, 8, 2, 128, 32, lp.KV_Q4, seed=50 + i) for i in range(3)]
+    qs = [_queries(B) for B in Bs]
+    W, mq, ms = 8 * 128, max(new), max(Bs[0].lens)
+    args = []
+    for B, q in zip(Bs, qs):
+        B.device()
+        args.append((B.up(q), B.alloc(B.tokens * W * 4), B.alloc(K.attn_paged_ws_bytes(B.cache, 8, B.batch, B.tokens, mq, ms))))
+    cuda.sync()
+
+    def launch(i, stream):
+        B, (dq, do, ws) = Bs[i], args[i]
+        for _ in range(3):
+            K.attn_paged(B.cache, dq, W, do, W, 8, B.dstarts, B.dlens, B.batch, B.tokens, mq, ms, 1.0 / np.sqrt(128.0), ws,
+                         stream, ws_bytes=ws.nbytes)
+
+    s, s0, s1 = (cuda.stream() for _ in range(3))
+    g0, g1 = (HipGraph(s, lambda st, i=i: launch(i, st)) for i in range(2))
+    want = [B.attention(q.reshape(B.tokens, 8, 128), 1.0 / np.sqrt(128.0)) for B, q in zip(Bs, qs)]
+    for _ in range(4):
+        for B, (_, do, _) in zip(Bs, args):
+            cuda.htod_async(do, np.full((B.tokens, W), 7, np.float32), s)
+        cuda.sync()
+        for _ in range(5):
+            g0.launch(s0)
+            g1.launch(s1)
+            launch(2, s)
+        for st in (s, s0, s1):
+            cuda.sync_stream(st)
+        for B, (_, do, _), w in zip(Bs, args, want):
+            _close(cuda.download(do, (B.tokens, 8, 128), np.float32), w)
+    g0.close()
+    g1.close()
+    for st in (s, s0, s1):
+        cuda.destroy_stream(st)
+    for B in Bs:
+        B.free()
+
+
+def test_attention_on_more_streams_than_have_counters(cuda, K):
+    """The same bits on 70 streams, whether the counters are a stream's or the
+    workspace's."""
+    B = Batch(cuda, [1, 1], [2500, 300], 8, 2, 128, 16, lp.KV_Q4, seed=52)
+    q = _queries(B)
+    B.device()
+    streams = [cuda.stream() for _ in range(70)]
+    outs = [_attn(K, B, q, stream=s) for s in streams]
+    _close(outs[0].reshape(2, 8, 128), B.attention(q.reshape(2, 8, 128), 1.0 / np.sqrt(128.0)))
+    for o in outs[1:]:
+        assert np.array_equal(o, outs[0])
+    for s in streams:
+        cuda.destroy_stream(s)
     B.free()
