@@ -32,13 +32,12 @@ constexpr int kStepSyncAttn = 17 * kSyncStride;
 constexpr int kStepSyncGemv = kStepSyncAttn + kAttnFusedMaxKvHeads * kSyncStride;
 constexpr int kStepSyncDone = kStepSyncGemv + kSyncStride;  // KV (or query) heads complete
 constexpr int kStepSyncErr = kStepSyncDone + kSyncStride;   // waits that gave up (lp_step_errors_sync)
-// then one per (sequence, KV head) of paged attention, or row of log probabilities,
-// whose parts workgroups share: 64 bytes apart (1,184 arrivals at 32 words of one
-// line took 10 us)
-constexpr int kPagedSync = kStepSyncErr + kSyncStride;
+constexpr int kSyncWords = kStepSyncErr + kSyncStride;
+// and of their own, one per (sequence, KV head) of paged attention or row of log
+// probabilities whose parts workgroups share: 64 bytes apart (1,184 arrivals at 32
+// words of one line took 10 us)
 constexpr int kPagedStride = 16;
 constexpr int kPagedPairs = 1024;
-constexpr int kSyncWords = kPagedSync + kPagedPairs * kPagedStride;
 constexpr int kMaxTopK = 16;           // largest top_k the device router accepts
 constexpr int kMaxExperts = 1024;      // largest expert count the device router accepts
 constexpr int kTopkFusedMaxT = 8;      // largest T routed by the one-workgroup top-k + dispatch kernel

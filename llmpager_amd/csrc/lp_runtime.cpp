@@ -266,6 +266,7 @@ struct lp_ctx {
     // destroying the capture stream and routing on a stream created later
     // never shares counters with the graph's replays.
     int32_t* sync = nullptr;
+    int32_t* join_sync = nullptr;  // a slot's kPagedPairs counters of join_counters, zero between launches too
     std::mutex sync_mu;
     hipStream_t sync_owner[kSyncSlots] = {};  // slot i belongs to sync_owner[i] when sync_used[i]
     bool sync_used[kSyncSlots] = {};
@@ -445,6 +446,9 @@ int lp_init(int device, const char* hsaco_dir, lp_ctx** out) {
     }
     e = hipMalloc(reinterpret_cast<void**>(&c->sync), (size_t)kSyncSlots * kSyncWords * 4);
     if (e == hipSuccess) e = hipMemset(c->sync, 0, (size_t)kSyncSlots * kSyncWords * 4);
+    const size_t joins = (size_t)kSyncSlots * kPagedPairs * kPagedStride * 4;
+    if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void**>(&c->join_sync), joins);
+    if (e == hipSuccess) e = hipMemset(c->join_sync, 0, joins);
     if (e == hipSuccess) e = hipDeviceSynchronize();
     if (e != hipSuccess) {
         lp_destroy(c);
@@ -466,6 +470,7 @@ void lp_destroy(lp_ctx* c) {
     if (c->sync) {
         (void)hipDeviceSynchronize();
         (void)hipFree(c->sync);
+        (void)hipFree(c->join_sync);
     }
     delete c;
 }
@@ -1185,7 +1190,7 @@ static int join_counters(lp_ctx* c, lp_stream s, uint64_t at, int n, uint64_t* s
     if (!ours && hipStreamIsCapturing((hipStream_t)s, &st) != hipSuccess) (void)hipGetLastError();
     const int slot = ours || st == hipStreamCaptureStatusNone ? sync_slot(c, s) : -1;
     if (slot >= 0) {
-        *sync = sync_words(c, slot) + kPagedSync * 4;
+        *sync = reinterpret_cast<uint64_t>(c->join_sync) + (uint64_t)slot * kPagedPairs * kPagedStride * 4;
         return LP_OK;
     }
     *sync = at;
