@@ -16,8 +16,8 @@
 // that the lanes' two largest do not rule out.  Keys are put in one by one where
 // they are few, else sorted 64 at a time across the lanes.
 //
-// A row's parts are joined by the workgroup that ends last.  2,048 rows of 49,152
-// without alternatives take 93 us, 5.1 TB/s: a copy's rate.  32 rows of 151,936
+// A row's parts are joined by the workgroup that ends last.  777 rows of 151,936
+// without alternatives take 91 us, 5.2 TB/s: a copy's rate.  32 rows of 151,936
 // take 10 us without alternatives, 16 with one, 20 with twenty and 35 with 64; one
 // such row 6 and 10 to 15: there the chain of a block's load, its exponentials,
 // the sort and the join counts, 1 to 3 us each.

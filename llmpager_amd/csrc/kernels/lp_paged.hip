@@ -1,7 +1,7 @@
 // gfx950 kernels of a batch's KV cache in pages: the new tokens' queries and
 // keys normed per head and rotated with keys and values written into their
 // pages (lp_kv_append_*), and attention of one or many new tokens a sequence
-// over its pages (lp_attn_paged_*).
+// over its pages (lp_attn_few_*, lp_attn_many_* and lp_attn_join_*).
 //
 // A page holds page_rows rows of one KV head, as fp16 [page_rows, head_dim] or
 // as a q4 region (f16 scales [page_rows, head_dim / 32], then nibbles
@@ -134,7 +134,7 @@ __device__ __forceinline__ int sequence_of(uint64_t q_starts, int batch, int tok
 // far position needs it, and a 4-bit code then is that of the exact value
 // whatever the order of the sums.  Vector fp64 runs at fp32's rate here, but
 // its divisions, square roots and sines are long: they are short series and
-// Newton steps from fp32 (2,115 tokens of 32 + 2 x 4 heads into 4-bit pages, 100
+// Newton steps from fp32 (2,404 tokens of 32 + 2 x 4 heads into 4-bit pages, 100
 // MB in all: 41 us with the library's, 27.4 with these, 3.6 TB/s).
 // ---------------------------------------------------------------------------
 // (by value: a choice between members of a block makes the compiler keep it in memory)
@@ -371,7 +371,7 @@ __device__ __forceinline__ uint64_t rec_sums(const AttnPagedArgs& a) {
 //            has; the waits count what was sent for since.  The pages of the
 //            next chunks are looked up together, 64 blocks of 16 rows at a time.
 //   scores   S^T = K Q^T on v_mfma_f32_16x16x32_f16: cache rows as M, the query
-//            rows as N, as fp16 hi + lo images of q scale log2 e (2^-21 of it is
+//            rows as N, as fp16 hi + lo images of q scale log2 e (2^-22 of it is
 //            left out), two MFMAs a step, begun at minus the running maximum.
 //   softmax  lane (query n, kb) holds rows 16 t + 4 kb + v of the chunk, so e^ of
 //            them stays in the lane; the running maximum is raised only when a
@@ -393,6 +393,12 @@ __device__ __forceinline__ uint64_t rec_sums(const AttnPagedArgs& a) {
 // zeroed.  fp16 rows that only some of the queries see (several new tokens) may
 // hold NaN or infinity, which zero probabilities would not keep out: a chunk
 // with one is added row by row.
+//
+// The cache's bytes bound it, the launch and a workgroup's chain of round trips
+// (lengths, pages, first rows, join) where they are few: 64 sequences of up to
+// 4,000 16-bit rows 70 us, 4.6 TB/s; 32 of up to 8,192 4-bit rows 31 us, 3.2 TB/s
+// with some 9 us before the first and after the last row, 5.2 in between; one of
+// 1,500 rows 10.5 us.
 // ---------------------------------------------------------------------------
 template <int D, bool Q4>
 struct Few {
@@ -965,10 +971,12 @@ LP_ATTN_FEW(q4_d128_n2, 1, 128, true, 2)
 // What would hold the accumulators twice, a branch that computes them in another
 // way, stays out of the loop.
 //
-// 2,048 tokens of 32 heads behind 6,000 rows of 16 bits: 419 us, 563 TFLOP/s of the
-// formula's and twice that of MFMA work, what a large fp16 product reaches; 12 x 80
-// query rows of 4 heads behind 6,000 rows of 4 bits: 36 us, of which a chunk takes
-// about 3 us and the launch with what comes before the first one 10.
+// 2,048 tokens of 32 heads on 4 KV heads behind 6,001 rows of 16 bits: 423 us, 557
+// TFLOP/s of the formula's and twice that of MFMA work, what a large fp16 product
+// reaches; 12 sequences of up to 5 tokens, 16 heads to a KV head, behind up to
+// 6,000 rows of 4 bits: 36 us, of which a chunk takes about 3 us and the launch with
+// what comes before the first one 10; six prompts of up to 700 tokens, 32 heads on
+// 4: 52 us, the longest one's last tiles.
 // ---------------------------------------------------------------------------
 namespace {
 

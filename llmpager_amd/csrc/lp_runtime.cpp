@@ -1142,7 +1142,7 @@ int lp_kv_append_paged(lp_ctx* c, const lp_kv_cache* cache, uint64_t q, int q_st
     const int rows = heads + 2 * cache->kv_heads, per = 256 / D;  // rows a wave takes at a time
     // Waves that share a token's rows: one pass each while the tokens are few,
     // else about 8192 in all, so that the angles are made less often and a
-    // wave's next rows load behind its present ones (2,115 tokens of 32 + 2 x 4
+    // wave's next rows load behind its present ones (2,404 tokens of 32 + 2 x 4
     // heads: 8,192 waves 27.4 us, 24,576 32.6).
     const int want = std::max(1, std::min(8192 / tokens, (rows + per - 1) / per));
     a.rows_per_part = ((rows + want - 1) / want + per - 1) / per * per;
@@ -1156,8 +1156,8 @@ int lp_kv_append_paged(lp_ctx* c, const lp_kv_cache* cache, uint64_t q, int q_st
 
 // How attention of many query rows is split over the rows of a context: into
 // spans of whole chunks of 64, as long as `wgs` workgroups of them are about 512
-// in all, and at most kPagedMaxSplits spans.  (48 tiles of 6,000 rows: 11 spans of
-// up to 9 chunks 36 us, 10 of up to 10 38.6.)
+// in all, and at most kPagedMaxSplits spans.  (48 tiles, up to 6,005 rows: 11 spans
+// of up to 9 chunks 36 us, 10 of up to 10 38.6.)
 static void paged_spans(int64_t wgs, int max_seq, int* span, int* splits) {
     const int64_t each = std::max((wgs * max_seq + 511) / 512, ((int64_t)max_seq + kPagedMaxSplits - 1) / kPagedMaxSplits);
     *span = (int)std::min<int64_t>((std::max<int64_t>(each, 1) + 63) / 64 * 64, INT32_MAX / 64 * 64);
@@ -1210,8 +1210,8 @@ static PagedPlan paged_plan(const lp_kv_cache* c, int heads, int batch, int toke
         const int unit = c->format == LP_KV_Q4 ? 256 : 128;
         const int units = std::max(1, (p.max_seq + unit - 1) / unit);
         p.min_units = (units + kFewParts - 1) / kFewParts;
-        // 512 shares, two workgroups a CU (32 contexts of 4 bits, 18,000 rows: 33 us,
-        // 256 shares 44; 64 of 16 bits: 70 us, 768 shares 76)
+        // 512 shares, two workgroups a CU (32 contexts of up to 8,192 4-bit rows: 33 us,
+        // 256 shares 44; 64 of up to 4,001 16-bit ones: 70 us, 768 shares 76)
         if (pairs <= kPagedPairs && batch <= kFewBatch && units > 1)
             p.shares = (int)std::min<int64_t>(std::max(512, pairs), (int64_t)pairs * units);
         if (p.shares) p.bytes = with_counters((uint64_t)p.shares * p.rows * (c->head_dim * 4 + 8), pairs);
