@@ -140,7 +140,16 @@ __device__ __forceinline__ uint32_t xor_lane(uint32_t v) {
     if constexpr (X == 7) return dpp(v, std::integral_constant<int, 0x141>());   // mirrored within eight
     if constexpr (X == 8) return dpp(v, std::integral_constant<int, 0x128>());   // rotated within a row of 16
     if constexpr (X == 15) return dpp(v, std::integral_constant<int, 0x140>());  // mirrored within a row
-    return (uint32_t)__shfl_xor((int)v, X, 64);
+    if constexpr (X == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return lane_id() & 16 ? r[0] : r[1];
+    }
+    if constexpr (X == 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return lane_id() & 32 ? r[0] : r[1];
+    }
+    if constexpr (X == 31) return xor_lane<16>(xor_lane<15>(v));
+    if constexpr (X == 63) return xor_lane<32>(xor_lane<31>(v));
 }
 
 // A key per lane: value key, then ~id; 0: none.
@@ -234,7 +243,10 @@ struct Best : Keys {
             Keys k;
             k.hi = (uint32_t)(key >> 32), k.lo = (uint32_t)key;
             k.sort();
-            merge(k);
+            if (__builtin_amdgcn_readfirstlane((int)hi))
+                merge(k);
+            else
+                hi = k.hi, lo = k.lo;
             held = 0;
             __builtin_amdgcn_wave_barrier();
         };
