@@ -1032,9 +1032,14 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
 
     uint32_t kreg[W], vreg[W];
     uint32_t ks = 0, vs = 0;
-    auto page_for = [&](int c) {
-        const int p = page_of(a.c, b, min(c + srow, r1 - 1));
-        return c + srow < r1 ? p : -1;
+    // a row's page, asked for and, later, looked at: what asks waits for nothing
+    auto ask_page = [&](int c) {  // (r1 is within the table's width)
+        const uint32_t col = (uint32_t)(min(c + srow, r1 - 1) >> a.c.page_log2);
+        return gptr<int>(a.c.table)[(uint64_t)(uint32_t)b * (uint32_t)a.c.max_pages + col];
+    };
+    auto page_for = [&](int asked, int c) {
+        asm volatile("" : "+v"(asked));
+        return c + srow < r1 && (uint32_t)asked < (uint32_t)a.c.pages ? asked : -1;
     };
     auto load_rows = [&](uint32_t (&r)[W], uint32_t& s, uint64_t pool, int c, int pg) {
         const uint32_t pr = (uint32_t)((c + srow) & pmask);
@@ -1122,10 +1127,12 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
     };
     int pg = -1, pg1 = -1;  // of the chunk in the registers, and of the one after it
     if (r0 < r1) {
-        pg = page_for(r0);
+        pg = ask_page(r0);
+        const int next = ask_page(r0 + CR);
+        pg = page_for(pg, r0);
         load_rows(kreg, ks, a.c.k_pages, r0, pg);
         load_rows(vreg, vs, a.c.v_pages, r0, pg);
-        pg1 = page_for(r0 + CR);
+        pg1 = page_for(next, r0 + CR);
     }
 
     // ---- the wave's query rows
@@ -1172,14 +1179,15 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
         pg = pg1;
         load_rows(kreg, ks, a.c.k_pages, c, pg);
         load_rows(vreg, vs, a.c.v_pages, c, pg);
-        pg1 = page_for(c + CR);
     };
     const bool none = r0 >= r1;
     if (!none) {
         if (!Q4 && special(r0, pg)) mend(Finite(), r0, pg);
         store_rows(Finite(), 0, r0, pg);
+        const int next = ask_page(r0 + 2 * CR);
         load_next(r0 + CR);
         if (!Q4 && special(r0 + CR, pg)) mend(Finite(), r0 + CR, pg);
+        pg1 = page_for(next, r0 + 2 * CR);
         __syncthreads();
     }
     int buf = 0;
@@ -1254,6 +1262,7 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
         uint64_t there = ~0ull;
 #pragma unroll
         for (int i = 0; i < 4; ++i) there &= *(LP_LDS u64_any*)(ll + M::kFlags + buf * 32 + i * 8);
+        const int next = ask_page(c + 3 * CR);
         f32x16_t s0 = zero();
         store_begin(Finite(), buf ^ 1, c + CR, pg);
         step_end();
@@ -1313,6 +1322,7 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
             }
         }
         if (!Q4 && special(c + 2 * CR, pg)) mend(Finite(), c + 2 * CR, pg);
+        pg1 = page_for(next, c + 3 * CR);
         __syncthreads();
     }
     // ---- values that are no finite numbers: again, these alone, row by row and each
@@ -1328,7 +1338,7 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
         if (__builtin_amdgcn_readfirstlane(any))
 #pragma unroll 1
             for (int c = r0; c < r1; c += CR) {
-                pg = page_for(c);
+                pg = page_for(ask_page(c), c);
                 load_rows(kreg, ks, a.c.k_pages, c, pg);
                 load_rows(vreg, vs, a.c.v_pages, c, pg);
                 if (!Q4) mend(Odd(), c, pg);
