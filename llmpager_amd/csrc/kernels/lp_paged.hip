@@ -444,7 +444,7 @@ __device__ __forceinline__ int few_units(const SeqView& s, int unit) {
 // last.  They were written through to agent scope in this launch; the sums, whole
 // cache lines that nothing here has read before, are read as usual, maximum and
 // sum of a row, which share a line with other pairs', at agent scope.
-template <int D>
+template <int D, int NT>
 __device__ __forceinline__ void few_join(const AttnPagedArgs& a, uint8_t* lds, const SeqView& sv, int g, int nrows, int first, int S) {
     float* const wt = reinterpret_cast<float*>(lds);  // [row][kFewParts]
     const int wave = (int)(threadIdx.x >> 6), lane = lane_id();
@@ -462,16 +462,37 @@ __device__ __forceinline__ void few_join(const AttnPagedArgs& a, uint8_t* lds, c
         if (lane < S) wt[row * kFewParts + lane] = L == 0.0f ? 0.0f : f / L;
     }
     __syncthreads();
+    // all of a thread's pieces at once: their loads are what this takes
     constexpr int TR = D / 4;
-    for (int k = (int)threadIdx.x; k < nrows * TR; k += 256) {
-        const int row = k / TR, d4 = k % TR, i = row / a.group, h = g * a.group + (row - i * a.group);
-        f32x4_t A = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto pieces = [&](auto number) {
+        constexpr int N = decltype(number)::value;
+        f32x4_t A[N];
+        uint64_t from[N];
+        const float* w[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int k = (int)threadIdx.x + 256 * i, row = min(k / TR, nrows - 1);
+            A[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            from[i] = a.part + (uint64_t)(uint32_t)(first * a.rows + row) * (D * 4) + 16 * (k % TR);
+            w[i] = wt + row * kFewParts;
+        }
 #pragma unroll 8
         for (int s = 0; s < S; ++s)
-            A += gptr<f32x4_t>(a.part + (uint64_t)(uint32_t)((first + s) * a.rows + row) * (D * 4))[d4] * wt[row * kFewParts + s];
-        const uint64_t o = a.out + ((uint64_t)(uint32_t)(sv.t0 + i) * (uint32_t)a.out_stride + (uint32_t)(h * D)) * 4;
-        gptr_w<f32x4_t>(o)[d4] = A;
-    }
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                A[i] += gptr<f32x4_t>(from[i] + (uint64_t)(uint32_t)(s * a.rows) * (D * 4))[0] * w[i][s];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int k = (int)threadIdx.x + 256 * i, row = k / TR, t = row / a.group, h = g * a.group + (row - t * a.group);
+            if (row >= nrows) continue;
+            const uint64_t o = a.out + ((uint64_t)(uint32_t)(sv.t0 + t) * (uint32_t)a.out_stride + (uint32_t)(h * D)) * 4;
+            gptr_w<f32x4_t>(o)[k % TR] = A[i];
+        }
+    };
+    if (nrows * TR <= 256)
+        pieces(std::integral_constant<int, 1>());
+    else
+        pieces(std::integral_constant<int, 16 * NT * TR / 256>());
 }
 
 // One part of a pair: units [u0, u1) of (sequence view sv, KV head g).
@@ -933,7 +954,7 @@ __device__ __forceinline__ void few_body(const AttnPagedArgs& a) {
         flag = o;
     }
     __syncthreads();
-    if (flag == parts - 1) few_join<D>(a, lds, sv, g, sv.n * a.group, (int)blockIdx.x - part, parts);
+    if (flag == parts - 1) few_join<D, NT>(a, lds, sv, g, sv.n * a.group, (int)blockIdx.x - part, parts);
 }
 
 }  // namespace

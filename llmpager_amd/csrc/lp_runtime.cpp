@@ -1211,9 +1211,12 @@ static PagedPlan paged_plan(const lp_kv_cache* c, int heads, int batch, int toke
         const int units = std::max(1, (p.max_seq + unit - 1) / unit);
         p.min_units = (units + kFewParts - 1) / kFewParts;
         // 512 shares, two workgroups a CU (32 contexts of up to 8,192 4-bit rows: 33 us,
-        // 256 shares 44; 64 of up to 4,001 16-bit ones: 70 us, 768 shares 76)
+        // 256 shares 44; 64 of up to 4,001 16-bit ones: 70 us, 768 shares 76); 256 for
+        // more than 16 query rows of 128, whose registers leave room for one (12 contexts
+        // of up to 6,000 rows: 29 us with 4 bits, 33 with 16; 512 shares 35 and 40)
+        const int shares = p.rows > 16 && c->head_dim == 128 ? 256 : 512;
         if (pairs <= kPagedPairs && batch <= kFewBatch && units > 1)
-            p.shares = (int)std::min<int64_t>(std::max(512, pairs), (int64_t)pairs * units);
+            p.shares = (int)std::min<int64_t>(std::max(shares, pairs), (int64_t)pairs * units);
         if (p.shares) p.bytes = with_counters((uint64_t)p.shares * p.rows * (c->head_dim * 4 + 8), pairs);
     } else {
         p.tiles = (p.rows + kManyRows - 1) / kManyRows;
