@@ -1456,17 +1456,27 @@ __device__ __forceinline__ void join_body(const AttnPagedArgs& a) {
     for (int o = 32; o >= 1; o >>= 1) L += shfl_xor(L, o);
     constexpr int C = D / 64;
     float A[C] = {};
-#pragma unroll 8
-    for (int s = 0; s < S; ++s) {
-        const float fs = __shfl(f, s, 64);
-        const uint64_t at = a.part + (r0 + (uint64_t)(uint32_t)s * (uint32_t)a.rows) * (D * 4);
-        if constexpr (C == 2) {
-            const float2 v = gptr<float2>(at)[lane];
-            A[0] = __builtin_fmaf(fs, v.x, A[0]);
-            A[1] = __builtin_fmaf(fs, v.y, A[1]);
-        } else {
-            A[0] = __builtin_fmaf(fs, gptr<float>(at)[lane], A[0]);
+    // sixteen records' loads at a time, for they are what this takes (512 rows of 59
+    // records 9.5 us, eight at a time 17)
+    for (int s0 = 0; s0 < S; s0 += 16) {
+        float x[16][C];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+            const uint64_t at = a.part + (r0 + (uint64_t)(uint32_t)min(s0 + u, S - 1) * (uint32_t)a.rows) * (D * 4);
+            if constexpr (C == 2) {
+                const float2 v = gptr<float2>(at)[lane];
+                x[u][0] = v.x, x[u][1] = v.y;
+            } else {
+                x[u][0] = gptr<float>(at)[lane];
+            }
         }
+#pragma unroll
+        for (int u = 0; u < 16; ++u)
+            if (s0 + u < S) {
+                const float fs = __shfl(f, s0 + u, 64);
+#pragma unroll
+                for (int i = 0; i < C; ++i) A[i] = __builtin_fmaf(fs, x[u][i], A[i]);
+            }
     }
     const int i = row / a.group, h = g * a.group + (row - i * a.group);
     const uint64_t o = a.out + ((uint64_t)(uint32_t)(sv.t0 + i) * (uint32_t)a.out_stride + (uint32_t)(h * D)) * 4;

@@ -527,3 +527,18 @@ def test_attention_on_more_streams_than_have_counters(cuda, K):
     for s in streams:
         cuda.destroy_stream(s)
     B.free()
+
+
+@FORMATS
+@pytest.mark.parametrize("new,past,heads,kv,dim", [
+    ([2, 1], [3000, 700], 32, 2, 128),      # 32 query rows of a KV head, and 16 of them
+    ([4], [2000], 6, 1, 128),
+    ([3, 3, 1], [900, 4000, 0], 8, 1, 64),
+    ([1, 1], [2000, 130], 12, 1, 128),
+    ([1], [9000], 17, 1, 64),
+    ([8, 2, 5], [1500, 6000, 31], 16, 4, 128),
+])
+def test_attention_of_two_tiles_in_parts(cuda, K, fmt, new, past, heads, kv, dim):
+    """9 to 32 query rows of a KV head over contexts in parts: every share of the
+    threads that join them."""
+    _check_attn(K, Batch(cuda, new, past, heads, kv, dim, 16, fmt, seed=heads))
