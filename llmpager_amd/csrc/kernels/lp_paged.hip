@@ -992,8 +992,8 @@ LP_ATTN_FEW(q4_d128_n2, 1, 128, true, 2)
 // What would hold the accumulators twice, a branch that computes them in another
 // way, stays out of the loop.
 //
-// 2,048 tokens of 32 heads on 4 KV heads behind 6,001 rows of 16 bits: 420 us, 561
-// TFLOP/s of the formula's and twice that of MFMA work, what a large fp16 product
+// 2,048 tokens of 32 heads on 4 KV heads behind 6,001 rows of 16 bits: 410 to 430
+// us, 550 to 575 TFLOP/s of the formula's and twice that of MFMA work, what a large fp16 product
 // reaches; 12 sequences of up to 5 tokens, 16 heads to a KV head, behind up to
 // 6,000 rows of 4 bits: 34 us, of which a chunk takes about 2.8 us (the steps' vector
 // work, a wave's alone) and the launch with what comes before the first one 10; six
