@@ -252,8 +252,10 @@ uint64_t lp_kv_page_bytes(int page_rows, int head_dim, int format);
 /* The new tokens of a batch: token t of sequence b, q_starts[b] <= t <
  * q_starts[b + 1] (device i32 [batch + 1], rising), has position seq_lens[b] -
  * (q_starts[b + 1] - t): seq_lens (device i32 [batch]) count the new tokens.
- * Tokens behind the last sequence (q_starts[batch] .. tokens - 1) are padding
- * and everything of theirs is left as it was.  At most 4096 sequences.
+ * Tokens before the first sequence and behind the last (0 .. q_starts[0] - 1,
+ * q_starts[batch] .. tokens - 1) are padding and everything of theirs is left as
+ * it was, so q_starts + b, seq_lens + b and rows b .. of the table are a call
+ * over some of the sequences.  At most 4096 sequences.
  *
  * Per token, rmsnorm of each query head with q_norm and each key head with
  * k_norm (f32 [head_dim]; 0: none), NeoX rotate-half rope of both, pair

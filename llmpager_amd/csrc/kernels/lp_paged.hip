@@ -111,8 +111,8 @@ __device__ __forceinline__ void sincos_f64(double r, double& sn, double& cs) {
     cs = (q + 1) & 2 ? -b : b;
 }
 
-// The token's sequence (batch for a token behind the last one): the sequences
-// that end at or before it.
+// The token's sequence: the sequences that end at or before it (batch for a token
+// behind the last one; a token before the first one's start is none of sequence 0's).
 __device__ __forceinline__ int sequence_of(uint64_t q_starts, int batch, int token) {
     int b = 0;
     for (int i = 0; i < batch; i += 64) {
@@ -148,7 +148,8 @@ __device__ __forceinline__ void append_body(const KvAppendPagedArgs& a) {
     const int token = w / a.parts;
     if (token >= a.tokens) return;  // whole waves
     const int b = sequence_of(a.q_starts, a.batch, token);
-    if (b >= a.batch) return;  // behind the last sequence: left as it was
+    // before the first sequence or behind the last: left as it was
+    if (b >= a.batch || token < gptr<int>(a.q_starts)[b]) return;
     const int pos = gptr<int>(a.seq_lens)[b] - (gptr<int>(a.q_starts)[b + 1] - token);
     const int page = page_of(a.c, b, pos), prow = pos & ((1 << a.c.page_log2) - 1);
     // pos inv_freq in radians, less whole turns (2 pi in two parts)
