@@ -282,6 +282,7 @@ typedef uint32_t u32_any __attribute__((may_alias));
 typedef uint64_t u64_any __attribute__((may_alias));
 typedef u32x4_t u32x4_any __attribute__((may_alias));
 typedef f32x4_t f32x4_any __attribute__((may_alias));
+typedef float f32_any __attribute__((may_alias));
 typedef float2 float2_any __attribute__((may_alias));
 
 __device__ __forceinline__ f32x4_t mfma16(const u32x4_t& a, const u32x4_t& b, f32x4_t c) {
@@ -291,7 +292,8 @@ __device__ __forceinline__ f32x4_t mfma16(const u32x4_t& a, const u32x4_t& b, f3
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Two values as fp16, cut towards zero, and what that leaves out of each, rounded
-// to fp16 (one mixed multiply-add each): 2^-22 of a value is left out.
+// to fp16 (one mixed multiply-add each): 2^-22 of a value is left out, or 2^-25
+// where that is more.
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
     const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
     hi = __builtin_bit_cast(uint32_t, h);
@@ -317,6 +319,15 @@ __device__ __forceinline__ u32x4_t nibbles8(uint32_t w, const half2_t (&s)[4], c
     r[3] = nibble_pair(w >> 8, s[3], c[3]);
     return r;
 }
+
+// Probabilities are held relative to a base kLift powers of two below the maximum that
+// was current when it was set, which a score may pass by kSlack more before the base
+// is raised: the largest is near 2^kLift and none is above 2^15, an image's reach.  What
+// the images leave out of a small one is then 2^-34 of the largest at most (with the
+// maximum for a base 2^-25, of one 17 nats below it a third).
+// A wider lift raises the base more often (38 tokens of 12 sequences: 40.3 us, with
+// kLift 11 and kSlack 4 41.2).
+constexpr float kLift = 9.0f, kSlack = 6.0f;
 
 __device__ __forceinline__ bool odd_halves(uint32_t w) {  // a NaN or infinity among the two
     return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u;
@@ -373,14 +384,18 @@ __device__ __forceinline__ uint64_t rec_sums(const AttnPagedArgs& a) {
 //            next chunks are looked up together, 64 blocks of 16 rows at a time.
 //   scores   S^T = K Q^T on v_mfma_f32_16x16x32_f16: cache rows as M, the query
 //            rows as N, as fp16 hi + lo images of q scale log2 e (2^-22 of it is
-//            left out), two MFMAs a step, begun at minus the running maximum.
+//            left out), two MFMAs a step, begun at minus the base.
 //   softmax  lane (query n, kb) holds rows 16 t + 4 kb + v of the chunk, so e^ of
-//            them stays in the lane; the running maximum is raised only when a
-//            score passes it by 2^8, which spares the rescaling and the exchange
-//            between lanes.
+//            them stays in the lane; the base is raised only when a score passes
+//            what it allows (kLift, kSlack), which spares the rescaling and the
+//            exchange between lanes.
 //   context  O^T = V^T P^T: the probabilities (hi + lo) are the B operand where
 //            they lie, V^T comes through the transposing LDS reads (4 x 16 fp16
 //            or 16 x 16 nibbles to a 16-lane group), a row of ones gives the sum.
+//            Every kFold rows of a wave the sums are added to a second set, so that
+//            a matrix product is never rounded to the last place of a sum that one
+//            large probability or a long context has made (17 nats below one row,
+//            400,000 others came out 2.8e-3 off, 6e-6 with it and kLift).
 //
 // Rows lie in LDS as they are, 16-byte pieces changed round within the row
 // (few_turn) so that 16 rows' same piece, and the rows of a transposing read, each
@@ -411,6 +426,7 @@ struct Few {
     static constexpr int kVals = kRows, kKScale = 2 * kRows, kVScale = kKScale + SP * 256, kTurned = kVScale + SP * 256;
     static constexpr int kWave = kTurned + (Q4 ? 2 * CR * G * 2 : 0);  // values' scales s and -72 s, turned
     static constexpr int kKeyOps = PC + 2 * SP, kValOps = PC;
+    static constexpr int kFold = 1024 / CR;                  // chunks of a wave between additions
     static constexpr int MS = D + 4;                         // floats of a row in the merge
     static constexpr int kMerge = 4 * 16 * MS * 4 + 4 * 16 * 8;
     static constexpr int kLds = 4 * kWave > kMerge ? 4 * kWave : kMerge;
@@ -604,14 +620,25 @@ __device__ __forceinline__ void few_part(const AttnPagedArgs& a, uint8_t* lds, c
     }
     const int all = seen_rows(a, sv, 0);  // rows below it are seen by every query row
 
-    float m[NT];  // the running maximum, -inf before the first score
+    float m[NT];  // the base, -inf before the first score
     f32x4_t acc[NT][DT], sum[NT];
+    f32x4_t acc2[NT][DT];  // and what was put aside
+    float sum2[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        m[nt] = -INFINITY, sum[nt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        m[nt] = -INFINITY, sum[nt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}, sum2[nt] = 0.0f;
 #pragma unroll
-        for (int d = 0; d < DT; ++d) acc[nt][d] = sum[nt];
+        for (int d = 0; d < DT; ++d) acc[nt][d] = sum[nt], acc2[nt][d] = sum[nt];
     }
+    auto fold = [&] {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            sum2[nt] += sum[nt][0], sum[nt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int d = 0; d < DT; ++d) acc2[nt][d] += acc[nt][d], acc[nt][d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    };
+    int until_fold = 1;  // (a context's first row is often the large one)
     for (; c < r1; c += 4 * CR) {
         wait_loads<F::kValOps>();  // the keys (and scales) are here
         // a bit per block of 16 rows: its page is there
@@ -702,20 +729,20 @@ __device__ __forceinline__ void few_part(const AttnPagedArgs& a, uint8_t* lds, c
             for (int t = 0; t < MT; ++t)
 #pragma unroll
                 for (int v = 0; v < 4; ++v) mx = fmaxf(mx, s[nt][t][v]);
-            if (__ballot(mx > (m[nt] == -INFINITY ? -INFINITY : 8.0f))) {
+            if (__ballot(mx > (m[nt] == -INFINITY ? -INFINITY : kLift + kSlack))) {
                 mx = fmaxf(mx, shfl_xor(mx, 16));
                 mx = fmaxf(mx, shfl_xor(mx, 32));
                 const bool first = m[nt] == -INFINITY;
-                const float by = first ? (mx == -INFINITY ? 0.0f : mx) : fmaxf(mx, 0.0f);
+                const float by = first ? (mx == -INFINITY ? 0.0f : mx - kLift) : fmaxf(mx - kLift, 0.0f);
                 const float f = first ? 0.0f : exp2_hw(-by);
 #pragma unroll
                 for (int t = 0; t < MT; ++t)
 #pragma unroll
                     for (int v = 0; v < 4; ++v) s[nt][t][v] -= by;
-                sum[nt] *= f;
+                sum[nt] *= f, sum2[nt] *= f;
 #pragma unroll
-                for (int d = 0; d < DT; ++d) acc[nt][d] *= f;
-                m[nt] = first ? mx : m[nt] + by;
+                for (int d = 0; d < DT; ++d) acc[nt][d] *= f, acc2[nt][d] *= f;
+                m[nt] = first ? mx - kLift : m[nt] + by;
             }
 #pragma unroll
             for (int w = 0; w < CR / 32; ++w)
@@ -838,7 +865,9 @@ __device__ __forceinline__ void few_part(const AttnPagedArgs& a, uint8_t* lds, c
             wait_loads<63>();  // the values are read
             send_values(c + 4 * CR);
         }
+        if (--until_fold == 0) fold(), until_fold = F::kFold;
     }
+    fold();
 
     // ---- the waves' sums meet, a query tile at a time: the output, or the part's record
     constexpr int MS = F::MS;
@@ -849,8 +878,8 @@ __device__ __forceinline__ void few_part(const AttnPagedArgs& a, uint8_t* lds, c
     for (int nt = 0; nt < NT; ++nt) {
         __syncthreads();
 #pragma unroll
-        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4_any*>(sums + (wave * 16 + n) * MS + 16 * d + 4 * kb) = acc[nt][d];
-        if (kb == 0) ml[wave * 16 + n] = make_float2(m[nt], sum[nt][0]);
+        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4_any*>(sums + (wave * 16 + n) * MS + 16 * d + 4 * kb) = acc2[nt][d];
+        if (kb == 0) ml[wave * 16 + n] = make_float2(m[nt], sum2[nt]);
         __syncthreads();
         constexpr int TR = D / 4;  // threads of a row
 #pragma unroll
@@ -960,12 +989,15 @@ __device__ __forceinline__ void few_body(const AttnPagedArgs& a) {
 
 }  // namespace
 
+// (waves a SIMD that the registers leave room for; with 4-bit rows of 128 the second set
+// of sums takes the third: 256 sequences' 4 KV heads over up to 2,000 rows 67 us, 62 with
+// three and one set, 95 with three and both, spilled)
 #define LP_ATTN_FEW(NAME, WAVES, D, Q4, NT) \
     extern "C" __global__ void __launch_bounds__(256, WAVES) lp_attn_few_##NAME(const AttnPagedArgs a) { few_body<D, Q4, NT>(a); }
 LP_ATTN_FEW(f16_d64, 2, 64, false, 1)
 LP_ATTN_FEW(f16_d128, 2, 128, false, 1)
 LP_ATTN_FEW(q4_d64, 3, 64, true, 1)
-LP_ATTN_FEW(q4_d128, 3, 128, true, 1)
+LP_ATTN_FEW(q4_d128, 2, 128, true, 1)
 LP_ATTN_FEW(f16_d64_n2, 2, 64, false, 2)
 LP_ATTN_FEW(f16_d128_n2, 1, 128, false, 2)
 LP_ATTN_FEW(q4_d64_n2, 2, 64, true, 2)
@@ -993,6 +1025,15 @@ LP_ATTN_FEW(q4_d128_n2, 1, 128, true, 2)
 // What would hold the accumulators twice, a branch that computes them in another
 // way, stays out of the loop.
 //
+// fp32 sums that hold one large probability are rounded to the last place of it at
+// each step of a matrix product, so that thousands of small ones behind it come out
+// wrong together, the low images' products first.  Every kLook chunks (and after the
+// first, the second and the fourth) a wave compares what they added with the sum so far;
+// where a query row's is, for each chunk, below kFaint of that, the accumulators are put
+// aside in memory, where the result goes, and begin again (one row 17 nats above
+// 100,000: 6.4e-3 off without this and kLift, 9e-6 with them; at worst, every time that
+// a wave looks, 2,048 tokens behind 6,001 rows take 440 us instead of 410).
+//
 // 2,048 tokens of 32 heads on 4 KV heads behind 6,001 rows of 16 bits: 410 to 430
 // us, 550 to 575 TFLOP/s of the formula's and twice that of MFMA work, what a large fp16 product
 // reaches; 12 sequences of up to 5 tokens, 16 heads to a KV head, behind up to
@@ -1011,13 +1052,17 @@ __device__ __forceinline__ f32x16_t mfma32(const u32x4_t& a, const u32x4_t& b, f
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
 }
 
+constexpr int kLook = 8;  // chunks
+constexpr float kFaint = 0x1p-8f;
+
 template <int D>
 struct ManyRows {
     static constexpr int CR = 64;
     static constexpr int RSK = D * 2 + 16, RSV = D * 2 + 64;
     static constexpr int kBuf = CR * (RSK + RSV);
     static constexpr int kFlags = 2 * kBuf;  // 4 waves' ballots of rows there per buffer, 4 words of odd values
-    static constexpr int kLds = kFlags + 2 * 4 * 8 + 4 * 4;
+    static constexpr int kAside = kFlags + 2 * 4 * 8 + 4 * 4;  // a thread's sum put aside, with its base
+    static constexpr int kLds = kAside + 256 * 8;
 };
 
 template <int D, bool Q4>
@@ -1192,7 +1237,12 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
     uint32_t klane = lbase + (uint32_t)(n * RSK + 16 * h);
     uint32_t vlane = lbase + (uint32_t)(CR * RSK + (4 * h + (lane >> 2 & 3)) * RSV + 32 * (lane >> 4 & 1) + 8 * (lane & 3));
     asm volatile("" : "+v"(klane), "+v"(vlane));
-    float m = -INFINITY, l = 0.0f;
+    // the base, the lane's sum since the last look at it, and what went before that and is
+    // in the accumulators
+    float m = -INFINITY, l = 0.0f, lseg = 0.0f;
+    // (in LDS, for the loop has no register left) the sum of what was put aside, with its base
+    LP_LDS f32_any* const aside = (LP_LDS f32_any*)(ll + M::kAside + tid * 8);
+    bool put = false;
     f32x16_t acc[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -1250,18 +1300,88 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
         for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
         return mx;
     };
-    // to a larger maximum; what the sums so far are to be multiplied by
+    // to a larger base; what the sums so far are to be multiplied by
     auto raise = [&](float mx) {
-        mx = fmaxf(mx, shfl_xor(mx, 32));
+        mx = fmaxf(mx, shfl_xor(mx, 32)) - kLift;
         const float mn = fmaxf(m, mx);
         const float f = m == -INFINITY ? 0.0f : exp2_hw(m - mn);
-        l *= f;
+        l *= f, lseg *= f;
         m = mn;
         return f;
     };
     auto scale = [&](float f) {
 #pragma unroll
         for (int d = 0; d < DT; ++d) acc[d] *= f;
+    };
+    // the lane's part of the query row's output or record: columns 32 d + 8 e .., 4-bit
+    // ones' place 4 h + r of eight column (4 h + r) / 2 + 4 (r % 2)
+    struct Place {
+        uint64_t at, rec;
+        int h;
+        bool on, direct;
+    };
+    auto place = [&] {
+        int me = lane;  // behind the asm so that nothing of this is kept in registers meanwhile
+        asm volatile("" : "+v"(me));
+        Place p;
+        const int r = row0 + 32 * wave + (me & 31), t = r / a.group, head = g * a.group + (r - t * a.group);
+        p.h = me >> 5, p.on = r < nrows, p.direct = vis <= a.span;
+        p.rec = rec_index(a, bg, split, r);
+        p.at = p.direct ? a.out + ((uint64_t)(uint32_t)(sv.t0 + t) * (uint32_t)a.out_stride + (uint32_t)(head * D)) * 4
+                        : a.part + p.rec * (D * 4);
+        return p;
+    };
+    auto get4 = [&](const Place& p, int d, int e) {
+        if constexpr (Q4) {
+            const uint64_t o = p.at + (32 * d + 8 * e + 2 * p.h) * 4;
+            const float2 x = gptr<float2>(o)[0], y = gptr<float2>(o)[2];
+            return f32x4_t{x.x, y.x, x.y, y.y};
+        } else {
+            return gptr<f32x4_t>(p.at + (32 * d + 8 * e + 4 * p.h) * 4)[0];
+        }
+    };
+    auto put4 = [&](const Place& p, int d, int e, const f32x4_t& x) {
+        if constexpr (Q4) {
+            const uint64_t o = p.at + (32 * d + 8 * e + 2 * p.h) * 4;
+            gptr_w<float2>(o)[0] = make_float2(x[0], x[2]);
+            gptr_w<float2>(o)[2] = make_float2(x[1], x[3]);
+        } else {
+            gptr_w<f32x4_t>(p.at + (32 * d + 8 * e + 4 * p.h) * 4)[0] = x;
+        }
+    };
+    auto part4 = [&](int d, int e) {
+        return f32x4_t{acc[d][4 * e], acc[d][4 * e + 1], acc[d][4 * e + 2], acc[d][4 * e + 3]};
+    };
+    // the sum that was put aside, and what goes with it is to be multiplied by (no base:
+    // it is 0, or a NaN that stays)
+    auto sum_aside = [&](float& f) {
+        const float x = aside[0], from = aside[1];
+        f = from == -INFINITY ? 1.0f : exp2_hw(from - m);
+        return x * f;
+    };
+    // what `chunks` chunks have added since the last time against what the accumulators hold
+    auto look = [&](int chunks) {
+        const bool faint = __ballot(l > 0.0f && l < lseg * (kFaint * (float)chunks)) != 0;
+        lseg += l, l = 0.0f;
+        if (!faint) return;
+        float f = 1.0f, sum = 0.0f;
+        if (put) sum = sum_aside(f);
+        const Place p = place();
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (p.on) {
+                    f32x4_t x = part4(d, e);
+                    if (put) x += get4(p, d, e) * f;
+                    put4(p, d, e, x);
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) acc[d][4 * e + u] = 0.0f;
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        aside[0] = sum + lseg, aside[1] = m;
+        lseg = 0.0f, put = true;
     };
     // piece j of KS of a half's probabilities, and their images
     auto probs = [&](const f32x16_t& s, float base, int j, uint32_t (&hi)[8], uint32_t (&lo)[8]) {
@@ -1303,7 +1423,7 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
             const bool whole = c + CR <= wall && __builtin_amdgcn_readfirstlane((int)(there == ~0ull));
             if (!whole) mask(c, 0, s0);
             float mx = top(s0);
-            if (__ballot(mx > m + 8.0f)) scale(raise(mx));
+            if (__ballot(mx > m + (kLift + kSlack))) scale(raise(mx));
             // (the wave that is further goes first: 12 sequences' 80 rows 36.1 us without, 34.5
             // with it, one prompt of 2,048 83.3 and 85.8)
             __builtin_amdgcn_s_setprio(1);
@@ -1324,7 +1444,7 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
             }
             if (!whole) mask(c, 1, s1);
             mx = top(s1);
-            const bool up = __ballot(mx > m + 8.0f);
+            const bool up = __ballot(mx > m + (kLift + kSlack));
             float f = 1.0f;
             if (up) f = raise(mx);
             base = m == -INFINITY ? 0.0f : m;
@@ -1349,6 +1469,8 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
             }
         }
         __builtin_amdgcn_s_setprio(0);
+        const int done = (c - r0) / CR + 1;  // (a chunk that some do not see says nothing)
+        if ((done % kLook == 0 || done == 1 || done == 2 || done == 4) && c + CR <= wall) look(done <= kLook ? (done + 1) / 2 : kLook);
         if (!Q4 && special(c + 2 * CR, pg)) mend(Finite(), c + 2 * CR, pg);
         pg1 = page_for(next, c + 3 * CR);
         __syncthreads();
@@ -1407,26 +1529,22 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
                 __syncthreads();
             }
     }
-    if (!on) return;  // the halves of a query row are on or off together
+    const Place p = place();
+    if (!p.on) return;  // the halves of a query row are on or off together
+    l += lseg;
+    float fput = 1.0f;
+    if (put) l += sum_aside(fput);
     l += shfl_xor(l, 32);
-    const bool direct = vis <= a.span;
-    const uint64_t rec = rec_index(a, bg, split, row);
-    const float f = !direct ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-    const uint64_t o = direct ? a.out + ((uint64_t)(uint32_t)(sv.t0 + qi) * (uint32_t)a.out_stride + (uint32_t)(qh_ * D)) * 4
-                              : a.part + rec * (D * 4);
+    const float f = !p.direct ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float x0 = acc[d][4 * e] * f, x1 = acc[d][4 * e + 1] * f, x2 = acc[d][4 * e + 2] * f, x3 = acc[d][4 * e + 3] * f;
-            if constexpr (Q4) {  // place 4 h + r of eight holds column (4 h + r) / 2 + 4 (r % 2)
-                gptr_w<float2>(o + (32 * d + 8 * e + 2 * h) * 4)[0] = make_float2(x0, x2);
-                gptr_w<float2>(o + (32 * d + 8 * e + 2 * h + 4) * 4)[0] = make_float2(x1, x3);
-            } else {
-                gptr_w<f32x4_t>(o + (32 * d + 8 * e + 4 * h) * 4)[0] = f32x4_t{x0, x1, x2, x3};
-            }
+            f32x4_t x = part4(d, e);
+            if (put) x += get4(p, d, e) * fput;
+            put4(p, d, e, x * f);
         }
-    if (!direct && h == 0) gptr_w<float2>(rec_sums<D>(a))[rec] = make_float2(m, l);
+    if (!p.direct && p.h == 0) gptr_w<float2>(rec_sums<D>(a))[p.rec] = make_float2(m, l);
 }
 
 }  // namespace

@@ -1,11 +1,11 @@
 """lp_kv_append_paged and lp_attn_paged where they are most easily wrong: part of a
-batch's sequences."""
+batch's sequences, one row far above thousands of others."""
 import numpy as np
 import pytest
 
 import llmpager_amd as lp
-from _paged import Batch
-from test_gpu_paged import EPS, FORMATS, _append_inputs, _close, _f32
+from _paged import GROUP, Batch, q4
+from test_gpu_paged import ATTN_TOL, EPS, FORMATS, _append_inputs, _attn, _close, _f32
 
 pytestmark = pytest.mark.gpu
 
@@ -79,3 +79,103 @@ def test_attention_of_some_sequences(cuda, K, fmt, new, past, b0, b1):
     assert (got[:t0] == 7).all() and (got[t1:] == 7).all()
     _close(got[t0:t1], B.attention(q.reshape(B.tokens, 4, 64), 0.125)[t0:t1])
     B.free()
+
+
+# ---- one row far above the others ------------------------------------------------
+# In units of the largest probability: an image's smallest step is 2^-24 of 2^9, so a
+# small probability is off by 2^-34 at most, N of them, all alike, by N 2^-34 (2.3e-5 at
+# 400,000); an fp32 sum that holds the large one is rounded by 2^-24 of it a matrix product
+# of 16 or 32 rows and image, for 1,024 rows or fewer before it is put aside: 2^7 2^-24 =
+# 7.6e-6; the sums put aside are one addition per 1,024 rows, of either sign as the values
+# vary: a quarter of 2^-24 x 200 = 3e-6.  Together 3.4e-5 of the mean |v|, which is below a
+# third of the largest here: 1e-5 of that.
+
+
+class Shared:
+    """`seqs` sequences over one context of `rows` rows, `new` query tokens each: rows
+    `at` have `gap` nats more than the others, values a common part."""
+
+    def __init__(self, cuda, fmt, dim, rows, at, gap, seqs, new, heads, pad=0, spread=0.0, seed=0):
+        page = 256
+        B = self.B = Batch(cuda, [new], [page], heads, 1, dim, page, fmt, seed=seed)
+        rng = B.rng
+        cols = -(-rows // page)
+        B.pages, B.cols, B.batch = cols, cols, seqs
+        order = rng.permutation(cols).astype(np.int32)
+        B.table = np.tile(order, (seqs, 1))
+        B.lens, B.new = [rows] * seqs, [new] * seqs
+        B.live, B.tokens = seqs * new, seqs * new + pad
+        B.starts = (np.arange(seqs + 1) * new).astype(np.int32)
+        k = rng.standard_normal((cols * page, dim), np.float32) * np.float32(spread)
+        k[at] = gap / np.sqrt(dim)
+        v = 1 + rng.standard_normal((cols * page, dim), np.float32) / 2
+        B.pools, self.held = [], []
+        for x in (k, v):
+            if fmt == lp.KV_F16:
+                y = x.astype(np.float16)
+                held, raw = y.astype(np.float64), y.view(np.uint8).reshape(cols, -1)
+            else:
+                codes, s = q4(x.astype(np.float64))
+                held = ((codes - 8.0).reshape(len(x), -1, GROUP) * s[..., None]).reshape(len(x), -1)
+                raw = np.concatenate((s.astype(np.float16).view(np.uint8).reshape(cols, -1),
+                                      (codes[:, 0::2] | codes[:, 1::2] << 4).reshape(cols, -1)), 1)
+            pool = np.empty((cols, 1, raw.shape[1]), np.uint8)
+            pool[order, 0] = raw
+            B.pools.append(pool)
+            self.held.append(held[:rows])
+        # every sequence asks the same
+        self.q = (1.0 + 0.01 * rng.standard_normal((new, heads, dim))).astype(np.float32)
+        self.rows = rows
+
+    def check(self, K, **kw):
+        B, n, H = self.B, len(self.q), self.B.heads
+        q = np.zeros((B.tokens, H * B.dim), np.float32)
+        q[:B.live] = np.tile(self.q.reshape(n, -1), (B.batch, 1))
+        B.device()
+        got = _attn(K, B, q, max_seq=self.rows, **kw)
+        k, v = self.held
+        want = np.empty((n, H, B.dim))
+        for i in range(n):
+            L = self.rows - n + 1 + i
+            s = self.q[i].astype(np.float64) @ k[:L].T / np.sqrt(B.dim)
+            p = np.exp(s - s.max(-1, keepdims=True))
+            want[i] = p @ v[:L] / p.sum(-1, keepdims=True)
+        got = got[:B.live].reshape(B.batch, n, H, B.dim)
+        err = np.abs(got - want).max()
+        print("largest error", err, "of", np.abs(v).max())
+        assert err <= ATTN_TOL * np.abs(v).max()
+        B.free()
+
+
+@FORMATS
+@pytest.mark.parametrize("dim,rows,gap,at,spread", [
+    (128, 8192, 12.0, 0, 0.0), (64, 8192, 15.0, 0, 0.3), (128, 8192, 17.0, 0, 0.0), (64, 8192, 18.0, 4000, 0.0),
+    (128, 8192, 18.0, 8100, 0.2), (64, 100003, 12.0, 0, 0.0), (128, 100003, 17.0, 5, 0.0), (64, 100003, 19.0, 0, 0.3),
+    (128, 100003, 20.0, 70000, 0.0), (128, 100003, 24.0, 3, 0.0)])
+def test_one_row_above_many_many_query_rows(cuda, K, fmt, dim, rows, gap, at, spread):
+    """40 query rows that walk the whole context (bounds as if there were 512 tiles)."""
+    Shared(cuda, fmt, dim, rows, at, gap, 1, 5, 8, pad=8192, spread=spread, seed=int(gap)).check(K, max_q=8192)
+
+
+@FORMATS
+@pytest.mark.parametrize("rows,gap", [(8192, 17.0), (100003, 17.0), (100003, 19.0)])
+def test_one_row_above_many_in_spans(cuda, K, fmt, rows, gap):
+    Shared(cuda, fmt, 128, rows, 9, gap, 1, 5, 8, seed=int(gap)).check(K)
+
+
+@FORMATS
+@pytest.mark.parametrize("dim,seqs,heads,new,rows,gap,at", [
+    (64, 512, 2, 1, 32768, 12.0, 0), (128, 512, 2, 1, 32768, 17.0, 0), (64, 512, 5, 4, 32768, 18.0, 20000),
+    (128, 256, 9, 2, 32768, 17.0, 32000), (64, 512, 2, 1, 400003, 13.0, 7), (64, 512, 2, 1, 400003, 17.0, 0),
+    (64, 512, 5, 4, 400003, 19.0, 3), (128, 512, 2, 1, 400003, 17.0, 300000), (128, 256, 9, 2, 400003, 18.0, 0),
+    (128, 512, 2, 1, 400003, 24.0, 0)])
+def test_one_row_above_many_few_query_rows(cuda, K, fmt, dim, seqs, heads, new, rows, gap, at):
+    """As many sequences as workgroups: each walks a whole context, its waves a quarter
+    of it each."""
+    Shared(cuda, fmt, dim, rows, at, gap, seqs, new, heads, seed=int(gap)).check(K)
+
+
+@FORMATS
+@pytest.mark.parametrize("rows,gap", [(8192, 17.0), (100003, 18.0)])
+def test_one_row_above_many_in_parts(cuda, K, fmt, rows, gap):
+    Shared(cuda, fmt, 128, rows, 1, gap, 1, 1, 8, seed=int(gap)).check(K)
