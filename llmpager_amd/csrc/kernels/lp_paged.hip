@@ -408,7 +408,10 @@ __device__ __forceinline__ uint64_t rec_sums(const AttnPagedArgs& a) {
 // Rows past the sequence, or of absent pages, are masked and their values
 // zeroed.  fp16 rows that only some of the queries see (several new tokens) may
 // hold NaN or infinity, which zero probabilities would not keep out: a chunk
-// with one is added row by row.
+// with one is added row by row.  In a chunk that all queries see nothing is looked
+// for, and an image of 0 makes a NaN of an infinity: a wave whose sums are no finite
+// numbers looks through its rows for what they are to be (few_odd; to look in each
+// chunk instead: 64 sequences of up to 4,000 rows 72.6 us, 70.5 so).
 //
 // The cache's bytes bound it, the launch and a workgroup's chain of round trips
 // (lengths, pages, first rows, join) where they are few: 64 sequences of up to
@@ -510,6 +513,63 @@ __device__ __forceinline__ void few_join(const AttnPagedArgs& a, uint8_t* lds, c
         pieces(std::integral_constant<int, 1>());
     else
         pieces(std::integral_constant<int, 16 * NT * TR / 256>());
+}
+
+// The wave's columns of 16-bit values that are no finite numbers, of the rows that each
+// query sees: infinities of one sign make the sum that, others NaN, and so does a row
+// whose score is not finite.  Lane (n, kb) holds columns 16 d + 4 kb + u of query n.
+template <int D, int NT, int DT>
+__device__ __forceinline__ void few_odd(const AttnPagedArgs& a, int b, int g, int c, int r1, const int (&last)[NT], f32x4_t (&acc)[NT][DT]) {
+    constexpr int CR = Few<D, false>::CR, kRow = D * 2;
+    const int lane = lane_id(), kb = lane >> 4, pmask = (1 << a.c.page_log2) - 1;
+    uint32_t up[NT] = {}, down[NT] = {}, nan[NT] = {};  // bit 4 d + u
+    for (; c < r1; c += 4 * CR)
+        for (int c16 = c; c16 < c + CR; c16 += 16) {
+            const int page = c16 < r1 ? page_of(a.c, b, c16) : -1;
+            if (page < 0) continue;  // the same in all lanes
+            const uint64_t off = (uint64_t)(uint32_t)((c16 & pmask) * kRow);
+            const uint64_t v = page_at<D, false>(a.c, a.c.v_pages, page, g) + off, k = page_at<D, false>(a.c, a.c.k_pages, page, g) + off;
+            uint32_t x[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                x[r] = D == 128 ? gptr<uint32_t>(v)[r * 64 + lane] : (uint32_t)gptr<uint16_t>(v)[r * 64 + lane];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                if (!__ballot(odd_halves(x[r])) || c16 + r >= r1) continue;
+                const uint32_t y = D == 128 ? gptr<uint32_t>(k)[r * 64 + lane] : (uint32_t)gptr<uint16_t>(k)[r * 64 + lane];
+                const bool score = !__ballot(odd_halves(y));
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const uint32_t e = gptr<uint16_t>(v)[r * D + 16 * d + 4 * kb + u], bit = 1u << (4 * d + u);
+                        if ((e & 0x7c00u) != 0x7c00u) continue;
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            if (c16 + r > last[nt]) continue;
+                            if (!score || (e & 0x3ffu))
+                                nan[nt] |= bit;
+                            else if (e & 0x8000u)
+                                down[nt] |= bit;
+                            else
+                                up[nt] |= bit;
+                        }
+                    }
+            }
+        }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const uint32_t bit = 1u << (4 * d + u);
+                const bool p = up[nt] & bit, m = down[nt] & bit;
+                if ((nan[nt] & bit) || (p && m))
+                    acc[nt][d][u] = __builtin_nanf("");
+                else if (p || m)
+                    acc[nt][d][u] = p ? INFINITY : -INFINITY;
+            }
 }
 
 // One part of a pair: units [u0, u1) of (sequence view sv, KV head g).
@@ -868,6 +928,16 @@ __device__ __forceinline__ void few_part(const AttnPagedArgs& a, uint8_t* lds, c
         if (--until_fold == 0) fold(), until_fold = F::kFold;
     }
     fold();
+    if constexpr (!Q4) {
+        f32x4_t odd = {0.0f, 0.0f, 0.0f, 0.0f};  // or NaN
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) odd[u] = __builtin_fmaf(acc2[nt][d][u], 0.0f, odd[u]);
+        if (__builtin_expect(__ballot(!(odd[0] + odd[1] + odd[2] + odd[3] == 0.0f)) != 0, 0)) few_odd<D, NT, DT>(a, b, g, (u0 * 4 + wave) * CR, r1, last, acc2);
+    }
 
     // ---- the waves' sums meet, a query tile at a time: the output, or the part's record
     constexpr int MS = F::MS;

@@ -1,5 +1,6 @@
 """lp_kv_append_paged and lp_attn_paged where they are most easily wrong: part of a
-batch's sequences, one row far above thousands of others."""
+batch's sequences, one row far above thousands of others, values that are no finite
+numbers in any place."""
 import numpy as np
 import pytest
 
@@ -179,3 +180,37 @@ def test_one_row_above_many_few_query_rows(cuda, K, fmt, dim, seqs, heads, new, 
 @pytest.mark.parametrize("rows,gap", [(8192, 17.0), (100003, 18.0)])
 def test_one_row_above_many_in_parts(cuda, K, fmt, rows, gap):
     Shared(cuda, fmt, 128, rows, 1, gap, 1, 1, 8, seed=int(gap)).check(K)
+
+
+# ---- values that are no finite numbers ---------------------------------------------
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new,past,heads,kv", [
+    ([1], [700], 4, 2), ([1, 1, 1], [4000, 33, 300], 16, 2), ([3], [900], 8, 2), ([7, 2], [2000, 600], 8, 2)])
+def test_few_rows_see_no_numbers(cuda, K, dim, new, past, heads, kv):
+    """Infinities that every query sees, in chunks that are whole and in the last one:
+    of the row with the largest score, of one with hardly any probability, two of
+    opposite signs in one column, a NaN."""
+    B = Batch(cuda, new, past, heads, kv, dim, 16, lp.KV_F16, seed=90 + dim)
+    q = _f32(B.rng, B.tokens, heads * dim)
+    for b, L in enumerate(B.lens):
+        rows = B.rng.permutation(min(L, past[b]))[:6]
+        first = q[int(B.starts[b])].reshape(kv, -1, dim)[:, 0]
+        B.put(int(rows[0]), first.astype(np.float16), None, b)              # the largest score
+        B.put(int(rows[1]), (-2 * first).astype(np.float16), None, b)       # about 34 nats below
+        for i, (c, x) in enumerate([(3, np.inf), (7, -np.inf), (9, np.inf), (9, -np.inf), (11, np.nan), (13, -np.inf)]):
+            v = B.rng.standard_normal((kv, dim)).astype(np.float16)
+            v[:, c] = x
+            B.put(int(rows[i]), None, v, b)
+        w = np.ones((kv, dim), np.float16)
+        w[:, 17] = np.inf
+        B.put(L - new[b], None, w, b)  # in the last chunk
+    B.device()
+    got = _attn(K, B, q).reshape(B.tokens, heads, dim)
+    want = B.attention(q.reshape(B.tokens, heads, dim), 1.0 / np.sqrt(dim))
+    assert np.isinf(want).any() and np.isnan(want).any()
+    fine = np.isfinite(want)
+    assert np.array_equal(got[~fine], want[~fine], equal_nan=True)
+    _close(got[fine], want[fine])
+    B.free()
