@@ -230,11 +230,14 @@ enum { LP_KV_F16 = 0, LP_KV_Q4 = 1 };
 /* One layer's cache.  Its pools hold `pages` pages of page_rows rows for every
  * KV head: page p of KV head g at pool + (p * kv_heads + g) * lp_kv_page_bytes,
  * as fp16 [page_rows, head_dim] or as a q4 region [page_rows, head_dim] of
- * group 32 (quant.rs:1-22: f16 scales, then nibbles holding q + 8).  Row r of
- * sequence b is row r % page_rows of page table[b][r / page_rows].  An entry
- * outside 0 .. pages - 1 holds no rows: nothing is appended to it and
- * attention leaves its rows out.  Sequences may share pages that are only
- * read. */
+ * group 32 (quant.rs:1-22: f16 scales, then nibbles holding q + 8) whose scales
+ * have at most 7 significant bits and lie within 2^-17 .. 896, as the append
+ * leaves them: attention multiplies out n s - 72 s (n = q + 72) in fp16, which
+ * is exact for those; of other scales it makes values that are off by up to
+ * s / 28, and from 910 on no numbers.  Row r of sequence b is row r % page_rows
+ * of page table[b][r / page_rows].  An entry outside 0 .. pages - 1 holds no
+ * rows: nothing is appended to it and attention leaves its rows out.  Sequences
+ * may share pages that are only read. */
 typedef struct lp_kv_cache {
     uint64_t k_pages, v_pages; /* device pools, 16-byte aligned */
     uint64_t table;            /* device i32 [batch, max_pages] */
