@@ -286,8 +286,10 @@ int lp_kv_append_paged(lp_ctx* ctx, const lp_kv_cache* cache, uint64_t q, int q_
  * larger length is taken as max_seq (or as what the table's width holds).  The
  * bounds decide how the work is split, so a capture may be replayed with other
  * q_starts, seq_lens and tables within them.  q and out: f32 rows as above,
- * which must not overlap.  The products take q scale log2(e) as two fp16 images:
- * below 2^16.  Scales in q4 pages are finite, as the append leaves them.
+ * which must not overlap.  The products take q scale log2(e), below 2^16, to
+ * 2^-22 of each value or, of one below 1/8, to 2^-25: a score is off by the sum
+ * of that times the key's values, so keys in the hundreds beside queries in the
+ * thousandths cost it bits that 32-bit products would keep.
  * workspace: lp_attn_paged_ws_bytes bytes, 256-byte aligned (0 bytes: may be 0);
  * two calls that overlap, replays of graphs among them, need one each. */
 uint64_t lp_attn_paged_ws_bytes(const lp_kv_cache* cache, int heads, int batch, int tokens, int max_q, int max_seq);
