@@ -271,7 +271,8 @@ uint64_t lp_kv_page_bytes(int page_rows, int head_dim, int format);
  * within 2^-17 .. 896, and round(x / scale) within -7 .. 7 (NaN as 0), of
  * values computed in 64 bits.  k_out, v_out (f32 [tokens, kv_heads, head_dim],
  * or 0): also the rows as the pages hold them.  A position outside the table's
- * width is not appended.  Two tokens with one place leave one of the two there. */
+ * width is not appended.  Two tokens with one place leave a mixture of the two
+ * there. */
 int lp_kv_append_paged(lp_ctx* ctx, const lp_kv_cache* cache, uint64_t q, int q_stride, uint64_t k, int k_stride,
                        uint64_t v, int v_stride, uint64_t q_norm, uint64_t k_norm, float eps, uint64_t inv_freq,
                        float mscale, uint64_t q_out, int q_out_stride, uint64_t k_out, uint64_t v_out, int heads,
