@@ -266,7 +266,6 @@ struct lp_ctx {
     // destroying the capture stream and routing on a stream created later
     // never shares counters with the graph's replays.
     int32_t* sync = nullptr;
-    int32_t* join_sync = nullptr;  // a slot's kPagedPairs counters of join_counters, zero between launches too
     std::mutex sync_mu;
     hipStream_t sync_owner[kSyncSlots] = {};  // slot i belongs to sync_owner[i] when sync_used[i]
     bool sync_used[kSyncSlots] = {};
@@ -274,6 +273,14 @@ struct lp_ctx {
     hipStream_t cap_stream = nullptr;         // a capture in progress on this stream ...
     int cap_slot = -1;                        // ... routes through this (the graph's) slot
     bool cap_prof = false;                    // lp_graph_capture_begin: the profiling switch to restore
+    // kPagedPairs counters each of join_counters, zero between launches too: slots of
+    // their own, so that calls that can do without one take none from those above
+    int32_t* join_sync = nullptr;
+    struct JoinSlot {
+        bool used;
+        hipStream_t stream;  // its owner, or (graph >= 0)
+        int graph;           // the graph that owns this slot of `sync`
+    } join_slots[kSyncSlots] = {};
     int step_spin = kStepSpinMax;             // polls before a wait of lp_attn_block or lp_attn_fused gives up
     // decode gate/up through lp_moe_gateup_bal (LLMPAGER_HIP_GATEUP_BAL=0 at
     // lp_init turns it off, for comparison)
@@ -536,6 +543,13 @@ int lp_stream_destroy(lp_ctx* c, lp_stream s) {
             if (c->sync_used[i] && !c->sync_graph[i] && c->sync_owner[i] == (hipStream_t)s) {
                 HIPCHK(hipStreamSynchronize((hipStream_t)s));
                 c->sync_used[i] = false;
+                break;
+            }
+        }
+        for (lp_ctx::JoinSlot& j : c->join_slots) {
+            if (j.used && j.graph < 0 && j.stream == (hipStream_t)s) {
+                HIPCHK(hipStreamSynchronize((hipStream_t)s));
+                j.used = false;
                 break;
             }
         }
@@ -1175,20 +1189,34 @@ struct PagedPlan {
 static uint64_t counters_at(uint64_t records) { return (records + 63) / 64 * 64; }
 static uint64_t with_counters(uint64_t records, int counters) { return counters_at(records) + (uint64_t)counters * kPagedStride * 4; }
 
+// The slot of join counters of a graph being captured (its slot of `sync`), or of a
+// stream; -1: none is free.
+static int join_slot(lp_ctx* c, hipStream_t s, int graph) {
+    std::lock_guard<std::mutex> g(c->sync_mu);
+    int free_slot = -1;
+    for (int i = 0; i < kSyncSlots; ++i) {
+        const lp_ctx::JoinSlot& j = c->join_slots[i];
+        if (j.used && j.graph == graph && (graph >= 0 || j.stream == s)) return i;
+        if (!j.used && free_slot < 0) free_slot = i;
+    }
+    if (free_slot >= 0) c->join_slots[free_slot] = {true, s, graph};
+    return free_slot;
+}
+
 // The arrival counters of a call whose last workgroups join the others' parts: its
 // stream's, zero between launches.  But what the caller captures into a graph may
 // be replayed beside other calls of that stream and other graphs captured from it,
 // and a stream may be one more than the context has counters for: there they are
 // the workspace's, cleared by a launch of its own.
 static int join_counters(lp_ctx* c, lp_stream s, uint64_t at, int n, uint64_t* sync) {
-    bool ours;
+    int graph;
     {
         std::lock_guard<std::mutex> g(c->sync_mu);
-        ours = c->cap_slot >= 0 && c->cap_stream == (hipStream_t)s;
+        graph = c->cap_slot >= 0 && c->cap_stream == (hipStream_t)s ? c->cap_slot : -1;
     }
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    if (!ours && hipStreamIsCapturing((hipStream_t)s, &st) != hipSuccess) (void)hipGetLastError();
-    const int slot = ours || st == hipStreamCaptureStatusNone ? sync_slot(c, s) : -1;
+    if (graph < 0 && hipStreamIsCapturing((hipStream_t)s, &st) != hipSuccess) (void)hipGetLastError();
+    const int slot = graph >= 0 || st == hipStreamCaptureStatusNone ? join_slot(c, (hipStream_t)s, graph) : -1;
     if (slot >= 0) {
         *sync = reinterpret_cast<uint64_t>(c->join_sync) + (uint64_t)slot * kPagedPairs * kPagedStride * 4;
         return LP_OK;
@@ -2156,6 +2184,8 @@ static void graph_slot_free(lp_ctx* c, int slot) {
     if (slot < 0 || slot >= kSyncSlots) return;
     c->sync_used[slot] = false;
     c->sync_graph[slot] = false;
+    for (lp_ctx::JoinSlot& j : c->join_slots)
+        if (j.used && j.graph == slot) j.used = false;
 }
 
 static void capture_end(lp_ctx* c) {
