@@ -1205,9 +1205,10 @@ static int join_slot(lp_ctx* c, hipStream_t s, int graph) {
 
 // The arrival counters of a call whose last workgroups join the others' parts: its
 // stream's, zero between launches.  But what the caller captures into a graph may
-// be replayed beside other calls of that stream and other graphs captured from it,
-// and a stream may be one more than the context has counters for: there they are
-// the workspace's, cleared by a launch of its own.
+// be replayed beside other calls of that stream and other graphs captured from it, a
+// stream may be one more than the context has counters for, and hipStreamPerThread is
+// one handle for a stream of each host thread: there they are the workspace's, cleared
+// by a launch of its own.
 static int join_counters(lp_ctx* c, lp_stream s, uint64_t at, int n, uint64_t* sync) {
     int graph;
     {
@@ -1216,7 +1217,8 @@ static int join_counters(lp_ctx* c, lp_stream s, uint64_t at, int n, uint64_t* s
     }
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
     if (graph < 0 && hipStreamIsCapturing((hipStream_t)s, &st) != hipSuccess) (void)hipGetLastError();
-    const int slot = graph >= 0 || st == hipStreamCaptureStatusNone ? join_slot(c, (hipStream_t)s, graph) : -1;
+    const bool own = graph >= 0 || (st == hipStreamCaptureStatusNone && (hipStream_t)s != hipStreamPerThread);
+    const int slot = own ? join_slot(c, (hipStream_t)s, graph) : -1;
     if (slot >= 0) {
         *sync = reinterpret_cast<uint64_t>(c->join_sync) + (uint64_t)slot * kPagedPairs * kPagedStride * 4;
         return LP_OK;

@@ -1,5 +1,7 @@
 """lp_attn_paged and lp_logprobs beside the calls that need a stream's arrival
 counters, on many streams."""
+import threading
+
 import numpy as np
 import pytest
 
@@ -89,3 +91,51 @@ def test_streams_and_graphs_give_their_counters_back(cuda, K):
         _close(cuda.download(do, (2, 8, 128), np.float32, s), want)
         cuda.destroy_stream(s)
     B.free()
+
+
+PER_THREAD = 2  # hipStreamPerThread: one handle, a stream for each host thread
+
+
+def test_threads_on_their_own_streams_by_one_handle(cuda, K):
+    """Four host threads, each with its workspaces, on the handle that names a stream
+    of each of them."""
+    Bs, jobs = [], []
+    for i in range(4):
+        B = Batch(cuda, [1, 1], [2500 + 300 * i, 300], 8, 2, 128, 16, lp.KV_Q4, seed=10 + i)
+        q = _queries(B)
+        B.device()
+        x = B.rng.standard_normal((2, 50021)).astype(np.float32)
+        Bs.append(B)
+        jobs.append((B.up(q), B.alloc(2 * 4096), B.alloc(K.attn_paged_ws_bytes(B.cache, 8, 2, 2, 1, max(B.lens))),
+                     B.up(x), B.up(np.array([3, 4], np.int32)), B.alloc(256), B.alloc(256), B.alloc(256),
+                     B.alloc(K.logprobs_ws_bytes(2, 50021, 5)),
+                     B.attention(q.reshape(2, 8, 128), 1.0 / np.sqrt(128.0)), logprobs(x, np.array([3, 4]), 5)))
+    cuda.sync()
+    start, failed = threading.Barrier(4), []
+
+    def run(B, job):
+        dq, do, ws, dx, dt, dl, di, dp, ws2, att, (wl, _, wi, wp) = job
+        try:
+            cuda.bind_thread()
+            start.wait()
+            for _ in range(5):
+                for _ in range(20):
+                    K.attn_paged(B.cache, dq, 1024, do, 1024, 8, B.dstarts, B.dlens, 2, 2, 1, max(B.lens),
+                                 1.0 / np.sqrt(128.0), ws, PER_THREAD, ws_bytes=ws.nbytes)
+                    K.logprobs(dx, 50021, 2, 50021, dt, dl, 0, 5, di, dp, ws2, PER_THREAD, ws_bytes=ws2.nbytes)
+                _close(cuda.download(do, (2, 8, 128), np.float32, PER_THREAD), att)
+                _same(cuda.download(dl, (2,), np.float32, PER_THREAD), wl)
+                assert np.array_equal(cuda.download(di, (2, 5), np.int32, PER_THREAD), wi)
+                _same(cuda.download(dp, (2, 5), np.float32, PER_THREAD), wp)
+        except BaseException as e:  # to the test's own thread
+            failed.append(e)
+
+    threads = [threading.Thread(target=run, args=a) for a in zip(Bs, jobs)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for B in Bs:
+        B.free()
+    if failed:
+        raise failed[0]
