@@ -1,14 +1,15 @@
 // gfx950 kernels that read rows of logits: log probabilities of given tokens,
 // the rows' entropies and their top alternatives.
 //
-// With M the row's largest logit, S = sum e^(x - M) and Y = sum e^(x - M) (x - M):
-//   log p(x) = (x - M) - log S,   entropy = log S - Y / S.
+// With M the row's largest logit, n the number of those equal to it, s = sum e^(x - M)
+// over the others, S = n + s and Y = sum e^(x - M) (x - M):
+//   log p(x) = (x - M) - log S,   entropy = log S - Y / S,   log S = log n + log(1 + s / n).
 // Logits are read once.  A workgroup takes a part of a row and each of its
 // waves 4096 bytes at a time, 16 logits a lane; M is the wave's running maximum,
 // raised for the wave as a whole when a block passes it, which few blocks do.
 // In a row that is sure of one token the entropy is all in what the other terms
 // add to the 1 of the largest, so logits equal to M are counted apart and the
-// others' sums kept beside the count; sums of 16 are added up in 64 bits.
+// others' sums kept beside the count to the end; sums of 16 are added up in 64 bits.
 //
 // The alternatives: lane i of a wave holds its i-th best as a key in the order of
 // (value, lowest id first), and a block is looked through only if one of its
@@ -51,6 +52,9 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
         t += __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(u >> 32), l) << 32 |
                                             (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, l));
     return t;
+}
+__device__ __forceinline__ int wave_sum_i32(int v) {
+    return (int)wave_reduce_u32((uint32_t)v, 0u, [](uint32_t a, uint32_t b) { return a + b; });
 }
 // (NaN counts as nothing)
 __device__ __forceinline__ float wave_top(float v) {
@@ -273,9 +277,13 @@ __device__ __forceinline__ f32x4_t load4(const LP_GLOBAL float* x, int e, int n)
     return r;
 }
 
-// What a row's sums make of it.
+// What a row's sums make of it: log(n + s), of a small r = s / n by the series of
+// log(1 + r), whose first term left out is 2^-53 of it.
 __device__ __forceinline__ double row_lse(const Sums& t) {
-    return t.m - t.m == 0.0f ? log(t.s + (double)t.n) : (double)__builtin_nanf("");
+    if (t.m - t.m != 0.0f) return (double)__builtin_nanf("");
+    const double n = (double)t.n, r = t.s / n;
+    if (!(r < 0x1p-10)) return log(n + t.s);
+    return (t.n == 1 ? 0.0 : log(n)) + r * (1.0 - r * (0.5 - r * (1.0 / 3.0 - r * (0.25 - r * 0.2))));
 }
 
 // The row's results, by the wave that holds its sums and best: lane i alternative i.
@@ -298,19 +306,21 @@ __device__ __forceinline__ void finish(const LogprobArgs& a, int row, const Sums
     }
 }
 
-// The sums of other waves or parts, one per lane (m = -inf, s = 0 where there
+// The sums of other waves or parts, one per lane (m = -inf, s = n = 0 where there
 // is none), as one.
-__device__ __forceinline__ Sums join(float m, double s, double y) {
+__device__ __forceinline__ Sums join(float m, double s, double y, int n) {
     Sums t;
     t.m = wave_top(m);
-    double f = m == t.m ? 1.0 : (double)exp_neg(m - t.m);
     if (m == -INFINITY) {
-        f = 0.0;
-        y = 0.0, m = t.m;
+        s *= 0.0, y = 0.0, n = 0;  // -inf adds nothing; a NaN stays one
+    } else if (m != t.m) {  // its maximum is one of the others
+        const double f = (double)exp_neg(m - t.m), all = s + (double)n;
+        y = f * (y + ((double)m - (double)t.m) * all);
+        s = f * all, n = 0;
     }
-    // s holds the count of its maximum
-    t.y = wave_sum_f64(f * (y + (m == t.m ? 0.0 : ((double)m - (double)t.m) * s)));
-    t.s = wave_sum_f64(f * s);
+    t.y = wave_sum_f64(y);
+    t.s = wave_sum_f64(s);
+    t.n = wave_sum_i32(n);
     return t;
 }
 
@@ -318,6 +328,7 @@ __device__ __forceinline__ Sums join(float m, double s, double y) {
 template <bool TOP>
 __device__ __forceinline__ void scan(const LogprobArgs& a, int row, int part, Sums& t, Best& best) {
     __shared__ float lm[4];
+    __shared__ int ln[4];
     __shared__ double lsum[2][4];
     __shared__ uint64_t lk[TOP ? 4 : 1][64];  // a wave's room, then its best
     const uint64_t at = a.logits + (uint64_t)row * (uint32_t)a.stride * 4;
@@ -358,12 +369,14 @@ __device__ __forceinline__ void scan(const LogprobArgs& a, int row, int part, Su
             }
         }
     }
-    const double ws = wave_sum_f64(t.s + (double)t.n), wy = wave_sum_f64(t.y);
-    if (lane == 0) lm[wave] = t.m, lsum[0][wave] = ws, lsum[1][wave] = wy;
+    const double ws = wave_sum_f64(t.s), wy = wave_sum_f64(t.y);
+    const int wn = wave_sum_i32(t.n);
+    if (lane == 0) lm[wave] = t.m, lsum[0][wave] = ws, lsum[1][wave] = wy, ln[wave] = wn;
     if constexpr (TOP) lk[wave][lane] = (uint64_t)best.hi << 32 | best.lo;
     __syncthreads();
     if (wave) return;
-    t = join(lane < 4 ? lm[lane & 3] : -INFINITY, lane < 4 ? lsum[0][lane & 3] : 0.0, lane < 4 ? lsum[1][lane & 3] : 0.0);
+    t = join(lane < 4 ? lm[lane & 3] : -INFINITY, lane < 4 ? lsum[0][lane & 3] : 0.0, lane < 4 ? lsum[1][lane & 3] : 0.0,
+             lane < 4 ? ln[lane & 3] : 0);
     if constexpr (TOP)
         for (int w = 1; w < 4; ++w) {
             Keys k;
@@ -372,7 +385,7 @@ __device__ __forceinline__ void scan(const LogprobArgs& a, int row, int part, Su
         }
 }
 
-// Records: per (row, part) s, y, m (32 bytes); behind all of them the keys of its
+// Records: per (row, part) s, y, m and n (32 bytes); behind all of them the keys of its
 // alternatives, a row's parts' one behind the other.
 __device__ __forceinline__ uint64_t rec_at(const LogprobArgs& a, int row, int part) {
     return a.part + ((uint64_t)(uint32_t)row * (uint32_t)a.parts + (uint32_t)part) * 32;
@@ -390,10 +403,12 @@ __device__ __forceinline__ void join_row(const LogprobArgs& a, int row) {
     const int lane = lane_id();
     float m = -INFINITY;
     double s = 0.0, y = 0.0;
+    int n = 0;
     if (lane < a.parts) {
         const uint64_t r = rec_at(a, row, lane);
         s = __builtin_bit_cast(double, get64(r)), y = __builtin_bit_cast(double, get64(r + 8));
-        m = __uint_as_float((uint32_t)get64(r + 16));
+        const uint64_t mn = get64(r + 16);
+        m = __uint_as_float((uint32_t)mn), n = (int)(mn >> 32);
     }
     Best best;
     if constexpr (TOP) {
@@ -411,7 +426,7 @@ __device__ __forceinline__ void join_row(const LogprobArgs& a, int row) {
             best.take(h, [&](int i) { return l[i]; }, a.top, room);
         }
     }
-    finish(a, row, join(m, s, y), best);
+    finish(a, row, join(m, s, y, n), best);
 }
 
 template <bool TOP>
@@ -429,7 +444,7 @@ __device__ __forceinline__ void logprobs_body(const LogprobArgs& a) {
     if (lane_id() == 0) {
         put64(r, __builtin_bit_cast(uint64_t, t.s));
         put64(r + 8, __builtin_bit_cast(uint64_t, t.y));
-        put64(r + 16, __float_as_uint(t.m));
+        put64(r + 16, (uint64_t)(uint32_t)t.n << 32 | __float_as_uint(t.m));
     }
     if (TOP && lane_id() < a.top) put64(keys_at(a, row, part) + 8 * lane_id(), (uint64_t)best.hi << 32 | best.lo);
     // the row's last part joins them: nothing waits
