@@ -1256,19 +1256,21 @@ static PagedPlan paged_plan(const lp_kv_cache* c, int heads, int batch, int toke
     return p;
 }
 
-// One query row per (token, query head): their number per KV head and its
-// products with the sequences stay within 32 bits.
-static int check_queries(int heads, int batch, int tokens, int max_q, int max_seq) {
+// One query row per (token, query head): their number per KV head is a 32-bit one, and
+// their workgroups a grid.
+static int check_queries(int heads, int kv_heads, int batch, int tokens, int max_q, int max_seq) {
     if (max_q < 0 || max_seq < 0) return fail(LP_E_INVALID, "attn_paged: negative max_q or max_seq");
-    if ((int64_t)batch * std::min(max_q, tokens) * heads > INT32_MAX / 256)
-        return fail(LP_E_UNSUPPORTED, "attn_paged: batch x max_q x heads must be below 2^23");
+    const int64_t rows = (int64_t)std::min(max_q, tokens) * (heads / kv_heads);
+    if (rows > INT32_MAX / 2 || (rows && (int64_t)batch * kv_heads * ((rows + kManyRows - 1) / kManyRows) > INT32_MAX / 256))
+        return fail(LP_E_UNSUPPORTED, "attn_paged: batch x kv_heads x blocks of 128 query rows (max_q x heads / kv_heads) "
+                                      "must be below 2^23");
     return LP_OK;
 }
 
 uint64_t lp_attn_paged_ws_bytes(const lp_kv_cache* cache, int heads, int batch, int tokens, int max_q, int max_seq) {
     PagedCache pc;
     if (check_paged("attn_paged", cache, &pc) || check_batch("attn_paged", heads, cache->kv_heads, batch, tokens, 4, 4) ||
-        check_queries(heads, batch, tokens, max_q, max_seq))
+        check_queries(heads, cache->kv_heads, batch, tokens, max_q, max_seq))
         return 0;
     return paged_plan(cache, heads, batch, tokens, max_q, max_seq).bytes;
 }
@@ -1295,7 +1297,7 @@ int lp_attn_paged(lp_ctx* c, const lp_kv_cache* cache, uint64_t q, int q_stride,
     if (int r = check_rows("attn_paged: q", q, q_stride, (int64_t)heads * D)) return r;
     if (int r = check_rows("attn_paged: out", out, out_stride, (int64_t)heads * D)) return r;
     if (q == out) return fail(LP_E_INVALID, "attn_paged: out must not be q");
-    if (int r = check_queries(heads, batch, tokens, max_q, max_seq)) return r;
+    if (int r = check_queries(heads, cache->kv_heads, batch, tokens, max_q, max_seq)) return r;
     const PagedPlan plan = paged_plan(cache, heads, batch, tokens, max_q, max_seq);
     if (int r = check_workspace("attn_paged", plan.bytes, workspace, ws_bytes)) return r;
     if (int r = check_ctx(c)) return r;

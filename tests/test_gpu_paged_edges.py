@@ -214,3 +214,19 @@ def test_few_rows_see_no_numbers(cuda, K, dim, new, past, heads, kv):
     assert np.array_equal(got[~fine], want[~fine], equal_nan=True)
     _close(got[fine], want[fine])
     B.free()
+
+
+# ---- one prompt's bound for many sequences ---------------------------------------------
+
+
+@FORMATS
+def test_a_prompt_and_many_single_tokens(cuda, K, fmt):
+    """64 sequences, one with 150 new tokens and the others with one, bounds of 2,048
+    new tokens: 65,536 blocks of 128 query rows, almost all of them empty."""
+    B = Batch(cuda, [1] * 20 + [150] + [1] * 43, [30 * b % 700 for b in range(64)], 64, 4, 64, 16, fmt, seed=7, pad=2048 - 213)
+    q = _f32(B.rng, B.tokens, 64 * 64)
+    B.device()
+    got = _attn(K, B, q, max_q=2048, max_seq=1000)
+    _close(got[:B.live].reshape(-1, 64, 64), B.attention(q.reshape(-1, 64, 64), 0.125)[:B.live])
+    assert (got[B.live:] == 7).all()
+    B.free()

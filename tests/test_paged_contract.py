@@ -1,8 +1,11 @@
 """What lp_kv_cache, lp_kv_append_paged, lp_attn_paged and lp_logprobs state in
 include/llmpager_hip.h, on the CPU."""
 import numpy as np
+import pytest
 
+import llmpager_amd as lp
 from _paged import q4
+from test_paged_host import INVALID, UNSUPPORTED, _attn, _cache, _said
 
 
 def test_scales_that_a_q4_page_may_hold():
@@ -28,3 +31,21 @@ def test_scales_as_the_append_makes_them():
     m, _ = np.frexp(s)
     assert s.min() == 2.0 ** -17 and s.max() == 896.0 and np.array_equal(m * 128, np.rint(m * 128))
     assert np.array_equal(s.astype(np.float16).astype(np.float64), s)
+
+
+@pytest.mark.parametrize("kv,heads,batch,tokens,max_q,taken", [
+    (2, 64, 64, 4096, 2048, True),           # 64 sequences, of which one has 2,048 tokens
+    (8, 64, 4096, 8192, 4096, False),        # 8,388,608 blocks of 128 query rows
+    (8, 64, 4095, 8192, 4096, True),
+    (2, 8, 4096, 1 << 30, 1 << 30, False),
+    (1, 1 << 20, 4, 1 << 20, 1 << 11, False),  # 2^31 query rows
+    (1, 4, 4096, 4096, 1, True),
+])
+def test_bounds_of_the_query_rows(kv, heads, batch, tokens, max_q, taken):
+    c = _cache(kv_heads=kv)
+    kw = dict(heads=heads, batch=batch, tokens=tokens, max_q=max_q, q_stride=heads * 128, out_stride=heads * 128)
+    if taken:
+        assert _attn(c, **kw) == INVALID and "null context" in _said(), _said()
+    else:
+        assert _attn(c, **kw) == UNSUPPORTED and "query rows" in _said(), _said()
+        assert lp.lib().lp_attn_paged_ws_bytes(c, heads, batch, tokens, max_q, 60) == 0
