@@ -1234,6 +1234,7 @@ static PagedPlan paged_plan(const lp_kv_cache* c, int heads, int batch, int toke
     p.max_seq = (int)std::min<int64_t>(max_seq, (int64_t)c->max_pages * c->page_rows);
     p.rows = p.max_q * (heads / c->kv_heads);
     p.splits = 1, p.span = INT32_MAX;
+    if (!p.rows) return p;  // nothing to do: no workspace
     const int pairs = batch * c->kv_heads;
     if (p.rows <= kFewRows) {
         // a workgroup's unit: a chunk for each of its four waves

@@ -5,7 +5,7 @@ import pytest
 
 import llmpager_amd as lp
 from _paged import q4
-from test_paged_host import INVALID, UNSUPPORTED, _attn, _cache, _said
+from test_paged_host import INVALID, P, UNSUPPORTED, _attn, _cache, _logprobs, _said
 
 
 def test_scales_that_a_q4_page_may_hold():
@@ -49,3 +49,40 @@ def test_bounds_of_the_query_rows(kv, heads, batch, tokens, max_q, taken):
     else:
         assert _attn(c, **kw) == UNSUPPORTED and "query rows" in _said(), _said()
         assert lp.lib().lp_attn_paged_ws_bytes(c, heads, batch, tokens, max_q, 60) == 0
+
+
+@pytest.mark.parametrize("kw", [dict(tokens=0), dict(max_q=0), dict(batch=0), dict(tokens=0, batch=0)])
+def test_a_call_without_queries_needs_no_workspace(kw):
+    c = _cache(max_pages=4096)
+    n = dict(batch=2, tokens=3, max_q=2)
+    n.update(kw)
+    assert lp.lib().lp_attn_paged_ws_bytes(c, 4, n["batch"], n["tokens"], n["max_q"], 60000) == 0
+    assert _attn(c, workspace=0, ws_bytes=0, max_seq=60000, **kw) == INVALID and "null context" in _said(), _said()
+
+
+@pytest.mark.parametrize("kw,attn", [
+    (dict(), True), (dict(tokens=900, max_q=900, q_stride=1024), True), (dict(tokens=20000, max_q=20000, batch=50), False)])
+def test_workspaces_of_calls_that_need_one(kw, attn):
+    """What test_workspaces_checked looks at where a workspace is needed, and calls
+    that are known to need one."""
+    c = _cache(max_pages=4096)
+    n = dict(batch=2, tokens=3, max_q=2, max_seq=60000)
+    n.update(kw)
+    need = lp.lib().lp_attn_paged_ws_bytes(c, 4, n["batch"], n["tokens"], n["max_q"], 60000)
+    assert (need > 0) == attn
+    kw = dict(n, ws_bytes=need)
+    assert _attn(c, **kw) == INVALID and "null context" in _said()
+    if attn:
+        assert _attn(c, **dict(kw, ws_bytes=need - 1)) == INVALID and "workspace" in _said()
+        assert _attn(c, **dict(kw, workspace=0)) == INVALID and "null workspace" in _said()
+        assert _attn(c, **dict(kw, workspace=P + 64)) == UNSUPPORTED and "workspace" in _said()
+
+
+def test_log_probabilities_that_need_a_workspace():
+    need = lp.lib().lp_logprobs_ws_bytes(2, 151936, 5)
+    assert need > 0 and lp.lib().lp_logprobs_ws_bytes(3000, 151936, 5) == 0
+    kw = dict(vocab=151936, stride=151936)
+    assert _logprobs(ws_bytes=need, **kw) == INVALID and "null context" in _said()
+    assert _logprobs(ws_bytes=need - 1, **kw) == INVALID and "workspace" in _said()
+    assert _logprobs(workspace=0, **kw) == INVALID and "null workspace" in _said()
+    assert _logprobs(workspace=P + 64, **kw) == UNSUPPORTED and "workspace" in _said()
