@@ -266,11 +266,13 @@ uint64_t lp_kv_page_bytes(int page_rows, int head_dim, int format);
  * both factors times mscale; queries to q_out, keys and values into their
  * pages.  q, k, v and q_out are f32 rows, tokens *_stride floats apart (a
  * multiple of 4; 16-byte aligned), so they may be parts of one projection's
- * output; q_out may be q.  An fp16 page rounds to nearest even.  A q4 page
- * takes scale = max|x| / 7 of each group, rounded to 7 significant bits and kept
- * within 2^-17 .. 896, and round(x / scale) within -7 .. 7 (NaN as 0), of
+ * output; q_out may be q, with q's stride (what is written must not overlap
+ * other tokens' rows that are read).  An fp16 page rounds to nearest even.  A q4
+ * page takes scale = max|x| / 7 of each group, rounded to 7 significant bits and
+ * kept within 2^-17 .. 896, and round(x / scale) within -7 .. 7 (NaN as 0), of
  * values computed in 64 bits.  k_out, v_out (f32 [tokens, kv_heads, head_dim],
- * or 0): also the rows as the pages hold them.  A position outside the table's
+ * or 0): also the rows as the pages hold them; they may be k and v where these
+ * lie so.  A position outside the table's
  * width is not appended.  Two tokens with one place leave a mixture of the two
  * there. */
 int lp_kv_append_paged(lp_ctx* ctx, const lp_kv_cache* cache, uint64_t q, int q_stride, uint64_t k, int k_stride,
