@@ -487,7 +487,8 @@ __device__ __forceinline__ void write_ximage(const lpk::RouteArgs& a, int t) {
 // image copies behind a tile's weight loads; the callers wait explicitly.  Base
 // may come from a vector register just before (v_readfirstlane): a memory
 // instruction may read such a scalar register five wait states later, which the
-// compiler does not count for an asm statement.
+// compiler does not count for an asm statement.  (lp_moe_gateup_bal at 32 tokens
+// 42.3 us, and 42.3 with one wait where a base is made.)
 __device__ __forceinline__ void lds_copy16(uint64_t base, uint32_t off, uint32_t lds) {
     asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
 }
