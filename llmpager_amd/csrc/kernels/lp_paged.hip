@@ -1494,8 +1494,9 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
             if (!whole) mask(c, 0, s0);
             float mx = top(s0);
             if (__ballot(mx > m + (kLift + kSlack))) scale(raise(mx));
-            // (the wave that is further goes first: 12 sequences' 80 rows 36.1 us without, 34.5
-            // with it, one prompt of 2,048 83.3 and 85.8)
+            // (the wave that is further goes first: 12 sequences' 80 rows 40.8 us without, 39.3
+            // with it, 2,048 tokens behind 14,000 852 and 832, two of 1,000 of dim 64 117 and
+            // 111; without context, 2,048 tokens or six prompts, both 84 and 55.8)
             __builtin_amdgcn_s_setprio(1);
             float base = m == -INFINITY ? 0.0f : m;
             uint32_t hi[8], lo[8];
