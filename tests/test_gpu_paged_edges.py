@@ -176,6 +176,20 @@ def test_one_row_above_many_few_query_rows(cuda, K, fmt, dim, seqs, heads, new, 
     Shared(cuda, fmt, dim, rows, at, gap, seqs, new, heads, seed=int(gap)).check(K)
 
 
+RISING = (np.array([100, 3000, 6000, 20000]), np.array([[13.0], [17.0], [24.0], [33.0]]))
+FALLING = (np.array([100, 3000, 6000, 20000]), np.array([[33.0], [30.0], [22.0], [19.0]]))
+
+
+@FORMATS
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("at,gap", [RISING, FALLING])
+@pytest.mark.parametrize("seqs,new,heads,pad", [(1, 5, 8, 8192), (512, 1, 2, 0)])
+def test_rows_above_what_came_before(cuda, K, fmt, dim, at, gap, seqs, new, heads, pad):
+    """Four large rows one behind the other: sums put aside at one base and met at
+    another, by many query rows and by few."""
+    Shared(cuda, fmt, dim, 33001, at, gap, seqs, new, heads, pad=pad, seed=dim).check(K, max_q=8192 if pad else None)
+
+
 @FORMATS
 @pytest.mark.parametrize("rows,gap", [(8192, 17.0), (100003, 18.0)])
 def test_one_row_above_many_in_parts(cuda, K, fmt, rows, gap):
