@@ -699,6 +699,7 @@ __device__ __forceinline__ void few_part(const AttnPagedArgs& a, uint8_t* lds, c
         }
     };
     int until_fold = 1;  // (a context's first row is often the large one)
+    bool odd_may = false;
     for (; c < r1; c += 4 * CR) {
         wait_loads<F::kValOps>();  // the keys (and scales) are here
         // a bit per block of 16 rows: its page is there
@@ -850,6 +851,7 @@ __device__ __forceinline__ void few_part(const AttnPagedArgs& a, uint8_t* lds, c
                 __builtin_amdgcn_wave_barrier();
             }
         }
+        odd_may |= whole || apart;
         if (apart) {
             // row by row, each for the queries that see it
 #pragma unroll
@@ -925,10 +927,10 @@ __device__ __forceinline__ void few_part(const AttnPagedArgs& a, uint8_t* lds, c
             wait_loads<63>();  // the values are read
             send_values(c + 4 * CR);
         }
-        if (--until_fold == 0) fold(), until_fold = F::kFold;
+        if (more && --until_fold == 0) fold(), until_fold = F::kFold;
     }
     fold();
-    if constexpr (!Q4) {
+    if (!Q4 && odd_may) {
         f32x4_t odd = {0.0f, 0.0f, 0.0f, 0.0f};  // or NaN
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
