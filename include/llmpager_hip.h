@@ -288,7 +288,9 @@ int lp_kv_append_paged(lp_ctx* ctx, const lp_kv_cache* cache, uint64_t q, int q_
  * sequence: a sequence's tokens past its first max_q are left as they were, a
  * larger length is taken as max_seq (or as what the table's width holds).
  * batch x kv_heads x blocks of 128 query rows (of max_q x heads / kv_heads, max_q
- * at most tokens) is below 2^23.  The bounds decide how the work is split, so a capture may be replayed with other
+ * at most tokens) is below 2^23.  The bounds decide how the work is split, for
+ * all sequences alike (single tokens beside a long prompt: two calls, each over
+ * its sequences, are faster), so a capture may be replayed with other
  * q_starts, seq_lens and tables within them.  q and out: f32 rows as above,
  * which must not overlap.  The products take q scale log2(e), below 2^16, to
  * 2^-22 of each value or, of one below 1/8, to 2^-25: a score is off by the sum

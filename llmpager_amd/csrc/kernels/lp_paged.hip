@@ -417,7 +417,7 @@ __device__ __forceinline__ uint64_t rec_sums(const AttnPagedArgs& a) {
 // (lengths, pages, first rows, join) where they are few: 64 sequences of up to
 // 4,000 16-bit rows 70 us, 4.6 TB/s; 32 of up to 8,192 4-bit rows 31 us, 3.2 TB/s
 // with some 9 us before the first and after the last row, 5.2 in between; one of
-// 1,500 rows 10.5 us.
+// 1,500 rows 10.8 us.
 // ---------------------------------------------------------------------------
 template <int D, bool Q4>
 struct Few {
@@ -1106,12 +1106,12 @@ LP_ATTN_FEW(q4_d128_n2, 1, 128, true, 2)
 // 100,000: 6.4e-3 off without this and kLift, 9e-6 with them; at worst, every time that
 // a wave looks, 2,048 tokens behind 6,001 rows take 440 us instead of 410).
 //
-// 2,048 tokens of 32 heads on 4 KV heads behind 6,001 rows of 16 bits: 410 to 430
-// us, 550 to 575 TFLOP/s of the formula's and twice that of MFMA work, what a large fp16 product
+// 2,048 tokens of 32 heads on 4 KV heads behind 6,001 rows of 16 bits: 407 to 418
+// us, 565 to 580 TFLOP/s of the formula's and twice that of MFMA work, what a large fp16 product
 // reaches; 12 sequences of up to 5 tokens, 16 heads to a KV head, behind up to
-// 6,000 rows of 4 bits: 34 us, of which a chunk takes about 2.8 us (the steps' vector
+// 6,000 rows of 4 bits: 35 us, of which a chunk takes about 2.8 us (the steps' vector
 // work, a wave's alone) and the launch with what comes before the first one 10; six
-// prompts of up to 700 tokens, 32 heads on 4: 52 us, the longest one's last tiles.
+// prompts of up to 700 tokens, 32 heads on 4: 53 us, the longest one's last tiles.
 // (Pages looked at as soon as asked for: 424 us, the prompts of one length 87
 // against 81.)
 // ---------------------------------------------------------------------------
