@@ -303,6 +303,83 @@ int lp_attn_paged(lp_ctx* ctx, const lp_kv_cache* cache, uint64_t q, int q_strid
                   int heads, uint64_t q_starts, uint64_t seq_lens, int batch, int tokens, int max_q, int max_seq,
                   float scale, uint64_t workspace, uint64_t ws_bytes, lp_stream s);
 
+/* ---- a step with drafted tokens ---------------------------------------------
+ * No reference counterparts.  The new tokens of a sequence are a tree: token
+ * q_starts[b] + i is its node i and parents[q_starts[b] + i] (device i32 [tokens])
+ * the node that it is drafted to follow, a lower one; with any other value it follows
+ * none.  Node 0 is the sequence's last token, drawn but not yet in the cache.  Node i
+ * of n has row p0 + i of the cache, p0 = seq_lens[b] - n, so rows and positions differ:
+ * node i stands at position p0 + its depth.  A step: lp_tree_layout; in each layer
+ * lp_kv_append_tree and lp_attn_tree; the lm_head; lp_verify_tree; lp_kv_keep.
+ * q_starts, seq_lens, padding and batch as for lp_kv_append_paged. */
+
+/* For each token depths[t] (i32), the nodes above it, and masks[t] (u64 [tokens,
+ * ceil(max_q / 64)]): bit j % 64 of word j / 64 for node j above it and itself.  A
+ * sequence has at most max_q tokens, max_q at most 1024; tokens past these are left as
+ * they were. */
+int lp_tree_layout(lp_ctx* ctx, uint64_t parents, uint64_t q_starts, int batch, int tokens, int max_q,
+                   uint64_t depths, uint64_t masks, lp_stream s);
+
+/* lp_kv_append_paged, but the angles are those of position p0 + depths[t] (device
+ * i32 [tokens], lp_tree_layout's or the caller's own). */
+int lp_kv_append_tree(lp_ctx* ctx, const lp_kv_cache* cache, uint64_t q, int q_stride, uint64_t k, int k_stride,
+                      uint64_t v, int v_stride, uint64_t q_norm, uint64_t k_norm, float eps, uint64_t inv_freq,
+                      float mscale, uint64_t q_out, int q_out_stride, uint64_t k_out, uint64_t v_out, int heads,
+                      uint64_t q_starts, uint64_t seq_lens, uint64_t depths, int batch, int tokens, lp_stream s);
+
+/* lp_attn_paged, but a token sees all rows before its sequence's new ones and, of
+ * these, row p0 + j where bit j of its mask is set (device u64 [tokens, ceil(max_q /
+ * 64)], 8-byte aligned; lp_tree_layout's, or any others: one without its own bit does not
+ * see itself, one without any in a sequence without other rows gets zeros).  Bits
+ * behind the sequence's tokens, or its first max_q, count as not set.  max_q at most 1024;
+ * the rest, the workspace among it, as for lp_attn_paged. */
+uint64_t lp_attn_tree_ws_bytes(const lp_kv_cache* cache, int heads, int batch, int tokens, int max_q, int max_seq);
+int lp_attn_tree(lp_ctx* ctx, const lp_kv_cache* cache, uint64_t q, int q_stride, uint64_t out, int out_stride,
+                 int heads, uint64_t q_starts, uint64_t seq_lens, uint64_t masks, int batch, int tokens, int max_q,
+                 int max_seq, float scale, uint64_t workspace, uint64_t ws_bytes, lp_stream s);
+
+/* Which drafted tokens stay.  logits: the target's, one f32 row a token, `stride`
+ * floats apart (-inf: a token that cannot be drawn); drafts (i32 [tokens]): the nodes'
+ * tokens (a root's is not looked at; one outside the vocabulary never stays);
+ * temperatures (f32 [batch], 0: all 1): of sequence b, p(x) of a row is e^(logit / T) over its
+ * sum, and with T <= 0 (or NaN) 1 for the largest logit, of equal ones the lowest id;
+ * uniforms: f32 [tokens] in 0 <= u < 1, independent of one another.  The walk begins
+ * at node 0 and ends at a node without a child that stays, or after max_depth (below
+ * 1024) drafted ones.
+ *   probs = 0, drafts that were chosen: node i draws a token, the first whose p with
+ * those of all lower ids is above uniforms[i].  The lowest child of i with that token stays and
+ * the walk goes on there; where there is none, the token is next[b].
+ *   probs, drafts that were sampled: row i (f32, `probs_stride` floats apart, >= 0) is the
+ * distribution q from which i's children were drawn, one by one.  They are tried in
+ * order, with p' = p: child c stays if uniforms[c] q(token) < p'(token), else p' becomes
+ * max(p' - q, 0) over its sum (p itself where that is 0).  next[b] is drawn from the last node's p' by
+ * uniforms of node 0.  T <= 0: the first child with the largest logit's token stays.
+ * Either way the tokens that stay and next have the target's distribution.
+ * path (i32 [batch, max_depth + 1]): the nodes that stay, from node 0 on, then -1;
+ * kept[b] their number; next[b] the token behind them.  A row with a NaN, with +inf or with
+ * nothing but -inf ends the walk with next[b] = -1, and a sequence without tokens has
+ * kept 0 and next -1.  Exponentials are good to 2^-41 and sums are in 64 bits.  vocab
+ * at most 2^19.
+ * workspace: lp_verify_tree_ws_bytes bytes (with_probs: whether probs is given),
+ * 256-byte aligned; two calls that overlap, replays of graphs among them, need one
+ * each.  Sampled drafts of which several are turned down in a sequence go on there with one
+ * workgroup, row by row: chains turn down one at most. */
+uint64_t lp_verify_tree_ws_bytes(int vocab, int batch, int tokens, int max_q, int max_depth, int with_probs);
+int lp_verify_tree(lp_ctx* ctx, uint64_t logits, int stride, int vocab, uint64_t drafts, uint64_t parents,
+                   uint64_t q_starts, int batch, int tokens, int max_q, int max_depth, uint64_t temperatures,
+                   uint64_t probs, int probs_stride, uint64_t uniforms, uint64_t path, uint64_t kept, uint64_t next,
+                   uint64_t workspace, uint64_t ws_bytes, lp_stream s);
+
+/* The rows of the tokens that stay, one behind the other: row p0 + i of sequence b
+ * becomes what row p0 + path[b][i] was, i < kept[b] (at most max_depth + 1 and the
+ * sequence's tokens), in the keys and values of `layers` caches (a host array) that share
+ * their table and shapes.  path must rise; an entry that is no node of the sequence, or
+ * a row whose page is not there, moves nothing.  lens_out (device i32 [batch], not
+ * seq_lens, or 0): the lengths then, p0 + kept[b]: the next step's new tokens come on top
+ * of them. */
+int lp_kv_keep(lp_ctx* ctx, const lp_kv_cache* caches, int layers, uint64_t path, int max_depth, uint64_t kept,
+               uint64_t q_starts, uint64_t seq_lens, uint64_t lens_out, int batch, lp_stream s);
+
 /* ---- logits ---------------------------------------------------------------- */
 
 /* Log probabilities from rows of logits (f32 [vocab], `stride` floats apart;

@@ -141,6 +141,16 @@ def _sig(lib):
         "lp_attn_paged_ws_bytes": (u64, [P(KvCache), i32, i32, i32, i32, i32]),
         "lp_attn_paged": (i32, [vp, P(KvCache), u64, i32, u64, i32, i32, u64, u64, i32, i32, i32, i32, f32, u64, u64,
                                 vp]),
+        "lp_tree_layout": (i32, [vp, u64, u64, i32, i32, i32, u64, u64, vp]),
+        "lp_kv_append_tree": (i32, [vp, P(KvCache), u64, i32, u64, i32, u64, i32, u64, u64, f32, u64, f32, u64, i32, u64,
+                                    u64, i32, u64, u64, u64, i32, i32, vp]),
+        "lp_attn_tree_ws_bytes": (u64, [P(KvCache), i32, i32, i32, i32, i32]),
+        "lp_attn_tree": (i32, [vp, P(KvCache), u64, i32, u64, i32, i32, u64, u64, u64, i32, i32, i32, i32, f32, u64, u64,
+                               vp]),
+        "lp_verify_tree_ws_bytes": (u64, [i32, i32, i32, i32, i32, i32]),
+        "lp_verify_tree": (i32, [vp, u64, i32, i32, u64, u64, u64, i32, i32, i32, i32, u64, u64, i32, u64, u64, u64, u64,
+                                 u64, u64, vp]),
+        "lp_kv_keep": (i32, [vp, P(KvCache), i32, u64, i32, u64, u64, u64, u64, i32, vp]),
         "lp_logprobs_ws_bytes": (u64, [i32, i32, i32]),
         "lp_logprobs": (i32, [vp, u64, i32, i32, i32, u64, u64, u64, i32, u64, u64, u64, u64, vp]),
         "lp_moe_ws_layout_get": (i32, [P(LayerDesc), i32, P(WsLayout)]),
@@ -587,6 +597,54 @@ class Kernels:
         DevPtr or an address with `ws_bytes` given."""
         _check(lib().lp_attn_paged(self.cuda.ctx, cache, q, q_stride, out, out_stride, heads, q_starts, seq_lens,
                                    batch, tokens, max_q, max_seq, scale, ws, _ws_bytes(ws, ws_bytes), stream))
+
+    # a step with drafted tokens (no kernels.rs counterparts)
+    def tree_layout(self, parents: int, q_starts: int, batch: int, tokens: int, max_q: int, depths: int, masks: int,
+                    stream=None) -> None:
+        """Depths of trees' nodes, and masks of the nodes above each and itself."""
+        _check(lib().lp_tree_layout(self.cuda.ctx, parents, q_starts, batch, tokens, max_q, depths, masks, stream))
+
+    def kv_append_tree(self, cache: KvCache, q: int, q_stride: int, k: int, k_stride: int, v: int, v_stride: int,
+                       q_norm: int, k_norm: int, eps: float, inv_freq: int, mscale: float, q_out: int,
+                       q_out_stride: int, k_out: int, v_out: int, heads: int, q_starts: int, seq_lens: int, depths: int,
+                       batch: int, tokens: int, stream=None) -> None:
+        """kv_append_paged with the angles of the nodes' depths."""
+        _check(lib().lp_kv_append_tree(self.cuda.ctx, cache, q, q_stride, k, k_stride, v, v_stride, q_norm, k_norm,
+                                       eps, inv_freq, mscale, q_out, q_out_stride, k_out, v_out, heads, q_starts,
+                                       seq_lens, depths, batch, tokens, stream))
+
+    def attn_tree_ws_bytes(self, cache: KvCache, heads: int, batch: int, tokens: int, max_q: int, max_seq: int) -> int:
+        return int(lib().lp_attn_tree_ws_bytes(cache, heads, batch, tokens, max_q, max_seq))
+
+    def attn_tree(self, cache: KvCache, q: int, q_stride: int, out: int, out_stride: int, heads: int, q_starts: int,
+                  seq_lens: int, masks: int, batch: int, tokens: int, max_q: int, max_seq: int, scale: float, ws: int,
+                  stream=None, ws_bytes: int | None = None) -> None:
+        """Attention of a batch's new tokens over their contexts and, of the new
+        rows, those that their masks name."""
+        _check(lib().lp_attn_tree(self.cuda.ctx, cache, q, q_stride, out, out_stride, heads, q_starts, seq_lens, masks,
+                                  batch, tokens, max_q, max_seq, scale, ws, _ws_bytes(ws, ws_bytes), stream))
+
+    def verify_tree_ws_bytes(self, vocab: int, batch: int, tokens: int, max_q: int, max_depth: int, with_probs: bool) -> int:
+        return int(lib().lp_verify_tree_ws_bytes(vocab, batch, tokens, max_q, max_depth, int(with_probs)))
+
+    def verify_tree(self, logits: int, stride: int, vocab: int, drafts: int, parents: int, q_starts: int, batch: int,
+                    tokens: int, max_q: int, max_depth: int, temperatures: int, probs: int, probs_stride: int,
+                    uniforms: int, path: int, kept: int, next_: int, ws: int, stream=None,
+                    ws_bytes: int | None = None) -> None:
+        """The drafted tokens that the target's logits keep, and the token behind
+        them (probs: 0, or the distributions that the drafts were drawn from)."""
+        _check(lib().lp_verify_tree(self.cuda.ctx, logits, stride, vocab, drafts, parents, q_starts, batch, tokens,
+                                    max_q, max_depth, temperatures, probs, probs_stride, uniforms, path, kept, next_,
+                                    ws, _ws_bytes(ws, ws_bytes), stream))
+
+    def kv_keep(self, caches, path: int, max_depth: int, kept: int, q_starts: int, seq_lens: int, lens_out: int,
+                batch: int, stream=None) -> None:
+        """The kept nodes' rows one behind the other in all layers' `caches` (a
+        sequence of KvCache, or a ctypes array of them)."""
+        if not isinstance(caches, C.Array):
+            caches = (KvCache * len(caches))(*caches)
+        _check(lib().lp_kv_keep(self.cuda.ctx, caches, len(caches), path, max_depth, kept, q_starts, seq_lens, lens_out,
+                                batch, stream))
 
     def logprobs_ws_bytes(self, rows: int, vocab: int, top: int) -> int:
         return int(lib().lp_logprobs_ws_bytes(rows, vocab, top))

@@ -4,7 +4,8 @@ Outputs (under llmpager_amd/lib/):
   lp_basic.hsaco, lp_moe.hsaco,
   lp_gemm.hsaco, lp_attn.hsaco,
   lp_step.hsaco, lp_mid.hsaco,
-  lp_paged.hsaco, lp_logits.hsaco kernels, hipcc --genco --offload-arch=gfx950
+  lp_paged.hsaco, lp_logits.hsaco,
+  lp_tree.hsaco, lp_verify.hsaco  kernels, hipcc --genco --offload-arch=gfx950
   libllmpager_hip.so              host runtime (g++), loads the code objects
                                   with hipModuleLoad at lp_init
 
@@ -26,7 +27,7 @@ ROOT = os.path.dirname(HERE)
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
 KERNEL_SOURCES = ["lp_basic.hip", "lp_moe.hip", "lp_gemm.hip", "lp_attn.hip", "lp_step.hip",
-                  "lp_mid.hip", "lp_paged.hip", "lp_logits.hip"]
+                  "lp_mid.hip", "lp_paged.hip", "lp_logits.hip", "lp_tree.hip", "lp_verify.hip"]
 HOST_SOURCES = ["lp_runtime.cpp", "lp_synth.cpp", "lp_cache.cpp", "lp_pager.cpp", "lp_pack.cpp"]
 HOST_HIP_SOURCES = ["lp_noalloc.hip"]
 

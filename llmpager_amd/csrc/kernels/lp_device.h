@@ -810,6 +810,18 @@ __device__ __forceinline__ float quad_rows(float s, float t) {
 // quad_rows result.
 __device__ __forceinline__ constexpr int quad_row_tok(int r) { return 2 * (r & 1) + (r >> 1); }
 
+// The token's sequence: the sequences that end at or before it (batch for a token
+// behind the last one; a token before the first one's start is none of sequence 0's).
+__device__ __forceinline__ int sequence_of(uint64_t q_starts, int batch, int token) {
+    int b = 0;
+    for (int i = 0; i < batch; i += 64) {
+        const int at = i + lane_id();
+        const bool past = at < batch && gptr<int>(q_starts)[at + 1] <= token;
+        b += __popcll(__ballot(past));
+    }
+    return __builtin_amdgcn_readfirstlane(b);
+}
+
 __device__ __forceinline__ int ilog2_pow2(int v) { return 31 - __builtin_clz(v); }
 
 }  // namespace lp

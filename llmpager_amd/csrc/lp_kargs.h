@@ -349,6 +349,7 @@ struct KvAppendPagedArgs {
     int32_t parts, rows_per_part;   // waves per token, and the rows (q, k and v heads) of each
     float eps, mscale;
     int32_t pad0;
+    uint64_t depths;                // i32 [tokens], where tokens are nodes of trees
 };
 
 struct AttnPagedArgs {
@@ -366,7 +367,30 @@ struct AttnPagedArgs {
     uint64_t sync;
     // lp_attn_many_*: workgroups of kManyRows query rows; rows of the context per
     // workgroup, and records per query row
-    int32_t tiles, splits, span, pad0;
+    int32_t tiles, splits, span;
+    // lp_attn_tree_*: u64 [tokens, words], bit j of a token's: it sees its sequence's new token j
+    int32_t words;
+    uint64_t masks;
+};
+
+constexpr int kTreeMaxNodes = 1024;    // new tokens of a sequence that is a tree
+
+struct TreeLayoutArgs {
+    uint64_t parents, q_starts;     // i32 [tokens], [batch + 1]
+    uint64_t depths, masks;         // i32 [tokens], u64 [tokens, words]
+    int32_t batch, tokens, max_q, words;
+};
+
+// lp_kv_keep_*: layers of a launch (its arguments hold their pools), and units of a
+// layer's rows that a wave moves.
+constexpr int kKeepLayers = 64;
+LPK_HD constexpr int keep_units(bool q4) { return q4 ? 192 : 128; }
+struct KvKeepArgs {
+    PagedCache c;                   // the table and shapes, which the layers share
+    uint64_t path, kept;            // i32 [batch, max_depth + 1], [batch]
+    uint64_t q_starts, seq_lens, lens_out;
+    int32_t batch, max_depth, layers, chunks;  // waves of a (sequence, layer)
+    uint64_t k_pages[kKeepLayers], v_pages[kKeepLayers];
 };
 
 struct LogprobArgs {
@@ -379,6 +403,30 @@ struct LogprobArgs {
     int32_t parts, per_part;        // workgroups of a row, and the logits of each (a multiple of kLogprobStep)
 };
 LPK_HD constexpr int logprob_rec(int top) { return 32 + 8 * top; }
+
+// Verification of drafted tokens.  A row's records: one a block of kVerifyBlock
+// logits, kVerifyLane a lane where they are joined.
+constexpr int kVerifyBlock = 1024;
+constexpr int kVerifyLane = 8;
+constexpr int kVerifyMaxVocab = 64 * kVerifyLane * kVerifyBlock;
+constexpr int kVerifyWaves = 16;       // of a workgroup of lp_verify_left
+struct VerifyState {                   // a sequence's walk down its tree
+    int32_t cur, last, len, pending;   // node; children up to it were tried; nodes so far; a pass is due
+    double taken, left;                // p - taken q is what is left of the row's distribution, `left` in all
+};
+struct VerifyArgs {
+    uint64_t logits, drafts, parents, q_starts;  // f32 rows; i32 [tokens], [tokens], [batch + 1]
+    uint64_t temps, probs, uniforms;   // f32 [batch] or 0; f32 rows or 0; f32 [tokens]
+    uint64_t path, kept, next;         // i32 [batch, max_depth + 1], [batch], [batch]
+    uint64_t part;                     // records [rows, blocks] of 16 bytes
+    uint64_t stats;                    // [tokens]: a row's sum, largest logit and draw, 16 bytes
+    uint64_t left;                     // f64 [batch, blocks]: sums of what is left of a row
+    uint64_t state;                    // VerifyState [batch]; by levels i32 [batch]
+    uint64_t sync;                     // arrival counters of the rows, then of the sequences
+    int32_t stride, probs_stride, vocab, batch, tokens, max_q, max_depth;
+    int32_t blocks, parts, per_part;   // blocks of a row; workgroups of a row and their blocks
+    int32_t level, row_counters;
+};
 
 struct ClearArgs {
     uint64_t at;  // 32-bit words to be 0

@@ -149,6 +149,32 @@ enum Fn {
     kLogprobs,
     kLogprobsTop,
     kClearWords,
+    kAppendTreeF16D64,
+    kAppendTreeF16D128,
+    kAppendTreeQ4D64,
+    kAppendTreeQ4D128,
+    kAttnTreeManyF16D64,
+    kAttnTreeManyF16D128,
+    kAttnTreeManyQ4D64,
+    kAttnTreeManyQ4D128,
+    kAttnTreeFewF16D64,
+    kAttnTreeFewF16D128,
+    kAttnTreeFewQ4D64,
+    kAttnTreeFewQ4D128,
+    kAttnTreeFewF16D64N2,
+    kAttnTreeFewF16D128N2,
+    kAttnTreeFewQ4D64N2,
+    kAttnTreeFewQ4D128N2,
+    kAttnTreeJoinD64,
+    kAttnTreeJoinD128,
+    kTreeLayout,
+    kKeepF16D64,
+    kKeepF16D128,
+    kKeepQ4D64,
+    kKeepQ4D128,
+    kVerifyRows,
+    kVerifyLeft,
+    kVerifyLevel,
     kNumFns
 };
 
@@ -212,11 +238,26 @@ const FnSpec kSpecs[kNumFns] = {
     {"lp_paged.hsaco", "lp_attn_join_d64"}, {"lp_paged.hsaco", "lp_attn_join_d128"},
     {"lp_logits.hsaco", "lp_logprobs"},      {"lp_logits.hsaco", "lp_logprobs_top"},
     {"lp_logits.hsaco", "lp_clear_words"},
+    {"lp_tree.hsaco", "lp_kv_append_tree_f16_d64"}, {"lp_tree.hsaco", "lp_kv_append_tree_f16_d128"},
+    {"lp_tree.hsaco", "lp_kv_append_tree_q4_d64"}, {"lp_tree.hsaco", "lp_kv_append_tree_q4_d128"},
+    {"lp_tree.hsaco", "lp_attn_tree_many_f16_d64"}, {"lp_tree.hsaco", "lp_attn_tree_many_f16_d128"},
+    {"lp_tree.hsaco", "lp_attn_tree_many_q4_d64"}, {"lp_tree.hsaco", "lp_attn_tree_many_q4_d128"},
+    {"lp_tree.hsaco", "lp_attn_tree_few_f16_d64"}, {"lp_tree.hsaco", "lp_attn_tree_few_f16_d128"},
+    {"lp_tree.hsaco", "lp_attn_tree_few_q4_d64"}, {"lp_tree.hsaco", "lp_attn_tree_few_q4_d128"},
+    {"lp_tree.hsaco", "lp_attn_tree_few_f16_d64_n2"}, {"lp_tree.hsaco", "lp_attn_tree_few_f16_d128_n2"},
+    {"lp_tree.hsaco", "lp_attn_tree_few_q4_d64_n2"}, {"lp_tree.hsaco", "lp_attn_tree_few_q4_d128_n2"},
+    {"lp_tree.hsaco", "lp_attn_tree_join_d64"}, {"lp_tree.hsaco", "lp_attn_tree_join_d128"},
+    {"lp_tree.hsaco", "lp_tree_layout"},
+    {"lp_tree.hsaco", "lp_kv_keep_f16_d64"}, {"lp_tree.hsaco", "lp_kv_keep_f16_d128"},
+    {"lp_tree.hsaco", "lp_kv_keep_q4_d64"}, {"lp_tree.hsaco", "lp_kv_keep_q4_d128"},
+    {"lp_verify.hsaco", "lp_verify_rows"},   {"lp_verify.hsaco", "lp_verify_left"},
+    {"lp_verify.hsaco", "lp_verify_level"},
 };
 
 const char* const kModules[] = {"lp_basic.hsaco", "lp_moe.hsaco", "lp_gemm.hsaco", "lp_attn.hsaco",
-                                "lp_step.hsaco", "lp_mid.hsaco", "lp_paged.hsaco", "lp_logits.hsaco"};
-constexpr int kNumModules = 8;
+                                "lp_step.hsaco", "lp_mid.hsaco", "lp_paged.hsaco", "lp_logits.hsaco",
+                                "lp_tree.hsaco", "lp_verify.hsaco"};
+constexpr int kNumModules = 10;
 
 std::string library_dir() {
     Dl_info info;
@@ -1130,29 +1171,33 @@ static int check_batch(const char* who, int heads, int kv_heads, int batch, int 
     return LP_OK;
 }
 
-int lp_kv_append_paged(lp_ctx* c, const lp_kv_cache* cache, uint64_t q, int q_stride, uint64_t k, int k_stride,
-                       uint64_t v, int v_stride, uint64_t q_norm, uint64_t k_norm, float eps, uint64_t inv_freq,
-                       float mscale, uint64_t q_out, int q_out_stride, uint64_t k_out, uint64_t v_out, int heads,
-                       uint64_t q_starts, uint64_t seq_lens, int batch, int tokens, lp_stream s) {
+// lp_kv_append_paged, or lp_kv_append_tree with its depths.
+static int append_call(const char* name, lp_ctx* c, const lp_kv_cache* cache, uint64_t q, int q_stride, uint64_t k,
+                       int k_stride, uint64_t v, int v_stride, uint64_t q_norm, uint64_t k_norm, float eps,
+                       uint64_t inv_freq, float mscale, uint64_t q_out, int q_out_stride, uint64_t k_out, uint64_t v_out,
+                       int heads, uint64_t q_starts, uint64_t seq_lens, bool tree, uint64_t depths, int batch, int tokens,
+                       lp_stream s) {
+    const std::string who(name);
     KvAppendPagedArgs a{};
-    if (int r = check_paged("kv_append_paged", cache, &a.c)) return r;
-    if (int r = check_batch("kv_append_paged", heads, cache->kv_heads, batch, tokens, q_starts, seq_lens)) return r;
+    if (int r = check_paged(name, cache, &a.c)) return r;
+    if (int r = check_batch(name, heads, cache->kv_heads, batch, tokens, q_starts, seq_lens)) return r;
     const int D = cache->head_dim;
     if ((int64_t)heads + 2 * (int64_t)cache->kv_heads > INT32_MAX / 256)
-        return fail(LP_E_UNSUPPORTED, "kv_append_paged: too many heads");
-    if (int r = check_rows("kv_append_paged: q", q, q_stride, (int64_t)heads * D)) return r;
-    if (int r = check_rows("kv_append_paged: k", k, k_stride, (int64_t)cache->kv_heads * D)) return r;
-    if (int r = check_rows("kv_append_paged: v", v, v_stride, (int64_t)cache->kv_heads * D)) return r;
-    if (int r = check_rows("kv_append_paged: q_out", q_out, q_out_stride, (int64_t)heads * D)) return r;
+        return fail(LP_E_UNSUPPORTED, who + ": too many heads");
+    if (int r = check_rows(who + ": q", q, q_stride, (int64_t)heads * D)) return r;
+    if (int r = check_rows(who + ": k", k, k_stride, (int64_t)cache->kv_heads * D)) return r;
+    if (int r = check_rows(who + ": v", v, v_stride, (int64_t)cache->kv_heads * D)) return r;
+    if (int r = check_rows(who + ": q_out", q_out, q_out_stride, (int64_t)heads * D)) return r;
     if (!inv_freq || inv_freq % 8 || q_norm % 8 || k_norm % 8 || k_out % 16 || v_out % 16)
-        return fail(LP_E_INVALID, "kv_append_paged: null inv_freq, or a misaligned pointer");
+        return fail(LP_E_INVALID, who + ": null inv_freq, or a misaligned pointer");
+    if (tree && (!depths || depths % 4)) return fail(LP_E_INVALID, who + ": depths null or not 4-byte aligned");
     if (int r = check_ctx(c)) return r;
     if (!batch || !tokens) return LP_OK;
     a.q = q, a.k = k, a.v = v, a.q_norm = q_norm, a.k_norm = k_norm, a.inv_freq = inv_freq;
     a.q_out = q_out, a.k_out = k_out, a.v_out = v_out, a.q_starts = q_starts, a.seq_lens = seq_lens;
     a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride, a.q_out_stride = q_out_stride;
     a.heads = heads, a.batch = batch, a.tokens = tokens;
-    a.eps = eps, a.mscale = mscale;
+    a.eps = eps, a.mscale = mscale, a.depths = depths;
     const int rows = heads + 2 * cache->kv_heads, per = 256 / D;  // rows a wave takes at a time
     // Waves that share a token's rows: one pass each while the tokens are few,
     // else about 8192 in all, so that the angles are made less often and a
@@ -1162,10 +1207,17 @@ int lp_kv_append_paged(lp_ctx* c, const lp_kv_cache* cache, uint64_t q, int q_st
     a.rows_per_part = ((rows + want - 1) / want + per - 1) / per * per;
     a.parts = (rows + a.rows_per_part - 1) / a.rows_per_part;
     const int64_t waves = (int64_t)tokens * a.parts;
-    if (waves > INT32_MAX / 256) return fail(LP_E_UNSUPPORTED, "kv_append_paged: too many tokens");
-    const Fn f = cache->format == LP_KV_Q4 ? (D == 64 ? kAppendQ4D64 : kAppendQ4D128)
-                                           : (D == 64 ? kAppendF16D64 : kAppendF16D128);
-    return launch(c, f, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, s, a);
+    if (waves > INT32_MAX / 256) return fail(LP_E_UNSUPPORTED, who + ": too many tokens");
+    const int which = (cache->format == LP_KV_Q4 ? 2 : 0) + (D == 128 ? 1 : 0);
+    return launch(c, (Fn)((tree ? kAppendTreeF16D64 : kAppendF16D64) + which), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, s, a);
+}
+
+int lp_kv_append_paged(lp_ctx* c, const lp_kv_cache* cache, uint64_t q, int q_stride, uint64_t k, int k_stride,
+                       uint64_t v, int v_stride, uint64_t q_norm, uint64_t k_norm, float eps, uint64_t inv_freq,
+                       float mscale, uint64_t q_out, int q_out_stride, uint64_t k_out, uint64_t v_out, int heads,
+                       uint64_t q_starts, uint64_t seq_lens, int batch, int tokens, lp_stream s) {
+    return append_call("kv_append_paged", c, cache, q, q_stride, k, k_stride, v, v_stride, q_norm, k_norm, eps, inv_freq,
+                       mscale, q_out, q_out_stride, k_out, v_out, heads, q_starts, seq_lens, false, 0, batch, tokens, s);
 }
 
 // How attention of many query rows is split over the rows of a context: into
@@ -1207,8 +1259,8 @@ static int join_slot(lp_ctx* c, hipStream_t s, int graph) {
 // stream's, zero between launches.  But what the caller captures into a graph may
 // be replayed beside other calls of that stream and other graphs captured from it, a
 // stream may be one more than the context has counters for, and hipStreamPerThread is
-// one handle for a stream of each host thread: there they are the workspace's, cleared
-// by a launch of its own.
+// one handle for a stream of each host thread: there, and for more than kPagedPairs, they
+// are the workspace's, cleared by a launch of its own.
 static int join_counters(lp_ctx* c, lp_stream s, uint64_t at, int n, uint64_t* sync) {
     int graph;
     {
@@ -1217,7 +1269,7 @@ static int join_counters(lp_ctx* c, lp_stream s, uint64_t at, int n, uint64_t* s
     }
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
     if (graph < 0 && hipStreamIsCapturing((hipStream_t)s, &st) != hipSuccess) (void)hipGetLastError();
-    const bool own = graph >= 0 || (st == hipStreamCaptureStatusNone && (hipStream_t)s != hipStreamPerThread);
+    const bool own = n <= kPagedPairs && (graph >= 0 || (st == hipStreamCaptureStatusNone && (hipStream_t)s != hipStreamPerThread));
     const int slot = own ? join_slot(c, (hipStream_t)s, graph) : -1;
     if (slot >= 0) {
         *sync = reinterpret_cast<uint64_t>(c->join_sync) + (uint64_t)slot * kPagedPairs * kPagedStride * 4;
@@ -1259,21 +1311,38 @@ static PagedPlan paged_plan(const lp_kv_cache* c, int heads, int batch, int toke
 
 // One query row per (token, query head): their number per KV head is a 32-bit one, and
 // their workgroups a grid.
-static int check_queries(int heads, int kv_heads, int batch, int tokens, int max_q, int max_seq) {
-    if (max_q < 0 || max_seq < 0) return fail(LP_E_INVALID, "attn_paged: negative max_q or max_seq");
+static int check_queries(const char* who, int heads, int kv_heads, int batch, int tokens, int max_q, int max_seq) {
+    const std::string w(who);
+    if (max_q < 0 || max_seq < 0) return fail(LP_E_INVALID, w + ": negative max_q or max_seq");
     const int64_t rows = (int64_t)std::min(max_q, tokens) * (heads / kv_heads);
     if (rows > INT32_MAX / 2 || (rows && (int64_t)batch * kv_heads * ((rows + kManyRows - 1) / kManyRows) > INT32_MAX / 256))
-        return fail(LP_E_UNSUPPORTED, "attn_paged: batch x kv_heads x blocks of 128 query rows (max_q x heads / kv_heads) "
-                                      "must be below 2^23");
+        return fail(LP_E_UNSUPPORTED, w + ": batch x kv_heads x blocks of 128 query rows (max_q x heads / kv_heads) "
+                                          "must be below 2^23");
     return LP_OK;
 }
 
-uint64_t lp_attn_paged_ws_bytes(const lp_kv_cache* cache, int heads, int batch, int tokens, int max_q, int max_seq) {
+// New tokens of a sequence that is a tree.
+static int check_nodes(const char* who, int max_q) {
+    if (max_q < 0) return fail(LP_E_INVALID, std::string(who) + ": negative max_q");
+    if (max_q > kTreeMaxNodes)
+        return fail(LP_E_UNSUPPORTED, std::string(who) + ": at most " + std::to_string(kTreeMaxNodes) + " nodes a sequence");
+    return LP_OK;
+}
+
+static uint64_t attn_ws(const char* who, const lp_kv_cache* cache, int heads, int batch, int tokens, int max_q, int max_seq) {
     PagedCache pc;
-    if (check_paged("attn_paged", cache, &pc) || check_batch("attn_paged", heads, cache->kv_heads, batch, tokens, 4, 4) ||
-        check_queries(heads, cache->kv_heads, batch, tokens, max_q, max_seq))
+    if (check_paged(who, cache, &pc) || check_batch(who, heads, cache->kv_heads, batch, tokens, 4, 4) ||
+        check_queries(who, heads, cache->kv_heads, batch, tokens, max_q, max_seq))
         return 0;
     return paged_plan(cache, heads, batch, tokens, max_q, max_seq).bytes;
+}
+
+uint64_t lp_attn_paged_ws_bytes(const lp_kv_cache* cache, int heads, int batch, int tokens, int max_q, int max_seq) {
+    return attn_ws("attn_paged", cache, heads, batch, tokens, max_q, max_seq);
+}
+
+uint64_t lp_attn_tree_ws_bytes(const lp_kv_cache* cache, int heads, int batch, int tokens, int max_q, int max_seq) {
+    return check_nodes("attn_tree", max_q) ? 0 : attn_ws("attn_tree", cache, heads, batch, tokens, max_q, max_seq);
 }
 
 // A workspace of at least `need` bytes (none of 0).
@@ -1288,19 +1357,25 @@ static int check_workspace(const char* who, uint64_t need, uint64_t ws, uint64_t
     return LP_OK;
 }
 
-int lp_attn_paged(lp_ctx* c, const lp_kv_cache* cache, uint64_t q, int q_stride, uint64_t out, int out_stride, int heads,
-                  uint64_t q_starts, uint64_t seq_lens, int batch, int tokens, int max_q, int max_seq, float scale,
-                  uint64_t workspace, uint64_t ws_bytes, lp_stream s) {
+// lp_attn_paged, or lp_attn_tree with its masks.
+static int attn_call(const char* name, lp_ctx* c, const lp_kv_cache* cache, uint64_t q, int q_stride, uint64_t out,
+                     int out_stride, int heads, uint64_t q_starts, uint64_t seq_lens, bool tree, uint64_t masks, int batch,
+                     int tokens, int max_q, int max_seq, float scale, uint64_t workspace, uint64_t ws_bytes, lp_stream s) {
+    const std::string who(name);
     AttnPagedArgs a{};
-    if (int r = check_paged("attn_paged", cache, &a.c)) return r;
-    if (int r = check_batch("attn_paged", heads, cache->kv_heads, batch, tokens, q_starts, seq_lens)) return r;
+    if (int r = check_paged(name, cache, &a.c)) return r;
+    if (int r = check_batch(name, heads, cache->kv_heads, batch, tokens, q_starts, seq_lens)) return r;
     const int D = cache->head_dim;
-    if (int r = check_rows("attn_paged: q", q, q_stride, (int64_t)heads * D)) return r;
-    if (int r = check_rows("attn_paged: out", out, out_stride, (int64_t)heads * D)) return r;
-    if (q == out) return fail(LP_E_INVALID, "attn_paged: out must not be q");
-    if (int r = check_queries(heads, cache->kv_heads, batch, tokens, max_q, max_seq)) return r;
+    if (int r = check_rows(who + ": q", q, q_stride, (int64_t)heads * D)) return r;
+    if (int r = check_rows(who + ": out", out, out_stride, (int64_t)heads * D)) return r;
+    if (q == out) return fail(LP_E_INVALID, who + ": out must not be q");
+    if (tree) {
+        if (int r = check_nodes(name, max_q)) return r;
+        if (!masks || masks % 8) return fail(LP_E_INVALID, who + ": masks null or not 8-byte aligned");
+    }
+    if (int r = check_queries(name, heads, cache->kv_heads, batch, tokens, max_q, max_seq)) return r;
     const PagedPlan plan = paged_plan(cache, heads, batch, tokens, max_q, max_seq);
-    if (int r = check_workspace("attn_paged", plan.bytes, workspace, ws_bytes)) return r;
+    if (int r = check_workspace(name, plan.bytes, workspace, ws_bytes)) return r;
     if (int r = check_ctx(c)) return r;
     if (!batch || !tokens || !max_q) return LP_OK;
     a.q = q, a.out = out, a.q_starts = q_starts, a.seq_lens = seq_lens;
@@ -1308,22 +1383,189 @@ int lp_attn_paged(lp_ctx* c, const lp_kv_cache* cache, uint64_t q, int q_stride,
     a.heads = heads, a.group = heads / cache->kv_heads, a.batch = batch, a.tokens = tokens;
     a.max_q = plan.max_q, a.max_seq = plan.max_seq, a.rows = plan.rows;
     a.splits = plan.splits, a.span = plan.span, a.part = workspace;
-    a.scale = scale;
+    a.scale = scale, a.masks = masks, a.words = (max_q + 63) / 64;
     const int pairs = batch * cache->kv_heads, which = (cache->format == LP_KV_Q4 ? 2 : 0) + (D == 128 ? 1 : 0);
     if (plan.rows <= kFewRows) {
         // (no shares, with more pairs than there are counters: a workgroup per pair)
         a.shares = plan.shares, a.min_units = plan.min_units;
         if (a.shares)
             if (int r = join_counters(c, s, workspace + plan.bytes - (uint64_t)pairs * kPagedStride * 4, pairs, &a.sync)) return r;
-        const Fn f = (Fn)(kAttnFewF16D64 + (plan.rows > 16 ? 4 : 0) + which);
+        const Fn f = (Fn)((tree ? kAttnTreeFewF16D64 : kAttnFewF16D64) + (plan.rows > 16 ? 4 : 0) + which);
         return launch(c, f, dim3((unsigned)(a.shares ? a.shares : pairs)), dim3(256), 0, s, a);
     }
     a.tiles = plan.tiles;
     const unsigned wgs = (unsigned)((int64_t)pairs * plan.tiles * plan.splits);
-    if (int r = launch(c, (Fn)(kAttnManyF16D64 + which), dim3(wgs), dim3(256), 0, s, a)) return r;
+    if (int r = launch(c, (Fn)((tree ? kAttnTreeManyF16D64 : kAttnManyF16D64) + which), dim3(wgs), dim3(256), 0, s, a)) return r;
     if (plan.splits == 1) return LP_OK;
     const int64_t rows = (int64_t)pairs * plan.rows;
-    return launch(c, D == 64 ? kAttnJoinD64 : kAttnJoinD128, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+    return launch(c, (Fn)((tree ? kAttnTreeJoinD64 : kAttnJoinD64) + (D == 128 ? 1 : 0)), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+}
+
+int lp_attn_paged(lp_ctx* c, const lp_kv_cache* cache, uint64_t q, int q_stride, uint64_t out, int out_stride, int heads,
+                  uint64_t q_starts, uint64_t seq_lens, int batch, int tokens, int max_q, int max_seq, float scale,
+                  uint64_t workspace, uint64_t ws_bytes, lp_stream s) {
+    return attn_call("attn_paged", c, cache, q, q_stride, out, out_stride, heads, q_starts, seq_lens, false, 0, batch,
+                     tokens, max_q, max_seq, scale, workspace, ws_bytes, s);
+}
+
+// ---- a step with drafted tokens (lp_tree.hip, lp_verify.hip) ------------------------
+
+int lp_tree_layout(lp_ctx* c, uint64_t parents, uint64_t q_starts, int batch, int tokens, int max_q, uint64_t depths,
+                   uint64_t masks, lp_stream s) {
+    if (int r = check_batch("tree_layout", 1, 1, batch, tokens, q_starts, q_starts)) return r;
+    if (int r = check_nodes("tree_layout", max_q)) return r;
+    if (!parents || !depths || !masks || parents % 4 || depths % 4 || masks % 8)
+        return fail(LP_E_INVALID, "tree_layout: null or misaligned pointer");
+    if (int r = check_ctx(c)) return r;
+    if (!batch || !tokens || !max_q) return LP_OK;
+    TreeLayoutArgs a{parents, q_starts, depths, masks, batch, tokens, max_q, (max_q + 63) / 64};
+    return launch(c, kTreeLayout, dim3((unsigned)(batch * a.words)), dim3(256), 0, s, a);
+}
+
+int lp_kv_append_tree(lp_ctx* c, const lp_kv_cache* cache, uint64_t q, int q_stride, uint64_t k, int k_stride,
+                      uint64_t v, int v_stride, uint64_t q_norm, uint64_t k_norm, float eps, uint64_t inv_freq,
+                      float mscale, uint64_t q_out, int q_out_stride, uint64_t k_out, uint64_t v_out, int heads,
+                      uint64_t q_starts, uint64_t seq_lens, uint64_t depths, int batch, int tokens, lp_stream s) {
+    return append_call("kv_append_tree", c, cache, q, q_stride, k, k_stride, v, v_stride, q_norm, k_norm, eps, inv_freq,
+                       mscale, q_out, q_out_stride, k_out, v_out, heads, q_starts, seq_lens, true, depths, batch, tokens, s);
+}
+
+int lp_attn_tree(lp_ctx* c, const lp_kv_cache* cache, uint64_t q, int q_stride, uint64_t out, int out_stride, int heads,
+                 uint64_t q_starts, uint64_t seq_lens, uint64_t masks, int batch, int tokens, int max_q, int max_seq,
+                 float scale, uint64_t workspace, uint64_t ws_bytes, lp_stream s) {
+    return attn_call("attn_tree", c, cache, q, q_stride, out, out_stride, heads, q_starts, seq_lens, true, masks, batch,
+                     tokens, max_q, max_seq, scale, workspace, ws_bytes, s);
+}
+
+// How a verification goes over its rows, and its workspace.
+struct VerifyPlan {
+    bool levels;                // a launch for each node down, else all rows in one
+    int blocks, parts, per_part;
+    int left_parts, left_per;   // of what is left of a row (sampled drafts)
+    int counters, row_counters;
+    uint64_t stats, left, state, records, bytes;  // offsets; where the records end
+};
+
+static VerifyPlan verify_plan(int vocab, int batch, int tokens, int max_q, int max_depth, bool probs) {
+    VerifyPlan p{};
+    if (!batch || !tokens || !max_q) return p;
+    p.blocks = (vocab + kVerifyBlock - 1) / kVerifyBlock;
+    // bytes a microsecond, and a launch's microseconds
+    const double rate = 4.5e6, launch = 6.0, row = 4.0 * vocab / rate;
+    const int downs = std::min(max_depth, max_q - 1) + 1;
+    p.levels = !probs && tokens * row > downs * (launch + batch * row);
+    const int rows = p.levels ? batch : tokens;
+    // about 2048 workgroups in all, four blocks at a time in each
+    const int steps = (p.blocks + 3) / 4, want = std::max(1, std::min(2048 / std::max(rows, 1), steps));
+    p.per_part = (steps + want - 1) / want * 4;
+    p.parts = (p.blocks + p.per_part - 1) / p.per_part;
+    p.row_counters = !p.levels && p.parts > 1 ? tokens : 0;
+    p.counters = p.row_counters + batch;
+    auto take = [&](uint64_t n) {
+        const uint64_t at = p.records;
+        p.records = align256(p.records + n);
+        return at;
+    };
+    take((uint64_t)rows * p.blocks * 16);
+    p.stats = take(p.levels ? 0 : (uint64_t)tokens * 16);
+    if (probs) {
+        const int all = (p.blocks + kVerifyWaves - 1) / kVerifyWaves;
+        const int each = std::max(1, std::min(512 / batch, all));
+        p.left_per = (all + each - 1) / each * kVerifyWaves;
+        p.left_parts = (p.blocks + p.left_per - 1) / p.left_per;
+        p.left = take((uint64_t)batch * p.blocks * 8);
+    }
+    p.state = take((uint64_t)batch * sizeof(VerifyState));
+    p.bytes = with_counters(p.records, p.counters);
+    return p;
+}
+
+static int check_verify(int vocab, int batch, int tokens, int max_q, int max_depth) {
+    if (vocab <= 0 || max_depth < 0) return fail(LP_E_INVALID, "verify_tree: need vocab >= 1 and max_depth >= 0");
+    if (int r = check_batch("verify_tree", 1, 1, batch, tokens, 4, 4)) return r;
+    if (int r = check_nodes("verify_tree", max_q)) return r;
+    if (vocab > kVerifyMaxVocab)
+        return fail(LP_E_UNSUPPORTED, "verify_tree: at most " + std::to_string(kVerifyMaxVocab) + " logits a row");
+    if (max_depth >= kTreeMaxNodes)
+        return fail(LP_E_UNSUPPORTED, "verify_tree: max_depth must be below " + std::to_string(kTreeMaxNodes));
+    if (tokens > INT32_MAX / 256) return fail(LP_E_UNSUPPORTED, "verify_tree: too many tokens");
+    return LP_OK;
+}
+
+uint64_t lp_verify_tree_ws_bytes(int vocab, int batch, int tokens, int max_q, int max_depth, int with_probs) {
+    if (check_verify(vocab, batch, tokens, max_q, max_depth)) return 0;
+    return verify_plan(vocab, batch, tokens, max_q, max_depth, with_probs != 0).bytes;
+}
+
+int lp_verify_tree(lp_ctx* c, uint64_t logits, int stride, int vocab, uint64_t drafts, uint64_t parents,
+                   uint64_t q_starts, int batch, int tokens, int max_q, int max_depth, uint64_t temperatures,
+                   uint64_t probs, int probs_stride, uint64_t uniforms, uint64_t path, uint64_t kept, uint64_t next,
+                   uint64_t workspace, uint64_t ws_bytes, lp_stream s) {
+    if (int r = check_verify(vocab, batch, tokens, max_q, max_depth)) return r;
+    if (stride < vocab || (probs && probs_stride < vocab))
+        return fail(LP_E_INVALID, "verify_tree: a stride is smaller than a row");
+    if (!logits || !drafts || !parents || !q_starts || !uniforms || !path || !kept || !next ||
+        (logits | drafts | parents | q_starts | temperatures | probs | uniforms | path | kept | next) % 4)
+        return fail(LP_E_INVALID, "verify_tree: null or misaligned pointer");
+    const VerifyPlan p = verify_plan(vocab, batch, tokens, max_q, max_depth, probs != 0);
+    if (int r = check_workspace("verify_tree", p.bytes, workspace, ws_bytes)) return r;
+    if (int r = check_ctx(c)) return r;
+    if (!p.bytes) return LP_OK;
+    VerifyArgs a{};
+    a.logits = logits, a.drafts = drafts, a.parents = parents, a.q_starts = q_starts;
+    a.temps = temperatures, a.probs = probs, a.uniforms = uniforms, a.path = path, a.kept = kept, a.next = next;
+    a.part = workspace, a.stats = workspace + p.stats, a.left = workspace + p.left, a.state = workspace + p.state;
+    a.stride = stride, a.probs_stride = probs_stride, a.vocab = vocab, a.batch = batch, a.tokens = tokens;
+    a.max_q = max_q, a.max_depth = max_depth;
+    a.blocks = p.blocks, a.parts = p.parts, a.per_part = p.per_part, a.row_counters = p.row_counters;
+    if (int r = join_counters(c, s, workspace + counters_at(p.records), p.counters, &a.sync)) return r;
+    if (p.levels) {
+        const int downs = std::min(max_depth, max_q - 1) + 1;
+        for (a.level = 0; a.level < downs; ++a.level)
+            if (int r = launch(c, kVerifyLevel, dim3((unsigned)(batch * p.parts)), dim3(256), 0, s, a)) return r;
+        return LP_OK;
+    }
+    if (int r = launch(c, kVerifyRows, dim3((unsigned)(tokens * p.parts)), dim3(256), 0, s, a)) return r;
+    if (!probs) return LP_OK;
+    a.parts = p.left_parts, a.per_part = p.left_per;
+    return launch(c, kVerifyLeft, dim3((unsigned)(batch * p.left_parts)), dim3(64 * kVerifyWaves), 0, s, a);
+}
+
+int lp_kv_keep(lp_ctx* c, const lp_kv_cache* caches, int layers, uint64_t path, int max_depth, uint64_t kept,
+               uint64_t q_starts, uint64_t seq_lens, uint64_t lens_out, int batch, lp_stream s) {
+    if (layers < 0 || max_depth < 0) return fail(LP_E_INVALID, "kv_keep: negative layers or max_depth");
+    KvKeepArgs a{};
+    for (int l = 0; l < std::max(layers, 1); ++l) {
+        const lp_kv_cache* k = caches ? caches + l : nullptr;
+        if (int r = check_paged("kv_keep", k, &a.c)) return r;
+        if (k->table != caches->table || k->pages != caches->pages || k->page_rows != caches->page_rows ||
+            k->max_pages != caches->max_pages || k->kv_heads != caches->kv_heads || k->head_dim != caches->head_dim ||
+            k->format != caches->format)
+            return fail(LP_E_INVALID, "kv_keep: the layers' caches must share their table and shapes");
+    }
+    if (int r = check_batch("kv_keep", 1, 1, batch, 0, q_starts, seq_lens)) return r;
+    if (max_depth >= kTreeMaxNodes)
+        return fail(LP_E_UNSUPPORTED, "kv_keep: max_depth must be below " + std::to_string(kTreeMaxNodes));
+    if (!path || !kept || path % 4 || kept % 4 || lens_out % 4) return fail(LP_E_INVALID, "kv_keep: null or misaligned pointer");
+    if (lens_out && lens_out == seq_lens) return fail(LP_E_INVALID, "kv_keep: lens_out must not be seq_lens");
+    const bool q4 = caches->format == LP_KV_Q4;
+    const int D = caches->head_dim, units = q4 ? D / 64 + D / 8 : D / 8;  // of a row of one head
+    const int64_t chunks = (2 * (int64_t)caches->kv_heads * units + keep_units(q4) - 1) / keep_units(q4);
+    if (chunks * std::min(std::max(layers, 1), kKeepLayers) * batch > INT32_MAX / 256)
+        return fail(LP_E_UNSUPPORTED, "kv_keep: too many heads for this batch");
+    if (int r = check_ctx(c)) return r;
+    if (!batch || !layers) return LP_OK;
+    a.path = path, a.kept = kept, a.q_starts = q_starts, a.seq_lens = seq_lens;
+    a.batch = batch, a.max_depth = max_depth, a.chunks = (int)chunks;
+    for (int l0 = 0; l0 < layers; l0 += kKeepLayers) {
+        a.layers = std::min(layers - l0, kKeepLayers);
+        a.lens_out = l0 ? 0 : lens_out;
+        for (int l = 0; l < a.layers; ++l) a.k_pages[l] = caches[l0 + l].k_pages, a.v_pages[l] = caches[l0 + l].v_pages;
+        const int64_t waves = chunks * a.layers * batch;
+        const Fn f = (Fn)(kKeepF16D64 + (q4 ? 2 : 0) + (D == 128 ? 1 : 0));
+        if (int r = launch(c, f, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, s, a)) return r;
+    }
+    return LP_OK;
 }
 
 // ---- logits (lp_logits.hip) ---------------------------------------------------------

@@ -289,6 +289,37 @@ extern "C" {
         heads: c_int, q_starts: u64, seq_lens: u64, batch: c_int, tokens: c_int, max_q: c_int, max_seq: c_int,
         scale: f32, workspace: u64, ws_bytes: u64, s: lp_stream,
     ) -> c_int;
+    pub fn lp_tree_layout(
+        ctx: *mut lp_ctx, parents: u64, q_starts: u64, batch: c_int, tokens: c_int, max_q: c_int, depths: u64,
+        masks: u64, s: lp_stream,
+    ) -> c_int;
+    pub fn lp_kv_append_tree(
+        ctx: *mut lp_ctx, cache: *const lp_kv_cache, q: u64, q_stride: c_int, k: u64, k_stride: c_int, v: u64,
+        v_stride: c_int, q_norm: u64, k_norm: u64, eps: f32, inv_freq: u64, mscale: f32, q_out: u64,
+        q_out_stride: c_int, k_out: u64, v_out: u64, heads: c_int, q_starts: u64, seq_lens: u64, depths: u64,
+        batch: c_int, tokens: c_int, s: lp_stream,
+    ) -> c_int;
+    pub fn lp_attn_tree_ws_bytes(
+        cache: *const lp_kv_cache, heads: c_int, batch: c_int, tokens: c_int, max_q: c_int, max_seq: c_int,
+    ) -> u64;
+    pub fn lp_attn_tree(
+        ctx: *mut lp_ctx, cache: *const lp_kv_cache, q: u64, q_stride: c_int, out: u64, out_stride: c_int,
+        heads: c_int, q_starts: u64, seq_lens: u64, masks: u64, batch: c_int, tokens: c_int, max_q: c_int,
+        max_seq: c_int, scale: f32, workspace: u64, ws_bytes: u64, s: lp_stream,
+    ) -> c_int;
+    pub fn lp_verify_tree_ws_bytes(
+        vocab: c_int, batch: c_int, tokens: c_int, max_q: c_int, max_depth: c_int, with_probs: c_int,
+    ) -> u64;
+    pub fn lp_verify_tree(
+        ctx: *mut lp_ctx, logits: u64, stride: c_int, vocab: c_int, drafts: u64, parents: u64, q_starts: u64,
+        batch: c_int, tokens: c_int, max_q: c_int, max_depth: c_int, temperatures: u64, probs: u64,
+        probs_stride: c_int, uniforms: u64, path: u64, kept: u64, next: u64, workspace: u64, ws_bytes: u64,
+        s: lp_stream,
+    ) -> c_int;
+    pub fn lp_kv_keep(
+        ctx: *mut lp_ctx, caches: *const lp_kv_cache, layers: c_int, path: u64, max_depth: c_int, kept: u64,
+        q_starts: u64, seq_lens: u64, lens_out: u64, batch: c_int, s: lp_stream,
+    ) -> c_int;
     pub fn lp_logprobs_ws_bytes(rows: c_int, vocab: c_int, top: c_int) -> u64;
     pub fn lp_logprobs(
         ctx: *mut lp_ctx, logits: u64, stride: c_int, rows: c_int, vocab: c_int, targets: u64, logp: u64,

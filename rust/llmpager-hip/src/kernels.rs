@@ -309,6 +309,95 @@ impl Kernels {
         check(rc, "attn_paged")
     }
 
+    /// Depths of trees' nodes, and masks of the nodes above each and itself.
+    #[allow(clippy::too_many_arguments)]
+    pub fn tree_layout(
+        &self, cuda: &Cuda, parents: CUdeviceptr, q_starts: CUdeviceptr, batch: i32, tokens: i32, max_q: i32,
+        depths: CUdeviceptr, masks: CUdeviceptr, stream: CUstream,
+    ) -> Result<()> {
+        let rc = unsafe {
+            ffi::lp_tree_layout(cuda.ctx, parents, q_starts, batch, tokens, max_q, depths, masks, stream)
+        };
+        check(rc, "tree_layout")
+    }
+
+    /// [`Self::kv_append_paged`] with the angles of the nodes' depths.
+    #[allow(clippy::too_many_arguments)]
+    pub fn kv_append_tree(
+        &self, cuda: &Cuda, cache: &lp_kv_cache, q: CUdeviceptr, q_stride: i32, k: CUdeviceptr, k_stride: i32,
+        v: CUdeviceptr, v_stride: i32, q_norm: CUdeviceptr, k_norm: CUdeviceptr, eps: f32, inv_freq: CUdeviceptr,
+        mscale: f32, q_out: CUdeviceptr, q_out_stride: i32, k_out: CUdeviceptr, v_out: CUdeviceptr, heads: i32,
+        q_starts: CUdeviceptr, seq_lens: CUdeviceptr, depths: CUdeviceptr, batch: i32, tokens: i32, stream: CUstream,
+    ) -> Result<()> {
+        let rc = unsafe {
+            ffi::lp_kv_append_tree(
+                cuda.ctx, cache, q, q_stride, k, k_stride, v, v_stride, q_norm, k_norm, eps, inv_freq, mscale, q_out,
+                q_out_stride, k_out, v_out, heads, q_starts, seq_lens, depths, batch, tokens, stream,
+            )
+        };
+        check(rc, "kv_append_tree")
+    }
+
+    /// Workspace bytes for [`Self::attn_tree`].
+    pub fn attn_tree_ws_bytes(&self, cache: &lp_kv_cache, heads: i32, batch: i32, tokens: i32, max_q: i32, max_seq: i32) -> u64 {
+        unsafe { ffi::lp_attn_tree_ws_bytes(cache, heads, batch, tokens, max_q, max_seq) }
+    }
+
+    /// Attention of a batch's new tokens over their contexts and, of the new
+    /// rows, those that their masks name.
+    #[allow(clippy::too_many_arguments)]
+    pub fn attn_tree(
+        &self, cuda: &Cuda, cache: &lp_kv_cache, q: CUdeviceptr, q_stride: i32, out: CUdeviceptr, out_stride: i32,
+        heads: i32, q_starts: CUdeviceptr, seq_lens: CUdeviceptr, masks: CUdeviceptr, batch: i32, tokens: i32,
+        max_q: i32, max_seq: i32, scale: f32, ws: CUdeviceptr, ws_bytes: u64, stream: CUstream,
+    ) -> Result<()> {
+        let rc = unsafe {
+            ffi::lp_attn_tree(
+                cuda.ctx, cache, q, q_stride, out, out_stride, heads, q_starts, seq_lens, masks, batch, tokens, max_q,
+                max_seq, scale, ws, ws_bytes, stream,
+            )
+        };
+        check(rc, "attn_tree")
+    }
+
+    /// Workspace bytes for [`Self::verify_tree`].
+    pub fn verify_tree_ws_bytes(&self, vocab: i32, batch: i32, tokens: i32, max_q: i32, max_depth: i32, with_probs: bool) -> u64 {
+        unsafe { ffi::lp_verify_tree_ws_bytes(vocab, batch, tokens, max_q, max_depth, with_probs as i32) }
+    }
+
+    /// The drafted tokens that the target's logits keep, and the token behind
+    /// them (`probs`: 0, or the distributions that the drafts were drawn from).
+    #[allow(clippy::too_many_arguments)]
+    pub fn verify_tree(
+        &self, cuda: &Cuda, logits: CUdeviceptr, stride: i32, vocab: i32, drafts: CUdeviceptr, parents: CUdeviceptr,
+        q_starts: CUdeviceptr, batch: i32, tokens: i32, max_q: i32, max_depth: i32, temperatures: CUdeviceptr,
+        probs: CUdeviceptr, probs_stride: i32, uniforms: CUdeviceptr, path: CUdeviceptr, kept: CUdeviceptr,
+        next: CUdeviceptr, ws: CUdeviceptr, ws_bytes: u64, stream: CUstream,
+    ) -> Result<()> {
+        let rc = unsafe {
+            ffi::lp_verify_tree(
+                cuda.ctx, logits, stride, vocab, drafts, parents, q_starts, batch, tokens, max_q, max_depth,
+                temperatures, probs, probs_stride, uniforms, path, kept, next, ws, ws_bytes, stream,
+            )
+        };
+        check(rc, "verify_tree")
+    }
+
+    /// The kept nodes' rows one behind the other in all layers' caches.
+    #[allow(clippy::too_many_arguments)]
+    pub fn kv_keep(
+        &self, cuda: &Cuda, caches: &[lp_kv_cache], path: CUdeviceptr, max_depth: i32, kept: CUdeviceptr,
+        q_starts: CUdeviceptr, seq_lens: CUdeviceptr, lens_out: CUdeviceptr, batch: i32, stream: CUstream,
+    ) -> Result<()> {
+        let rc = unsafe {
+            ffi::lp_kv_keep(
+                cuda.ctx, caches.as_ptr(), caches.len() as i32, path, max_depth, kept, q_starts, seq_lens, lens_out,
+                batch, stream,
+            )
+        };
+        check(rc, "kv_keep")
+    }
+
     /// Workspace bytes for [`Self::logprobs`].
     pub fn logprobs_ws_bytes(&self, rows: i32, vocab: i32, top: i32) -> u64 {
         unsafe { ffi::lp_logprobs_ws_bytes(rows, vocab, top) }
