@@ -13,7 +13,7 @@
 // the next token is drawn from R / Z.  At temperature 0 both go by the largest logit.
 //
 // A draw is where a running sum over the vocabulary passes a border, and a value of 1e-7
-// of the whole is many tokens' there: exponentials are made to 2^-42 and all sums in 64
+// of the whole is many tokens' there: exponentials are made to 2^-40 and all sums in 64
 // bits, so that the token is that of the formula.  Vector fp64 runs at fp32's rate here.
 //
 // A wave takes blocks of 1024 logits and leaves a record of each, its largest logit and the sum
@@ -26,29 +26,47 @@
 
 namespace {
 
-constexpr double kNone = -800.0;  // e^ of it is 0
+constexpr double kNone = -700.0;     // e^ of it, of anything below and of -infinity,
+constexpr double kNothing = 1e-290;  // counts as nothing
 
-// e^d for kNone <= d <= 0: d = k ln 2 + r, |r| <= ln 2 / 2, Taylor's series of e^r, whose
-// first term left out is 2^-42.
-__device__ __forceinline__ double exp_f64(double d) {
-    const double k = rint(d * 1.4426950408889634);
-    const double r = __builtin_fma(-k, 0.6931471805599453, d);
-    auto by_r = [&](double y, double c) { return __builtin_fma(y, r, c); };
-    double y = by_r(2.7557319223985888e-7, 2.7557319223985893e-6);  // 1 / 10!, 1 / 9!, ...
-    y = by_r(y, 2.4801587301587302e-5);
-    y = by_r(y, 1.9841269841269841e-4);
-    y = by_r(y, 1.3888888888888889e-3);
-    y = by_r(y, 8.3333333333333333e-3);
-    y = by_r(y, 4.1666666666666667e-2);
-    y = by_r(y, 0.16666666666666667);
-    y = by_r(y, 0.5);
-    y = by_r(y, 1.0);
-    y = by_r(y, 1.0);
-    return __builtin_amdgcn_ldexp(y, (int)k);
+// e^((x - m) / T): d = n ln 2 + r, |r| <= ln 2 / 2, and 2^n by the exponent's bits.  The
+// polynomial has the smallest largest relative error of those of degree 8 that are 1 at
+// 0: 2^-40.  (Taylor's of degree 10 with rounding and scaling instructions of their own is
+// 22 fp64 instructions of 2.1 ns a wave and SIMD, this 17 and one of 1.3.)  N at a time, a
+// step of all before the next, for a step waits for the one before it.
+// (A NaN counts as none here; rows with one are found by their logits.)
+template <int N>
+__device__ __forceinline__ void exp_over(const float* x, float m, double inv_t, double* e) {
+    typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+    constexpr double kRound = 6755399441055744.0;  // 1.5 2^52: the sum's last bits are the whole number
+    constexpr double C[8] = {0.00019914665993177232, 0.0013889154943716253, 0.008333268780697685, 0.04166666453742114,
+                             0.16666666873210403, 0.500000000045801, 0.999999999983073, 1.0};
+    double d[N], t[N], y[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) d[i] = ((double)x[i] - (double)m) * inv_t;
+#pragma unroll
+    for (int i = 0; i < N; ++i) d[i] = fmax(d[i], kNone);
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] = __builtin_fma(d[i], 1.4426950408889634, kRound);
+#pragma unroll
+    for (int i = 0; i < N; ++i) d[i] = __builtin_fma(t[i] - kRound, -0.6931471805599453, d[i]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) y[i] = __builtin_fma(2.473298746639189e-05, d[i], C[0]);
+#pragma unroll
+    for (int k = 1; k < 8; ++k)
+#pragma unroll
+        for (int i = 0; i < N; ++i) y[i] = __builtin_fma(y[i], d[i], C[k]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        u32x2_t u = __builtin_bit_cast(u32x2_t, y[i]);
+        u[1] += __builtin_bit_cast(u32x2_t, t[i])[0] << 20;
+        e[i] = __builtin_bit_cast(double, u);
+    }
 }
-// (a NaN counts as none here; rows with one are found by their logits)
 __device__ __forceinline__ double exp_over(float x, float m, double inv_t) {
-    return exp_f64(fmax(((double)x - (double)m) * inv_t, kNone));
+    double e;
+    exp_over<1>(&x, m, inv_t, &e);
+    return e;
 }
 
 template <int CTRL, int ROWS>
@@ -77,70 +95,103 @@ __device__ __forceinline__ void put64(uint64_t at, uint64_t v) { agent_store(rei
 __device__ __forceinline__ uint64_t get64(uint64_t at) { return agent_load(reinterpret_cast<const uint64_t*>(at)); }
 __device__ __forceinline__ double getf64(uint64_t at) { return __builtin_bit_cast(double, get64(at)); }
 
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
+
 constexpr int kPer = kVerifyBlock / 64;  // values of a lane in a block: 4 j + u is the block's 256 j + 4 lane + u
 constexpr int kBad = 0x7fffffff;
 
-// A block of a row; past its end `none`.
-__device__ __forceinline__ void load_block(float (&v)[kPer], uint64_t row, int block, int n, float none) {
-    const LP_GLOBAL float* const x = gptr<float>(row);
-    typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
+// A block of a row (what is past its end comes as 0): loads without a branch of a lane's
+// own, so that a wave works on one block while the next one's are under way.
+__device__ __forceinline__ void load_block(float (&v)[kPer], uint64_t row, int block, int n) {
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(uniform_u64(row)), (short)0, n * 4, kBufferWord3);
+    const int at = (block * kVerifyBlock + 4 * lane_id()) * 4;
+    if ((block + 1) * kVerifyBlock <= n) {
 #pragma unroll
-    for (int j = 0; j < kPer / 4; ++j) {
-        const int e = block * kVerifyBlock + 256 * j + 4 * lane_id();
-        if (e + 4 <= n) {
-            const f32x4_u w = *reinterpret_cast<const LP_GLOBAL f32x4_u*>(x + e);
+        for (int j = 0; j < kPer / 4; ++j) {
+            const f32x4_t w = __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, at + 1024 * j, 0, 0));
 #pragma unroll
             for (int u = 0; u < 4; ++u) v[4 * j + u] = w[u];
-        } else {
-#pragma unroll
-            for (int u = 0; u < 4; ++u) v[4 * j + u] = e + u < n ? x[e + u] : none;
         }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+            v[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, at + 1024 * (i / 4) + 4 * (i % 4), 0, 0));
+    }
+}
+// Logits past the row's end: -infinity.
+__device__ __forceinline__ void end_block(float (&v)[kPer], int block, int n) {
+    if ((block + 1) * kVerifyBlock <= n) return;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) v[i] = block * kVerifyBlock + 256 * (i / 4) + 4 * lane_id() + i % 4 < n ? v[i] : -INFINITY;
+}
+
+// The place in a block where the sums of the weights, `before` what went before them, pass
+// thr; at rounding's edge the last that adds to them, -1 where none does.  weights(j, e):
+// the lane's four of part j.
+template <typename F>
+__device__ __forceinline__ int find_in_block(const F& weights, double before, double thr) {
+    constexpr int N = kPer / 4;
+    double t[N], incl[N], e[4];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        weights(j, e);
+        t[j] = (e[0] + e[1]) + (e[2] + e[3]);
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) incl[j] = scan_f64(t[j]);
+    int in = -1, lane = 0;
+    double from = 0.0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const uint64_t some = __ballot(t[j] > kNothing), hit = __ballot(before + incl[j] > thr && t[j] > kNothing);
+        if (some) in = j, lane = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some), from = before + incl[j] - t[j];
+        if (hit) break;
+        before += lane_f64(incl[j], 63);
+    }
+    if (in < 0) return -1;
+    weights(in, e);
+    int u = -1;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if (u >= 0 && from > thr) continue;  // found
+        from += e[k];
+        if (e[k] > kNothing) u = k;
+    }
+    return 256 * in + 4 * lane + __builtin_amdgcn_readlane(u, lane);
+}
+// Part j of the lane's values.
+__device__ __forceinline__ void part_of(const float (&v)[kPer], int j, float (&x)[4]) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        x[u] = v[u];
+#pragma unroll
+        for (int k = 1; k < kPer / 4; ++k) x[u] = j == k ? v[4 * k + u] : x[u];
     }
 }
 
-// The place in the block where the sums of v, `before` what went before them, pass thr; at
-// rounding's edge the last that adds to them, -1 where none does.
-__device__ __forceinline__ int find_in_block(const double (&v)[kPer], double before, double thr) {
-    int at = -1;
-#pragma unroll
-    for (int j = 0; j < kPer / 4; ++j) {
-        const double t = (v[4 * j] + v[4 * j + 1]) + (v[4 * j + 2] + v[4 * j + 3]);
-        const double incl = before + scan_f64(t);
-        const uint64_t some = __ballot(t > 0.0), hit = __ballot(incl > thr && t > 0.0);
-        if (some) {
-            const int l = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some);
-            double c = incl - t;
-            int u = -1;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if (u >= 0 && c > thr) continue;  // found
-                c += v[4 * j + k];
-                if (v[4 * j + k] > 0.0) u = k;
-            }
-            at = 256 * j + 4 * l + __builtin_amdgcn_readlane(u, l);
-        }
-        if (hit) return at;
-        before = lane_f64(incl, 63);
-    }
-    return at;
-}
+// A row's blocks in LDS, for one wave.
+struct Room {
+    double w[kVerifyBlocks];  // their sums
+    float m[kVerifyBlocks];
+};
 
-// Which of a row's blocks holds the border: their sums w (block lane + 64 i) in order, and
-// `share` of the whole.  The border and what goes before the block are left in thr and
-// before; -1 where nothing adds to the sums.
-__device__ __forceinline__ int find_block(const double (&w)[kVerifyLane], double share, double& thr, double& before) {
-    double incl[kVerifyLane], all = 0.0;
-#pragma unroll
-    for (int i = 0; i < kVerifyLane; ++i) incl[i] = all + scan_f64(w[i]), all = lane_f64(incl[i], 63);
-    thr = share * all;
+// Which of a row's blocks holds the border: their sums in order, and `share` of the whole.
+// The border and what goes before the block are left in thr and before; -1 where nothing
+// adds to the sums.
+__device__ __forceinline__ int find_block(const double* w, int blocks, double share, double& thr, double& before) {
+    double all = 0.0;
+    for (int i = lane_id(); i - lane_id() < blocks; i += 64) all += i < blocks ? w[i] : 0.0;
+    thr = share * wave_sum_f64(all);
     int at = -1;
+    double done = 0.0;
     before = 0.0;
-#pragma unroll
-    for (int i = 0; i < kVerifyLane; ++i) {
-        const uint64_t some = __ballot(w[i] > 0.0), hit = __ballot(incl[i] > thr && w[i] > 0.0);
+    for (int i0 = 0; i0 < blocks; i0 += 64) {
+        const double x = i0 + lane_id() < blocks ? w[i0 + lane_id()] : 0.0, incl = done + scan_f64(x);
+        const uint64_t some = __ballot(x > kNothing), hit = __ballot(incl > thr && x > kNothing);
+        done = lane_f64(incl, 63);
         if (!some) continue;
         const int l = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some);
-        at = 64 * i + l, before = lane_f64(incl[i] - w[i], l);
+        at = i0 + l, before = lane_f64(incl - x, l);
         if (hit) break;
     }
     return at;
@@ -168,18 +219,20 @@ __device__ __forceinline__ uint64_t record(const VerifyArgs& a, int slot, int bl
     return a.part + ((uint64_t)(uint32_t)slot * (uint32_t)a.blocks + (uint32_t)block) * 16;
 }
 
-// The records of a part of row t (those of slot `slot`), by the whole workgroup: the block's
+// The records of a part of row t (those of slot `slot`), by the whole workgroup of WAVES: the block's
 // sum (NaN: a logit is NaN or infinite), its largest logit, and the first id of that.
+template <int WAVES>
 __device__ __forceinline__ void scan_part(const VerifyArgs& a, const Seq& s, int t, int slot, int part) {
-    const int wave = (int)(threadIdx.x >> 6), end = min(a.blocks, (part + 1) * a.per_part);
+    const int wave = wave_id(), end = min(a.blocks, (part + 1) * a.per_part);
     const uint64_t row = logits_row(a, t);
     float x[kPer], next[kPer];
     int blk = part * a.per_part + wave;
-    if (blk < end) load_block(next, row, blk, a.vocab, -INFINITY);
-    for (; blk < end; blk += 4) {
+    if (blk < end) load_block(next, row, blk, a.vocab);
+    for (; blk < end; blk += WAVES) {
 #pragma unroll
         for (int i = 0; i < kPer; ++i) x[i] = next[i];
-        if (blk + 4 < end) load_block(next, row, blk + 4, a.vocab, -INFINITY);
+        if (blk + WAVES < end) load_block(next, row, blk + WAVES, a.vocab);
+        end_block(x, blk, a.vocab);
         float mx = x[0];
         bool bad = false;
 #pragma unroll
@@ -188,9 +241,15 @@ __device__ __forceinline__ void scan_part(const VerifyArgs& a, const Seq& s, int
         double sum = 0.0;
         int id = kBad;
         if (s.temp > 0.0f) {
+            double some[4] = {};
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) sum += exp_over(x[i], mx, s.inv_t);
-            sum = wave_sum_f64(sum);
+            for (int i = 0; i < kPer; i += 4) {
+                double e[4];
+                exp_over<4>(x + i, mx, s.inv_t, e);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) some[u] += e[u];
+            }
+            sum = wave_sum_f64((some[0] + some[1]) + (some[2] + some[3]));
         } else {
 #pragma unroll
             for (int i = kPer - 1; i >= 0; --i) id = x[i] == mx ? blk * kVerifyBlock + 256 * (i / 4) + 4 * lane_id() + i % 4 : id;
@@ -205,65 +264,80 @@ __device__ __forceinline__ void scan_part(const VerifyArgs& a, const Seq& s, int
     }
 }
 
-// A row's records joined by a wave.
+// A row's records joined by a wave, the blocks' sums relative to the row's largest logit left
+// in `room`.
 struct Row {
-    float m;                // the largest logit
-    double s;               // the sum relative to it, NaN for a row from which nothing can be drawn
-    double w[kVerifyLane];  // the sums of blocks lane + 64 i
-    int first;              // the first id of the largest logit
+    float m;    // the largest logit
+    double s;   // the sum relative to it, NaN for a row from which nothing can be drawn
+    int first;  // the first id of the largest logit
 };
-__device__ __forceinline__ Row join_row(const VerifyArgs& a, const Seq& s, int slot) {
-    Row r;
-    float m[kVerifyLane];
-    int id[kVerifyLane];
+__device__ __forceinline__ Row join_row(const VerifyArgs& a, const Seq& s, int slot, Room& room) {
+    Row r{-INFINITY, 0.0, kBad};
     float mx = -INFINITY;
+    int id = kBad;
+    constexpr int N = 4;  // loads at a time
+    for (int b0 = lane_id(); b0 - lane_id() < a.blocks; b0 += 64 * N) {
+        uint64_t w[N], mi[N];
 #pragma unroll
-    for (int i = 0; i < kVerifyLane; ++i) {
-        const int blk = lane_id() + 64 * i;
-        r.w[i] = 0.0, m[i] = -INFINITY, id[i] = kBad;
-        if (64 * i < a.blocks && blk < a.blocks) {
-            const uint64_t at = record(a, slot, blk), mi = get64(at + 8);
-            r.w[i] = getf64(at), m[i] = __uint_as_float((uint32_t)mi), id[i] = (int)(mi >> 32);
+        for (int i = 0; i < N; ++i) {
+            const uint64_t at = record(a, slot, min(b0 + 64 * i, a.blocks - 1));
+            w[i] = get64(at), mi[i] = get64(at + 8);
         }
-        mx = fmaxf(mx, m[i]);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int blk = b0 + 64 * i;
+            if (blk >= a.blocks) continue;
+            const float m = __uint_as_float((uint32_t)mi[i]);
+            room.w[blk] = __builtin_bit_cast(double, w[i]), room.m[blk] = m;
+            if (m > mx) mx = m, id = (int)(mi[i] >> 32);  // blocks rise: the first of equal ones stays
+        }
     }
     r.m = wave_top(mx);
-    r.s = 0.0, r.first = kBad;
-#pragma unroll
-    for (int i = 0; i < kVerifyLane; ++i) {
-        if (64 * i >= a.blocks) continue;
-        if (m[i] == r.m) r.first = min(r.first, id[i]);
-        r.w[i] *= s.temp > 0.0f ? exp_over(m[i], r.m, s.inv_t) : 1.0;
-        r.s += wave_sum_f64(r.w[i]);
+    r.first = wave_least(mx == r.m ? id : kBad);
+    double sum = 0.0;
+    for (int blk = lane_id(); blk < a.blocks; blk += 64) {
+        double w = room.w[blk];
+        if (s.temp > 0.0f) w *= exp_over(room.m[blk], r.m, s.inv_t);
+        room.w[blk] = w;
+        sum += w;
     }
-    r.first = wave_least(r.first);
-    if (r.m == -INFINITY) r.s = __builtin_nan("");
+    r.s = r.m == -INFINITY ? __builtin_nan("") : wave_sum_f64(sum);
     return r;
 }
 
 // The token of row t that number u draws, -1: none can be.
-__device__ __forceinline__ int draw(const VerifyArgs& a, const Seq& s, int t, const Row& r, float u) {
+__device__ __forceinline__ int draw(const VerifyArgs& a, const Seq& s, int t, const Row& r, const Room& room, float u) {
     if (r.s != r.s) return -1;
     if (s.temp == 0.0f) return r.first;
     double thr, before;
-    const int blk = find_block(r.w, (double)u, thr, before);
+    const int blk = find_block(room.w, a.blocks, (double)u, thr, before);
     if (blk < 0) return -1;
     float x[kPer];
-    load_block(x, logits_row(a, t), blk, a.vocab, -INFINITY);
-    double v[kPer];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) v[i] = exp_over(x[i], r.m, s.inv_t);
-    const int at = find_in_block(v, before, thr);
+    load_block(x, logits_row(a, t), blk, a.vocab);
+    end_block(x, blk, a.vocab);
+    auto weights = [&](int j, double (&e)[4]) {
+        float y[4];
+        part_of(x, j, y);
+        exp_over<4>(y, r.m, s.inv_t, e);
+    };
+    const int at = find_in_block(weights, before, thr);
     return at < 0 ? -1 : blk * kVerifyBlock + at;
 }
 
-// What is left of a row's block: max(p - taken q, 0).
-__device__ __forceinline__ void left_block(const VerifyArgs& a, const Seq& s, int t, int blk, float m, double inv_s, double taken, double (&v)[kPer]) {
-    float x[kPer], q[kPer];
-    load_block(x, logits_row(a, t), blk, a.vocab, -INFINITY);
-    load_block(q, probs_row(a, t), blk, a.vocab, 0.0f);
+// What is left of a row: max(p - taken q, 0), four at a time.
+struct Left {
+    float m;
+    double inv_s, inv_t, taken;
+    __device__ __forceinline__ void operator()(const float (&x)[4], const float (&q)[4], double (&e)[4]) const {
+        exp_over<4>(x, m, inv_t, e);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) v[i] = fmax(__builtin_fma(-taken, (double)q[i], exp_over(x[i], m, s.inv_t) * inv_s), 0.0);
+        for (int u = 0; u < 4; ++u) e[u] = fmax(__builtin_fma(-taken, (double)q[u], e[u] * inv_s), 0.0);
+    }
+};
+__device__ __forceinline__ void load_both(const VerifyArgs& a, int t, int blk, float (&x)[kPer], float (&q)[kPer]) {
+    load_block(x, logits_row(a, t), blk, a.vocab);
+    load_block(q, probs_row(a, t), blk, a.vocab);
+    end_block(x, blk, a.vocab);
 }
 
 // A counter's last arrival (the calling wave's stores are done before it counts).
@@ -327,7 +401,8 @@ struct Nodes {
         if (a.probs && s.temp > 0.0f) {
             const float x = gptr<float>(logits_row(a, s.t0 + p))[token], q = gptr<float>(probs_row(a, s.t0 + p))[token];
             const float u = gptr<float>(a.uniforms)[s.t0 + i];
-            fits = (double)u * (double)q < exp_over(x, st.m, s.inv_t) / st.s;
+            const double pr = exp_over(x, st.m, s.inv_t) / st.s;
+            fits = pr > kNothing && (double)u * (double)q < pr;
         } else {
             fits = token == st.z;
         }
@@ -335,10 +410,10 @@ struct Nodes {
 };
 
 // A sequence's walk, by one wave, from node st.cur on until its end (true) or until what is
-// left of a row has to be summed (false; then, with the blocks' sums in `sums`, the walk goes on).
-__device__ __forceinline__ bool walk(const VerifyArgs& a, const Seq& s, int b, VerifyState& st, const double* sums) {
+// left of a row has to be summed (false; then, with the blocks' sums in `room`, the walk goes on).
+__device__ __forceinline__ bool walk(const VerifyArgs& a, const Seq& s, int b, VerifyState& st, Room& room) {
     const bool sampled = a.probs && s.temp > 0.0f;
-    if (!(st.left > 0.0)) st.taken = 0.0, st.left = 1.0;  // nothing is left: p again
+    if (!(st.left > kNothing)) st.taken = 0.0, st.left = 1.0;  // nothing is left: p again
     Nodes N;
     for (;;) {
         N.load(a, s, st.cur & ~63);
@@ -376,8 +451,8 @@ __device__ __forceinline__ bool walk(const VerifyArgs& a, const Seq& s, int b, V
                 if (!kids) continue;
                 const int k = __builtin_ctzll(kids), d = __builtin_amdgcn_readlane(N.token, k), t = s.t0 + st.cur;
                 const double q = (double)gptr<float>(probs_row(a, t))[d], u = (double)gptr<float>(a.uniforms)[s.t0 + i0 + k];
-                const double p = exp_over(gptr<float>(logits_row(a, t))[d], m, s.inv_t) / S;
-                if (u * q * st.left < fmax(__builtin_fma(-st.taken, q, p), 0.0)) {
+                const double p = __builtin_fma(-st.taken, q, exp_over(gptr<float>(logits_row(a, t))[d], m, s.inv_t) / S);
+                if (p > kNothing && u * q * st.left < p) {
                     to = i0 + k;
                     continue;
                 }
@@ -394,14 +469,20 @@ __device__ __forceinline__ bool walk(const VerifyArgs& a, const Seq& s, int b, V
             const int t = s.t0 + st.cur;
             const float u = gptr<float>(a.uniforms)[s.t0];
             if (st.taken == 0.0) {
-                next = draw(a, s, t, join_row(a, s, t), u);
+                const Row r = join_row(a, s, t, room);
+                next = draw(a, s, t, r, room, u);
             } else {
-                double w[kVerifyLane], thr, before, v[kPer];
-#pragma unroll
-                for (int i = 0; i < kVerifyLane; ++i) w[i] = lane_id() + 64 * i < a.blocks ? sums[lane_id() + 64 * i] : 0.0;
-                const int blk = find_block(w, (double)u, thr, before);
-                left_block(a, s, t, max(blk, 0), m, 1.0 / S, st.taken, v);
-                next = max(blk, 0) * kVerifyBlock + max(find_in_block(v, before, thr), 0);
+                double thr, before;
+                float x[kPer], q[kPer];
+                const int blk = max(0, find_block(room.w, a.blocks, (double)u, thr, before));
+                load_both(a, t, blk, x, q);
+                const Left left{m, 1.0 / S, s.inv_t, st.taken};
+                auto weights = [&](int j, double (&e)[4]) {
+                    float y[4], z[4];
+                    part_of(x, j, y), part_of(q, j, z);
+                    left(y, z, e);
+                };
+                next = blk * kVerifyBlock + max(0, find_in_block(weights, before, thr));
             }
         }
         put_end(a, b, st.len, next);
@@ -430,8 +511,9 @@ __device__ __forceinline__ int sequence_of_row(const VerifyArgs& a, int t) {
 
 // Every row at once: workgroup (row, part).  A row's last workgroup joins its records, a
 // sequence's last row walks down its tree.
-extern "C" __global__ void __launch_bounds__(256) lp_verify_rows(const VerifyArgs a) {
-    const int t = (int)blockIdx.x / a.parts, part = (int)blockIdx.x - t * a.parts, wave = (int)(threadIdx.x >> 6);
+extern "C" __global__ void __launch_bounds__(256, 4) lp_verify_rows(const VerifyArgs a) {
+    __shared__ Room room;
+    const int t = (int)blockIdx.x / a.parts, part = (int)blockIdx.x - t * a.parts, wave = wave_id();
     if (blockIdx.x == 0 && wave == 3)  // sequences without a token
         for (int b = lane_id(); b < a.batch; b += 64) {
             if (seq_of(a, b).n > 0) continue;
@@ -443,18 +525,18 @@ extern "C" __global__ void __launch_bounds__(256) lp_verify_rows(const VerifyArg
     if (b >= a.batch) return;  // whole workgroups, here and below
     const Seq s = seq_of(a, b);
     if (t < s.t0 || t - s.t0 >= s.n) return;
-    scan_part(a, s, t, t, part);
+    scan_part<4>(a, s, t, t, part);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     if (wave) return;
     if (a.parts > 1 && !last_of(a, t, a.parts)) return;
-    const Row r = join_row(a, s, t);
+    const Row r = join_row(a, s, t, room);
     const bool sampled = a.probs && s.temp > 0.0f;
-    put_stat(a, t, r, sampled ? -1 : draw(a, s, t, r, gptr<float>(a.uniforms)[t]));
+    put_stat(a, t, r, sampled ? -1 : draw(a, s, t, r, room, gptr<float>(a.uniforms)[t]));
     if (!last_of(a, a.row_counters + b, s.n)) return;
     VerifyState st{0, 0, 1, 0, 0.0, 1.0};
     put_node(a, b, 0, 0);
-    walk(a, s, b, st, nullptr);
+    walk(a, s, b, st, room);
     if (a.probs && lane_id() == 0) gptr_w<VerifyState>(a.state)[b] = st;
 }
 
@@ -462,21 +544,29 @@ extern "C" __global__ void __launch_bounds__(256) lp_verify_rows(const VerifyArg
 // part) sums a wave's blocks, the last one goes on with the walk, and where that needs
 // another row's or more taken from this one, sums that alone.
 extern "C" __global__ void __launch_bounds__(64 * kVerifyWaves) lp_verify_left(const VerifyArgs a) {
-    __shared__ double sums[64 * kVerifyLane];
+    __shared__ Room room;
     __shared__ VerifyState now;
     __shared__ int flag;
     const int b = (int)blockIdx.x / a.parts, part = (int)blockIdx.x - b * a.parts;
-    const int wave = (int)(threadIdx.x >> 6), lane = lane_id();
+    const int wave = wave_id(), lane = lane_id();
     VerifyState st = gptr<VerifyState>(a.state)[b];
     if (!st.pending) return;  // whole workgroups, here and below
     const Seq s = seq_of(a, b);
     const uint64_t mine = a.left + (uint64_t)(uint32_t)b * (uint32_t)a.blocks * 8;
     auto sum_block = [&](int blk) {
+        float x[kPer], q[kPer];
+        load_both(a, s.t0 + st.cur, blk, x, q);
         const Stat r = get_stat(a, s.t0 + st.cur);
-        double v[kPer], sum = 0.0;
-        left_block(a, s, s.t0 + st.cur, blk, r.m, 1.0 / r.s, st.taken, v);
+        const Left left{r.m, 1.0 / r.s, s.inv_t, st.taken};
+        double sum = 0.0;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) sum += v[i];
+        for (int j = 0; j < kPer / 4; ++j) {
+            float y[4], z[4];
+            double e[4];
+            part_of(x, j, y), part_of(q, j, z);
+            left(y, z, e);
+            sum += (e[0] + e[1]) + (e[2] + e[3]);
+        }
         return wave_sum_f64(sum);
     };
     for (int blk = part * a.per_part + wave; blk < min(a.blocks, (part + 1) * a.per_part); blk += kVerifyWaves) {
@@ -491,14 +581,14 @@ extern "C" __global__ void __launch_bounds__(64 * kVerifyWaves) lp_verify_left(c
     }
     __syncthreads();
     if (!flag) return;
-    for (int i = threadIdx.x; i < a.blocks; i += 64 * kVerifyWaves) sums[i] = getf64(mine + 8 * i);
+    for (int i = threadIdx.x; i < a.blocks; i += 64 * kVerifyWaves) room.w[i] = getf64(mine + 8 * i);
     for (;;) {
         __syncthreads();
         if (wave == 0) {
             double z = 0.0;
-            for (int i = lane; i < a.blocks; i += 64) z += sums[i];
+            for (int i = lane; i < a.blocks; i += 64) z += room.w[i];
             st.left = wave_sum_f64(z), st.pending = 0;
-            const bool done = walk(a, s, b, st, sums);
+            const bool done = walk(a, s, b, st, room);
             if (lane == 0) now = st, flag = done;
         }
         __syncthreads();
@@ -506,41 +596,87 @@ extern "C" __global__ void __launch_bounds__(64 * kVerifyWaves) lp_verify_left(c
         st = now;
         for (int blk = wave; blk < a.blocks; blk += kVerifyWaves) {
             const double sum = sum_block(blk);
-            if (lane == 0) sums[blk] = sum;
+            if (lane == 0) room.w[blk] = sum;
         }
     }
 }
 
-// By levels, chosen drafts: workgroup (sequence, part) of the row that the walk stands at,
-// whose last one goes a node down, for the next launch.
-extern "C" __global__ void __launch_bounds__(256) lp_verify_level(const VerifyArgs a) {
-    const int b = (int)blockIdx.x / a.parts, part = (int)blockIdx.x - b * a.parts, wave = (int)(threadIdx.x >> 6);
+// The rows of the path alone, chosen drafts: `parts` workgroups a sequence share the row
+// that the walk stands at.  Each takes a group of its blocks (the count of those that are
+// taken, beside the node's number); who ends a row's last group joins it, goes a node down
+// and says so, and all take groups of that one.  Nobody needs another one to go on: who finds
+// no group left looks for the next node for a while and leaves, and who ended the last
+// group is there to take all of the next row's if need be.  The last one to leave clears the words.
+//
+// 32 trees of up to 60 nodes, at most 6 of them kept, 151,936 logits: 67 us; a node is about
+// 11, of which 3 to 5 are the row's blocks, 4 the join and the draw, 2 word that it is done
+// (a launch for each node 75 us, half of a node's the launch; the words 64 bytes apart and
+// workgroups of four waves 103 us: many look at one memory channel).
+constexpr int kTaken = 0, kEnded = 1, kGone = 2, kLen = 3;  // words of a sequence
+constexpr int kOver = 0x7fff;                               // no node
+constexpr int kLooks = 64;                                  // about a microsecond each
+
+extern "C" __global__ void __launch_bounds__(64 * kPathWaves, 4) lp_verify_path(const VerifyArgs a) {
+    __shared__ Room room;
+    __shared__ int share;
+    const int b = (int)blockIdx.x / a.parts, part = (int)blockIdx.x - b * a.parts, wave = wave_id();
     const Seq s = seq_of(a, b);
-    const int cur = a.level ? gptr<int>(a.state)[b] : 0;
     if (s.n <= 0) {
-        if (a.level == 0 && part == 0 && wave == 0) {
-            put_end(a, b, 0, -1);
-            if (lane_id() == 0) gptr_w<int>(a.state)[b] = -1;
-        }
-        return;
+        if (part == 0 && wave == 0) put_end(a, b, 0, -1);
+        return;  // whole workgroups
     }
-    if (cur < 0) return;  // whole workgroups
-    const int t = s.t0 + cur;
-    scan_part(a, s, t, b, part);
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    if (wave) return;
-    if (a.parts > 1 && !last_of(a, a.row_counters + b, a.parts)) return;
-    const int z = draw(a, s, t, join_row(a, s, b), gptr<float>(a.uniforms)[t]);
-    int to = -1;
-    if (z >= 0 && a.level < a.max_depth)
-        for (int i0 = cur & ~63; i0 < s.n && to < 0; i0 += 64) {
-            const int i = i0 + lane_id();
-            const bool fits = i < s.n && i > cur && gptr<int>(a.parents)[s.t0 + i] == cur && gptr<int>(a.drafts)[s.t0 + i] == z;
-            const uint64_t fit = __ballot(fits);
-            if (fit) to = i0 + __builtin_ctzll(fit);
+    int* const word = reinterpret_cast<int*>(a.sync) + (uint64_t)(uint32_t)(b * a.row_counters) * kPagedStride;
+    int up = -1, token = -1;  // of the first 64 nodes, one a lane
+    if (lane_id() < s.n) up = gptr<int>(a.parents)[s.t0 + lane_id()], token = gptr<int>(a.drafts)[s.t0 + lane_id()];
+    for (;;) {
+        if (threadIdx.x == 0) {
+            int c = atomicAdd(word + kTaken, 1);
+            for (int look = 0; (c & 0xffff) >= a.parts && c >> 16 != kOver;) {
+                const int now = agent_load(word + kTaken);
+                if (now >> 16 != c >> 16)
+                    c = now >> 16 == kOver ? now : atomicAdd(word + kTaken, 1);
+                else if (++look == kLooks)
+                    c = kOver << 16;
+                else
+                    __builtin_amdgcn_s_sleep(2);
+            }
+            share = c;
         }
-    put_node(a, b, a.level, cur);
-    if (to < 0) put_end(a, b, a.level + 1, z);
-    if (lane_id() == 0) gptr_w<int>(a.state)[b] = to;
+        __syncthreads();
+        const int c = __builtin_amdgcn_readfirstlane(share), cur = c >> 16, t = s.t0 + cur;
+        if (cur == kOver) break;
+        const float u = gptr<float>(a.uniforms)[t];
+        scan_part<kPathWaves>(a, s, t, b, c & 0xffff);
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (wave) continue;
+        int ended = 0;
+        if (lane_id() == 0) ended = atomicAdd(word + kEnded, 1);
+        if (__builtin_amdgcn_readfirstlane(ended) != a.parts - 1) continue;
+        const int len = agent_load(word + kLen);
+        const Row r = join_row(a, s, b, room);
+        const int z = draw(a, s, t, r, room, u);
+        int to = -1;
+        if (z >= 0 && len < a.max_depth)
+            for (int i0 = cur & ~63; i0 < s.n && to < 0; i0 += 64) {
+                const int i = i0 + lane_id();
+                int p = up, d = token;
+                if (i0) {
+                    p = d = -1;
+                    if (i < s.n) p = gptr<int>(a.parents)[s.t0 + i], d = gptr<int>(a.drafts)[s.t0 + i];
+                }
+                const uint64_t fit = __ballot(i > cur && p == cur && d == z);
+                if (fit) to = i0 + __builtin_ctzll(fit);
+            }
+        if (lane_id() == 0) {
+            agent_store(word + kEnded, 0);
+            agent_store(word + kLen, len + 1);
+            __builtin_amdgcn_s_waitcnt(0);
+            atomicExch(word + kTaken, (to < 0 ? kOver : to) << 16);
+        }
+        put_node(a, b, len, cur);
+        if (to < 0) put_end(a, b, len + 1, z);
+    }
+    if (threadIdx.x == 0 && atomicAdd(word + kGone, 1) == a.parts - 1)
+        for (int i = 0; i < 4; ++i) agent_store(word + i, 0);
 }

@@ -405,11 +405,12 @@ struct LogprobArgs {
 LPK_HD constexpr int logprob_rec(int top) { return 32 + 8 * top; }
 
 // Verification of drafted tokens.  A row's records: one a block of kVerifyBlock
-// logits, kVerifyLane a lane where they are joined.
+// logits, at most kVerifyBlocks.
 constexpr int kVerifyBlock = 1024;
-constexpr int kVerifyLane = 8;
-constexpr int kVerifyMaxVocab = 64 * kVerifyLane * kVerifyBlock;
+constexpr int kVerifyBlocks = 512;
+constexpr int kVerifyMaxVocab = kVerifyBlocks * kVerifyBlock;
 constexpr int kVerifyWaves = 16;       // of a workgroup of lp_verify_left
+constexpr int kPathWaves = 8;          // and of lp_verify_path
 struct VerifyState {                   // a sequence's walk down its tree
     int32_t cur, last, len, pending;   // node; children up to it were tried; nodes so far; a pass is due
     double taken, left;                // p - taken q is what is left of the row's distribution, `left` in all
@@ -421,11 +422,11 @@ struct VerifyArgs {
     uint64_t part;                     // records [rows, blocks] of 16 bytes
     uint64_t stats;                    // [tokens]: a row's sum, largest logit and draw, 16 bytes
     uint64_t left;                     // f64 [batch, blocks]: sums of what is left of a row
-    uint64_t state;                    // VerifyState [batch]; by levels i32 [batch]
+    uint64_t state;                    // VerifyState [batch]
     uint64_t sync;                     // arrival counters of the rows, then of the sequences
     int32_t stride, probs_stride, vocab, batch, tokens, max_q, max_depth;
     int32_t blocks, parts, per_part;   // blocks of a row; workgroups of a row and their blocks
-    int32_t level, row_counters;
+    int32_t row_counters, pad0;        // of the rows; of the path: from a sequence's to the next one's
 };
 
 struct ClearArgs {

@@ -174,7 +174,7 @@ enum Fn {
     kKeepQ4D128,
     kVerifyRows,
     kVerifyLeft,
-    kVerifyLevel,
+    kVerifyPath,
     kNumFns
 };
 
@@ -251,7 +251,7 @@ const FnSpec kSpecs[kNumFns] = {
     {"lp_tree.hsaco", "lp_kv_keep_f16_d64"}, {"lp_tree.hsaco", "lp_kv_keep_f16_d128"},
     {"lp_tree.hsaco", "lp_kv_keep_q4_d64"}, {"lp_tree.hsaco", "lp_kv_keep_q4_d128"},
     {"lp_verify.hsaco", "lp_verify_rows"},   {"lp_verify.hsaco", "lp_verify_left"},
-    {"lp_verify.hsaco", "lp_verify_level"},
+    {"lp_verify.hsaco", "lp_verify_path"},
 };
 
 const char* const kModules[] = {"lp_basic.hsaco", "lp_moe.hsaco", "lp_gemm.hsaco", "lp_attn.hsaco",
@@ -1439,7 +1439,7 @@ int lp_attn_tree(lp_ctx* c, const lp_kv_cache* cache, uint64_t q, int q_stride, 
 
 // How a verification goes over its rows, and its workspace.
 struct VerifyPlan {
-    bool levels;                // a launch for each node down, else all rows in one
+    bool path;                  // the rows of the path one behind the other, else all at once
     int blocks, parts, per_part;
     int left_parts, left_per;   // of what is left of a row (sampled drafts)
     int counters, row_counters;
@@ -1450,24 +1450,27 @@ static VerifyPlan verify_plan(int vocab, int batch, int tokens, int max_q, int m
     VerifyPlan p{};
     if (!batch || !tokens || !max_q) return p;
     p.blocks = (vocab + kVerifyBlock - 1) / kVerifyBlock;
-    // bytes a microsecond, and a launch's microseconds
-    const double rate = 4.5e6, launch = 6.0, row = 4.0 * vocab / rate;
-    const int downs = std::min(max_depth, max_q - 1) + 1;
-    p.levels = !probs && tokens * row > downs * (launch + batch * row);
-    const int rows = p.levels ? batch : tokens;
-    // about 2048 workgroups in all, four blocks at a time in each
-    const int steps = (p.blocks + 3) / 4, want = std::max(1, std::min(2048 / std::max(rows, 1), steps));
-    p.per_part = (steps + want - 1) / want * 4;
+    // All rows take about 8 us and 3.3 TB/s; the path's a node 6.5 us and 4 TB/s, and how
+    // many there are is known to be at most that (151,936 logits, sequences x nodes: 1 x 26 14.7
+    // us and 42; 1 x 200 45 and 37; 8 x 60 62 and 71; 32 x 26 100 and 69; 32 x 60 205 and 71)
+    const double all = 8.0 + 4.0 * tokens * vocab / 3.3e6, node = 6.5 + 4.0 * batch * vocab / 4e6;
+    p.path = !probs && all > (std::min(max_depth, max_q - 1) + 1) * node;
+    const int rows = p.path ? batch : tokens;
+    // about as many waves as the registers leave room for, a block at a time in each
+    const int waves = p.path ? kPathWaves : 4, steps = (p.blocks + waves - 1) / waves;
+    const int want = std::max(1, std::min(5120 / waves / std::max(rows, 1), steps));
+    p.per_part = (steps + want - 1) / want * waves;
     p.parts = (p.blocks + p.per_part - 1) / p.per_part;
-    p.row_counters = !p.levels && p.parts > 1 ? tokens : 0;
-    p.counters = p.row_counters + batch;
+    // (a path's words as far apart as they fit, for many look at them)
+    p.row_counters = p.path ? std::max(1, std::min(16, kPagedPairs / batch)) : p.parts > 1 ? tokens : 0;
+    p.counters = p.path ? batch * p.row_counters : p.row_counters + batch;
     auto take = [&](uint64_t n) {
         const uint64_t at = p.records;
         p.records = align256(p.records + n);
         return at;
     };
     take((uint64_t)rows * p.blocks * 16);
-    p.stats = take(p.levels ? 0 : (uint64_t)tokens * 16);
+    p.stats = take(p.path ? 0 : (uint64_t)tokens * 16);
     if (probs) {
         const int all = (p.blocks + kVerifyWaves - 1) / kVerifyWaves;
         const int each = std::max(1, std::min(512 / batch, all));
@@ -1475,7 +1478,7 @@ static VerifyPlan verify_plan(int vocab, int batch, int tokens, int max_q, int m
         p.left_parts = (p.blocks + p.left_per - 1) / p.left_per;
         p.left = take((uint64_t)batch * p.blocks * 8);
     }
-    p.state = take((uint64_t)batch * sizeof(VerifyState));
+    p.state = take(probs ? (uint64_t)batch * sizeof(VerifyState) : 0);
     p.bytes = with_counters(p.records, p.counters);
     return p;
 }
@@ -1519,12 +1522,7 @@ int lp_verify_tree(lp_ctx* c, uint64_t logits, int stride, int vocab, uint64_t d
     a.max_q = max_q, a.max_depth = max_depth;
     a.blocks = p.blocks, a.parts = p.parts, a.per_part = p.per_part, a.row_counters = p.row_counters;
     if (int r = join_counters(c, s, workspace + counters_at(p.records), p.counters, &a.sync)) return r;
-    if (p.levels) {
-        const int downs = std::min(max_depth, max_q - 1) + 1;
-        for (a.level = 0; a.level < downs; ++a.level)
-            if (int r = launch(c, kVerifyLevel, dim3((unsigned)(batch * p.parts)), dim3(256), 0, s, a)) return r;
-        return LP_OK;
-    }
+    if (p.path) return launch(c, kVerifyPath, dim3((unsigned)(batch * p.parts)), dim3(64 * kPathWaves), 0, s, a);
     if (int r = launch(c, kVerifyRows, dim3((unsigned)(tokens * p.parts)), dim3(256), 0, s, a)) return r;
     if (!probs) return LP_OK;
     a.parts = p.left_parts, a.per_part = p.left_per;

@@ -144,14 +144,55 @@ def test_many_sequences(cuda, K, sampled):
     _check(cuda, K, Case(rng, sizes, 300, 3, sampled, pad=2))
 
 
-@pytest.mark.parametrize("sizes,vocab,max_depth", [([60] * 12, 60000, 8), ([100, 3, 0, 80, 1], 150000, 12), ([300], 200001, 7),
-                                                   ([64] * 30, 9001, 5)])
+def _path_alone(K, sizes, vocab, max_depth):
+    """Whether a call reads the rows of the path one behind the other: its workspace
+    has no records of the others."""
+    n = K.verify_tree_ws_bytes(vocab, len(sizes), sum(sizes) + 2, max(sizes), max_depth, False)
+    return n < sum(sizes) * (vocab // 1024) * 16
+
+
+@pytest.mark.parametrize("sizes,vocab,max_depth", [([100, 3, 0, 80, 1], 150000, 3), ([300], 200001, 7), ([64] * 40, 30001, 5),
+                                                   ([0, 200, 150, 90, 0, 200], 70001, 6), ([120] * 64, 3001, 4),
+                                                   ([1000, 1, 700], 60001, 6), ([7] * 1300, 3000, 2)])
 def test_large_trees(cuda, K, sizes, vocab, max_depth):
     """Sizes at which the rows of the path alone are read."""
+    assert _path_alone(K, sizes, vocab, max_depth)
     rng = np.random.default_rng(vocab)
     temps = [rng.choice([0.0, 0.7, 1.0]) for _ in sizes]
     w = _check(cuda, K, Case(rng, sizes, vocab, max_depth, temps=temps, pad=1, front=1))
     assert w[1].max() > 2
+
+
+@pytest.mark.parametrize("kind", ["temperatures", "drafts", "numbers", "rows", "max_q"])
+def test_large_trees_at_the_ends(cuda, K, kind):
+    """What the tests below look at, where the rows of the path alone are read."""
+    rng = np.random.default_rng(len(kind))
+    sizes, vocab = [200] * 6, 30001
+    assert _path_alone(K, sizes, vocab, 5)
+    c = Case(rng, sizes, vocab, 5, luck=0.9, front=1, pad=1, temps=[0, -1, np.nan, 1e-6, 0.01, 50] if kind == "temperatures" else [0, 0.7, 0.7, 1, 1, 1])
+    if kind == "drafts":
+        c.drafts[rng.random(c.T) < 0.2] = -1
+        c.drafts[rng.random(c.T) < 0.1] = vocab
+        for t in rng.choice(c.T, 100, replace=False):
+            c.parents[t] = rng.choice([-1, 199, 200, -2 ** 31, 2 ** 31 - 1])
+        c.trees = [c.parents[c.starts[b]:c.starts[b + 1]].tolist() for b in range(6)]
+    if kind == "numbers":
+        c.u[:] = rng.choice([0.0, 2.0 ** -24, 1 - 2.0 ** -24], c.T)
+        c.x[:, :2300] = -np.inf
+        c.x[:, 29000:] = -np.inf
+    if kind == "rows":
+        c.x[::4, 1029] = np.inf
+        c.x[2::4, vocab - 1] = np.nan
+    if kind != "max_q":
+        _check(cuda, K, c, cols=3, shift=1)
+        return
+    full, c.trees = c.trees, [t[:150] for t in c.trees]
+    want = c.want()
+    c.trees = full
+    c.device(cuda, K, max_q=150)
+    c.run(K)
+    _same(c.got(cuda), want)
+    c.m.free()
 
 
 @pytest.mark.parametrize("sampled", [False, True])
@@ -264,7 +305,7 @@ def test_distributions_that_end(cuda, K):
 
 def test_starts_that_fall_change_nothing(cuda, K):
     rng = np.random.default_rng(13)
-    for vocab, n in ((200, 4), (9000, 400)):  # all rows at once, and by levels
+    for vocab, n in ((200, 4), (33000, 400)):  # all rows at once, and those of the path
         c = Case(rng, [n, n, n], vocab, 3)
         c.starts[2] = c.starts[1] - 2
         c.device(cuda, K)
