@@ -436,6 +436,7 @@ struct Few {
     static constexpr int kMerge = 4 * 16 * MS * 4 + 4 * 16 * 8;
     static constexpr int kLds = 4 * kWave > kMerge ? 4 * kWave : kMerge;
     static_assert(kFewRows * kFewParts * 4 <= kMerge, "the parts' weights fit");
+    static_assert(2 * kFewBatch * 4 <= kLds, "the sequences' units and blocks fit");
 };
 
 // Where a row keeps piece p (16 bytes).
@@ -467,7 +468,7 @@ __device__ __forceinline__ int few_units(const SeqView& s, int unit) {
 // cache lines that nothing here has read before, are read as usual, maximum and
 // sum of a row, which share a line with other pairs', at agent scope.
 template <int D, int NT>
-__device__ __forceinline__ void few_join(const AttnPagedArgs& a, uint8_t* lds, const SeqView& sv, int g, int nrows, int first, int S) {
+__device__ __forceinline__ void few_join(const AttnPagedArgs& a, uint8_t* lds, const SeqView& sv, int g, int row0, int nrows, int first, int S) {
     float* const wt = reinterpret_cast<float*>(lds);  // [row][kFewParts]
     const int wave = (int)(threadIdx.x >> 6), lane = lane_id();
     const uint64_t* const ml = reinterpret_cast<const uint64_t*>(a.part + (uint64_t)(uint32_t)(a.shares * a.rows) * (D * 4));
@@ -505,7 +506,7 @@ __device__ __forceinline__ void few_join(const AttnPagedArgs& a, uint8_t* lds, c
                 A[i] += gptr<f32x4_t>(from[i] + (uint64_t)(uint32_t)(s * a.rows) * (D * 4))[0] * w[i][s];
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int k = (int)threadIdx.x + 256 * i, row = k / TR, t = row / a.group, h = g * a.group + (row - t * a.group);
+            const int k = (int)threadIdx.x + 256 * i, row = k / TR, t = (row0 + row) / a.group, h = g * a.group + (row0 + row - t * a.group);
             if (row >= nrows) continue;
             const uint64_t o = a.out + ((uint64_t)(uint32_t)(sv.t0 + t) * (uint32_t)a.out_stride + (uint32_t)(h * D)) * 4;
             gptr_w<f32x4_t>(o)[k % TR] = A[i];
@@ -574,15 +575,16 @@ __device__ __forceinline__ void few_odd(const AttnPagedArgs& a, const SeqView& s
             }
 }
 
-// One part of a pair: units [u0, u1) of (sequence view sv, KV head g).
+// One part of a pair: units [u0, u1) of (sequence view sv, KV head g).  TREE: for the 16 NT
+// query rows from row0 on.
 template <int D, bool Q4, int NT, bool TREE>
-__device__ __forceinline__ void few_part(const AttnPagedArgs& a, uint8_t* lds, const SeqView& sv, int b, int g, int u0, int u1,
+__device__ __forceinline__ void few_part(const AttnPagedArgs& a, uint8_t* lds, const SeqView& sv, int b, int g, int row0, int u0, int u1,
                                          bool direct) {
     using F = Few<D, Q4>;
     constexpr int CR = F::CR, MT = F::MT, G = F::G, DT = F::DT, PC = F::PC, SP = F::SP, KS = F::KS;
     const int wave = (int)(threadIdx.x >> 6), lane = lane_id(), n = lane & 15, kb = lane >> 4;
-    const int nrows = sv.n * a.group;
-    const int r1 = (int)min((int64_t)seen_rows(a, sv, nrows - 1), (int64_t)u1 * (4 * CR));
+    const int all_rows = sv.n * a.group, nrows = TREE ? min(all_rows - row0, 16 * NT) : all_rows;
+    const int r1 = (int)min((int64_t)seen_rows(a, sv, all_rows - 1), (int64_t)u1 * (4 * CR));
     LP_LDS uint8_t* const mine = (LP_LDS uint8_t*)(lds + wave * F::kWave);
     const uint32_t base = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)mine);
 
@@ -648,7 +650,7 @@ __device__ __forceinline__ void few_part(const AttnPagedArgs& a, uint8_t* lds, c
         f32x4_t x[NT][KS][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const int row = min(nt * 16 + n, nrows - 1), i = row / a.group, h = g * a.group + (row - i * a.group);
+            const int row = row0 + min(nt * 16 + n, nrows - 1), i = row / a.group, h = g * a.group + (row - i * a.group);
             last[nt] = nt * 16 + n < nrows ? (TREE ? i : sv.p0 + i) : -1;
             const uint64_t q = a.q + ((uint64_t)(uint32_t)(sv.t0 + i) * (uint32_t)a.q_stride + (uint32_t)(h * D)) * 4 +
                                (Q4 ? D : 32) * kb;
@@ -976,7 +978,7 @@ __device__ __forceinline__ void few_part(const AttnPagedArgs& a, uint8_t* lds, c
                 A += *reinterpret_cast<const f32x4_any*>(sums + (w * 16 + q) * MS + 4 * d4) * f;
             }
             if (direct) {
-                const int i = row / a.group, h = g * a.group + (row - i * a.group);
+                const int i = (row0 + row) / a.group, h = g * a.group + (row0 + row - i * a.group);
                 const uint64_t o = a.out + ((uint64_t)(uint32_t)(sv.t0 + i) * (uint32_t)a.out_stride + (uint32_t)(h * D)) * 4;
                 const float f = L == 0.0f ? 0.0f : 1.0f / L;
                 gptr_w<f32x4_t>(o)[d4] = A * f;
@@ -1000,45 +1002,56 @@ __device__ __forceinline__ void few_body(const AttnPagedArgs& a) {
     __shared__ __align__(1024) uint8_t lds[F::kLds];
     __shared__ int flag;
     const int lane = lane_id(), kv = a.c.kv_heads;
-    int b, g, part = 0, parts = 1, per = INT32_MAX / kUnit;
+    int b, g, part = 0, parts = 1, per = INT32_MAX / kUnit, tile = 0;
     SeqView sv{0, 0, 0, 0};
     if (a.shares) {
         // units in a lane each (64 sequences), or in LDS
         int* const many = reinterpret_cast<int*>(lds);
         const bool lanes = a.batch <= 64;
         int mine = 0, total = 0;
+        // TREE: a pair's blocks of 16 NT query rows, each with that many units
+        auto tiles_of = [&](const SeqView& s) { return s.n > 0 ? (s.n * a.group + 16 * NT - 1) / (16 * NT) : 0; };
+        int tiles = 1;
         if (lanes) {
             if (lane < a.batch) sv = seq_view(a, lane);
             mine = few_units(sv, kUnit);
-            total = __builtin_amdgcn_readlane(wave_incl_scan(mine), 63);
+            if constexpr (TREE) tiles = tiles_of(sv);
+            total = __builtin_amdgcn_readlane(wave_incl_scan(TREE ? mine * tiles : mine), 63);
         } else {
-            for (int i = threadIdx.x; i < (a.batch + 63 & ~63); i += 256)
+            for (int i = threadIdx.x; i < (a.batch + 63 & ~63); i += 256) {
                 many[i] = i < a.batch ? few_units(seq_view(a, i), kUnit) : 0;
+                if constexpr (TREE) many[kFewBatch + i] = i < a.batch ? tiles_of(seq_view(a, i)) : 0;
+            }
             __syncthreads();
-            for (int i = 0; i < a.batch; i += 64) total += __builtin_amdgcn_readlane(wave_incl_scan(many[i + lane]), 63);
+            for (int i = 0; i < a.batch; i += 64)
+                total += __builtin_amdgcn_readlane(wave_incl_scan(TREE ? many[i + lane] * many[kFewBatch + i + lane] : many[i + lane]), 63);
         }
         auto parts_of = [&](int u) { return (u + per - 1) / per; };
         per = max((total * kv + a.shares - 1) / a.shares, a.min_units);
         for (;; per += (per + 7) / 8) {
             int n = 0;
-            for (int i = 0; i < a.batch; i += 64) n += __builtin_amdgcn_readlane(wave_incl_scan(parts_of(lanes ? mine : many[i + lane])), 63);
+            for (int i = 0; i < a.batch; i += 64)
+                n += __builtin_amdgcn_readlane(wave_incl_scan(parts_of(lanes ? mine : many[i + lane]) * (!TREE ? 1 : lanes ? tiles : many[kFewBatch + i + lane])), 63);
             if (n * kv <= a.shares) break;  // one part a pair always fits
         }
         // the sequence whose parts hold the workgroup's number
         int before = 0, at = (int)blockIdx.x;
         for (b = 0;; b += 64) {
             if (b >= a.batch) return;  // whole workgroups, here and below
-            const int n = parts_of(lanes ? mine : many[b + lane]), incl = before + kv * wave_incl_scan(n);
+            const int ti = !TREE ? 1 : lanes ? tiles : many[kFewBatch + b + lane];
+            const int n = parts_of(lanes ? mine : many[b + lane]), incl = before + kv * wave_incl_scan(n * ti);
             const int i = __popcll(__ballot(incl <= at));
             if (i < 64) {
                 parts = __builtin_amdgcn_readlane(n, i);
-                at -= __builtin_amdgcn_readlane(incl, i) - kv * parts;
+                if constexpr (TREE) tiles = __builtin_amdgcn_readlane(ti, i);
+                at -= __builtin_amdgcn_readlane(incl, i) - kv * parts * (TREE ? tiles : 1);
                 b += i;
                 break;
             }
             before = __builtin_amdgcn_readlane(incl, 63);
         }
         g = at / parts, part = at - g * parts;
+        if constexpr (TREE) tile = g % tiles, g /= tiles;
         if (lanes) {
             sv = SeqView{__builtin_amdgcn_readlane(sv.t0, b), __builtin_amdgcn_readlane(sv.n, b),
                          __builtin_amdgcn_readlane(sv.len, b), __builtin_amdgcn_readlane(sv.p0, b)};
@@ -1048,12 +1061,14 @@ __device__ __forceinline__ void few_body(const AttnPagedArgs& a) {
         }
     } else {  // a workgroup per pair
         b = (int)blockIdx.x / kv, g = (int)blockIdx.x - b * kv;
+        if constexpr (TREE) tile = b % a.tiles, b /= a.tiles;
         sv = seq_view(a, b);
         if (sv.n <= 0) return;
+        if (TREE && tile * (16 * NT) >= sv.n * a.group) return;
     }
-    few_part<D, Q4, NT, TREE>(a, lds, sv, b, g, part * per, part * per + per, parts == 1);
+    few_part<D, Q4, NT, TREE>(a, lds, sv, b, g, TREE ? tile * (16 * NT) : 0, part * per, part * per + per, parts == 1);
     if (parts == 1) return;
-    int* const count = reinterpret_cast<int*>(a.sync) + (b * kv + g) * kPagedStride;
+    int* const count = reinterpret_cast<int*>(a.sync) + (TREE ? (b * kv + g) * a.tiles + tile : b * kv + g) * kPagedStride;
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -1062,7 +1077,8 @@ __device__ __forceinline__ void few_body(const AttnPagedArgs& a) {
         flag = o;
     }
     __syncthreads();
-    if (flag == parts - 1) few_join<D, NT>(a, lds, sv, g, sv.n * a.group, (int)blockIdx.x - part, parts);
+    const int row0 = TREE ? tile * (16 * NT) : 0, nrows = TREE ? min(sv.n * a.group - row0, 16 * NT) : sv.n * a.group;
+    if (flag == parts - 1) few_join<D, NT>(a, lds, sv, g, row0, nrows, (int)blockIdx.x - part, parts);
 }
 
 // ---------------------------------------------------------------------------

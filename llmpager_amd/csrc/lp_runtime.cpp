@@ -1232,7 +1232,8 @@ static void paged_spans(int64_t wgs, int max_seq, int* span, int* splits) {
 
 struct PagedPlan {
     int max_q, max_seq, rows;
-    int shares, min_units;    // few query rows
+    int few;                  // query rows of a block of lp_attn_few_* (0: many)
+    int shares, min_units;    // of these
     int tiles, span, splits;  // many
     uint64_t bytes;           // of the records and, with shares, the pairs' counters
 };
@@ -1289,6 +1290,7 @@ static PagedPlan paged_plan(const lp_kv_cache* c, int heads, int batch, int toke
     if (!p.rows) return p;  // nothing to do: no workspace
     const int pairs = batch * c->kv_heads;
     if (p.rows <= kFewRows) {
+        p.few = p.rows > 16 ? 32 : 16;
         // a workgroup's unit: a chunk for each of its four waves
         const int unit = c->format == LP_KV_Q4 ? 256 : 128;
         const int units = std::max(1, (p.max_seq + unit - 1) / unit);
@@ -1306,6 +1308,33 @@ static PagedPlan paged_plan(const lp_kv_cache* c, int heads, int batch, int toke
         paged_spans((int64_t)pairs * p.tiles, p.max_seq, &p.span, &p.splits);
         if (p.splits > 1) p.bytes = (uint64_t)pairs * p.splits * p.rows * (c->head_dim + 2) * 4;
     }
+    return p;
+}
+
+// Attention of trees.  More than 16 query rows go to lp_attn_tree_few_*, too, in blocks of 16
+// of them that have parts of their own, while blocks times units of the longest context are
+// few: a block's chain of round trips is shorter, and its parts are joined where they end.
+// Else as paged_plan.  (Heads 32 on 4 of 128, sequences x tokens over rows: 1 x 26 over 1,500 17.4
+// us against 20.8, 1 x 60 22 against 30, 4 x 60 25.8 against 33.3 and over 3,000 39.2 against 40.8,
+// 8 x 32 over 3,000 50 against 42; with 4 bits 16.2 against 21.2, 19.8 against 32.5, 24.5 against
+// 34.4, 37.9 against 41.5 and 46.8 against 42.2.  16-bit contexts that are many as well
+// are read too often: 16 x 8 over 3,000 43 against 32.5.  17 to 32 rows: 64 x 4 over 4,000 with 16
+// bits 91 against 83, 32 x 4 over 3,000 37 against 41; with 4 bits 55 against 63.)
+constexpr int kTreeUnits = 5760, kTreeUnits32 = 8192, kTreePairUnits = 1024;
+static PagedPlan tree_plan(const lp_kv_cache* c, int heads, int batch, int tokens, int max_q, int max_seq) {
+    PagedPlan p = paged_plan(c, heads, batch, tokens, max_q, max_seq);
+    if (p.few) p.tiles = 1;
+    if (p.rows <= 16) return p;
+    const bool q4 = c->format == LP_KV_Q4;
+    const int unit = q4 ? 256 : 128, units = std::max(1, (p.max_seq + unit - 1) / unit), tiles = (p.rows + 15) / 16;
+    const int64_t pairs = (int64_t)batch * c->kv_heads, blocks = pairs * tiles;
+    if (blocks > kPagedPairs || batch > kFewBatch) return p;
+    if (p.few ? !q4 && blocks * units > kTreeUnits32
+              : blocks * units > kTreeUnits || (!q4 && pairs * units > kTreePairUnits))
+        return p;
+    p = PagedPlan{p.max_q, p.max_seq, 16, 16, 0, (units + kFewParts - 1) / kFewParts, tiles, INT32_MAX, 1, 0};
+    if (units > 1) p.shares = (int)std::min<int64_t>(std::max<int64_t>(512, blocks), blocks * units);
+    if (p.shares) p.bytes = with_counters((uint64_t)p.shares * p.rows * (c->head_dim * 4 + 8), (int)blocks);
     return p;
 }
 
@@ -1329,20 +1358,21 @@ static int check_nodes(const char* who, int max_q) {
     return LP_OK;
 }
 
-static uint64_t attn_ws(const char* who, const lp_kv_cache* cache, int heads, int batch, int tokens, int max_q, int max_seq) {
+static uint64_t attn_ws(const char* who, bool tree, const lp_kv_cache* cache, int heads, int batch, int tokens, int max_q,
+                        int max_seq) {
     PagedCache pc;
     if (check_paged(who, cache, &pc) || check_batch(who, heads, cache->kv_heads, batch, tokens, 4, 4) ||
         check_queries(who, heads, cache->kv_heads, batch, tokens, max_q, max_seq))
         return 0;
-    return paged_plan(cache, heads, batch, tokens, max_q, max_seq).bytes;
+    return (tree ? tree_plan : paged_plan)(cache, heads, batch, tokens, max_q, max_seq).bytes;
 }
 
 uint64_t lp_attn_paged_ws_bytes(const lp_kv_cache* cache, int heads, int batch, int tokens, int max_q, int max_seq) {
-    return attn_ws("attn_paged", cache, heads, batch, tokens, max_q, max_seq);
+    return attn_ws("attn_paged", false, cache, heads, batch, tokens, max_q, max_seq);
 }
 
 uint64_t lp_attn_tree_ws_bytes(const lp_kv_cache* cache, int heads, int batch, int tokens, int max_q, int max_seq) {
-    return check_nodes("attn_tree", max_q) ? 0 : attn_ws("attn_tree", cache, heads, batch, tokens, max_q, max_seq);
+    return check_nodes("attn_tree", max_q) ? 0 : attn_ws("attn_tree", true, cache, heads, batch, tokens, max_q, max_seq);
 }
 
 // A workspace of at least `need` bytes (none of 0).
@@ -1374,7 +1404,7 @@ static int attn_call(const char* name, lp_ctx* c, const lp_kv_cache* cache, uint
         if (!masks || masks % 8) return fail(LP_E_INVALID, who + ": masks null or not 8-byte aligned");
     }
     if (int r = check_queries(name, heads, cache->kv_heads, batch, tokens, max_q, max_seq)) return r;
-    const PagedPlan plan = paged_plan(cache, heads, batch, tokens, max_q, max_seq);
+    const PagedPlan plan = (tree ? tree_plan : paged_plan)(cache, heads, batch, tokens, max_q, max_seq);
     if (int r = check_workspace(name, plan.bytes, workspace, ws_bytes)) return r;
     if (int r = check_ctx(c)) return r;
     if (!batch || !tokens || !max_q) return LP_OK;
@@ -1385,13 +1415,14 @@ static int attn_call(const char* name, lp_ctx* c, const lp_kv_cache* cache, uint
     a.splits = plan.splits, a.span = plan.span, a.part = workspace;
     a.scale = scale, a.masks = masks, a.words = (max_q + 63) / 64;
     const int pairs = batch * cache->kv_heads, which = (cache->format == LP_KV_Q4 ? 2 : 0) + (D == 128 ? 1 : 0);
-    if (plan.rows <= kFewRows) {
+    if (plan.few) {
         // (no shares, with more pairs than there are counters: a workgroup per pair)
-        a.shares = plan.shares, a.min_units = plan.min_units;
+        a.shares = plan.shares, a.min_units = plan.min_units, a.tiles = plan.tiles;
+        const int blocks = pairs * std::max(plan.tiles, 1);
         if (a.shares)
-            if (int r = join_counters(c, s, workspace + plan.bytes - (uint64_t)pairs * kPagedStride * 4, pairs, &a.sync)) return r;
-        const Fn f = (Fn)((tree ? kAttnTreeFewF16D64 : kAttnFewF16D64) + (plan.rows > 16 ? 4 : 0) + which);
-        return launch(c, f, dim3((unsigned)(a.shares ? a.shares : pairs)), dim3(256), 0, s, a);
+            if (int r = join_counters(c, s, workspace + plan.bytes - (uint64_t)blocks * kPagedStride * 4, blocks, &a.sync)) return r;
+        const Fn f = (Fn)((tree ? kAttnTreeFewF16D64 : kAttnFewF16D64) + (plan.few > 16 ? 4 : 0) + which);
+        return launch(c, f, dim3((unsigned)(a.shares ? a.shares : blocks)), dim3(256), 0, s, a);
     }
     a.tiles = plan.tiles;
     const unsigned wgs = (unsigned)((int64_t)pairs * plan.tiles * plan.splits);

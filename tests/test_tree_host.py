@@ -152,10 +152,18 @@ def test_workspaces_checked(probs, vocab, batch, tokens, max_q, max_depth):
         assert _verify(**dict(kw, workspace=0, ws_bytes=0, **none)) == INVALID and "null context" in _said()
 
 
-def test_attention_workspaces_are_those_of_the_paged_one():
-    for q, seq in ((1, 60), (7, 6000), (256, 40000)):
-        c = _cache(max_pages=4096)
-        assert lp.lib().lp_attn_tree_ws_bytes(c, 8, 3, 600, q, seq) == lp.lib().lp_attn_paged_ws_bytes(c, 8, 3, 600, q, seq)
+def test_attention_workspaces_checked():
+    c = _cache(max_pages=4096)
+    for heads, batch, q, seq in ((4, 2, 2, 60000), (64, 1, 26, 1500), (64, 16, 32, 6000), (64, 4, 1024, 60000)):
+        kw = dict(heads=heads, q_stride=heads * 128, out_stride=heads * 128, batch=batch, tokens=batch * q, max_q=q, max_seq=seq)
+        need = lp.lib().lp_attn_tree_ws_bytes(c, heads, batch, batch * q, q, seq)
+        assert _attn(c, ws_bytes=need, **kw) == INVALID and "null context" in _said()
+        if need:
+            assert _attn(c, ws_bytes=need - 1, **kw) == INVALID and "workspace" in _said()
+            assert _attn(c, workspace=0, **kw) == INVALID and "null workspace" in _said()
+            assert _attn(c, workspace=P + 64, **kw) == UNSUPPORTED and "workspace" in _said()
+    assert lp.lib().lp_attn_tree_ws_bytes(c, 64, 16, 512, 32, 6000) > 0
+    assert _attn(c, workspace=0, ws_bytes=0, max_q=0, max_seq=60000) == INVALID and "null context" in _said()
 
 
 # ---- the formulas -------------------------------------------------------------------
