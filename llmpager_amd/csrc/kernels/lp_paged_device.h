@@ -361,6 +361,16 @@ __device__ __forceinline__ bool tree_sees_row(const AttnPagedArgs& a, const SeqV
 __device__ __forceinline__ uint64_t rec_index(const AttnPagedArgs& a, int bg, int split, int row) {
     return ((uint64_t)(uint32_t)bg * (uint32_t)a.splits + (uint32_t)split) * (uint32_t)a.rows + (uint32_t)row;
 }
+// lp_attn_tree_many_*: kManyRows records a workgroup, {maximum, sum} behind all of them; then
+// of each block of query rows its first workgroup and, above it, how many it has.
+template <int D>
+__device__ __forceinline__ uint64_t tree_rec_sums(const AttnPagedArgs& a) {
+    return a.part + (uint64_t)(uint32_t)a.shares * (kManyRows * D * 4);
+}
+template <int D>
+__device__ __forceinline__ uint64_t tree_blocks(const AttnPagedArgs& a) {
+    return tree_rec_sums<D>(a) + (uint64_t)(uint32_t)a.shares * (kManyRows * 8);
+}
 template <int D>
 __device__ __forceinline__ uint64_t rec_sums(const AttnPagedArgs& a) {
     return a.part + (uint64_t)(uint32_t)(a.batch * a.c.kv_heads) * (uint32_t)a.splits * (uint32_t)a.rows * (D * 4);
@@ -436,7 +446,7 @@ struct Few {
     static constexpr int kMerge = 4 * 16 * MS * 4 + 4 * 16 * 8;
     static constexpr int kLds = 4 * kWave > kMerge ? 4 * kWave : kMerge;
     static_assert(kFewRows * kFewParts * 4 <= kMerge, "the parts' weights fit");
-    static_assert(2 * kFewBatch * 4 <= kLds, "the sequences' units and blocks fit");
+    static_assert(2 * kFewBatch * 4 <= kLds, "the sequences' units and blocks fit (share_of)");
 };
 
 // Where a row keeps piece p (16 bytes).
@@ -995,31 +1005,33 @@ __device__ __forceinline__ void few_part(const AttnPagedArgs& a, uint8_t* lds, c
     }
 }
 
-template <int D, bool Q4, int NT, bool TREE>
-__device__ __forceinline__ void few_body(const AttnPagedArgs& a) {
-    using F = Few<D, Q4>;
-    constexpr int kUnit = 4 * F::CR;
-    __shared__ __align__(1024) uint8_t lds[F::kLds];
-    __shared__ int flag;
+// The workgroup's part: units (of UNIT rows of the context) part per .. of sequence b's KV head
+// g; TREE: for its block `tile` of ROWS query rows, each of which has all of them.  Every
+// workgroup finds its own from the lengths.
+struct Share {
+    int b, g, tile, part, parts, per;  // b < 0: none
+    SeqView sv;
+};
+template <int UNIT, int ROWS, bool TREE>
+__device__ __forceinline__ Share share_of(const AttnPagedArgs& a, int* many) {
     const int lane = lane_id(), kv = a.c.kv_heads;
-    int b, g, part = 0, parts = 1, per = INT32_MAX / kUnit, tile = 0;
+    int b, g, part = 0, parts = 1, per = INT32_MAX / UNIT, tile = 0;
     SeqView sv{0, 0, 0, 0};
+    const Share none{-1, 0, 0, 0, 1, 0, sv};
     if (a.shares) {
         // units in a lane each (64 sequences), or in LDS
-        int* const many = reinterpret_cast<int*>(lds);
         const bool lanes = a.batch <= 64;
         int mine = 0, total = 0;
-        // TREE: a pair's blocks of 16 NT query rows, each with that many units
-        auto tiles_of = [&](const SeqView& s) { return s.n > 0 ? (s.n * a.group + 16 * NT - 1) / (16 * NT) : 0; };
+        auto tiles_of = [&](const SeqView& s) { return s.n > 0 ? (s.n * a.group + ROWS - 1) / ROWS : 0; };
         int tiles = 1;
         if (lanes) {
             if (lane < a.batch) sv = seq_view(a, lane);
-            mine = few_units(sv, kUnit);
+            mine = few_units(sv, UNIT);
             if constexpr (TREE) tiles = tiles_of(sv);
             total = __builtin_amdgcn_readlane(wave_incl_scan(TREE ? mine * tiles : mine), 63);
         } else {
             for (int i = threadIdx.x; i < (a.batch + 63 & ~63); i += 256) {
-                many[i] = i < a.batch ? few_units(seq_view(a, i), kUnit) : 0;
+                many[i] = i < a.batch ? few_units(seq_view(a, i), UNIT) : 0;
                 if constexpr (TREE) many[kFewBatch + i] = i < a.batch ? tiles_of(seq_view(a, i)) : 0;
             }
             __syncthreads();
@@ -1028,7 +1040,7 @@ __device__ __forceinline__ void few_body(const AttnPagedArgs& a) {
         }
         auto parts_of = [&](int u) { return (u + per - 1) / per; };
         per = max((total * kv + a.shares - 1) / a.shares, a.min_units);
-        for (;; per += (per + 7) / 8) {
+        for (;; per += ROWS == kManyRows ? (per + 63) / 64 : (per + 7) / 8) {
             int n = 0;
             for (int i = 0; i < a.batch; i += 64)
                 n += __builtin_amdgcn_readlane(wave_incl_scan(parts_of(lanes ? mine : many[i + lane]) * (!TREE ? 1 : lanes ? tiles : many[kFewBatch + i + lane])), 63);
@@ -1037,7 +1049,7 @@ __device__ __forceinline__ void few_body(const AttnPagedArgs& a) {
         // the sequence whose parts hold the workgroup's number
         int before = 0, at = (int)blockIdx.x;
         for (b = 0;; b += 64) {
-            if (b >= a.batch) return;  // whole workgroups, here and below
+            if (b >= a.batch) return none;
             const int ti = !TREE ? 1 : lanes ? tiles : many[kFewBatch + b + lane];
             const int n = parts_of(lanes ? mine : many[b + lane]), incl = before + kv * wave_incl_scan(n * ti);
             const int i = __popcll(__ballot(incl <= at));
@@ -1063,9 +1075,23 @@ __device__ __forceinline__ void few_body(const AttnPagedArgs& a) {
         b = (int)blockIdx.x / kv, g = (int)blockIdx.x - b * kv;
         if constexpr (TREE) tile = b % a.tiles, b /= a.tiles;
         sv = seq_view(a, b);
-        if (sv.n <= 0) return;
-        if (TREE && tile * (16 * NT) >= sv.n * a.group) return;
+        if (sv.n <= 0) return none;
+        if (TREE && tile * ROWS >= sv.n * a.group) return none;
     }
+    return Share{b, g, tile, part, parts, per, sv};
+}
+
+template <int D, bool Q4, int NT, bool TREE>
+__device__ __forceinline__ void few_body(const AttnPagedArgs& a) {
+    using F = Few<D, Q4>;
+    constexpr int kUnit = 4 * F::CR;
+    __shared__ __align__(1024) uint8_t lds[F::kLds];
+    __shared__ int flag;
+    const int kv = a.c.kv_heads;
+    const Share t = share_of<kUnit, 16 * NT, TREE>(a, reinterpret_cast<int*>(lds));
+    if (t.b < 0) return;  // whole workgroups, here and below
+    const SeqView sv = t.sv;
+    const int b = t.b, g = t.g, tile = t.tile, part = t.part, parts = t.parts, per = t.per;
     few_part<D, Q4, NT, TREE>(a, lds, sv, b, g, TREE ? tile * (16 * NT) : 0, part * per, part * per + per, parts == 1);
     if (parts == 1) return;
     int* const count = reinterpret_cast<int*>(a.sync) + (TREE ? (b * kv + g) * a.tiles + tile : b * kv + g) * kPagedStride;
@@ -1157,16 +1183,36 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
     // at once, two a CU, the second ones go from the shortest up (426 us, 419).
     const int pairs = a.batch * a.c.kv_heads, total = pairs * a.tiles;
     int id = (int)blockIdx.x % total;
-    const int split = (int)blockIdx.x / total;
+    int split = (int)blockIdx.x / total;
     if (id >= 256 && total <= 512) id = total - 1 - (id - 256);
-    const int bg = (id + id / pairs + split) % pairs, tile = a.tiles - 1 - id / pairs;
-    const int b = bg / a.c.kv_heads, g = bg - b * a.c.kv_heads;
-    const SeqView sv = seq_view(a, b);
+    int bg = (id + id / pairs + split) % pairs, tile = a.tiles - 1 - id / pairs;
+    int b = bg / a.c.kv_heads, g = bg - b * a.c.kv_heads;
+    SeqView sv = seq_view(a, b);
+    // TREE: a pair's blocks all walk the same rows of the context, so that where there are
+    // parts at all they are shared out by the lengths in memory, as for few query rows (16
+    // sequences of up to 32 tokens, 32 heads on 4 of 128, behind up to 6,000 4-bit rows, 60 % of
+    // that on average: 81 us, 87 with spans of the bounds; where there is a block for each of
+    // 512 workgroups the order above stays, 150 us against 158 of four sequences).
+    int nth = 0, parts = 1, per = INT32_MAX / CR;
+    if (TREE && a.shares) {
+        const Share t = share_of<CR, kManyRows, true>(a, reinterpret_cast<int*>(lds));
+        if (t.b < 0) return;
+        sv = t.sv, b = t.b, g = t.g, tile = t.tile, nth = t.part, parts = t.parts, per = t.per, split = (int)blockIdx.x;
+        if (nth == 0 && tid == 0)
+            gptr_w<uint64_t>(tree_blocks<D>(a))[(b * a.c.kv_heads + g) * a.tiles + tile] = (uint64_t)(uint32_t)parts << 32 | blockIdx.x;
+    }
+    if constexpr (TREE) {  // (scalars, that nothing spills)
+        sv.t0 = __builtin_amdgcn_readfirstlane(sv.t0), sv.n = __builtin_amdgcn_readfirstlane(sv.n);
+        sv.len = __builtin_amdgcn_readfirstlane(sv.len), sv.p0 = __builtin_amdgcn_readfirstlane(sv.p0);
+        b = __builtin_amdgcn_readfirstlane(b), g = __builtin_amdgcn_readfirstlane(g), tile = __builtin_amdgcn_readfirstlane(tile);
+        nth = __builtin_amdgcn_readfirstlane(nth), parts = __builtin_amdgcn_readfirstlane(parts), per = __builtin_amdgcn_readfirstlane(per);
+    }
     const int nrows = sv.n * a.group, row0 = tile * kManyRows;
     if (row0 >= nrows) return;  // whole workgroups, here and below
     const int vis = seen_rows(a, sv, (TREE ? nrows : min(row0 + kManyRows, nrows)) - 1);
-    const int r0 = split * a.span, r1 = min(vis, r0 + a.span);
-    if (r0 >= r1 && split > 0) return;
+    const int r0 = TREE ? nth * per * CR : split * a.span;
+    const int r1 = TREE ? (int)min((int64_t)vis, ((int64_t)nth + 1) * per * CR) : min(vis, r0 + a.span);
+    if (r0 >= r1 && split > 0 && !TREE) return;
     const uint32_t lbase = (uint32_t)(uintptr_t)(LP_LDS uint8_t*)lds;
     LP_LDS uint8_t* const ll = (LP_LDS uint8_t*)lds;
 
@@ -1402,8 +1448,8 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
         asm volatile("" : "+v"(me));
         Place p;
         const int r = row0 + 32 * wave + (me & 31), t = r / a.group, head = g * a.group + (r - t * a.group);
-        p.h = me >> 5, p.on = r < nrows, p.direct = vis <= a.span;
-        p.rec = rec_index(a, bg, split, r);
+        p.h = me >> 5, p.on = r < nrows, p.direct = TREE ? parts == 1 : vis <= a.span;
+        p.rec = TREE ? (uint64_t)(uint32_t)split * kManyRows + (uint32_t)(r - row0) : rec_index(a, bg, split, r);
         p.at = p.direct ? a.out + ((uint64_t)(uint32_t)(sv.t0 + t) * (uint32_t)a.out_stride + (uint32_t)(head * D)) * 4
                         : a.part + p.rec * (D * 4);
         return p;
@@ -1622,7 +1668,7 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
             if (put) x += get4(p, d, e) * fput;
             put4(p, d, e, x * f);
         }
-    if (!p.direct && p.h == 0) gptr_w<float2>(rec_sums<D>(a))[p.rec] = make_float2(m, l);
+    if (!p.direct && p.h == 0) gptr_w<float2>(TREE ? tree_rec_sums<D>(a) : rec_sums<D>(a))[p.rec] = make_float2(m, l);
 }
 
 // The records of a query row of a sequence with several splits, joined: a wave
@@ -1636,12 +1682,22 @@ __device__ __forceinline__ void join_body(const AttnPagedArgs& a) {
     const int nrows = sv.n * a.group;
     if (row >= nrows) return;
     // the rows that its workgroup walked
-    const int vis = seen_rows(a, sv, (TREE ? nrows : min(row / kManyRows * kManyRows + kManyRows, nrows)) - 1);
-    if (vis <= a.span) return;  // written directly
-    const int S = __builtin_amdgcn_readfirstlane((vis + a.span - 1) / a.span);
-    const uint64_t r0 = rec_index(a, bg, 0, row);
+    int S;
+    uint64_t r0;
+    if constexpr (TREE) {
+        const uint64_t block = gptr<uint64_t>(tree_blocks<D>(a))[bg * a.tiles + row / kManyRows];
+        S = __builtin_amdgcn_readfirstlane((int)(block >> 32));
+        if (S == 1) return;  // written directly
+        r0 = (uint64_t)(uint32_t)block * kManyRows + (uint32_t)(row % kManyRows);
+    } else {
+        const int vis = seen_rows(a, sv, min(row / kManyRows * kManyRows + kManyRows, nrows) - 1);
+        if (vis <= a.span) return;  // written directly
+        S = __builtin_amdgcn_readfirstlane((vis + a.span - 1) / a.span);
+        r0 = rec_index(a, bg, 0, row);
+    }
+    const int step = TREE ? kManyRows : a.rows;
     float2 x = make_float2(-INFINITY, 0.0f);
-    if (lane < S) x = gptr<float2>(rec_sums<D>(a))[r0 + (uint64_t)(uint32_t)lane * (uint32_t)a.rows];
+    if (lane < S) x = gptr<float2>(TREE ? tree_rec_sums<D>(a) : rec_sums<D>(a))[r0 + (uint64_t)(uint32_t)lane * (uint32_t)step];
     const float M = wave_max(x.x);
     const float f = x.x == -INFINITY ? 1.0f : exp2_hw(x.x - M);
     float L = f * x.y;
@@ -1655,7 +1711,7 @@ __device__ __forceinline__ void join_body(const AttnPagedArgs& a) {
 #pragma unroll
         for (int u = 0; u < 16; ++u) {
             if (s0 + u >= S) break;
-            const uint64_t at = a.part + (r0 + (uint64_t)(uint32_t)(s0 + u) * (uint32_t)a.rows) * (D * 4);
+            const uint64_t at = a.part + (r0 + (uint64_t)(uint32_t)(s0 + u) * (uint32_t)step) * (D * 4);
             if constexpr (C == 2) {
                 const float2 v = gptr<float2>(at)[lane];
                 x[u][0] = v.x, x[u][1] = v.y;

@@ -361,8 +361,9 @@ struct AttnPagedArgs {
     int32_t rows;                   // query rows of a (sequence, KV head): max_q group
     float scale;
     uint64_t part;                  // records of the parts of a context
-    // lp_attn_few_*: workgroups for the pairs' parts (0: a workgroup per pair), the
-    // fewest units of a part, arrival counters of the pairs
+    // lp_attn_few_*, lp_attn_tree_many_*: workgroups for the pairs' parts (0: a workgroup per
+    // pair, many: and block of query rows), the fewest units of a part; few: arrival counters of
+    // the pairs
     int32_t shares, min_units;
     uint64_t sync;
     // lp_attn_many_*: workgroups of kManyRows query rows; rows of the context per

@@ -1314,7 +1314,8 @@ static PagedPlan paged_plan(const lp_kv_cache* c, int heads, int batch, int toke
 // Attention of trees.  More than 16 query rows go to lp_attn_tree_few_*, too, in blocks of 16
 // of them that have parts of their own, while blocks times units of the longest context are
 // few: a block's chain of round trips is shorter, and its parts are joined where they end.
-// Else as paged_plan.  (Heads 32 on 4 of 128, sequences x tokens over rows: 1 x 26 over 1,500 17.4
+// Else as paged_plan, but that where the rows of the context are split, 512 workgroups, two a CU,
+// share out what they turn out to be (at 64 rows a unit).  (Heads 32 on 4 of 128, sequences x tokens over rows: 1 x 26 over 1,500 17.4
 // us against 20.8, 1 x 60 22 against 30, 4 x 60 25.8 against 33.3 and over 3,000 39.2 against 40.8,
 // 8 x 32 over 3,000 50 against 42; with 4 bits 16.2 against 21.2, 19.8 against 32.5, 24.5 against
 // 34.4, 37.9 against 41.5 and 46.8 against 42.2.  16-bit contexts that are many as well
@@ -1328,10 +1329,16 @@ static PagedPlan tree_plan(const lp_kv_cache* c, int heads, int batch, int token
     const bool q4 = c->format == LP_KV_Q4;
     const int unit = q4 ? 256 : 128, units = std::max(1, (p.max_seq + unit - 1) / unit), tiles = (p.rows + 15) / 16;
     const int64_t pairs = (int64_t)batch * c->kv_heads, blocks = pairs * tiles;
-    if (blocks > kPagedPairs || batch > kFewBatch) return p;
-    if (p.few ? !q4 && blocks * units > kTreeUnits32
-              : blocks * units > kTreeUnits || (!q4 && pairs * units > kTreePairUnits))
+    const bool fit = blocks <= kPagedPairs && batch <= kFewBatch;
+    if (p.few && (!fit || (!q4 && blocks * units > kTreeUnits32))) return p;
+    if (!p.few && (!fit || blocks * units > kTreeUnits || (!q4 && pairs * units > kTreePairUnits))) {
+        if (p.splits == 1) return p;
+        const int chunks = (p.max_seq + 63) / 64;
+        p.shares = (int)std::min<int64_t>(512, pairs * p.tiles * chunks);
+        p.min_units = std::max(2, (chunks + kFewParts - 1) / kFewParts);
+        p.bytes = (uint64_t)p.shares * kManyRows * (c->head_dim * 4 + 8) + (uint64_t)pairs * p.tiles * 8;
         return p;
+    }
     p = PagedPlan{p.max_q, p.max_seq, 16, 16, 0, (units + kFewParts - 1) / kFewParts, tiles, INT32_MAX, 1, 0};
     if (units > 1) p.shares = (int)std::min<int64_t>(std::max<int64_t>(512, blocks), blocks * units);
     if (p.shares) p.bytes = with_counters((uint64_t)p.shares * p.rows * (c->head_dim * 4 + 8), (int)blocks);
@@ -1425,7 +1432,8 @@ static int attn_call(const char* name, lp_ctx* c, const lp_kv_cache* cache, uint
         return launch(c, f, dim3((unsigned)(a.shares ? a.shares : blocks)), dim3(256), 0, s, a);
     }
     a.tiles = plan.tiles;
-    const unsigned wgs = (unsigned)((int64_t)pairs * plan.tiles * plan.splits);
+    if (tree) a.shares = plan.shares, a.min_units = plan.min_units;
+    const unsigned wgs = a.shares ? (unsigned)a.shares : (unsigned)((int64_t)pairs * plan.tiles * plan.splits);
     if (int r = launch(c, (Fn)((tree ? kAttnTreeManyF16D64 : kAttnManyF16D64) + which), dim3(wgs), dim3(256), 0, s, a)) return r;
     if (plan.splits == 1) return LP_OK;
     const int64_t rows = (int64_t)pairs * plan.rows;

@@ -355,6 +355,18 @@ def test_attention_many_sequences_in_blocks(cuda, K, fmt):
 
 
 @pytest.mark.parametrize("fmt,dim", FORMS)
+@pytest.mark.parametrize("n", [3, 64, 80])
+def test_attention_of_many_rows_shared_out(cuda, K, fmt, dim, n):
+    """128 query rows and more a workgroup, whose parts go by the lengths in memory: some
+    sequences have none, some one, some several; in lanes, and past as many sequences."""
+    rng = np.random.default_rng(dim)
+    long, bound = (1000, 4000) if n > 3 else (6000, 96000)
+    past = [0, long] + [int(p) for p in rng.integers(0, long // 2, n - 2)]
+    trees = [random_tree(rng, 14), random_tree(rng, 9)] + [random_tree(rng, int(k)) if k else [] for k in rng.integers(0, 14, n - 2)]
+    _check_attn(K, Trees(cuda, trees, past, 16, 1, dim, 16, fmt, seed=n, cols=bound // 16), bound)
+
+
+@pytest.mark.parametrize("fmt,dim", FORMS)
 @pytest.mark.parametrize("n,heads", [(3, 8), (9, 2), (40, 8), (130, 8)])
 def test_attention_long_contexts(cuda, K, fmt, dim, n, heads):
     """Contexts that many workgroups share, ragged ones, and joins of their parts."""
