@@ -1321,7 +1321,7 @@ static PagedPlan paged_plan(const lp_kv_cache* c, int heads, int batch, int toke
 // 34.4, 37.9 against 41.5 and 46.8 against 42.2.  16-bit contexts that are many as well
 // are read too often: 16 x 8 over 3,000 43 against 32.5.  17 to 32 rows: 64 x 4 over 4,000 with 16
 // bits 91 against 83, 32 x 4 over 3,000 37 against 41; with 4 bits 55 against 63.)
-constexpr int kTreeUnits = 5760, kTreeUnits32 = 8192, kTreePairUnits = 1024;
+constexpr int kTreeUnits = 5760, kTreeUnits32 = 8192, kTreePairUnits = 1024, kTreeUnitsOne = 1280;
 static PagedPlan tree_plan(const lp_kv_cache* c, int heads, int batch, int tokens, int max_q, int max_seq) {
     PagedPlan p = paged_plan(c, heads, batch, tokens, max_q, max_seq);
     if (p.few) p.tiles = 1;
@@ -1340,7 +1340,11 @@ static PagedPlan tree_plan(const lp_kv_cache* c, int heads, int batch, int token
         return p;
     }
     p = PagedPlan{p.max_q, p.max_seq, 16, 16, 0, (units + kFewParts - 1) / kFewParts, tiles, INT32_MAX, 1, 0};
-    if (units > 1) p.shares = (int)std::min<int64_t>(std::max<int64_t>(512, blocks), blocks * units);
+    // 512 shares, two workgroups a CU; one a CU, half the parts to join, where either has only a unit
+    // or a few (heads 32 on 4 of 128: 26 tokens over 1,500 16-bit rows 16.6 us against 19, 40 18.0 against
+    // 20.6, 8 over 4,000 15.8 against 19.1, but 64 over 3,000 27.8 against 25.5; heads of 64: no gain)
+    const int shares = c->head_dim == 128 && blocks * units <= kTreeUnitsOne ? 256 : 512;
+    if (units > 1) p.shares = (int)std::min<int64_t>(std::max<int64_t>(shares, blocks), blocks * units);
     if (p.shares) p.bytes = with_counters((uint64_t)p.shares * p.rows * (c->head_dim * 4 + 8), (int)blocks);
     return p;
 }
