@@ -358,8 +358,8 @@ int lp_attn_tree(lp_ctx* ctx, const lp_kv_cache* cache, uint64_t q, int q_stride
  * path (i32 [batch, max_depth + 1]): the nodes that stay, from node 0 on, then -1;
  * kept[b] their number; next[b] the token behind them.  A row with a NaN, with +inf or with
  * nothing but -inf ends the walk with next[b] = -1, and a sequence without tokens has
- * kept 0 and next -1.  Exponentials are good to 2^-41 and sums are in 64 bits.  vocab
- * at most 2^19.
+ * kept 0 and next -1.  Exponentials are good to 2^-40 and sums are in 64 bits; a token whose
+ * logit / T is 660 or more below the largest is never drawn.  vocab at most 2^19.
  * workspace: lp_verify_tree_ws_bytes bytes (with_probs: whether probs is given),
  * 256-byte aligned; two calls that overlap, replays of graphs among them, need one
  * each.  Sampled drafts of which several are turned down in a sequence go on there with one
@@ -373,7 +373,7 @@ int lp_verify_tree(lp_ctx* ctx, uint64_t logits, int stride, int vocab, uint64_t
 /* The rows of the tokens that stay, one behind the other: row p0 + i of sequence b
  * becomes what row p0 + path[b][i] was, i < kept[b] (at most max_depth + 1 and the
  * sequence's tokens), in the keys and values of `layers` caches (a host array) that share
- * their table and shapes.  path must rise; an entry that is no node of the sequence, or
+ * their table and shapes, each with pools of its own.  path must rise; an entry that is no node of the sequence, or
  * a row whose page is not there, moves nothing.  lens_out (device i32 [batch], not
  * seq_lens, or 0): the lengths then, p0 + kept[b]: the next step's new tokens come on top
  * of them. */

@@ -514,14 +514,14 @@ __device__ __forceinline__ int sequence_of_row(const VerifyArgs& a, int t) {
 extern "C" __global__ void __launch_bounds__(256, 4) lp_verify_rows(const VerifyArgs a) {
     __shared__ Room room;
     const int t = (int)blockIdx.x / a.parts, part = (int)blockIdx.x - t * a.parts, wave = wave_id();
-    if (blockIdx.x == 0 && wave == 3)  // sequences without a token
-        for (int b = lane_id(); b < a.batch; b += 64) {
-            if (seq_of(a, b).n > 0) continue;
-            for (int i = 0; i <= a.max_depth; ++i) gptr_w<int>(a.path)[(uint64_t)(uint32_t)b * (uint32_t)(a.max_depth + 1) + (uint32_t)i] = -1;
-            gptr_w<int>(a.kept)[b] = 0, gptr_w<int>(a.next)[b] = -1;
-            if (a.probs) gptr_w<VerifyState>(a.state)[b].pending = 0;
-        }
     const int b = sequence_of_row(a, t);
+    if (blockIdx.x == 0 && wave == 3)  // sequences without a token, or where no row has a sequence all
+        for (int i = lane_id(); i < a.batch; i += 64) {
+            if (b < a.batch && seq_of(a, i).n > 0) continue;
+            for (int j = 0; j <= a.max_depth; ++j) gptr_w<int>(a.path)[(uint64_t)(uint32_t)i * (uint32_t)(a.max_depth + 1) + (uint32_t)j] = -1;
+            gptr_w<int>(a.kept)[i] = 0, gptr_w<int>(a.next)[i] = -1;
+            if (a.probs) gptr_w<VerifyState>(a.state)[i].pending = 0;
+        }
     if (b >= a.batch) return;  // whole workgroups, here and below
     const Seq s = seq_of(a, b);
     if (t < s.t0 || t - s.t0 >= s.n) return;

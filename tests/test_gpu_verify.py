@@ -2,7 +2,7 @@
 whole step with drafted tokens as a program runs it.
 
 Paths and tokens are whole numbers and have to be equal.  Both sides' sums are 64-bit, the
-device's exponentials good to 2^-41: a border between two tokens is off by 1e-12 of the whole
+device's exponentials good to 2^-40: a border between two tokens is off by 1e-12 of the whole
 at most, and of 2^24 numbers u the chance that one lies that near any of 2^19 borders is below
 1e-6 a draw."""
 import numpy as np
@@ -314,6 +314,21 @@ def test_starts_that_fall_change_nothing(cuda, K):
         c.m.free()
         c = Case(rng, [n, n, n], vocab, 3)  # and the calls behind it are as ever
         _check(cuda, K, c)
+
+
+def test_starts_that_fall_with_sampled_drafts(cuda, K):
+    """No row has a sequence then, and none is left a walk to go on with, whatever the
+    workspace held before."""
+    rng = np.random.default_rng(14)
+    c = Case(rng, [4, 4, 4], 200, 3, True)
+    c.starts[2] = c.starts[1] - 2
+    c.device(cuda, K)
+    cuda.htod_async(c.ws, np.full(c.ws.nbytes, 0x5a, np.uint8))
+    c.run(K)
+    path, kept, after = c.got(cuda)
+    assert (path == -1).all() and (kept == 0).all() and (after == -1).all()
+    c.m.free()
+    _check(cuda, K, Case(rng, [4, 4, 4], 200, 3, True))  # and the calls behind it are as ever
 
 
 @pytest.mark.parametrize("sampled", [False, True])
