@@ -1010,6 +1010,7 @@ __device__ __forceinline__ void few_part(const AttnPagedArgs& a, uint8_t* lds, c
 // workgroup finds its own from the lengths.
 struct Share {
     int b, g, tile, part, parts, per;  // b < 0: none
+    int slot;                          // its number, a block's parts one behind the other
     SeqView sv;
 };
 template <int UNIT, int ROWS, bool TREE>
@@ -1017,18 +1018,20 @@ __device__ __forceinline__ Share share_of(const AttnPagedArgs& a, int* many) {
     const int lane = lane_id(), kv = a.c.kv_heads;
     int b, g, part = 0, parts = 1, per = INT32_MAX / UNIT, tile = 0;
     SeqView sv{0, 0, 0, 0};
-    const Share none{-1, 0, 0, 0, 1, 0, sv};
-    if (a.shares) {
+    const Share none{-1, 0, 0, 0, 1, 0, 0, sv};
+    constexpr bool SORT = ROWS == kManyRows;
+    int at = (int)blockIdx.x, slot = at;
+    if (a.shares || SORT) {
         // units in a lane each (64 sequences), or in LDS
         const bool lanes = a.batch <= 64;
-        int mine = 0, total = 0;
+        int mine = 0, total = 0, even = 0;
         auto tiles_of = [&](const SeqView& s) { return s.n > 0 ? (s.n * a.group + ROWS - 1) / ROWS : 0; };
         int tiles = 1;
         if (lanes) {
             if (lane < a.batch) sv = seq_view(a, lane);
             mine = few_units(sv, UNIT);
             if constexpr (TREE) tiles = tiles_of(sv);
-            total = __builtin_amdgcn_readlane(wave_incl_scan(TREE ? mine * tiles : mine), 63);
+            if (a.shares) total = __builtin_amdgcn_readlane(wave_incl_scan(TREE ? mine * tiles : mine), 63);
         } else {
             for (int i = threadIdx.x; i < (a.batch + 63 & ~63); i += 256) {
                 many[i] = i < a.batch ? few_units(seq_view(a, i), UNIT) : 0;
@@ -1039,31 +1042,55 @@ __device__ __forceinline__ Share share_of(const AttnPagedArgs& a, int* many) {
                 total += __builtin_amdgcn_readlane(wave_incl_scan(TREE ? many[i + lane] * many[kFewBatch + i + lane] : many[i + lane]), 63);
         }
         auto parts_of = [&](int u) { return (u + per - 1) / per; };
-        per = max((total * kv + a.shares - 1) / a.shares, a.min_units);
-        for (;; per += ROWS == kManyRows ? (per + 63) / 64 : (per + 7) / 8) {
+        if (a.shares) per = max((total * kv + a.shares - 1) / a.shares, a.min_units);
+        for (; a.shares; per += SORT ? (per + 63) / 64 : (per + 7) / 8) {
             int n = 0;
             for (int i = 0; i < a.batch; i += 64)
                 n += __builtin_amdgcn_readlane(wave_incl_scan(parts_of(lanes ? mine : many[i + lane]) * (!TREE ? 1 : lanes ? tiles : many[kFewBatch + i + lane])), 63);
             if (n * kv <= a.shares) break;  // one part a pair always fits
         }
-        // the sequence whose parts hold the workgroup's number
-        int before = 0, at = (int)blockIdx.x;
-        for (b = 0;; b += 64) {
+        // the sequence whose parts hold the workgroup's number, SORT: the largest parts first, and
+        // where all are on the card at once, the second one of a CU, number 256 + i, from the smallest up
+        int before = 0;
+        if constexpr (SORT) {
+            const int slots = a.shares ? a.shares : a.batch * kv * a.tiles;
+            if (at >= 256 && slots <= 512) at = slots - 1 - (at - 256);
+            slot = at;
+        }
+        if (SORT && lanes) {
+            int n = mine > 0, size = mine;
+            if (a.shares) n = parts_of(mine), size = (mine + max(n, 1) - 1) / max(n, 1);
+            for (int j = 0; j < a.batch; ++j) {
+                const int other = __builtin_amdgcn_readlane(size, j);
+                before += other > size || (other == size && j < lane) ? __builtin_amdgcn_readlane(n * tiles, j) : 0;
+            }
+            before *= kv;
+            const uint64_t hit = __ballot(at >= before && at < before + kv * n * tiles);
+            if (!hit) return none;
+            b = __builtin_ctzll(hit), at -= __builtin_amdgcn_readlane(before, b);
+            parts = __builtin_amdgcn_readlane(n, b), tiles = __builtin_amdgcn_readlane(tiles, b), even = __builtin_amdgcn_readlane(mine, b);
+        } else for (b = 0;; b += 64) {
             if (b >= a.batch) return none;
             const int ti = !TREE ? 1 : lanes ? tiles : many[kFewBatch + b + lane];
             const int n = parts_of(lanes ? mine : many[b + lane]), incl = before + kv * wave_incl_scan(n * ti);
             const int i = __popcll(__ballot(incl <= at));
             if (i < 64) {
                 parts = __builtin_amdgcn_readlane(n, i);
-                if constexpr (TREE) tiles = __builtin_amdgcn_readlane(ti, i);
+                if constexpr (TREE) tiles = __builtin_amdgcn_readlane(ti, i), even = __builtin_amdgcn_readlane(lanes ? mine : many[b + lane], i);
                 at -= __builtin_amdgcn_readlane(incl, i) - kv * parts * (TREE ? tiles : 1);
                 b += i;
                 break;
             }
             before = __builtin_amdgcn_readlane(incl, 63);
         }
-        g = at / parts, part = at - g * parts;
-        if constexpr (TREE) tile = g % tiles, g /= tiles;
+        if constexpr (TREE) per = parts == 1 ? even : (even + parts - 1) / parts;  // (as many parts, of one size)
+        if constexpr (SORT) {  // a KV head's workgroups to few XCDs, to which consecutive ones go in turn
+            g = at % kv, tile = at / kv, part = tile % parts, tile /= parts;
+            slot += (g * tiles + tile) * parts + part - at;
+        } else {
+            g = at / parts, part = at - g * parts;
+            if constexpr (TREE) tile = g % tiles, g /= tiles;
+        }
         if (lanes) {
             sv = SeqView{__builtin_amdgcn_readlane(sv.t0, b), __builtin_amdgcn_readlane(sv.n, b),
                          __builtin_amdgcn_readlane(sv.len, b), __builtin_amdgcn_readlane(sv.p0, b)};
@@ -1078,7 +1105,7 @@ __device__ __forceinline__ Share share_of(const AttnPagedArgs& a, int* many) {
         if (sv.n <= 0) return none;
         if (TREE && tile * ROWS >= sv.n * a.group) return none;
     }
-    return Share{b, g, tile, part, parts, per, sv};
+    return Share{b, g, tile, part, parts, per, slot, sv};
 }
 
 template <int D, bool Q4, int NT, bool TREE>
@@ -1188,24 +1215,25 @@ __device__ __forceinline__ void many_body(const AttnPagedArgs& a) {
     int bg = (id + id / pairs + split) % pairs, tile = a.tiles - 1 - id / pairs;
     int b = bg / a.c.kv_heads, g = bg - b * a.c.kv_heads;
     SeqView sv = seq_view(a, b);
-    // TREE: a pair's blocks all walk the same rows of the context, so that where there are
-    // parts at all they are shared out by the lengths in memory, as for few query rows (16
-    // sequences of up to 32 tokens, 32 heads on 4 of 128, behind up to 6,000 4-bit rows, 60 % of
-    // that on average: 81 us, 87 with spans of the bounds; where there is a block for each of
-    // 512 workgroups the order above stays, 150 us against 158 of four sequences).
+    // TREE: a pair's blocks all walk the same rows of the context, so that their order and,
+    // where there are several, their parts go by the lengths in memory: 32 heads on 4 of 128,
+    // 16 sequences of up to 32 tokens behind up to 6,000 4-bit rows 80 us, 87 with spans of the
+    // bound; 64 on 4, 4 of up to 256 behind up to 3,000 16-bit ones 135 us and 8 of 250 behind
+    // 6,000 352, in the order above 149 and 436.
     int nth = 0, parts = 1, per = INT32_MAX / CR;
-    if (TREE && a.shares) {
+    if (TREE && (a.shares || a.batch <= 64)) {
         const Share t = share_of<CR, kManyRows, true>(a, reinterpret_cast<int*>(lds));
         if (t.b < 0) return;
-        sv = t.sv, b = t.b, g = t.g, tile = t.tile, nth = t.part, parts = t.parts, per = t.per, split = (int)blockIdx.x;
-        if (nth == 0 && tid == 0)
-            gptr_w<uint64_t>(tree_blocks<D>(a))[(b * a.c.kv_heads + g) * a.tiles + tile] = (uint64_t)(uint32_t)parts << 32 | blockIdx.x;
+        sv = t.sv, b = t.b, g = t.g, tile = t.tile, nth = t.part, parts = t.parts, per = t.per, split = t.slot;
+        if (a.shares && nth == 0 && tid == 0)
+            gptr_w<uint64_t>(tree_blocks<D>(a))[(b * a.c.kv_heads + g) * a.tiles + tile] = (uint64_t)(uint32_t)parts << 32 | (uint32_t)split;
     }
     if constexpr (TREE) {  // (scalars, that nothing spills)
         sv.t0 = __builtin_amdgcn_readfirstlane(sv.t0), sv.n = __builtin_amdgcn_readfirstlane(sv.n);
         sv.len = __builtin_amdgcn_readfirstlane(sv.len), sv.p0 = __builtin_amdgcn_readfirstlane(sv.p0);
         b = __builtin_amdgcn_readfirstlane(b), g = __builtin_amdgcn_readfirstlane(g), tile = __builtin_amdgcn_readfirstlane(tile);
         nth = __builtin_amdgcn_readfirstlane(nth), parts = __builtin_amdgcn_readfirstlane(parts), per = __builtin_amdgcn_readfirstlane(per);
+        split = __builtin_amdgcn_readfirstlane(split);
     }
     const int nrows = sv.n * a.group, row0 = tile * kManyRows;
     if (row0 >= nrows) return;  // whole workgroups, here and below

@@ -1315,13 +1315,16 @@ static PagedPlan paged_plan(const lp_kv_cache* c, int heads, int batch, int toke
 // of them that have parts of their own, while blocks times units of the longest context are
 // few: a block's chain of round trips is shorter, and its parts are joined where they end.
 // Else as paged_plan, but that where the rows of the context are split, 512 workgroups, two a CU,
-// share out what they turn out to be (at 64 rows a unit).  (Heads 32 on 4 of 128, sequences x tokens over rows: 1 x 26 over 1,500 17.4
-// us against 20.8, 1 x 60 22 against 30, 4 x 60 25.8 against 33.3 and over 3,000 39.2 against 40.8,
-// 8 x 32 over 3,000 50 against 42; with 4 bits 16.2 against 21.2, 19.8 against 32.5, 24.5 against
-// 34.4, 37.9 against 41.5 and 46.8 against 42.2.  16-bit contexts that are many as well
-// are read too often: 16 x 8 over 3,000 43 against 32.5.  17 to 32 rows: 64 x 4 over 4,000 with 16
-// bits 91 against 83, 32 x 4 over 3,000 37 against 41; with 4 bits 55 against 63.)
-constexpr int kTreeUnits = 5760, kTreeUnits32 = 8192, kTreePairUnits = 1024, kTreeUnitsOne = 1280;
+// share out what they turn out to be (at 64 rows a unit).  Heads 32 on 4 of 128, sequences x
+// tokens over rows, few against many: 16 bits 1 x 60 over 3,000 25 us against 32, 4 x 60 over 1,500 25 against
+// 33 and over 3,000 40 against 39, 8 x 32 over 1,500 28 against 33, 1 x 250 over 1,500 37 against 40; where the
+// contexts are many as well they are read too often: 8 x 12 over 3,000 28 against 30, 8 x 16 43 against 33, 16 x 16
+// over 1,400 37 against 33.  4 bits: 4 x 60 over 3,000 37 against 43, 8 x 32 over 3,000 37 against 40 and
+// over 4,000 48 against 44, 16 x 16 over 3,000 40 and 40.  Heads of 64 have half the work: 16 x 32
+// over 1,500 18 against 26.  17 to 32 rows: 64 x 4 over 4,000 with 16 bits 91 against 83,
+// 32 x 4 over 3,000 37 against 41; with 4 bits 55 against 63.
+constexpr int kTreeUnitsQ4 = 6144, kTreeUnits = 7168, kTreeUnitsWide = 5760, kTreePairUnits = 448, kTreePairUnitsWide = 1024;
+constexpr int kTreeUnits32 = 8192, kTreeUnitsOne = 1280;
 static PagedPlan tree_plan(const lp_kv_cache* c, int heads, int batch, int tokens, int max_q, int max_seq) {
     PagedPlan p = paged_plan(c, heads, batch, tokens, max_q, max_seq);
     if (p.few) p.tiles = 1;
@@ -1331,7 +1334,9 @@ static PagedPlan tree_plan(const lp_kv_cache* c, int heads, int batch, int token
     const int64_t pairs = (int64_t)batch * c->kv_heads, blocks = pairs * tiles;
     const bool fit = blocks <= kPagedPairs && batch <= kFewBatch;
     if (p.few && (!fit || (!q4 && blocks * units > kTreeUnits32))) return p;
-    if (!p.few && (!fit || blocks * units > kTreeUnits || (!q4 && pairs * units > kTreePairUnits))) {
+    const int64_t work = blocks * units * c->head_dim / 128, reads = q4 ? 0 : pairs * units * c->head_dim / 128;
+    const int most = q4 ? kTreeUnitsQ4 : reads <= kTreePairUnits ? kTreeUnits : kTreeUnitsWide;
+    if (!p.few && (!fit || work > most || reads > kTreePairUnitsWide)) {
         if (p.splits == 1) return p;
         const int chunks = (p.max_seq + 63) / 64;
         p.shares = (int)std::min<int64_t>(512, pairs * p.tiles * chunks);

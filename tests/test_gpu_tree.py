@@ -366,6 +366,19 @@ def test_attention_of_many_rows_shared_out(cuda, K, fmt, dim, n):
     _check_attn(K, Trees(cuda, trees, past, 16, 1, dim, 16, fmt, seed=n, cols=bound // 16), bound)
 
 
+@pytest.mark.parametrize("fmt", [lp.KV_F16, lp.KV_Q4])
+@pytest.mark.parametrize("n,kv,group", [(40, 8, 16), (64, 9, 4), (66, 8, 4), (5, 5, 16)])
+def test_attention_a_workgroup_a_block(cuda, K, fmt, n, kv, group):
+    """Blocks of 128 query rows that no other workgroup helps with: by their lengths, in one
+    round and in several, and of more sequences than lanes."""
+    rng = np.random.default_rng(n)
+    nodes = [9, 0, 1] + [int(k) for k in rng.integers(0, 10, n - 3)]
+    if n == 5:
+        nodes = [150, 0, 90, 150, 17]
+    past = [290, 40, 2] + [int(p) for p in rng.integers(0, 290, n - 3)]
+    _check_attn(K, Trees(cuda, [random_tree(rng, k) if k else [] for k in nodes], past, kv * group, kv, 64, 16, fmt, seed=n))
+
+
 @pytest.mark.parametrize("fmt,dim", FORMS)
 @pytest.mark.parametrize("n,heads", [(3, 8), (9, 2), (40, 8), (130, 8)])
 def test_attention_long_contexts(cuda, K, fmt, dim, n, heads):
