@@ -511,6 +511,10 @@ __device__ __forceinline__ int sequence_of_row(const VerifyArgs& a, int t) {
 
 // Every row at once: workgroup (row, part).  A row's last workgroup joins its records, a
 // sequence's last row walks down its tree.
+//
+// 26 rows of 151,936 logits 14.5 us: the launch, two blocks a wave, the join, the draw and the
+// walk, one behind the other.  116 rows 31 us, 600 rows 119: 3.1 TB/s; loads alone took 93, and the
+// exponentials' 18 instructions a logit are 51 more, half of which the four waves of a SIMD hide.
 extern "C" __global__ void __launch_bounds__(256, 4) lp_verify_rows(const VerifyArgs a) {
     __shared__ Room room;
     const int t = (int)blockIdx.x / a.parts, part = (int)blockIdx.x - t * a.parts, wave = wave_id();
@@ -542,7 +546,8 @@ extern "C" __global__ void __launch_bounds__(256, 4) lp_verify_rows(const Verify
 
 // What is left of a row, for the sequences whose walk stands there: workgroup (sequence,
 // part) sums a wave's blocks, the last one goes on with the walk, and where that needs
-// another row's or more taken from this one, sums that alone.
+// another row's or more taken from this one, sums that alone.  32 chains of 6 nodes, 151,936
+// logits: 12 us for 39 MB, mostly one chain: a wave's blocks, the arrival, the walk and its draw.
 extern "C" __global__ void __launch_bounds__(64 * kVerifyWaves) lp_verify_left(const VerifyArgs a) {
     __shared__ Room room;
     __shared__ VerifyState now;
