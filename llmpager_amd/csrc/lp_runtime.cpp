@@ -1561,13 +1561,17 @@ int lp_verify_tree(lp_ctx* c, uint64_t logits, int stride, int vocab, uint64_t d
     const VerifyPlan p = verify_plan(vocab, batch, tokens, max_q, max_depth, probs != 0);
     if (int r = check_workspace("verify_tree", p.bytes, workspace, ws_bytes)) return r;
     if (int r = check_ctx(c)) return r;
-    if (!p.bytes) return LP_OK;
+    if (!batch) return LP_OK;
     VerifyArgs a{};
     a.logits = logits, a.drafts = drafts, a.parents = parents, a.q_starts = q_starts;
     a.temps = temperatures, a.probs = probs, a.uniforms = uniforms, a.path = path, a.kept = kept, a.next = next;
     a.part = workspace, a.stats = workspace + p.stats, a.left = workspace + p.left, a.state = workspace + p.state;
     a.stride = stride, a.probs_stride = probs_stride, a.vocab = vocab, a.batch = batch, a.tokens = tokens;
     a.max_q = max_q, a.max_depth = max_depth;
+    if (!tokens || !max_q) {  // no sequence has a token: its workgroup says so and ends there
+        a.parts = 1;
+        return launch(c, kVerifyPath, dim3((unsigned)batch), dim3(64 * kPathWaves), 0, s, a);
+    }
     a.blocks = p.blocks, a.parts = p.parts, a.per_part = p.per_part, a.row_counters = p.row_counters;
     if (int r = join_counters(c, s, workspace + counters_at(p.records), p.counters, &a.sync)) return r;
     if (p.path) return launch(c, kVerifyPath, dim3((unsigned)(batch * p.parts)), dim3(64 * kPathWaves), 0, s, a);
