@@ -26,8 +26,11 @@
 
 namespace {
 
-constexpr double kNone = -700.0;     // e^ of it, of anything below and of -infinity,
-constexpr double kNothing = 1e-290;  // counts as nothing
+// A token 660 or more below the row's largest can't be drawn: its e^, made from no lower exponent
+// than kNone, is e^-660 at most (kNothing is 1e-11 of it above that, more than its error).  Such a
+// weight is 0 wherever one is looked for: a border of 0 lies below all of them, and a block's or
+// four tokens' sum of them says nothing of what any one of them is.  (In the sums they may stay.)
+constexpr double kNone = -700.0, kNothing = 2.3208225942028e-287;
 
 // e^((x - m) / T): d = n ln 2 + r, |r| <= ln 2 / 2, and 2^n by the exponent's bits.  The
 // polynomial has the smallest largest relative error of those of degree 8 that are 1 at
@@ -126,8 +129,8 @@ __device__ __forceinline__ void end_block(float (&v)[kPer], int block, int n) {
 }
 
 // The place in a block where the sums of the weights, `before` what went before them, pass
-// thr; at rounding's edge the last that adds to them, -1 where none does.  weights(j, e):
-// the lane's four of part j.
+// thr; at rounding's edge the last that is not 0, -1 where none is.  weights(j, e): the
+// lane's four of part j, 0 for what can't be drawn.
 template <typename F>
 __device__ __forceinline__ int find_in_block(const F& weights, double before, double thr) {
     constexpr int N = kPer / 4;
@@ -143,7 +146,7 @@ __device__ __forceinline__ int find_in_block(const F& weights, double before, do
     double from = 0.0;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-        const uint64_t some = __ballot(t[j] > kNothing), hit = __ballot(before + incl[j] > thr && t[j] > kNothing);
+        const uint64_t some = __ballot(t[j] > 0.0), hit = __ballot(before + incl[j] > thr && t[j] > 0.0);
         if (some) in = j, lane = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some), from = before + incl[j] - t[j];
         if (hit) break;
         before += lane_f64(incl[j], 63);
@@ -155,7 +158,7 @@ __device__ __forceinline__ int find_in_block(const F& weights, double before, do
     for (int k = 0; k < 4; ++k) {
         if (u >= 0 && from > thr) continue;  // found
         from += e[k];
-        if (e[k] > kNothing) u = k;
+        if (e[k] > 0.0) u = k;
     }
     return 256 * in + 4 * lane + __builtin_amdgcn_readlane(u, lane);
 }
@@ -187,7 +190,7 @@ __device__ __forceinline__ int find_block(const double* w, int blocks, double sh
     before = 0.0;
     for (int i0 = 0; i0 < blocks; i0 += 64) {
         const double x = i0 + lane_id() < blocks ? w[i0 + lane_id()] : 0.0, incl = done + scan_f64(x);
-        const uint64_t some = __ballot(x > kNothing), hit = __ballot(incl > thr && x > kNothing);
+        const uint64_t some = __ballot(x > 0.0), hit = __ballot(incl > thr && x > 0.0);
         done = lane_f64(incl, 63);
         if (!some) continue;
         const int l = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some);
@@ -297,7 +300,10 @@ __device__ __forceinline__ Row join_row(const VerifyArgs& a, const Seq& s, int s
     double sum = 0.0;
     for (int blk = lane_id(); blk < a.blocks; blk += 64) {
         double w = room.w[blk];
-        if (s.temp > 0.0f) w *= exp_over(room.m[blk], r.m, s.inv_t);
+        if (s.temp > 0.0f) {  // 0 where not even the largest can be drawn, but NaN stays
+            const double e = exp_over(room.m[blk], r.m, s.inv_t);
+            w = e > kNothing || w != w ? w * e : 0.0;
+        }
         room.w[blk] = w;
         sum += w;
     }
@@ -319,19 +325,22 @@ __device__ __forceinline__ int draw(const VerifyArgs& a, const Seq& s, int t, co
         float y[4];
         part_of(x, j, y);
         exp_over<4>(y, r.m, s.inv_t, e);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) e[u] = e[u] > kNothing ? e[u] : 0.0;
     };
     const int at = find_in_block(weights, before, thr);
     return at < 0 ? -1 : blk * kVerifyBlock + at;
 }
 
-// What is left of a row: max(p - taken q, 0), four at a time.
+// What is left of a row: max(p - taken q, 0), four at a time.  What can't be drawn comes as 0,
+// since kNothing is taken off, which is less than the last bit of any but the smallest.
 struct Left {
     float m;
     double inv_s, inv_t, taken;
     __device__ __forceinline__ void operator()(const float (&x)[4], const float (&q)[4], double (&e)[4]) const {
         exp_over<4>(x, m, inv_t, e);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) e[u] = fmax(__builtin_fma(-taken, (double)q[u], e[u] * inv_s), 0.0);
+        for (int u = 0; u < 4; ++u) e[u] = fmax(__builtin_fma(-taken, (double)q[u], __builtin_fma(e[u], inv_s, -kNothing * inv_s)), 0.0);
     }
 };
 __device__ __forceinline__ void load_both(const VerifyArgs& a, int t, int blk, float (&x)[kPer], float (&q)[kPer]) {
@@ -401,8 +410,8 @@ struct Nodes {
         if (a.probs && s.temp > 0.0f) {
             const float x = gptr<float>(logits_row(a, s.t0 + p))[token], q = gptr<float>(probs_row(a, s.t0 + p))[token];
             const float u = gptr<float>(a.uniforms)[s.t0 + i];
-            const double pr = exp_over(x, st.m, s.inv_t) / st.s;
-            fits = pr > kNothing && (double)u * (double)q < pr;
+            const double e = exp_over(x, st.m, s.inv_t);
+            fits = e > kNothing && (double)u * (double)q < e / st.s;
         } else {
             fits = token == st.z;
         }
@@ -413,7 +422,7 @@ struct Nodes {
 // left of a row has to be summed (false; then, with the blocks' sums in `room`, the walk goes on).
 __device__ __forceinline__ bool walk(const VerifyArgs& a, const Seq& s, int b, VerifyState& st, Room& room) {
     const bool sampled = a.probs && s.temp > 0.0f;
-    if (!(st.left > kNothing)) st.taken = 0.0, st.left = 1.0;  // nothing is left: p again
+    if (!(st.left > 0.0)) st.taken = 0.0, st.left = 1.0;  // nothing is left: p again
     Nodes N;
     for (;;) {
         N.load(a, s, st.cur & ~63);
@@ -451,8 +460,8 @@ __device__ __forceinline__ bool walk(const VerifyArgs& a, const Seq& s, int b, V
                 if (!kids) continue;
                 const int k = __builtin_ctzll(kids), d = __builtin_amdgcn_readlane(N.token, k), t = s.t0 + st.cur;
                 const double q = (double)gptr<float>(probs_row(a, t))[d], u = (double)gptr<float>(a.uniforms)[s.t0 + i0 + k];
-                const double p = __builtin_fma(-st.taken, q, exp_over(gptr<float>(logits_row(a, t))[d], m, s.inv_t) / S);
-                if (p > kNothing && u * q * st.left < p) {
+                const double e = exp_over(gptr<float>(logits_row(a, t))[d], m, s.inv_t), p = __builtin_fma(-st.taken, q, e / S);
+                if (e > kNothing && p > 0.0 && u * q * st.left < p) {
                     to = i0 + k;
                     continue;
                 }
