@@ -1585,7 +1585,7 @@ int lp_kv_keep(lp_ctx* c, const lp_kv_cache* caches, int layers, uint64_t path, 
                uint64_t q_starts, uint64_t seq_lens, uint64_t lens_out, int batch, lp_stream s) {
     if (layers < 0 || max_depth < 0) return fail(LP_E_INVALID, "kv_keep: negative layers or max_depth");
     KvKeepArgs a{};
-    for (int l = 0; l < std::max(layers, 1); ++l) {
+    for (int l = 0; l < layers; ++l) {
         const lp_kv_cache* k = caches ? caches + l : nullptr;
         if (int r = check_paged("kv_keep", k, &a.c)) return r;
         if (k->table != caches->table || k->pages != caches->pages || k->page_rows != caches->page_rows ||
@@ -1598,19 +1598,21 @@ int lp_kv_keep(lp_ctx* c, const lp_kv_cache* caches, int layers, uint64_t path, 
         return fail(LP_E_UNSUPPORTED, "kv_keep: max_depth must be below " + std::to_string(kTreeMaxNodes));
     if (!path || !kept || path % 4 || kept % 4 || lens_out % 4) return fail(LP_E_INVALID, "kv_keep: null or misaligned pointer");
     if (lens_out && lens_out == seq_lens) return fail(LP_E_INVALID, "kv_keep: lens_out must not be seq_lens");
-    const bool q4 = caches->format == LP_KV_Q4;
-    const int D = caches->head_dim, units = q4 ? D / 64 + D / 8 : D / 8;  // of a row of one head
-    const int64_t chunks = (2 * (int64_t)caches->kv_heads * units + keep_units(q4) - 1) / keep_units(q4);
+    // without layers a wave a sequence, whose cache has no heads and no pages
+    const bool q4 = layers && caches->format == LP_KV_Q4;
+    const int D = layers ? caches->head_dim : 64, units = q4 ? D / 64 + D / 8 : D / 8;  // of a row of one head
+    const int64_t chunks = layers ? (2 * (int64_t)caches->kv_heads * units + keep_units(q4) - 1) / keep_units(q4) : 1;
     if (chunks * std::min(std::max(layers, 1), kKeepLayers) * batch > INT32_MAX / 256)
         return fail(LP_E_UNSUPPORTED, "kv_keep: too many heads for this batch");
     if (int r = check_ctx(c)) return r;
-    if (!batch || !layers) return LP_OK;
+    if (!batch || (!layers && !lens_out)) return LP_OK;
     a.path = path, a.kept = kept, a.q_starts = q_starts, a.seq_lens = seq_lens;
     a.batch = batch, a.max_depth = max_depth, a.chunks = (int)chunks;
-    for (int l0 = 0; l0 < layers; l0 += kKeepLayers) {
-        a.layers = std::min(layers - l0, kKeepLayers);
+    for (int l0 = 0; l0 < std::max(layers, 1); l0 += kKeepLayers) {
+        const int n = std::min(layers - l0, kKeepLayers);
+        a.layers = std::max(n, 1);
         a.lens_out = l0 ? 0 : lens_out;
-        for (int l = 0; l < a.layers; ++l) a.k_pages[l] = caches[l0 + l].k_pages, a.v_pages[l] = caches[l0 + l].v_pages;
+        for (int l = 0; l < n; ++l) a.k_pages[l] = caches[l0 + l].k_pages, a.v_pages[l] = caches[l0 + l].v_pages;
         const int64_t waves = chunks * a.layers * batch;
         const Fn f = (Fn)(kKeepF16D64 + (q4 ? 2 : 0) + (D == 128 ? 1 : 0));
         if (int r = launch(c, f, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, s, a)) return r;
