@@ -375,8 +375,9 @@ int lp_verify_tree(lp_ctx* ctx, uint64_t logits, int stride, int vocab, uint64_t
  * becomes what row p0 + path[b][i] was, i < kept[b] (at most max_depth + 1 and the
  * sequence's tokens), in the keys and values of `layers` caches (a host array) that share
  * their table and shapes, each with pools of its own.  path must rise; an entry that is no node of the sequence, or
- * a row whose page is not there, moves nothing.  lens_out (device i32 [batch], not seq_lens, or 0):
- * the lengths then, p0 + kept[b]: the next step's new tokens come on top of them.  Without layers (caches: may be 0) it writes these alone. */
+ * a row whose page is not there, moves nothing.  lens_out (device i32 [batch], or 0; over
+ * none of the arrays that are read): the lengths then, p0 + kept[b]: the next step's new tokens
+ * come on top of them.  Without layers (caches: may be 0) it writes these alone. */
 int lp_kv_keep(lp_ctx* ctx, const lp_kv_cache* caches, int layers, uint64_t path, int max_depth, uint64_t kept,
                uint64_t q_starts, uint64_t seq_lens, uint64_t lens_out, int batch, lp_stream s);
 

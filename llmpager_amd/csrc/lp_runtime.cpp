@@ -1597,7 +1597,11 @@ int lp_kv_keep(lp_ctx* c, const lp_kv_cache* caches, int layers, uint64_t path, 
     if (max_depth >= kTreeMaxNodes)
         return fail(LP_E_UNSUPPORTED, "kv_keep: max_depth must be below " + std::to_string(kTreeMaxNodes));
     if (!path || !kept || path % 4 || kept % 4 || lens_out % 4) return fail(LP_E_INVALID, "kv_keep: null or misaligned pointer");
-    if (lens_out && lens_out == seq_lens) return fail(LP_E_INVALID, "kv_keep: lens_out must not be seq_lens");
+    // one wave writes a length while others read what it is made of
+    const uint64_t lens = 4 * (uint64_t)std::max(batch, 1);
+    auto over = [&](uint64_t p, uint64_t n) { return lens_out < p + n && p < lens_out + lens; };
+    if (lens_out && (over(seq_lens, lens) || over(kept, lens) || over(q_starts, lens + 4) || over(path, lens * (max_depth + 1))))
+        return fail(LP_E_INVALID, "kv_keep: lens_out must not overlap seq_lens, kept, q_starts or path");
     // without layers a wave a sequence, whose cache has no heads and no pages
     const bool q4 = layers && caches->format == LP_KV_Q4;
     const int D = layers ? caches->head_dim : 64, units = q4 ? D / 64 + D / 8 : D / 8;  // of a row of one head
