@@ -449,9 +449,12 @@ class Cuda:
 
     # convenience
     def upload(self, a: np.ndarray, stream: int | None = None) -> int:
+        """A new buffer with a's values.  They are there when this returns, for work on any
+        stream (one of `stream()` does not wait for the null stream) and whatever becomes of a."""
         a = np.ascontiguousarray(a)
         p = self.alloc_device(max(a.nbytes, 1))
         self.htod_async(p, a, stream)
+        self.sync_stream(stream)
         return p
 
     def download(self, p: int, shape, dtype, stream: int | None = None) -> np.ndarray:
