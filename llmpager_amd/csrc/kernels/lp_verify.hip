@@ -27,10 +27,11 @@
 namespace {
 
 // A token 660 or more below the row's largest can't be drawn: its e^, made from no lower exponent
-// than kNone, is e^-660 at most (kNothing is 1e-11 of it above that, more than its error).  Such a
-// weight is 0 wherever one is looked for: a border of 0 lies below all of them, and a block's or
-// four tokens' sum of them says nothing of what any one of them is.  (In the sums they may stay.)
+// than kNone, is e^-660 at most (kNothing is 1e-11 of it above that, more than its error).  A sum
+// of four or of a block's 1024 holds a larger weight than `least` if it is above that many times it,
+// and some to spare at each step, so that what is found in the sums is found below them too.
 constexpr double kNone = -700.0, kNothing = 2.3208225942028e-287;
+constexpr double kOfFour = 4.1, kOfBlock = 1100.0;
 
 // e^((x - m) / T): d = n ln 2 + r, |r| <= ln 2 / 2, and 2^n by the exponent's bits.  The
 // polynomial has the smallest largest relative error of those of degree 8 that are 1 at
@@ -129,10 +130,10 @@ __device__ __forceinline__ void end_block(float (&v)[kPer], int block, int n) {
 }
 
 // The place in a block where the sums of the weights, `before` what went before them, pass
-// thr; at rounding's edge the last that is not 0, -1 where none is.  weights(j, e): the
-// lane's four of part j, 0 for what can't be drawn.
+// thr; at rounding's edge the last above `least`, -1 where none is.  weights(j, e): the
+// lane's four of part j.
 template <typename F>
-__device__ __forceinline__ int find_in_block(const F& weights, double before, double thr) {
+__device__ __forceinline__ int find_in_block(const F& weights, double before, double thr, double least) {
     constexpr int N = kPer / 4;
     double t[N], incl[N], e[4];
 #pragma unroll
@@ -146,7 +147,7 @@ __device__ __forceinline__ int find_in_block(const F& weights, double before, do
     double from = 0.0;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-        const uint64_t some = __ballot(t[j] > 0.0), hit = __ballot(before + incl[j] > thr && t[j] > 0.0);
+        const uint64_t some = __ballot(t[j] > kOfFour * least), hit = __ballot(before + incl[j] > thr && t[j] > kOfFour * least);
         if (some) in = j, lane = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some), from = before + incl[j] - t[j];
         if (hit) break;
         before += lane_f64(incl[j], 63);
@@ -158,7 +159,7 @@ __device__ __forceinline__ int find_in_block(const F& weights, double before, do
     for (int k = 0; k < 4; ++k) {
         if (u >= 0 && from > thr) continue;  // found
         from += e[k];
-        if (e[k] > 0.0) u = k;
+        if (e[k] > least) u = k;
     }
     return 256 * in + 4 * lane + __builtin_amdgcn_readlane(u, lane);
 }
@@ -179,9 +180,9 @@ struct Room {
 };
 
 // Which of a row's blocks holds the border: their sums in order, and `share` of the whole.
-// The border and what goes before the block are left in thr and before; -1 where nothing
-// adds to the sums.
-__device__ __forceinline__ int find_block(const double* w, int blocks, double share, double& thr, double& before) {
+// The border and what goes before the block are left in thr and before; -1 where no sum
+// holds a weight above `least`.
+__device__ __forceinline__ int find_block(const double* w, int blocks, double share, double least, double& thr, double& before) {
     double all = 0.0;
     for (int i = lane_id(); i - lane_id() < blocks; i += 64) all += i < blocks ? w[i] : 0.0;
     thr = share * wave_sum_f64(all);
@@ -190,7 +191,7 @@ __device__ __forceinline__ int find_block(const double* w, int blocks, double sh
     before = 0.0;
     for (int i0 = 0; i0 < blocks; i0 += 64) {
         const double x = i0 + lane_id() < blocks ? w[i0 + lane_id()] : 0.0, incl = done + scan_f64(x);
-        const uint64_t some = __ballot(x > 0.0), hit = __ballot(incl > thr && x > 0.0);
+        const uint64_t some = __ballot(x > kOfBlock * least), hit = __ballot(incl > thr && x > kOfBlock * least);
         done = lane_f64(incl, 63);
         if (!some) continue;
         const int l = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some);
@@ -300,10 +301,7 @@ __device__ __forceinline__ Row join_row(const VerifyArgs& a, const Seq& s, int s
     double sum = 0.0;
     for (int blk = lane_id(); blk < a.blocks; blk += 64) {
         double w = room.w[blk];
-        if (s.temp > 0.0f) {  // 0 where not even the largest can be drawn, but NaN stays
-            const double e = exp_over(room.m[blk], r.m, s.inv_t);
-            w = e > kNothing || w != w ? w * e : 0.0;
-        }
+        if (s.temp > 0.0f) w *= exp_over(room.m[blk], r.m, s.inv_t);
         room.w[blk] = w;
         sum += w;
     }
@@ -311,24 +309,50 @@ __device__ __forceinline__ Row join_row(const VerifyArgs& a, const Seq& s, int s
     return r;
 }
 
+// The first token of row t that can be drawn.  (A border of 0 lies below all sums, also those of
+// tokens that can't be; the numbers above 0 are 2^-149 at least, beside which a row's 2^19 such
+// weights are nothing, so that only 0 has to look at each.)
+__device__ __forceinline__ int draw_first(const VerifyArgs& a, const Seq& s, int t, const Row& r, const Room& room) {
+    for (int b0 = 0; b0 < a.blocks; b0 += 64) {
+        const int i = b0 + lane_id();
+        const uint64_t some = __ballot(i < a.blocks && exp_over(room.m[min(i, a.blocks - 1)], r.m, s.inv_t) > kNothing);
+        if (!some) continue;
+        const int blk = b0 + __builtin_ctzll(some);
+        float x[kPer];
+        load_block(x, logits_row(a, t), blk, a.vocab);
+        end_block(x, blk, a.vocab);
+        int id = kBad;
+#pragma unroll 1
+        for (int j = kPer / 4 - 1; j >= 0; --j) {
+            float y[4];
+            double e[4];
+            part_of(x, j, y);
+            exp_over<4>(y, r.m, s.inv_t, e);
+#pragma unroll
+            for (int u = 3; u >= 0; --u) id = e[u] > kNothing ? blk * kVerifyBlock + 256 * j + 4 * lane_id() + u : id;
+        }
+        return wave_least(id);
+    }
+    return -1;
+}
+
 // The token of row t that number u draws, -1: none can be.
 __device__ __forceinline__ int draw(const VerifyArgs& a, const Seq& s, int t, const Row& r, const Room& room, float u) {
     if (r.s != r.s) return -1;
     if (s.temp == 0.0f) return r.first;
     double thr, before;
-    const int blk = find_block(room.w, a.blocks, (double)u, thr, before);
-    if (blk < 0) return -1;
     float x[kPer];
+    if (!(u > 0.0f)) return draw_first(a, s, t, r, room);
+    const int blk = find_block(room.w, a.blocks, (double)u, kNothing, thr, before);
+    if (blk < 0) return -1;
     load_block(x, logits_row(a, t), blk, a.vocab);
     end_block(x, blk, a.vocab);
     auto weights = [&](int j, double (&e)[4]) {
         float y[4];
         part_of(x, j, y);
         exp_over<4>(y, r.m, s.inv_t, e);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) e[u] = e[u] > kNothing ? e[u] : 0.0;
     };
-    const int at = find_in_block(weights, before, thr);
+    const int at = find_in_block(weights, before, thr, kNothing);
     return at < 0 ? -1 : blk * kVerifyBlock + at;
 }
 
@@ -483,7 +507,7 @@ __device__ __forceinline__ bool walk(const VerifyArgs& a, const Seq& s, int b, V
             } else {
                 double thr, before;
                 float x[kPer], q[kPer];
-                const int blk = max(0, find_block(room.w, a.blocks, (double)u, thr, before));
+                const int blk = max(0, find_block(room.w, a.blocks, (double)u, 0.0, thr, before));
                 load_both(a, t, blk, x, q);
                 const Left left{m, 1.0 / S, s.inv_t, st.taken};
                 auto weights = [&](int j, double (&e)[4]) {
@@ -491,7 +515,7 @@ __device__ __forceinline__ bool walk(const VerifyArgs& a, const Seq& s, int b, V
                     part_of(x, j, y), part_of(q, j, z);
                     left(y, z, e);
                 };
-                next = blk * kVerifyBlock + max(0, find_in_block(weights, before, thr));
+                next = blk * kVerifyBlock + max(0, find_in_block(weights, before, thr, 0.0));
             }
         }
         put_end(a, b, st.len, next);

@@ -32,10 +32,11 @@ def test_without_tokens(cuda, K, sampled, batch, max_depth, tokens, max_q, start
     shapes = ((batch, max_depth + 1), (batch,), (batch,))
     out = [m.up(np.full(s, 7, np.int32)) for s in shapes]
     assert K.verify_tree_ws_bytes(50, batch, tokens, max_q, max_depth, sampled) == 0
+    fill = [np.full(s, 7, np.int32) for s in shapes]
     for stream in (None, cuda.stream()):
         if stream is not None:
-            for d, s in zip(out, shapes):
-                cuda.htod_async(d, np.full(s, 7, np.int32), stream)
+            for d, f in zip(out, fill):
+                cuda.htod_async(d, f, stream)
         K.verify_tree(x, 50, 50, i, i, ds, batch, tokens, max_q, max_depth, 0, x if sampled else 0, 50, x, *out, 0, stream, ws_bytes=0)
         path, kept, after = (cuda.download(d, s, np.int32, stream) for d, s in zip(out, shapes))
         assert (path == -1).all() and (kept == 0).all() and (after == -1).all()
@@ -118,7 +119,7 @@ def test_what_is_left_far_below(cuda, K, gap, vocab):
 
 @pytest.mark.parametrize("gap", GAPS)
 def test_draws_of_0_on_large_trees(cuda, K, gap):
-    """The same where the rows of the path alone are read."""
+    """The same, and by the smallest number above 0, where the rows of the path alone are read."""
     sizes, vocab = [200] * 6, 30001
     assert _path_alone(K, sizes, vocab, 5)
     rng = np.random.default_rng(5)
@@ -126,7 +127,8 @@ def test_draws_of_0_on_large_trees(cuda, K, gap):
     c.x[:] = -gap
     c.x[:, 12345] = 0.0
     c.x[::2, 777] = 0.0
-    c.u[:] = rng.choice([0.0, 0.75], c.T)
+    c.u[:] = rng.choice(np.array([0.0, 2.0 ** -149, 0.75], np.float32), c.T)
+    assert (c.u > 0).any() and (c.u[c.u > 0] < 1e-40).any()
     c.drafts[:] = rng.choice([0, 777, 12345], c.T)
     w = _check_cut(cuda, K, c)
     assert (gap < 660) == (w[2] == 0).any()
