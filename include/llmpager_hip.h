@@ -358,7 +358,7 @@ int lp_attn_tree(lp_ctx* ctx, const lp_kv_cache* cache, uint64_t q, int q_stride
  * path (i32 [batch, max_depth + 1]): the nodes that stay, from node 0 on, then -1;
  * kept[b] their number; next[b] the token behind them.  A row with a NaN, with +inf or with
  * nothing but -inf ends the walk with next[b] = -1, and a sequence without tokens has
- * kept 0 and next -1.  Exponentials are good to 2^-40 and sums are in 64 bits; a token whose
+ * kept 0 and next -1 (so have all where q_starts do not rise).  Exponentials are good to 2^-40 and sums are in 64 bits; a token whose
  * logit / T is 660 or more below the largest is as one of -inf: never drawn, never kept,
  * nothing of what is left of p'.  vocab at most 2^19.
  * workspace: lp_verify_tree_ws_bytes bytes (with_probs: whether probs is given),

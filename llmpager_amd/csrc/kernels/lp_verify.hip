@@ -656,7 +656,7 @@ constexpr int kLooks = 64;                                  // about a microseco
 
 extern "C" __global__ void __launch_bounds__(64 * kPathWaves, 4) lp_verify_path(const VerifyArgs a) {
     __shared__ Room room;
-    __shared__ int share;
+    __shared__ int share, fell[kPathWaves];
     const int b = (int)blockIdx.x / a.parts, part = (int)blockIdx.x - b * a.parts, wave = wave_id();
     const Seq s = seq_of(a, b);
     if (s.n <= 0) {
@@ -666,6 +666,15 @@ extern "C" __global__ void __launch_bounds__(64 * kPathWaves, 4) lp_verify_path(
     int* const word = reinterpret_cast<int*>(a.sync) + (uint64_t)(uint32_t)(b * a.row_counters) * kPagedStride;
     int up = -1, token = -1;  // of the first 64 nodes, one a lane
     if (lane_id() < s.n) up = gptr<int>(a.parents)[s.t0 + lane_id()], token = gptr<int>(a.drafts)[s.t0 + lane_id()];
+    // where the starts do not rise no row has a sequence, as in lp_verify_rows: seen by the
+    // other waves while the first one waits for its group (by that one, or by who ends the
+    // root's row, 0.9 to 1.5 us more)
+    if (wave) {
+        bool falls = false;
+        for (int i = 64 * (wave - 1) + lane_id(); i < a.batch; i += 64 * (kPathWaves - 1)) falls |= gptr<int>(a.q_starts)[i + 1] < gptr<int>(a.q_starts)[i];
+        const bool some = __ballot(falls) != 0;
+        if (lane_id() == 0) fell[wave] = some;
+    }
     for (;;) {
         if (threadIdx.x == 0) {
             int c = atomicAdd(word + kTaken, 1);
@@ -694,8 +703,9 @@ extern "C" __global__ void __launch_bounds__(64 * kPathWaves, 4) lp_verify_path(
         const int len = agent_load(word + kLen);
         const Row r = join_row(a, s, b, room);
         const int z = draw(a, s, t, r, room, u);
+        const bool none = __ballot(lane_id() > 0 && lane_id() < kPathWaves && fell[lane_id() % kPathWaves]) != 0;
         int to = -1;
-        if (z >= 0 && len < a.max_depth)
+        if (z >= 0 && len < a.max_depth && !none)
             for (int i0 = cur & ~63; i0 < s.n && to < 0; i0 += 64) {
                 const int i = i0 + lane_id();
                 int p = up, d = token;
@@ -712,8 +722,8 @@ extern "C" __global__ void __launch_bounds__(64 * kPathWaves, 4) lp_verify_path(
             __builtin_amdgcn_s_waitcnt(0);
             atomicExch(word + kTaken, (to < 0 ? kOver : to) << 16);
         }
-        put_node(a, b, len, cur);
-        if (to < 0) put_end(a, b, len + 1, z);
+        if (!none) put_node(a, b, len, cur);
+        if (to < 0) put_end(a, b, none ? 0 : len + 1, none ? -1 : z);
     }
     if (threadIdx.x == 0 && atomicAdd(word + kGone, 1) == a.parts - 1)
         for (int i = 0; i < 4; ++i) agent_store(word + i, 0);

@@ -132,3 +132,40 @@ def test_draws_of_0_on_large_trees(cuda, K, gap):
     c.drafts[:] = rng.choice([0, 777, 12345], c.T)
     w = _check_cut(cuda, K, c)
     assert (gap < 660) == (w[2] == 0).any()
+
+
+# ---- starts that do not rise, temperatures without end ------------------------------------
+
+
+@pytest.mark.parametrize("sampled", [False, True])
+@pytest.mark.parametrize("vocab,n,batch", [(200, 4, 3), (33000, 400, 3), (3001, 120, 70)])
+def test_starts_that_fall_leave_no_sequences(cuda, K, vocab, n, batch, sampled):
+    """Whether all rows are read or those of the path alone."""
+    rng = np.random.default_rng(13)
+    c = Case(rng, [n] * batch, vocab, 3, sampled)
+    assert sampled or _path_alone(K, [n] * batch, vocab, 3) == (n > 4)
+    c.starts[batch - 1] = c.starts[batch - 2] - 2
+    c.device(cuda, K)
+    c.run(K)
+    path, kept, after = c.got(cuda)
+    assert (path == -1).all() and (kept == 0).all() and (after == -1).all()
+    c.m.free()
+    c = Case(rng, [n] * batch, vocab, 3, sampled).device(cuda, K)  # and the calls behind it are as ever
+    c.run(K)
+    _same(c.got(cuda), c.want())
+    c.m.free()
+
+
+@pytest.mark.parametrize("sampled", [False, True])
+@pytest.mark.parametrize("sizes,vocab", [([8, 5], 3000), ([200] * 3, 40000)])
+def test_infinite_temperatures(cuda, K, sampled, sizes, vocab):
+    """Every token that can be drawn at all is as likely as any other."""
+    rng = np.random.default_rng(15)
+    c = Case(rng, sizes, vocab, 5, sampled, temps=[1.0] * len(sizes))
+    c.x[:, 100:120] = -np.inf
+    c.temps[:] = np.inf
+    c.device(cuda, K)
+    c.run(K)
+    flat = np.where(c.x == -np.inf, -np.inf, 0.0)
+    _same(c.got(cuda), verify(flat, c.drafts, c.trees, c.starts, np.ones(len(sizes)), c.u, c.q, c.max_depth))
+    c.m.free()
