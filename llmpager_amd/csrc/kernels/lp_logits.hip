@@ -34,6 +34,10 @@ namespace {
 constexpr int kPer = 16;               // logits of a lane in a block
 constexpr int kBlock = 64 * kPer;      // and of a wave
 
+__device__ __forceinline__ int wave_sum_i32(int v) {
+    return (int)wave_reduce_u32((uint32_t)v, 0u, [](uint32_t a, uint32_t b) { return a + b; });
+}
+
 // e^d for d <= 0: the hardware's base-2 exponential, with what the product
 // d log2 e is rounded by put back, so that it is good to a few units of 2^-24
 // at any d.
@@ -238,6 +242,15 @@ struct Best : Keys {
         flush();
     }
 };
+
+// Four logits from index e of a row; those outside [0, n) are -inf.
+__device__ __forceinline__ f32x4_t load4(const LP_GLOBAL float* x, int e, int n) {
+    if (e >= 0 && e + 4 <= n) return *reinterpret_cast<const LP_GLOBAL f32x4_t*>(x + e);
+    f32x4_t r;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) r[u] = e + u >= 0 && e + u < n ? x[e + u] : -INFINITY;
+    return r;
+}
 
 // What a row's sums make of it: log(n + s), of a small r = s / n by the series of
 // log(1 + r), whose first term left out is 2^-53 of it.

@@ -26,23 +26,11 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
                                             (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, l));
     return t;
 }
-__device__ __forceinline__ int wave_sum_i32(int v) {
-    return (int)wave_reduce_u32((uint32_t)v, 0u, [](uint32_t a, uint32_t b) { return a + b; });
-}
 // (NaN counts as nothing)
 __device__ __forceinline__ float wave_top(float v) {
     return __uint_as_float(wave_reduce_u32(__float_as_uint(v), 0xff800000u, [](uint32_t a, uint32_t b) {
         return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
     }));
-}
-
-// Four logits from index e of a row; those outside [0, n) are -inf.
-__device__ __forceinline__ f32x4_t load4(const LP_GLOBAL float* x, int e, int n) {
-    if (e >= 0 && e + 4 <= n) return *reinterpret_cast<const LP_GLOBAL f32x4_t*>(x + e);
-    f32x4_t r;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) r[u] = e + u >= 0 && e + u < n ? x[e + u] : -INFINITY;
-    return r;
 }
 
 }  // namespace
