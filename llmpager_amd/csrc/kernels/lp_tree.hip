@@ -5,7 +5,7 @@
 #include "lp_paged_device.h"
 
 // Append: the angles are the depths', the rest that of lp_paged.hip and bound like it, by the
-// launch or the copy rate: 1,347 tokens of 32 sequences, 64 + 2 x 4 heads of 128, 16-bit
+// launch or the copy rate: 1,273 tokens of 32 sequences, 64 + 2 x 4 heads of 128, 16-bit
 // pages: 22 us, 4.2 TB/s of 91 MB (17.3 us at the rate of a large copy).
 extern "C" __global__ void __launch_bounds__(256) lp_kv_append_tree_f16_d64(const KvAppendPagedArgs a) { append_body<64, false, true>(a); }
 extern "C" __global__ void __launch_bounds__(256) lp_kv_append_tree_f16_d128(const KvAppendPagedArgs a) { append_body<128, false, true>(a); }
@@ -15,9 +15,11 @@ extern "C" __global__ void __launch_bounds__(256) lp_kv_append_tree_q4_d128(cons
 // Attention: a chunk of rows before the new ones is walked as in lp_paged.hip, one that
 // holds new ones has each query row's scores taken from its token's mask.  26 tokens of 32
 // heads on 4 of 128 over 1,526 16-bit rows 16.6 us: the launch, a chain of round trips
-// (lengths, pages, rows), two units a workgroup and the join of up to 6 parts.  16 sequences of up to 32 tokens,
+// (lengths, pages, rows), three units a workgroup and the join of up to 4 parts.  16 sequences of up to 32 tokens,
 // up to 6,032 4-bit rows: 70 us and 10 of the join; its 8,212 chunks of 128 query rows by 64 are 59 us of matrix
-// work on 256 CUs, of which the fullest has 36 and the mean 32.  4 sequences of up to 256 tokens, 64 heads on
+// work on 256 CUs, of which the fullest has 36 and the mean 32.  27 % of the chunks' query rows are none (96 to
+// 256 rows a sequence and KV head), 20 % of their waves have none at all, which do a quarter of
+// a full one's matrix work still: by the waves that have some it would be 47 us.  4 sequences of up to 256 tokens, 64 heads on
 // 4, 3,257 16-bit rows and fewer: 135 us, 15,612 chunks, 112 us of matrix work, 73 chunks on the fullest CU and
 // 61 on the mean; parts of them cost more in records and joins than they even out (1,024 workgroups
 // 164 us where 512 took 163, of the 16 sequences 93 against 87).

@@ -1322,7 +1322,8 @@ static PagedPlan paged_plan(const lp_kv_cache* c, int heads, int batch, int toke
 // over 1,400 37 against 33.  4 bits: 4 x 60 over 3,000 37 against 43, 8 x 32 over 3,000 37 against 40 and
 // over 4,000 48 against 44, 16 x 16 over 3,000 40 and 40.  Heads of 64 have half the work: 16 x 32
 // over 1,500 18 against 26.  17 to 32 rows: 64 x 4 over 4,000 with 16 bits 91 against 83,
-// 32 x 4 over 3,000 37 against 41; with 4 bits 55 against 63.
+// 32 x 4 over 3,000 37 against 41; with 4 bits 55 against 63.  (Other shapes, 64 heads on 4, 32 on 8 or few
+// to a KV head, go by the same lines, which have not been measured with them.)
 constexpr int kTreeUnitsQ4 = 6144, kTreeUnits = 7168, kTreeUnitsWide = 5760, kTreePairUnits = 448, kTreePairUnitsWide = 1024;
 constexpr int kTreeUnits32 = 8192, kTreeUnitsOne = 1280;
 static PagedPlan tree_plan(const lp_kv_cache* c, int heads, int batch, int tokens, int max_q, int max_seq) {
